@@ -580,6 +580,43 @@ ts_status ts_rescale_inplace(void* x, int64_t n, ts_dtype dtype, const float* no
                              const float* used, float* hint_out, ts_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* Global gradient norm and clipping                                         */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * The lists are HOST arrays of `count` entries: device pointers (NULL only for an empty
+ * tensor), numbers of elements, and ts_dtype codes. They are read before the call returns. Each
+ * tensor is contiguous; any element-aligned address will do. The lists' order and the tensors'
+ * sizes alone fix the order of the sums.
+ *
+ * norm = sqrt(sum over all tensors of x^2), summed in double and rounded to fp32 once.
+ * Workspace: ts_grad_norm_workspace_size(count) bytes, 8-byte aligned.
+ */
+size_t ts_grad_norm_workspace_size(int64_t count);
+ts_status ts_grad_norm(const void* const* tensors, const int64_t* numels,
+                       const int32_t* dtypes, int64_t count, float* norm,
+                       void* workspace, size_t workspace_bytes, ts_stream_t stream);
+
+/*
+ * out = x * min(1, max_norm / (*norm + 1e-6)) with a norm formed before (on the device; by
+ * ts_grad_norm, or combined over ranks): fp32 product, rounded once. An out entry may be its
+ * tensor (in place; nothing is written when the factor is 1) and otherwise overlaps no other
+ * buffer; out_dtypes[i] is the tensor's dtype or TS_F32. A NaN norm makes every output NaN.
+ */
+ts_status ts_grad_scale(const void* const* tensors, void* const* outs, const int64_t* numels,
+                        const int32_t* dtypes, const int32_t* out_dtypes, int64_t count,
+                        const float* norm, float max_norm, ts_stream_t stream);
+
+/*
+ * Both at once: *norm = the tensors' norm, out = x * min(1, max_norm / (norm + 1e-6)).
+ * Counterpart of the trainer's clip_grad_norm_ call (trainers/sota_trainer.py:2214-2245).
+ */
+ts_status ts_grad_clip(const void* const* tensors, void* const* outs, const int64_t* numels,
+                       const int32_t* dtypes, const int32_t* out_dtypes, int64_t count,
+                       float max_norm, float* norm, void* workspace, size_t workspace_bytes,
+                       ts_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* Measurement                                                               */
 /* ------------------------------------------------------------------------ */
 

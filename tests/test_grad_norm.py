@@ -1,0 +1,194 @@
+"""Gradient norm and clipping on the CPU: host checks of the C ABI and of the Python entry
+points, and the cutting of tensors into chunks."""
+import ctypes
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+from trainscale_amd import _lib
+from trainscale_amd.kernels import (clip_grad_norm_, clip_grads_with_norm_, clipped_grads,
+                                    get_total_norm)
+from trainscale_amd.kernels.grad_kernels import _is_dense, _refuse_overlap
+
+TS_OK, INVALID, DTYPE, SHAPE, WORKSPACE = 0, -1, -2, -3, -4
+CSRC = Path(__file__).resolve().parent.parent / "trainscale_amd" / "csrc"
+FAKE = ctypes.c_void_p(0x1000)  # never dereferenced: every call below ends on the host
+
+
+def _lists(ptrs, numels, dtypes):
+    n = len(ptrs)
+    return ((ctypes.c_void_p * n)(*ptrs), (ctypes.c_int64 * n)(*numels),
+            (ctypes.c_int32 * n)(*dtypes))
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return _lib.load()
+
+
+def test_norm_validation(lib):
+    need = lib.ts_grad_norm_workspace_size(2)
+
+    def call(ptrs=(0x1000, 0x2000), numels=(5, 7), dtypes=(0, 1), norm=FAKE, ws=FAKE, wsb=need,
+             count=2):
+        p, n, d = _lists(ptrs, numels, dtypes)
+        return lib.ts_grad_norm(p, n, d, count, norm, ws, wsb, None)
+
+    assert call(count=-1) == SHAPE
+    assert call(numels=(5, -1)) == SHAPE
+    assert call(dtypes=(0, 3)) == DTYPE
+    assert call(ptrs=(0x1000, None)) == INVALID
+    assert call(ptrs=(0x1002, 0x2000)) == INVALID  # an fp32 tensor off its elements
+    assert b"aligned" in lib.ts_last_error()
+    assert call(ptrs=(0x1000, 0x2001)) == INVALID
+    assert call(norm=None) == INVALID
+    assert call(ws=None) == WORKSPACE
+    assert call(ws=ctypes.c_void_p(0x1004)) == WORKSPACE
+    assert call(wsb=need - 1) == WORKSPACE
+    assert call(numels=(5, 1 << 62)) == SHAPE
+    assert lib.ts_grad_norm(None, None, None, 2, FAKE, FAKE, need, None) == INVALID
+
+
+def test_scale_and_clip_validation(lib):
+    need = lib.ts_grad_norm_workspace_size(1)
+
+    def scale(ptr=0x1000, out=0x2000, numel=5, dt=1, odt=1, norm=FAKE, max_norm=1.0):
+        p, n, d = _lists([ptr], [numel], [dt])
+        return lib.ts_grad_scale(p, (ctypes.c_void_p * 1)(out), n, d, (ctypes.c_int32 * 1)(odt), 1,
+                                 norm, max_norm, None)
+
+    assert scale(odt=2) == DTYPE  # bf16 into fp16
+    assert scale(dt=0, odt=1) == DTYPE  # fp32 into bf16
+    assert scale(out=None) == INVALID
+    assert scale(out=0x2002, odt=0) == INVALID
+    assert scale(norm=None) == INVALID
+    assert scale(max_norm=-1.0) == INVALID
+    assert scale(max_norm=float("nan")) == INVALID
+    assert scale(numel=0, ptr=None, out=None) == TS_OK  # an empty tensor is nothing to do
+    p, n, d = _lists([0x1000], [5], [1])
+    o, od = (ctypes.c_void_p * 1)(0x2000), (ctypes.c_int32 * 1)(0)
+    clip = lambda **k: lib.ts_grad_clip(p, o, n, d, od, 1, k.get("max_norm", 1.0),
+                                        k.get("norm", FAKE), k.get("ws", FAKE),
+                                        k.get("wsb", need), None)
+    assert clip(max_norm=-0.5) == INVALID
+    assert clip(norm=None) == INVALID
+    assert clip(wsb=8) == WORKSPACE
+    assert clip(ws=None) == WORKSPACE
+
+
+def test_python_refusals():
+    p = torch.nn.Parameter(torch.zeros(4))
+    p.grad = torch.zeros(4)
+    with pytest.raises(RuntimeError, match="GPU"):
+        clip_grad_norm_([p], 1.0)
+    with pytest.raises(ValueError, match="max_norm"):
+        clip_grad_norm_([p], -1.0)
+    with pytest.raises(ValueError, match="max_norm"):
+        clip_grads_with_norm_([p], float("nan"), torch.tensor(1.0))
+    with pytest.raises(ValueError, match="2-norm"):
+        clip_grad_norm_([p], 1.0, norm_type=1)
+    with pytest.raises(ValueError, match="2-norm"):
+        get_total_norm([p.grad], float("inf"))
+    with pytest.raises(TypeError, match="dtype"):
+        get_total_norm([torch.zeros(3, dtype=torch.float64)])
+    with pytest.raises(TypeError, match="sparse"):
+        get_total_norm([torch.zeros(3, 3).to_sparse()])
+    with pytest.raises(TypeError, match="expected tensors"):
+        get_total_norm([1.0])
+    with pytest.raises(TypeError, match="local tensor"):
+        get_total_norm([torch.zeros(3).as_subclass(type("Sharded", (torch.Tensor,), {}))])
+
+
+def test_nothing_to_clip():
+    assert float(clip_grad_norm_([torch.nn.Parameter(torch.zeros(3))], 1.0)) == 0.0
+    assert float(get_total_norm([])) == 0.0
+    assert float(clipped_grads([], 1.0, [])) == 0.0
+    clip_grads_with_norm_([], 1.0, torch.tensor(1.0))
+
+
+def test_dense_and_overlap():
+    t = torch.zeros(4, 6, 5)
+    assert _is_dense(t) and _is_dense(t.permute(2, 0, 1)) and _is_dense(t[1])
+    assert not _is_dense(t[:, 1:]) and not _is_dense(t[:, :, ::2])
+    assert not _is_dense(torch.zeros(1, 5).expand(3, 5))
+    flat = torch.zeros(100)
+    a, b = flat[:50], flat[50:]
+    _refuse_overlap("x", [a, b], [a, b])
+    with pytest.raises(ValueError, match="share memory"):
+        _refuse_overlap("x", [a, flat[49:]], [a, flat[49:]])
+    with pytest.raises(ValueError, match="share memory"):  # the same tensor twice
+        _refuse_overlap("x", [a, a], [a, a])
+    with pytest.raises(ValueError, match="share memory"):  # an output over another's gradient
+        _refuse_overlap("x", [b, torch.zeros(50)], [a, flat[20:70]])
+    with pytest.raises(ValueError, match="share memory"):  # a small one inside a large one
+        _refuse_overlap("x", [torch.zeros(100), flat[10:12]], [flat, torch.zeros(2)])
+    _refuse_overlap("x", [torch.zeros(50), torch.zeros(50)], [a, a])  # read twice
+    _refuse_overlap("x", [flat[:0], flat], [flat[:0], flat])
+
+
+DRIVER = r"""
+#include <cstdio>
+#include <initializer_list>
+#include <vector>
+#include "plan.hpp"
+using namespace ts_plan;
+int main() {
+  int fails = 0;
+  unsigned r = 12345;
+  for (int elt : {2, 4})
+    for (int count : {1, 2, 3, 100, kGradTensors})
+      for (int rep = 0; rep < 20; ++rep) {
+        std::vector<int64_t> numel(count);
+        std::vector<int32_t> end(count);
+        int64_t chunks = 0;
+        const int64_t per = kGradChunkBytes / elt;
+        for (int i = 0; i < count; ++i) {
+          r = r * 1664525u + 1013904223u;
+          const int64_t edge[] = {1, per - 1, per, per + 1, 3 * per, (int64_t)(r >> 12) + 1};
+          numel[i] = edge[r % 6];
+          chunks += grad_chunks(numel[i], elt);
+          end[i] = (int32_t)chunks;
+        }
+        // every chunk belongs to one tensor and holds at least one of its values; together
+        // they hold all of them
+        std::vector<int64_t> held(count, 0);
+        for (int64_t c = 0; c < chunks; ++c) {
+          const int t = grad_find_tensor(end, count, (int)c);
+          const int64_t first = (c - (t ? end[t - 1] : 0)) * per;
+          const int64_t left = numel[t] - first;
+          if (t < 0 || t >= count || c >= end[t] || first < 0 || left <= 0) { ++fails; continue; }
+          held[t] += left < per ? left : per;
+        }
+        for (int i = 0; i < count; ++i) fails += held[i] != numel[i];
+      }
+  // launches of a list: full ones, and at most one that is not full for each of three types
+  for (int64_t count = 1; count < 2000; ++count) {
+    int64_t most = 0;
+    for (int64_t a = 0; a <= 2; ++a)
+      for (int64_t b = 0; b <= 2; ++b) {
+        const int64_t n1 = count > a ? a : 0, n2 = count - n1 > b ? b : 0, n3 = count - n1 - n2;
+        int64_t l = 0;
+        for (int64_t n : {n1, n2, n3}) l += (n + kGradTensors - 1) / kGradTensors;
+        most = l > most ? l : most;
+      }
+    fails += most * kGradGrid > grad_norm_parts(count);
+  }
+  fails += grad_chunks(0, 2) != 0 || grad_norm_parts(0) < 1;
+  std::printf("%d failures\n", fails);
+  return fails != 0;
+}
+"""
+
+
+def test_chunks(tmp_path):
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("g++ not available")
+    src, exe = tmp_path / "chunks.cpp", tmp_path / "chunks"
+    src.write_text(DRIVER)
+    subprocess.run([gxx, "-O2", "-std=c++17", f"-I{CSRC}", str(src), "-o", str(exe)], check=True)
+    proc = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert proc.returncode == 0, proc.stdout + proc.stderr

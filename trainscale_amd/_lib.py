@@ -103,6 +103,10 @@ SIGNATURES = {
     "ts_swiglu_fwd": ([P, P, P, I64, I32, P], I32),
     "ts_swiglu_bwd": ([P, P, P, P, P, I64, I32, P], I32),
     "ts_rescale_inplace": ([P, I64, I32, P, P, P, P], I32),
+    "ts_grad_norm_workspace_size": ([I64], SZ),
+    "ts_grad_norm": ([P, P, P, I64, P, P, SZ, P], I32),
+    "ts_grad_scale": ([P, P, P, P, P, I64, P, F32, P], I32),
+    "ts_grad_clip": ([P, P, P, P, P, I64, F32, P, P, SZ, P], I32),
     "ts_stream_copy": ([P, P, I64, P], I32),
 }
 

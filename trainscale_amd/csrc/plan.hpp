@@ -492,4 +492,34 @@ TS_HOST_DEVICE inline RopeElems rope_elems(int j, int width, int half, bool inte
   return interleaved ? RopeElems{j * width, -1} : RopeElems{j * width, half + j * width};
 }
 
+// ---------------------------------------------------------------------------
+// Global gradient norm and clipping (grad_norm.hip): the tensors of a launch are cut into
+// chunks of kGradChunkBytes (of the gradients), numbered through; chunk_end[t] is the number of
+// chunks of tensors 0 .. t.
+// ---------------------------------------------------------------------------
+constexpr int kGradTensors = 128;               // tensors of one launch
+constexpr int kGradGrid = 2048;                 // most workgroups of a launch: 8 a CU
+constexpr int64_t kGradChunkBytes = 64 * 1024;
+constexpr int64_t kGradMaxChunks = 1ll << 30;   // 64 TiB of gradients
+
+TS_HOST_DEVICE inline int64_t grad_chunks(int64_t numel, int elt) {
+  const int64_t per = kGradChunkBytes / elt;
+  return numel / per + (numel % per != 0);
+}
+// The tensor that chunk c belongs to (c < end[count - 1]; no tensor is empty).
+template <typename A>
+TS_HOST_DEVICE inline int grad_find_tensor(const A& end, int count, int c) {
+  int lo = 0, hi = count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (c < end[mid]) hi = mid; else lo = mid + 1;
+  }
+  return lo;
+}
+// Doubles that the norm of `count` tensors may write: kGradGrid for each of its launches, of
+// which every type has at most one that is not full.
+inline int64_t grad_norm_parts(int64_t count) {
+  return count <= 0 ? 1 : (count / kGradTensors + 3) * kGradGrid;
+}
+
 }  // namespace ts_plan

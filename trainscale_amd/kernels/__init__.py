@@ -14,6 +14,12 @@ from .fused_kernels import (
     fast_cross_entropy_loss,
     swiglu_forward,
 )
+from .grad_kernels import (
+    clip_grad_norm_,
+    clip_grads_with_norm_,
+    clipped_grads,
+    get_total_norm,
+)
 from .layernorm_kernels import (
     FusedAddRMSLayerNormFunction,
     FusedRMSNorm,
@@ -68,4 +74,8 @@ __all__ = [
     "fast_rope_embedding",
     "inplace_rope_embedding",
     "precompute_freqs_cis",
+    "get_total_norm",
+    "clip_grad_norm_",
+    "clip_grads_with_norm_",
+    "clipped_grads",
 ]

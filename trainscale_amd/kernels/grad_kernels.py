@@ -1,0 +1,217 @@
+"""Global gradient norm over many tensors, and clipping.
+
+The trainer clips the global norm between the backward pass and the optimizer's step
+(data_pipeline/trainer/trainers/sota_trainer.py:2214-2245, through torch's ``clip_grad_norm_``).
+The functions here keep torch's names, arguments and arithmetic for the 2-norm:
+
+    norm = sqrt(sum of x^2 over all gradients),  gradients *= min(1, max_norm / (norm + 1e-6))
+
+A few launches cover every tensor of a model, whatever their number, sizes and types (fp32,
+bf16, fp16 mixed); the norm is summed in double in a fixed order and nothing waits for the host.
+A norm that is NaN makes every clipped gradient NaN, an infinite one zeros the finite gradients,
+as torch's arithmetic does.
+
+``clipped_grads`` writes the clipped gradients elsewhere, for optimizers that keep fp32 main
+gradients next to 16-bit ones: one pass instead of a copy and a scaling.
+"""
+from __future__ import annotations
+
+import math
+from typing import Iterable, List, Optional, Sequence, Union
+
+import torch
+from torch import Tensor
+
+from .. import _lib, ops
+
+__all__ = ["get_total_norm", "clip_grads_with_norm_", "clip_grad_norm_", "clipped_grads"]
+
+
+def _is_dense(t: Tensor) -> bool:
+    """Whether the elements fill their memory without gaps or overlaps, in any order."""
+    want = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != want:
+            return False
+        want *= size
+    return True
+
+
+def _checked(what: str, tensors: Union[Tensor, Iterable[Tensor]]) -> List[Tensor]:
+    """The tensors as a list: dense fp32/bf16/fp16 torch tensors on one GPU."""
+    tensors = [tensors] if isinstance(tensors, Tensor) else list(tensors)
+    dev = None
+    for t in tensors:
+        if not isinstance(t, Tensor):
+            raise TypeError(f"{what}: expected tensors, got {type(t).__name__}")
+        if type(t) not in (Tensor, torch.nn.Parameter):
+            raise TypeError(f"{what}: {type(t).__name__} is not supported: pass its local tensor")
+        if t.layout != torch.strided:
+            raise TypeError(f"{what}: sparse gradients are not supported")
+        if t.dtype not in _lib.DTYPE_CODE:
+            raise TypeError(f"{what}: unsupported dtype {t.dtype} (float32/bfloat16/float16)")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise RuntimeError(f"{what}: tensors are on different devices ({dev} vs {t.device})")
+    if tensors:
+        _lib.require_gpu(what, tensors[0])
+    return tensors
+
+
+def _storage_order(t: Tensor) -> Tensor:
+    """The values of t in an order of their own, contiguous: t itself where it is dense."""
+    return t if t.is_contiguous() or _is_dense(t) else t.contiguous()
+
+
+def _refuse_overlap(what: str, written: Sequence[Tensor], read: Sequence[Tensor]) -> None:
+    """Raises if a written tensor shares memory with another tensor of either list. A tensor of
+    `read` that is the written one at the same place in the list does not count."""
+    spans = []
+    for w, r in zip(written, read):
+        n = w.numel()
+        if n == 0:
+            continue
+        a = w.data_ptr()
+        spans.append((a, a + n * w.element_size(), True))
+        b = r.data_ptr()
+        if b != a or r.dtype != w.dtype:
+            spans.append((b, b + n * r.element_size(), False))
+    spans.sort()
+    end, end_written = 0, False
+    for a, b, is_written in spans:
+        if a < end and (is_written or end_written):
+            raise ValueError(f"{what}: gradients share memory: each must be written once")
+        if b > end:
+            end, end_written = b, is_written
+        elif is_written:
+            end_written = True
+
+
+def _max_norm(what: str, max_norm: float) -> float:
+    max_norm = float(max_norm)
+    if not max_norm >= 0:
+        raise ValueError(f"{what}: max_norm must be >= 0, got {max_norm}")
+    return max_norm
+
+
+def _check_norm_type(what: str, norm_type: float) -> None:
+    if float(norm_type) != 2.0:
+        raise ValueError(f"{what}: only the 2-norm is supported, got norm_type {norm_type}")
+
+
+def _grads(parameters: Union[Tensor, Iterable[Tensor]]) -> List[Tensor]:
+    """The gradients of the parameters that have one; a parameter given twice counts once."""
+    parameters = [parameters] if isinstance(parameters, Tensor) else parameters
+    seen = {id(p): p for p in parameters}
+    return [p.grad for p in seen.values() if p.grad is not None]
+
+
+def get_total_norm(tensors: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0,
+                   error_if_nonfinite: bool = False, foreach: Optional[bool] = None) -> Tensor:
+    """The 2-norm of all values of the tensors as a 0-dim fp32 tensor (torch's
+    ``get_total_norm``; foreach is accepted for its signature). Of an empty list 0, on the CPU.
+    Tensors are read only: they may share memory, and each counts as often as it is given."""
+    del foreach
+    _check_norm_type("get_total_norm", norm_type)
+    tensors = _checked("get_total_norm", tensors)
+    if not tensors:
+        return torch.tensor(0.0)
+    norm = ops.grad_norm([_storage_order(t.detach()) for t in tensors], tensors[0].device)
+    if error_if_nonfinite:
+        _raise_if_nonfinite(norm)
+    return norm
+
+
+def _raise_if_nonfinite(norm: Tensor) -> None:
+    if not math.isfinite(norm.item()):
+        raise RuntimeError("the total norm of the gradients is non-finite, so it cannot be "
+                           "clipped; pass error_if_nonfinite=False to scale them all the same")
+
+
+def _scale_in_place(what: str, grads: List[Tensor], launch) -> Optional[Tensor]:
+    """Runs launch(contiguous tensors) over the gradients; those that are not dense (slices of a
+    larger buffer) are scaled in a copy and copied back."""
+    for g in grads:
+        if any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
+            raise ValueError(f"{what}: a gradient's elements share memory (an expanded tensor)")
+    held = [_storage_order(g.detach()) for g in grads]
+    _refuse_overlap(what, held, held)
+    out = launch(held)
+    for g, h in zip(grads, held):
+        if h.data_ptr() != g.data_ptr():
+            with torch.no_grad():
+                g.copy_(h)
+    torch.autograd.graph.increment_version(grads)
+    return out
+
+
+def clip_grads_with_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float,
+                          total_norm: Tensor, foreach: Optional[bool] = None) -> None:
+    """Scales the parameters' gradients in place by min(1, max_norm / (total_norm + 1e-6))
+    (torch's ``clip_grads_with_norm_``): for a norm formed before, over the ranks of a sharded
+    model for instance. total_norm is a tensor of one value on the gradients' device."""
+    del foreach
+    what = "clip_grads_with_norm_"
+    max_norm = _max_norm(what, max_norm)
+    grads = _checked(what, _grads(parameters))
+    if not grads:
+        return
+    dev = grads[0].device
+    if not isinstance(total_norm, Tensor) or total_norm.numel() != 1:
+        raise TypeError(f"{what}: total_norm must be a tensor of one value")
+    _lib.require_gpu(what, grads[0], total_norm)
+    norm = total_norm.detach().to(torch.float32).reshape(())
+    _scale_in_place(what, grads, lambda t: ops.grad_scale(t, t, norm, max_norm, dev))
+
+
+def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float,
+                    norm_type: float = 2.0, error_if_nonfinite: bool = False,
+                    foreach: Optional[bool] = None) -> Tensor:
+    """Clips the global 2-norm of the parameters' gradients in place and returns the norm before
+    clipping, a 0-dim fp32 tensor (torch's ``clip_grad_norm_``; foreach is accepted for its
+    signature). Parameters without a gradient are skipped; a parameter given twice counts once.
+    Gradients that share memory with one another are refused. error_if_nonfinite waits for the
+    norm and raises, with the gradients unscaled, if it is not finite."""
+    del foreach
+    what = "clip_grad_norm_"
+    _check_norm_type(what, norm_type)
+    max_norm = _max_norm(what, max_norm)
+    grads = _checked(what, _grads(parameters))
+    if not grads:
+        return torch.tensor(0.0)
+    dev = grads[0].device
+    if error_if_nonfinite:
+        norm = ops.grad_norm([_storage_order(g.detach()) for g in grads], dev)
+        _raise_if_nonfinite(norm)
+        _scale_in_place(what, grads, lambda t: ops.grad_scale(t, t, norm, max_norm, dev))
+        return norm
+    return _scale_in_place(what, grads, lambda t: ops.grad_clip(t, t, max_norm, dev))
+
+
+def clipped_grads(grads: Sequence[Tensor], max_norm: float, out: Sequence[Tensor]) -> Tensor:
+    """out[i] = grads[i] * min(1, max_norm / (norm + 1e-6)), norm the global 2-norm of grads,
+    which is returned (0-dim fp32). out[i] has grads[i]'s shape, is contiguous, and is fp32 or of
+    the gradient's dtype: fp32 main gradients of 16-bit ones, for instance. It may be grads[i]
+    itself and otherwise shares no memory with any other tensor of the call."""
+    what = "clipped_grads"
+    max_norm = _max_norm(what, max_norm)
+    grads = _checked(what, grads)
+    out = _checked(what, out)
+    if len(out) != len(grads):
+        raise ValueError(f"{what}: {len(out)} outputs for {len(grads)} gradients")
+    if not grads:
+        return torch.tensor(0.0)
+    for g, o in zip(grads, out):
+        if o.shape != g.shape:
+            raise ValueError(f"{what}: output {tuple(o.shape)} for a gradient {tuple(g.shape)}")
+        if o.dtype not in (g.dtype, torch.float32):
+            raise TypeError(f"{what}: output dtype {o.dtype} for a gradient of {g.dtype}")
+        if not o.is_contiguous():
+            raise ValueError(f"{what}: outputs must be contiguous")
+    _lib.require_gpu(what, grads[0], out[0])
+    src = [g.detach() if g.is_contiguous() else g.detach().contiguous() for g in grads]
+    _refuse_overlap(what, out, src)
+    norm = ops.grad_clip(src, out, max_norm, grads[0].device)
+    torch.autograd.graph.increment_version(out)
+    return norm

@@ -8,6 +8,8 @@ wrappers with the reference's signatures (``trainscale_amd.kernels``,
 """
 from __future__ import annotations
 
+import ctypes
+
 from typing import Optional, Tuple
 
 import torch
@@ -520,3 +522,58 @@ def swiglu_backward(dout: Tensor, gate: Tensor, up: Tensor) -> Tuple[Tensor, Ten
                                 gate.numel(), _lib.dtype_code(gate, "swiglu"),
                                 _lib.stream_handle(dev)), "ts_swiglu_bwd")
     return dgate, dup
+
+
+# ---------------------------------------------------------------------------
+# Global gradient norm and clipping
+# ---------------------------------------------------------------------------
+
+def _host_lists(tensors, outs=None):
+    """The C ABI's host lists of contiguous tensors: pointers, element counts, dtype codes (and
+    the outputs' pointers and codes)."""
+    n = len(tensors)
+    code = _lib.DTYPE_CODE
+    lists = [(ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors]),
+             (ctypes.c_int64 * n)(*[t.numel() for t in tensors]),
+             (ctypes.c_int32 * n)(*[code[t.dtype] for t in tensors])]
+    if outs is not None:
+        lists += [(ctypes.c_void_p * n)(*[t.data_ptr() for t in outs]),
+                  (ctypes.c_int32 * n)(*[code[t.dtype] for t in outs])]
+    return lists
+
+
+def grad_norm(tensors, dev: torch.device) -> Tensor:
+    """The 2-norm of all values of contiguous tensors on `dev`: a 0-dim fp32 tensor."""
+    lib = _lib.load()
+    n = len(tensors)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    wsb = int(lib.ts_grad_norm_workspace_size(n))
+    ws = torch.empty((wsb,), dtype=torch.uint8, device=dev)
+    src, numel, dt = _host_lists(tensors)
+    with _lib.on_device(dev):
+        check(lib.ts_grad_norm(src, numel, dt, n, ptr(norm), ptr(ws), wsb,
+                               _lib.stream_handle(dev)), "ts_grad_norm")
+    return norm
+
+
+def grad_scale(tensors, outs, norm: Tensor, max_norm: float, dev: torch.device) -> None:
+    """outs = tensors * min(1, max_norm / (norm + 1e-6)); norm a 0-dim fp32 tensor on `dev`."""
+    lib = _lib.load()
+    src, numel, dt, dst, ddt = _host_lists(tensors, outs)
+    with _lib.on_device(dev):
+        check(lib.ts_grad_scale(src, dst, numel, dt, ddt, len(tensors), ptr(norm), max_norm,
+                                _lib.stream_handle(dev)), "ts_grad_scale")
+
+
+def grad_clip(tensors, outs, max_norm: float, dev: torch.device) -> Tensor:
+    """grad_norm, then grad_scale by it; returns the norm."""
+    lib = _lib.load()
+    n = len(tensors)
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    wsb = int(lib.ts_grad_norm_workspace_size(n))
+    ws = torch.empty((wsb,), dtype=torch.uint8, device=dev)
+    src, numel, dt, dst, ddt = _host_lists(tensors, outs)
+    with _lib.on_device(dev):
+        check(lib.ts_grad_clip(src, dst, numel, dt, ddt, n, max_norm, ptr(norm), ptr(ws), wsb,
+                               _lib.stream_handle(dev)), "ts_grad_clip")
+    return norm
