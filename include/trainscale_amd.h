@@ -580,6 +580,35 @@ ts_status ts_rescale_inplace(void* x, int64_t n, ts_dtype dtype, const float* no
                              const float* used, float* hint_out, ts_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* Token embedding                                                           */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * out[n, :] = scale * weight[ids[n], :] (fp32 product, rounded once); an id outside [0, V)
+ * gives a row of NaN. weight: [V, H] and out: [N, H] of dtype with row strides ldw, ldo; any
+ * H and any element-aligned address.
+ */
+ts_status ts_embedding_fwd(const int64_t* ids, int64_t N, const void* weight, int64_t ldw,
+                           ts_dtype dtype, int64_t V, int64_t H, float scale, void* out,
+                           int64_t ldo, ts_stream_t stream);
+
+/* Bytes of workspace ts_embedding_bwd needs (0 for sizes it refuses): about 16 N + H N / 8. */
+size_t ts_embedding_bwd_workspace_size(int64_t N, int64_t V, int64_t H);
+
+/*
+ * grad_weight[v, :] = scale * sum over n with ids[n] = v of dout[n, :], for every v in [0, V)
+ * (rows without a token are written as zeros): the tokens are sorted by id, each row is summed
+ * in fp32 in an order that the ids alone fix and rounded once. Tokens whose id is padding_idx
+ * or outside [0, V) contribute nothing (a padding_idx outside [0, V): none).
+ * dout: [N, H] of dtype, row stride ldd; grad_weight: [V, H] of dtype, contiguous. N and V at
+ * most 2^31 - 2. Workspace: 16-byte aligned.
+ */
+ts_status ts_embedding_bwd(const int64_t* ids, int64_t N, const void* dout, int64_t ldd,
+                           ts_dtype dtype, int64_t V, int64_t H, float scale,
+                           int64_t padding_idx, void* grad_weight, void* workspace,
+                           size_t workspace_bytes, ts_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* Global gradient norm and clipping                                         */
 /* ------------------------------------------------------------------------ */
 

@@ -214,7 +214,8 @@ def test_stays_inside(gpu, src, dst, n):
     lib = _lib.load()
     wsb = int(lib.ts_grad_norm_workspace_size(1))
     gw = flat(wsb, torch.uint8, gpu)
-    p, k, d, o, od = ops._host_lists([gx.t], [go.t])
+    li, lo = ops.HostList([gx.t]), ops.HostList([go.t])
+    p, k, d, o, od = map(ops._host, (li.ptr, li.numel, li.code, lo.ptr, lo.code))
     _lib.check(lib.ts_grad_clip(p, o, k, d, od, 1, 0.5, gn.p, gw.p, wsb, _lib.stream_handle(gpu)),
                "clip")
     assert gx.intact() and go.intact() and gn.intact() and gw.intact()

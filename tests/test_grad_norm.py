@@ -12,6 +12,7 @@ from trainscale_amd import _lib
 from trainscale_amd.kernels import (clip_grad_norm_, clip_grads_with_norm_, clipped_grads,
                                     get_total_norm)
 from trainscale_amd.kernels.grad_kernels import _is_dense, _refuse_overlap
+from trainscale_amd.ops import HostList
 
 TS_OK, INVALID, DTYPE, SHAPE, WORKSPACE = 0, -1, -2, -3, -4
 CSRC = Path(__file__).resolve().parent.parent / "trainscale_amd" / "csrc"
@@ -116,17 +117,24 @@ def test_dense_and_overlap():
     assert not _is_dense(torch.zeros(1, 5).expand(3, 5))
     flat = torch.zeros(100)
     a, b = flat[:50], flat[50:]
-    _refuse_overlap("x", [a, b], [a, b])
-    with pytest.raises(ValueError, match="share memory"):
-        _refuse_overlap("x", [a, flat[49:]], [a, flat[49:]])
-    with pytest.raises(ValueError, match="share memory"):  # the same tensor twice
-        _refuse_overlap("x", [a, a], [a, a])
-    with pytest.raises(ValueError, match="share memory"):  # an output over another's gradient
-        _refuse_overlap("x", [b, torch.zeros(50)], [a, flat[20:70]])
-    with pytest.raises(ValueError, match="share memory"):  # a small one inside a large one
-        _refuse_overlap("x", [torch.zeros(100), flat[10:12]], [flat, torch.zeros(2)])
-    _refuse_overlap("x", [torch.zeros(50), torch.zeros(50)], [a, a])  # read twice
-    _refuse_overlap("x", [flat[:0], flat], [flat[:0], flat])
+
+    def check(written, read=None):
+        w = HostList(written)
+        _refuse_overlap("x", w, w if read is None else HostList(read))
+
+    check([a, b])
+    check([a, b], [a, b])
+    for written, read in (([a, flat[49:]], None),
+                          ([a, a], None),  # the same tensor twice
+                          ([a, a], [a, a]),
+                          ([b, torch.zeros(50)], [a, flat[20:70]]),  # over another's gradient
+                          ([torch.zeros(100), flat[10:12]], [flat, torch.zeros(2)]),
+                          ([a.view(torch.bfloat16)[:50]], [a])):
+        with pytest.raises(ValueError, match="share memory"):
+            check(written, read)
+    check([torch.zeros(50), torch.zeros(50)], [a, a])  # read twice
+    check([flat[:0], flat])
+    check([torch.zeros(40), flat[60:]], [flat[:60].view(torch.bfloat16)[10:50], flat[:40]])
 
 
 DRIVER = r"""

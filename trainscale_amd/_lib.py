@@ -103,6 +103,9 @@ SIGNATURES = {
     "ts_swiglu_fwd": ([P, P, P, I64, I32, P], I32),
     "ts_swiglu_bwd": ([P, P, P, P, P, I64, I32, P], I32),
     "ts_rescale_inplace": ([P, I64, I32, P, P, P, P], I32),
+    "ts_embedding_fwd": ([P, I64, P, I64, I32, I64, I64, F32, P, I64, P], I32),
+    "ts_embedding_bwd_workspace_size": ([I64, I64, I64], SZ),
+    "ts_embedding_bwd": ([P, I64, P, I64, I32, I64, I64, F32, I64, P, P, SZ, P], I32),
     "ts_grad_norm_workspace_size": ([I64], SZ),
     "ts_grad_norm": ([P, P, P, I64, P, P, SZ, P], I32),
     "ts_grad_scale": ([P, P, P, P, P, I64, P, F32, P], I32),

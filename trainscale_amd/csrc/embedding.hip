@@ -1,0 +1,670 @@
+// Token embedding with scaling, and its gradient by sorted tokens, for gfx950:
+//   out[n, :]  = round(scale * weight[id[n], :])
+//   grad[v, :] = round(scale * sum over n with id[n] = v of dout[n, :])     (fp32 sums)
+// An id outside [0, V) gives a row of NaN and no gradient; the padding id gives no gradient.
+//
+// Forward: a gather, HBM-bound (one row read and one written per token). TPR lanes own a row,
+// its 16-byte vectors TPR apart.
+//
+// Backward: HBM-bound by the dense gradient (V rows written, N read). The tokens are sorted by
+// id, stably, so every gradient row is one run of the sorted list and is summed and written
+// once, without atomics on floats, in an order that depends on the ids alone. The sort is a
+// radix sort of (id, position) pairs by digits of up to 10 bits: ids below 2^20 take two passes
+// (a histogram and a scatter each), fewer than kSmallTokens tokens one launch in LDS. Padding
+// and out-of-range ids get the key V, behind all rows.
+//
+// Token frequencies are far from uniform (a frequent token, or one filler token in most places,
+// would leave one workgroup with thousands of rows), so runs are cut: wherever kChunk
+// neighbours in the sorted list, from a multiple of kChunk on, share one id, their sum is formed
+// beforehand as one fp32 row, and the same again over kChunk such sums. A row's sum then reads
+// at most 2 (kChunk - 1) token rows, as many rows of sums, and N / kChunk^2 rows of sums of
+// sums. Which stretches those are follows from the sorted ids: no list is kept.
+#include "common.hpp"
+#include "plan.hpp"
+
+namespace {
+
+using namespace ts;
+using ts_plan::kEmbedChunk;
+
+constexpr int kThreads = 256;
+constexpr int kWaveKeys = 256;                   // keys of a wave in one step: 4 a lane
+constexpr int kKeysPerLane = kWaveKeys / kWave;
+constexpr int kMaxBins = 1 << ts_plan::kEmbedMaxBits;
+
+// ---------------------------------------------------------------------------
+// Forward
+// ---------------------------------------------------------------------------
+
+// One 16-byte vector of a row, or the row's last elements (v == nvec, fewer than a vector).
+template <typename T>
+__device__ inline void load_part(const T* __restrict__ row, int v, int nvec, int tail,
+                                 float (&f)[Elt<T>::kVec]) {
+  constexpr int V = Elt<T>::kVec;
+  if (v < nvec) {
+    Elt<T>::unpack(ld16_any_stream(row + (int64_t)v * V), f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = i < tail ? Elt<T>::load1(row + (int64_t)v * V + i) : 0.f;
+  }
+}
+template <typename T>
+__device__ inline void store_part(T* __restrict__ row, int v, int nvec, int tail,
+                                  const float (&f)[Elt<T>::kVec]) {
+  constexpr int V = Elt<T>::kVec;
+  if (v < nvec) {
+    st16_any_stream(row + (int64_t)v * V, Elt<T>::pack(f));
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < tail) Elt<T>::store1(row + (int64_t)v * V + i, f[i]);
+  }
+}
+
+template <typename T, int TPR>
+__global__ __launch_bounds__(kThreads) void embed_fwd(const int64_t* __restrict__ ids, int64_t N,
+                                                      const T* __restrict__ w, int64_t ldw,
+                                                      int64_t V, int nvec, int tail, float scale,
+                                                      T* __restrict__ out, int64_t ldo) {
+  constexpr int VE = Elt<T>::kVec;
+  const int64_t n = (int64_t)blockIdx.x * (kThreads / TPR) + threadIdx.x / TPR;
+  if (n >= N) return;
+  const int64_t id = ids[n];
+  const bool in = id >= 0 && id < V;
+  const T* row = w + (in ? id : 0) * ldw;
+  T* o = out + n * ldo;
+  const int parts = nvec + (tail > 0);
+#pragma unroll 2
+  for (int v = threadIdx.x % TPR; v < parts; v += TPR) {
+    float f[VE];
+    load_part(row, v, nvec, tail, f);
+#pragma unroll
+    for (int i = 0; i < VE; ++i) f[i] = in ? f[i] * scale : __builtin_nanf("");
+    store_part(o, v, nvec, tail, f);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Sort of (key, position) by key
+// ---------------------------------------------------------------------------
+
+__device__ inline uint32_t key_of(int64_t id, int64_t V, int64_t padding) {
+  return id >= 0 && id < V && id != padding ? (uint32_t)id : (uint32_t)V;
+}
+
+// Lanes of the wave whose key is valid and has this lane's digit.
+__device__ inline uint64_t same_digit(uint32_t digit, int bits, bool valid) {
+  uint64_t m = __ballot(valid);
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (digit >> b) & 1u;
+    const uint64_t bal = __ballot(one);
+    m &= one ? bal : ~bal;
+  }
+  return m;
+}
+
+// Exclusive prefix sums over the workgroup's threads (kT of them); `lds` holds kT / 64 + 1.
+template <int kT>
+__device__ inline int block_exclusive(int v, int* lds) {
+  const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
+  int inc = v;
+#pragma unroll
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int u = __shfl_up(inc, d, kWave);
+    if (lane >= d) inc += u;
+  }
+  if (lane == kWave - 1) lds[wid] = inc;
+  __syncthreads();
+  int before = 0;
+#pragma unroll
+  for (int i = 0; i < kT / kWave; ++i) before += i < wid ? lds[i] : 0;
+  __syncthreads();
+  return before + inc - v;
+}
+
+// Ranks the wave's keys among equal digits of the wave, in their order: rank[r] for key r * 64 +
+// lane; cnt[digit] (the wave's own, cleared) ends as the digit's count.
+__device__ inline void wave_ranks(const uint32_t (&digit)[kKeysPerLane],
+                                  const bool (&valid)[kKeysPerLane], int bits, volatile int* cnt,
+                                  int (&rank)[kKeysPerLane]) {
+  const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+  for (int r = 0; r < kKeysPerLane; ++r) {
+    const uint64_t m = same_digit(digit[r], bits, valid[r]);
+    const int below = __popcll(m & ((1ull << lane) - 1));
+    const int prev = valid[r] ? cnt[digit[r]] : 0;
+    __builtin_amdgcn_wave_barrier();
+    if (valid[r] && below == 0) cnt[digit[r]] = prev + __popcll(m);
+    __builtin_amdgcn_wave_barrier();
+    rank[r] = prev + below;
+  }
+}
+
+// Whole sort in one workgroup: N <= kSmallTokens.
+constexpr int kSmallThreads = 512;
+static_assert(ts_plan::kEmbedSmallTokens == kSmallThreads / kWave * kWaveKeys, "keys of a workgroup");
+
+__global__ __launch_bounds__(kSmallThreads) void sort_small(const int64_t* __restrict__ ids, int N,
+                                                            int64_t V, int64_t padding, int bits,
+                                                            int passes, uint32_t* __restrict__ keys,
+                                                            uint32_t* __restrict__ vals) {
+  constexpr int kWaves = kSmallThreads / kWave;
+  __shared__ int cnt[kWaves][kMaxBins];
+  __shared__ uint2 held[ts_plan::kEmbedSmallTokens];
+  __shared__ int scan[kWaves];
+  const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
+  const int bins = 1 << bits;
+  constexpr int kPer = kMaxBins / kSmallThreads;  // bins of a thread
+  uint32_t key[kKeysPerLane], val[kKeysPerLane];
+  bool valid[kKeysPerLane];
+#pragma unroll
+  for (int r = 0; r < kKeysPerLane; ++r) {
+    const int i = wid * kWaveKeys + r * kWave + lane;
+    valid[r] = i < N;
+    key[r] = valid[r] ? key_of(ids[i], V, padding) : 0;
+    val[r] = (uint32_t)i;
+  }
+  for (int p = 0; p < passes; ++p) {
+    for (int i = threadIdx.x; i < kWaves * kMaxBins; i += kSmallThreads) (&cnt[0][0])[i] = 0;
+    __syncthreads();
+    uint32_t digit[kKeysPerLane];
+    int rank[kKeysPerLane];
+#pragma unroll
+    for (int r = 0; r < kKeysPerLane; ++r) digit[r] = (key[r] >> (p * bits)) & (uint32_t)(bins - 1);
+    wave_ranks(digit, valid, bits, cnt[wid], rank);
+    __syncthreads();
+    int mine = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      for (int w = 0; w < kWaves; ++w) mine += cnt[w][threadIdx.x * kPer + k];
+    int at = block_exclusive<kSmallThreads>(mine, scan);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k)
+      for (int w = 0; w < kWaves; ++w) {
+        const int c = cnt[w][threadIdx.x * kPer + k];
+        cnt[w][threadIdx.x * kPer + k] = at;
+        at += c;
+      }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kKeysPerLane; ++r)
+      if (valid[r]) held[cnt[wid][digit[r]] + rank[r]] = make_uint2(key[r], val[r]);
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kKeysPerLane; ++r) {
+      const int i = wid * kWaveKeys + r * kWave + lane;
+      if (valid[r]) {
+        const uint2 kv = held[i];
+        key[r] = kv.x;
+        val[r] = kv.y;
+      }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < kKeysPerLane; ++r) {
+    const int i = wid * kWaveKeys + r * kWave + lane;
+    if (valid[r]) {
+      keys[i] = key[r];
+      vals[i] = val[r];
+    }
+  }
+}
+
+// One pass over many workgroups: workgroup b owns keys [b * len, (b + 1) * len). First the
+// digits' counts, table[b][digit], then the scatter, whose workgroups each form the digits'
+// starts from the whole table (at most kEmbedMaxBlocks rows of it).
+template <bool kFirst>
+__global__ __launch_bounds__(kThreads) void sort_counts(const int64_t* __restrict__ ids,
+                                                        const uint32_t* __restrict__ keys_in,
+                                                        int64_t N, int64_t len, int64_t V,
+                                                        int64_t padding, int shift, int bits,
+                                                        int* __restrict__ table) {
+  __shared__ int cnt[kMaxBins];
+  const int bins = 1 << bits;
+  for (int d = threadIdx.x; d < bins; d += kThreads) cnt[d] = 0;
+  __syncthreads();
+  const int64_t first = (int64_t)blockIdx.x * len;
+  const int64_t end = first + len < N ? first + len : N;
+  for (int64_t i = first + threadIdx.x; i < end; i += kThreads) {
+    const uint32_t key = kFirst ? key_of(ids[i], V, padding) : keys_in[i];
+    atomicAdd(&cnt[(key >> shift) & (uint32_t)(bins - 1)], 1);
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < bins; d += kThreads) table[(int64_t)blockIdx.x * bins + d] = cnt[d];
+}
+
+template <bool kFirst>
+__global__ __launch_bounds__(kThreads) void sort_scatter(
+    const int64_t* __restrict__ ids, const uint32_t* __restrict__ keys_in,
+    const uint32_t* __restrict__ vals_in, int64_t N, int64_t len, int64_t V, int64_t padding,
+    int shift, int bits, const int* __restrict__ table, uint32_t* __restrict__ keys_out,
+    uint32_t* __restrict__ vals_out) {
+  constexpr int kWaves = kThreads / kWave;
+  constexpr int kPer = kMaxBins / kThreads;  // most bins of a thread
+  __shared__ int cnt[kWaves][kMaxBins];
+  __shared__ int base[kMaxBins];
+  __shared__ int scan[kWaves];
+  const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
+  const int bins = 1 << bits;
+  const int per = bins > kThreads ? bins / kThreads : 1;
+  {
+    int total[kPer], before[kPer], sum = 0;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      total[k] = before[k] = 0;
+      const int d = threadIdx.x * per + k;
+      if (k < per && d < bins) {
+#pragma unroll 8
+        for (int b = 0; b < (int)gridDim.x; ++b) {
+          const int c = table[(int64_t)b * bins + d];
+          total[k] += c;
+          before[k] += b < (int)blockIdx.x ? c : 0;
+        }
+      }
+      sum += total[k];
+    }
+    int at = block_exclusive<kThreads>(sum, scan);
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      const int d = threadIdx.x * per + k;
+      if (k < per && d < bins) base[d] = at + before[k];
+      at += total[k];
+    }
+  }
+  const int64_t first = (int64_t)blockIdx.x * len;
+  const int64_t end = first + len < N ? first + len : N;
+  for (int64_t start = first; start < end; start += kWaves * kWaveKeys) {
+    for (int i = threadIdx.x; i < kWaves * bins; i += kThreads) cnt[i >> bits][i & (bins - 1)] = 0;
+    __syncthreads();  // also orders base, and the last step's reads of cnt
+    uint32_t key[kKeysPerLane], val[kKeysPerLane], digit[kKeysPerLane];
+    bool valid[kKeysPerLane];
+    int rank[kKeysPerLane];
+#pragma unroll
+    for (int r = 0; r < kKeysPerLane; ++r) {
+      const int64_t i = start + wid * kWaveKeys + r * kWave + lane;
+      valid[r] = i < end;
+      if constexpr (kFirst) {
+        key[r] = valid[r] ? key_of(ids[i], V, padding) : 0;
+        val[r] = (uint32_t)i;
+      } else {
+        key[r] = valid[r] ? keys_in[i] : 0;
+        val[r] = valid[r] ? vals_in[i] : 0;
+      }
+      digit[r] = (key[r] >> shift) & (uint32_t)(bins - 1);
+    }
+    wave_ranks(digit, valid, bits, cnt[wid], rank);
+    __syncthreads();
+    for (int d = threadIdx.x; d < bins; d += kThreads) {
+      int at = base[d];
+#pragma unroll
+      for (int w = 0; w < kWaves; ++w) {
+        const int c = cnt[w][d];
+        cnt[w][d] = at;
+        at += c;
+      }
+      base[d] = at;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kKeysPerLane; ++r) {
+      if (valid[r]) {
+        const int pos = cnt[wid][digit[r]] + rank[r];
+        keys_out[pos] = key[r];
+        vals_out[pos] = val[r];
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Sums
+// ---------------------------------------------------------------------------
+
+// Adds token rows vals[i], i in [i0, i1), to acc: this lane's parts v0 + k * TPR.
+template <typename T, int TPR, int KV>
+__device__ inline void add_tokens(const T* __restrict__ dout, int64_t ldd,
+                                  const uint32_t* __restrict__ vals, int64_t i0, int64_t i1,
+                                  int v0, int nvec, int tail, float (&acc)[KV][Elt<T>::kVec]) {
+  constexpr int V = Elt<T>::kVec;
+  constexpr int kU = KV == 1 ? 8 : 4;  // token rows in flight
+  const int parts = nvec + (tail > 0);
+  for (int64_t i = i0; i < i1; i += kU) {
+    const T* row[kU];
+#pragma unroll
+    for (int u = 0; u < kU; ++u) row[u] = dout + (int64_t)vals[i + u < i1 ? i + u : i] * ldd;
+#pragma unroll
+    for (int k = 0; k < KV; ++k) {
+      const int v = v0 + k * TPR;
+      if (v < nvec) {
+        u32x4 q[kU];
+#pragma unroll
+        for (int u = 0; u < kU; ++u) q[u] = ld16_any_stream(row[u] + (int64_t)v * V);
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          float f[V];
+          Elt<T>::unpack(q[u], f);
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[k][e] += i + u < i1 ? f[e] : 0.f;
+        }
+      } else if (v < parts) {
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          float f[V];
+          load_part(row[u], v, nvec, tail, f);
+#pragma unroll
+          for (int e = 0; e < V; ++e) acc[k][e] += i + u < i1 ? f[e] : 0.f;
+        }
+      }
+    }
+  }
+}
+
+// Adds rows c0 .. c1 - 1 of fp32 sums.
+template <int V, int TPR, int KV>
+__device__ inline void add_sums(const float* __restrict__ sums, int64_t lds_, int64_t c0,
+                                int64_t c1, int v0, int parts, float (&acc)[KV][V]) {
+  constexpr int kU = KV == 1 ? 4 : 2;
+  for (int64_t c = c0; c < c1; c += kU) {
+#pragma unroll
+    for (int k = 0; k < KV; ++k) {
+      const int v = v0 + k * TPR;
+      if (v < parts) {
+        float4 q[kU][V / 4];
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+          for (int h = 0; h < V / 4; ++h)
+            q[u][h] = *reinterpret_cast<const float4*>(sums + (c + u < c1 ? c + u : c) * lds_ +
+                                                       (int64_t)v * V + 4 * h);
+#pragma unroll
+        for (int u = 0; u < kU; ++u)
+#pragma unroll
+          for (int h = 0; h < V / 4; ++h) {
+            const bool in = c + u < c1;
+            acc[k][4 * h] += in ? q[u][h].x : 0.f;
+            acc[k][4 * h + 1] += in ? q[u][h].y : 0.f;
+            acc[k][4 * h + 2] += in ? q[u][h].z : 0.f;
+            acc[k][4 * h + 3] += in ? q[u][h].w : 0.f;
+          }
+      }
+    }
+  }
+}
+
+// Sum of chunk c where all of it is one row's: from its kChunk tokens (kLevel 1), or from the
+// sums of its kChunk chunks (kLevel 2).
+template <typename T, int TPR, int KV, int kLevel>
+__global__ __launch_bounds__(kThreads) void embed_chunk_sums(
+    const T* __restrict__ dout, int64_t ldd, const uint32_t* __restrict__ keys,
+    const uint32_t* __restrict__ vals, int64_t chunks, uint32_t none, int nvec, int tail,
+    int slices, const float* __restrict__ sums_in, float* __restrict__ sums_out, int64_t lds_) {
+  constexpr int V = Elt<T>::kVec;
+  constexpr int64_t kSpan = kLevel == 1 ? kEmbedChunk : (int64_t)kEmbedChunk * kEmbedChunk;
+  const int64_t c = (int64_t)(blockIdx.x / slices) * (kThreads / TPR) + threadIdx.x / TPR;
+  if (c >= chunks) return;
+  const uint32_t key = keys[c * kSpan];
+  if (key == none || key != keys[c * kSpan + kSpan - 1]) return;
+  const int v0 = (int)(blockIdx.x % slices) * TPR * KV + threadIdx.x % TPR;
+  const int parts = nvec + (tail > 0);
+  float acc[KV][V] = {};
+  if constexpr (kLevel == 1)
+    add_tokens<T, TPR, KV>(dout, ldd, vals, c * kSpan, c * kSpan + kSpan, v0, nvec, tail, acc);
+  else
+    add_sums<V, TPR, KV>(sums_in, lds_, c * kEmbedChunk, (c + 1) * kEmbedChunk, v0, parts, acc);
+#pragma unroll
+  for (int k = 0; k < KV; ++k) {
+    const int v = v0 + k * TPR;
+    if (v < parts) {
+#pragma unroll
+      for (int h = 0; h < V / 4; ++h)
+        *reinterpret_cast<float4*>(sums_out + c * lds_ + (int64_t)v * V + 4 * h) =
+            make_float4(acc[k][4 * h], acc[k][4 * h + 1], acc[k][4 * h + 2], acc[k][4 * h + 3]);
+    }
+  }
+}
+
+// First index in keys[0, N) whose key is not below `key`.
+__device__ inline int64_t lower_bound(const uint32_t* __restrict__ keys, int64_t N, uint32_t key) {
+  int64_t lo = 0, hi = N;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) >> 1;
+    if (keys[mid] < key) lo = mid + 1; else hi = mid;
+  }
+  return lo;
+}
+
+// The gradient's rows. A workgroup takes kRows groups of kThreads / TPR neighbouring rows, the
+// groups a grid apart: the running workgroups write a compact window of the gradient, and
+// frequent tokens, whose ids are often neighbours, go to different workgroups. The bounds of all
+// its runs are searched at once at the start, a lane each.
+template <typename T, int TPR, int KV>
+__global__ __launch_bounds__(kThreads) void embed_grad_rows(
+    const T* __restrict__ dout, int64_t ldd, const uint32_t* __restrict__ keys,
+    const uint32_t* __restrict__ vals, int64_t N, int64_t V, int nvec, int tail, int slices,
+    int rows, const float* __restrict__ sums1, const float* __restrict__ sums2, int64_t lds_,
+    float scale, T* __restrict__ grad) {
+  constexpr int VE = Elt<T>::kVec;
+  constexpr int kSlots = kThreads / TPR;
+  __shared__ int64_t bound[ts_plan::kEmbedMaxRows * 2];
+  const int64_t group0 = blockIdx.x / slices;
+  const int64_t groups = gridDim.x / slices;
+  const int v0 = (int)(blockIdx.x % slices) * TPR * KV + threadIdx.x % TPR;
+  const int slot = threadIdx.x / TPR;
+  const int parts = nvec + (tail > 0);
+  const int64_t H = (int64_t)nvec * VE + tail;
+  for (int b = threadIdx.x; b < 2 * rows * kSlots; b += kThreads) {
+    const int64_t v = (group0 + (int64_t)(b / 2 / kSlots) * groups) * kSlots + b / 2 % kSlots;
+    bound[b] = v < V ? lower_bound(keys, N, (uint32_t)v + (b & 1)) : 0;
+  }
+  __syncthreads();
+  for (int j = 0; j < rows; ++j) {
+    const int64_t v = (group0 + (int64_t)j * groups) * kSlots + slot;
+    if (v >= V) break;
+    const int64_t s = bound[2 * (j * kSlots + slot)], e = bound[2 * (j * kSlots + slot) + 1];
+    float acc[KV][VE] = {};
+    if (s < e) {
+      const ts_plan::EmbedRun run = ts_plan::embed_run(s, e);
+      add_tokens<T, TPR, KV>(dout, ldd, vals, s, run.t0, v0, nvec, tail, acc);
+      add_sums<VE, TPR, KV>(sums1, lds_, run.a0, run.a1, v0, parts, acc);
+      add_sums<VE, TPR, KV>(sums2, lds_, run.b0, run.b1, v0, parts, acc);
+      add_sums<VE, TPR, KV>(sums1, lds_, run.c0, run.c1, v0, parts, acc);
+      add_tokens<T, TPR, KV>(dout, ldd, vals, run.t1, e, v0, nvec, tail, acc);
+    }
+    T* row = grad + v * H;
+#pragma unroll
+    for (int k = 0; k < KV; ++k) {
+      const int p = v0 + k * TPR;
+      if (p < parts) {
+#pragma unroll
+        for (int i = 0; i < VE; ++i) acc[k][i] *= scale;
+        store_part(row, p, nvec, tail, acc[k]);
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+
+template <typename T>
+ts_status fwd_typed(const int64_t* ids, int64_t N, const void* w, int64_t ldw, int64_t V, int64_t H,
+                    float scale, void* out, int64_t ldo, hipStream_t st) {
+  const int nvec = (int)(H / Elt<T>::kVec), tail = (int)(H % Elt<T>::kVec);
+  const int parts = nvec + (tail > 0);
+  const int tpr = ts_plan::embed_fwd_lanes(parts);
+  const int64_t per = kThreads / tpr, blocks = (N + per - 1) / per;
+  if (blocks > 0x7fffffff) return ts_host::fail(TS_ERR_SHAPE, "embedding_fwd: too many tokens");
+#define TS_FWD(R)                                                                             \
+  hipLaunchKernelGGL((embed_fwd<T, R>), dim3((unsigned)blocks), dim3(kThreads), 0, st, ids, N, \
+                     static_cast<const T*>(w), ldw, V, nvec, tail, scale, static_cast<T*>(out), ldo)
+  switch (tpr) {
+    case 8: TS_FWD(8); break;
+    case 32: TS_FWD(32); break;
+    case 128: TS_FWD(128); break;
+    default: TS_FWD(256); break;
+  }
+#undef TS_FWD
+  return ts_host::check_launch("embed_fwd");
+}
+
+struct BwdArgs {
+  const int64_t* ids;
+  int64_t N, V, H, padding, ldd;
+  const void* dout;
+  void* grad;
+  float scale;
+  uint8_t* ws;
+};
+
+// Sorts the tokens; *keys and *vals are where the sorted pairs end up.
+ts_status launch_sort(const BwdArgs& a, const ts_plan::EmbedWorkspace& w, const uint32_t** keys,
+                      const uint32_t** vals, hipStream_t st) {
+  const ts_plan::EmbedSort p = ts_plan::embed_sort(a.N, a.V);
+  uint32_t* k[2] = {reinterpret_cast<uint32_t*>(a.ws + w.keys[0]),
+                    reinterpret_cast<uint32_t*>(a.ws + w.keys[1])};
+  uint32_t* v[2] = {reinterpret_cast<uint32_t*>(a.ws + w.vals[0]),
+                    reinterpret_cast<uint32_t*>(a.ws + w.vals[1])};
+  *keys = k[0];
+  *vals = v[0];
+  if (a.N == 0) return TS_OK;
+  if (p.blocks == 0) {
+    hipLaunchKernelGGL(sort_small, dim3(1), dim3(kSmallThreads), 0, st, a.ids, (int)a.N, a.V,
+                       a.padding, p.bits, p.passes, k[0], v[0]);
+    return ts_host::check_launch("sort_small");
+  }
+  int* table = reinterpret_cast<int*>(a.ws + w.table);
+  const dim3 grid((unsigned)p.blocks), block(kThreads);
+  for (int i = 0; i < p.passes; ++i) {
+    const int shift = i * p.bits, to = i & 1, from = to ^ 1;
+    if (i == 0) {
+      hipLaunchKernelGGL(sort_counts<true>, grid, block, 0, st, a.ids, k[from], a.N, p.len, a.V,
+                         a.padding, shift, p.bits, table);
+      hipLaunchKernelGGL(sort_scatter<true>, grid, block, 0, st, a.ids, k[from], v[from], a.N,
+                         p.len, a.V, a.padding, shift, p.bits, table, k[to], v[to]);
+    } else {
+      hipLaunchKernelGGL(sort_counts<false>, grid, block, 0, st, a.ids, k[from], a.N, p.len, a.V,
+                         a.padding, shift, p.bits, table);
+      hipLaunchKernelGGL(sort_scatter<false>, grid, block, 0, st, a.ids, k[from], v[from], a.N,
+                         p.len, a.V, a.padding, shift, p.bits, table, k[to], v[to]);
+    }
+    const ts_status s = ts_host::check_launch("sort_scatter");
+    if (s != TS_OK) return s;
+    *keys = k[to];
+    *vals = v[to];
+  }
+  return TS_OK;
+}
+
+template <typename T, int TPR, int KV>
+ts_status bwd_shaped(const BwdArgs& a, const ts_plan::EmbedWorkspace& w, const uint32_t* keys,
+                     const uint32_t* vals, hipStream_t st) {
+  constexpr int VE = Elt<T>::kVec;
+  constexpr int kSlots = kThreads / TPR;
+  const int nvec = (int)(a.H / VE), tail = (int)(a.H % VE), parts = nvec + (tail > 0);
+  const int slices = (parts + TPR * KV - 1) / (TPR * KV);
+  const T* dout = static_cast<const T*>(a.dout);
+  float* sums1 = reinterpret_cast<float*>(a.ws + w.sums1);
+  float* sums2 = reinterpret_cast<float*>(a.ws + w.sums2);
+  const uint32_t none = (uint32_t)a.V;
+  const int64_t c1 = a.N / kEmbedChunk, c2 = c1 / kEmbedChunk;
+  const ts_plan::EmbedRows r = ts_plan::embed_rows(a.V, kSlots);
+  const int64_t b1 = (c1 + kSlots - 1) / kSlots * slices, b2 = (c2 + kSlots - 1) / kSlots * slices;
+  const int64_t blocks = r.groups * slices;
+  if (b1 > 0x7fffffff || blocks > 0x7fffffff)
+    return ts_host::fail(TS_ERR_SHAPE, "embedding_bwd: tensor too large");
+  if (c1 > 0)
+    hipLaunchKernelGGL((embed_chunk_sums<T, TPR, KV, 1>), dim3((unsigned)b1), dim3(kThreads), 0, st,
+                       dout, a.ldd, keys, vals, c1, none, nvec, tail, slices, sums2, sums1, w.ld);
+  if (c2 > 0)
+    hipLaunchKernelGGL((embed_chunk_sums<T, TPR, KV, 2>), dim3((unsigned)b2), dim3(kThreads), 0, st,
+                       dout, a.ldd, keys, vals, c2, none, nvec, tail, slices, sums1, sums2, w.ld);
+  hipLaunchKernelGGL((embed_grad_rows<T, TPR, KV>), dim3((unsigned)blocks), dim3(kThreads), 0, st,
+                     dout, a.ldd, keys, vals, a.N, a.V, nvec, tail, slices, r.rows, sums1, sums2,
+                     w.ld, a.scale, static_cast<T*>(a.grad));
+  return ts_host::check_launch("embed_grad_rows");
+}
+
+template <typename T>
+ts_status bwd_typed(const BwdArgs& a, hipStream_t st) {
+  const ts_plan::EmbedWorkspace w = ts_plan::embed_workspace(a.N, a.V, a.H);
+  const uint32_t *keys, *vals;
+  const ts_status s = launch_sort(a, w, &keys, &vals, st);
+  if (s != TS_OK) return s;
+  const int64_t parts = (a.H + Elt<T>::kVec - 1) / Elt<T>::kVec;
+  if (parts <= 8) return bwd_shaped<T, 8, 1>(a, w, keys, vals, st);
+  if (parts <= 32) return bwd_shaped<T, 32, 1>(a, w, keys, vals, st);
+  if (parts <= 128) return bwd_shaped<T, 128, 1>(a, w, keys, vals, st);
+  if (parts <= 256) return bwd_shaped<T, 256, 1>(a, w, keys, vals, st);
+  return bwd_shaped<T, 256, 2>(a, w, keys, vals, st);
+}
+
+bool bad_address(const void* p, ts_dtype t) {
+  return reinterpret_cast<uintptr_t>(p) % ts_host::dtype_size(t) != 0;
+}
+
+}  // namespace
+
+extern "C" ts_status ts_embedding_fwd(const int64_t* ids, int64_t N, const void* weight,
+                                      int64_t ldw, ts_dtype dtype, int64_t V, int64_t H,
+                                      float scale, void* out, int64_t ldo, ts_stream_t stream) {
+  using ts_host::fail;
+  if (!ts_host::valid_dtype(dtype))
+    return fail(TS_ERR_UNSUPPORTED_DTYPE, "embedding_fwd: bad dtype");
+  if (N < 0 || V < 0 || H < 0 || H > 0x7fffffff)
+    return fail(TS_ERR_SHAPE, "embedding_fwd: bad sizes");
+  if (N == 0 || H == 0) return TS_OK;
+  if (V == 0) return fail(TS_ERR_SHAPE, "embedding_fwd: no rows to look up");
+  if (ldw < H || ldo < H) return fail(TS_ERR_SHAPE, "embedding_fwd: row stride below the width");
+  if (ids == nullptr || weight == nullptr || out == nullptr)
+    return fail(TS_ERR_INVALID_ARGUMENT, "embedding_fwd: NULL pointer");
+  if (bad_address(weight, dtype) || bad_address(out, dtype) ||
+      reinterpret_cast<uintptr_t>(ids) % 8 != 0)
+    return fail(TS_ERR_INVALID_ARGUMENT, "embedding_fwd: a tensor is not aligned to its elements");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case TS_BF16: return fwd_typed<__bf16>(ids, N, weight, ldw, V, H, scale, out, ldo, st);
+    case TS_F16: return fwd_typed<_Float16>(ids, N, weight, ldw, V, H, scale, out, ldo, st);
+    case TS_F32: return fwd_typed<float>(ids, N, weight, ldw, V, H, scale, out, ldo, st);
+  }
+  return fail(TS_ERR_UNSUPPORTED_DTYPE, "embedding_fwd: bad dtype");
+}
+
+extern "C" size_t ts_embedding_bwd_workspace_size(int64_t N, int64_t V, int64_t H) {
+  if (N < 0 || V < 0 || H < 0 || N > ts_plan::kEmbedMaxIndex || V > ts_plan::kEmbedMaxIndex ||
+      H > 0x7fffffff)
+    return 0;
+  return (size_t)ts_plan::embed_workspace(N, V, H).bytes;
+}
+
+extern "C" ts_status ts_embedding_bwd(const int64_t* ids, int64_t N, const void* dout, int64_t ldd,
+                                      ts_dtype dtype, int64_t V, int64_t H, float scale,
+                                      int64_t padding_idx, void* grad_weight, void* workspace,
+                                      size_t workspace_bytes, ts_stream_t stream) {
+  using ts_host::fail;
+  if (!ts_host::valid_dtype(dtype))
+    return fail(TS_ERR_UNSUPPORTED_DTYPE, "embedding_bwd: bad dtype");
+  if (N < 0 || V < 0 || H < 0 || N > ts_plan::kEmbedMaxIndex || V > ts_plan::kEmbedMaxIndex ||
+      H > 0x7fffffff)
+    return fail(TS_ERR_SHAPE, "embedding_bwd: bad sizes");
+  if (V == 0 || H == 0) return TS_OK;
+  if (grad_weight == nullptr || (N > 0 && (ids == nullptr || dout == nullptr)))
+    return fail(TS_ERR_INVALID_ARGUMENT, "embedding_bwd: NULL pointer");
+  if (N > 0 && ldd < H) return fail(TS_ERR_SHAPE, "embedding_bwd: row stride below the width");
+  if (bad_address(grad_weight, dtype) || bad_address(dout, dtype) ||
+      reinterpret_cast<uintptr_t>(ids) % 8 != 0)
+    return fail(TS_ERR_INVALID_ARGUMENT, "embedding_bwd: a tensor is not aligned to its elements");
+  if (workspace_bytes < ts_embedding_bwd_workspace_size(N, V, H) || workspace == nullptr ||
+      !ts_host::aligned16(workspace))
+    return fail(TS_ERR_WORKSPACE, "embedding_bwd: workspace missing, too small or unaligned");
+  const BwdArgs a{ids, N, V, H, padding_idx, ldd, dout, grad_weight, scale,
+                  static_cast<uint8_t*>(workspace)};
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case TS_BF16: return bwd_typed<__bf16>(a, st);
+    case TS_F16: return bwd_typed<_Float16>(a, st);
+    case TS_F32: return bwd_typed<float>(a, st);
+  }
+  return fail(TS_ERR_UNSUPPORTED_DTYPE, "embedding_bwd: bad dtype");
+}

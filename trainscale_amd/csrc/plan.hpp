@@ -522,4 +522,103 @@ inline int64_t grad_norm_parts(int64_t count) {
   return count <= 0 ? 1 : (count / kGradTensors + 3) * kGradGrid;
 }
 
+// ---------------------------------------------------------------------------
+// Embedding gradient by sorted tokens (embedding.hip)
+// ---------------------------------------------------------------------------
+constexpr int kEmbedMaxBits = 10;        // of a radix digit
+constexpr int kEmbedSmallTokens = 2048;  // sorted by one workgroup, in LDS
+constexpr int kEmbedTile = 1024;         // keys of a sorting workgroup's step
+constexpr int64_t kEmbedMaxBlocks = 256;
+constexpr int64_t kEmbedMaxIndex = 0x7ffffffe;  // tokens and rows: 32-bit keys and positions
+// Neighbours of the sorted list whose sum is formed beforehand when they share an id.
+constexpr int kEmbedChunk = 32;
+
+struct EmbedSort {
+  int passes, bits;  // keys 0 .. V (V: no row) fit passes * bits bits
+  int64_t blocks;    // sorting workgroups (0: one workgroup sorts in LDS)
+  int64_t len;       // keys of each, a multiple of kEmbedTile
+};
+inline EmbedSort embed_sort(int64_t N, int64_t V) {
+  EmbedSort p{1, 1, 0, 0};
+  int need = 1;
+  while ((V >> need) != 0) ++need;
+  p.passes = (need + kEmbedMaxBits - 1) / kEmbedMaxBits;
+  p.bits = (need + p.passes - 1) / p.passes;
+  if (N <= kEmbedSmallTokens) return p;
+  p.len = (N + kEmbedMaxBlocks - 1) / kEmbedMaxBlocks;
+  p.len = (p.len + kEmbedTile - 1) / kEmbedTile * kEmbedTile;
+  p.blocks = (N + p.len - 1) / p.len;
+  return p;
+}
+
+// Byte offsets of the gradient's workspace, all multiples of 16, and fp32 elements of a row of
+// sums (whole vectors of the narrowest type, so every row of sums is 16-byte aligned).
+struct EmbedWorkspace {
+  int64_t keys[2], vals[2], table, sums1, sums2, ld, bytes;
+};
+inline EmbedWorkspace embed_workspace(int64_t N, int64_t V, int64_t H) {
+  EmbedWorkspace w;
+  const EmbedSort p = embed_sort(N, V);
+  const int64_t list = (N * 4 + 15) / 16 * 16;
+  int64_t at = 0;
+  for (int i = 0; i < 2; ++i) {
+    w.keys[i] = at;
+    at += i == 0 || p.blocks > 0 ? list : 0;
+    w.vals[i] = at;
+    at += i == 0 || p.blocks > 0 ? list : 0;
+  }
+  w.table = at;
+  at += (p.blocks << p.bits) * 4;
+  at = (at + 15) / 16 * 16;
+  w.ld = (H + 7) / 8 * 8;
+  w.sums1 = at;
+  at += N / kEmbedChunk * w.ld * 4;
+  w.sums2 = at;
+  at += N / kEmbedChunk / kEmbedChunk * w.ld * 4;
+  w.bytes = at > 0 ? at : 16;
+  return w;
+}
+
+// A run [s, e) of the sorted list: tokens [s, t0), sums of chunks [a0, a1), sums of sums
+// [b0, b1), sums of chunks [c0, c1), tokens [t1, e).
+struct EmbedRun {
+  int64_t t0, a0, a1, b0, b1, c0, c1, t1;
+};
+TS_HOST_DEVICE inline EmbedRun embed_run(int64_t s, int64_t e) {
+  const int64_t C = kEmbedChunk;
+  int64_t c0 = (s + C - 1) / C, c1 = e / C;  // whole chunks
+  if (c0 >= c1) return EmbedRun{e, 0, 0, 0, 0, 0, 0, e};
+  EmbedRun r{c0 * C, c0, c1, 0, 0, 0, 0, c1 * C};
+  const int64_t b0 = (c0 + C - 1) / C, b1 = c1 / C;
+  if (b0 < b1) {
+    r.a1 = b0 * C;
+    r.b0 = b0;
+    r.b1 = b1;
+    r.c0 = b1 * C;
+    r.c1 = c1;
+  }
+  return r;
+}
+
+// Rows of the gradient: each workgroup takes `rows` groups of `slots` neighbouring rows, `groups`
+// apart. Few rows for a small vocabulary (8 workgroups a CU first), more for a large one.
+constexpr int kEmbedMaxRows = 128;  // rows of a workgroup
+struct EmbedRows {
+  int64_t groups;
+  int rows;
+};
+inline EmbedRows embed_rows(int64_t V, int slots) {
+  const int64_t all = (V + slots - 1) / slots;
+  int64_t rows = all / (256 * 8);
+  const int64_t most = kEmbedMaxRows / slots < 16 ? kEmbedMaxRows / slots : 16;
+  if (rows > most) rows = most;
+  if (rows < 1) rows = 1;
+  return EmbedRows{(all + rows - 1) / rows, (int)rows};
+}
+
+// Lanes that own a row of `parts` vectors in the forward.
+inline int embed_fwd_lanes(int64_t parts) {
+  return parts <= 8 ? 8 : parts <= 32 ? 32 : parts <= 128 ? 128 : 256;
+}
+
 }  // namespace ts_plan

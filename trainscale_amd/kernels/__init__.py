@@ -4,6 +4,7 @@ The exports mirror the hot-path names of TrainScale's ``kernels/__init__.py``
 (data_pipeline/trainer/kernels/__init__.py:15-124): ``fast_rms_layernorm`` is
 the layernorm_kernels variant there, as here.
 """
+from .embedding_kernels import ScaledEmbedding, ScaledEmbeddingFunction, scaled_embedding
 from .fused_kernels import (
     Fast_CrossEntropyLoss,
     Fast_RMS_LayerNorm,
@@ -74,6 +75,9 @@ __all__ = [
     "fast_rope_embedding",
     "inplace_rope_embedding",
     "precompute_freqs_cis",
+    "ScaledEmbeddingFunction",
+    "ScaledEmbedding",
+    "scaled_embedding",
     "get_total_norm",
     "clip_grad_norm_",
     "clip_grads_with_norm_",

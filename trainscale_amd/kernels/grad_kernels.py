@@ -19,6 +19,7 @@ from __future__ import annotations
 import math
 from typing import Iterable, List, Optional, Sequence, Union
 
+import numpy as np
 import torch
 from torch import Tensor
 
@@ -40,52 +41,52 @@ def _is_dense(t: Tensor) -> bool:
 def _checked(what: str, tensors: Union[Tensor, Iterable[Tensor]]) -> List[Tensor]:
     """The tensors as a list: dense fp32/bf16/fp16 torch tensors on one GPU."""
     tensors = [tensors] if isinstance(tensors, Tensor) else list(tensors)
-    dev = None
-    for t in tensors:
-        if not isinstance(t, Tensor):
-            raise TypeError(f"{what}: expected tensors, got {type(t).__name__}")
-        if type(t) not in (Tensor, torch.nn.Parameter):
-            raise TypeError(f"{what}: {type(t).__name__} is not supported: pass its local tensor")
-        if t.layout != torch.strided:
-            raise TypeError(f"{what}: sparse gradients are not supported")
-        if t.dtype not in _lib.DTYPE_CODE:
-            raise TypeError(f"{what}: unsupported dtype {t.dtype} (float32/bfloat16/float16)")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise RuntimeError(f"{what}: tensors are on different devices ({dev} vs {t.device})")
-    if tensors:
-        _lib.require_gpu(what, tensors[0])
+    if not tensors:
+        return tensors
+    # over whole lists (a model has hundreds of tensors): the interpreter's time is the call's
+    for cls in {type(t) for t in tensors} - {Tensor, torch.nn.Parameter}:
+        if not issubclass(cls, Tensor):
+            raise TypeError(f"{what}: expected tensors, got {cls.__name__}")
+        raise TypeError(f"{what}: {cls.__name__} is not supported: pass its local tensor")
+    if {t.layout for t in tensors} != {torch.strided}:
+        raise TypeError(f"{what}: sparse gradients are not supported")
+    for dtype in {t.dtype for t in tensors}:
+        if dtype not in _lib.DTYPE_CODE:
+            raise TypeError(f"{what}: unsupported dtype {dtype} (float32/bfloat16/float16)")
+    if len({t.get_device() for t in tensors}) != 1:
+        raise RuntimeError(f"{what}: tensors are on different devices")
+    _lib.require_gpu(what, tensors[0])
     return tensors
 
 
-def _storage_order(t: Tensor) -> Tensor:
-    """The values of t in an order of their own, contiguous: t itself where it is dense."""
-    return t if t.is_contiguous() or _is_dense(t) else t.contiguous()
+def _storage_order(tensors: List[Tensor]) -> List[Tensor]:
+    """The tensors with their values contiguous, in an order of their own: dense ones themselves,
+    a copy of the others."""
+    return [t if t.is_contiguous() or _is_dense(t) else t.detach().contiguous() for t in tensors]
 
 
-def _refuse_overlap(what: str, written: Sequence[Tensor], read: Sequence[Tensor]) -> None:
+def _refuse_overlap(what: str, written: ops.HostList, read: ops.HostList) -> None:
     """Raises if a written tensor shares memory with another tensor of either list. A tensor of
     `read` that is the written one at the same place in the list does not count."""
-    spans = []
-    for w, r in zip(written, read):
-        n = w.numel()
-        if n == 0:
-            continue
-        a = w.data_ptr()
-        spans.append((a, a + n * w.element_size(), True))
-        b = r.data_ptr()
-        if b != a or r.dtype != w.dtype:
-            spans.append((b, b + n * r.element_size(), False))
-    spans.sort()
-    end, end_written = 0, False
-    for a, b, is_written in spans:
-        if a < end and (is_written or end_written):
-            raise ValueError(f"{what}: gradients share memory: each must be written once")
-        if b > end:
-            end, end_written = b, is_written
-        elif is_written:
-            end_written = True
+    start, end = written.ptr, written.end()
+    if read is not written:
+        rstart, rend = read.ptr, read.end()
+        other = (rstart != start) | (rend != end)
+        rstart, rend = rstart[other], rend[other]
+        # what is read may overlap: as disjoint stretches
+        order = np.argsort(rstart, kind="stable")
+        rstart, rend = rstart[order], rend[order]
+        if rend.size:
+            first = np.ones(rstart.size, dtype=bool)
+            first[1:] = rstart[1:] >= np.maximum.accumulate(rend)[:-1]
+            at = np.flatnonzero(first)
+            start = np.concatenate([start, rstart[at]])
+            end = np.concatenate([end, np.maximum.reduceat(rend, at)])
+    some = end > start
+    start, end = start[some], end[some]
+    order = np.argsort(start, kind="stable")
+    if (start[order][1:] < end[order][:-1]).any():
+        raise ValueError(f"{what}: gradients share memory: each must be written once")
 
 
 def _max_norm(what: str, max_norm: float) -> float:
@@ -102,9 +103,9 @@ def _check_norm_type(what: str, norm_type: float) -> None:
 
 def _grads(parameters: Union[Tensor, Iterable[Tensor]]) -> List[Tensor]:
     """The gradients of the parameters that have one; a parameter given twice counts once."""
-    parameters = [parameters] if isinstance(parameters, Tensor) else parameters
-    seen = {id(p): p for p in parameters}
-    return [p.grad for p in seen.values() if p.grad is not None]
+    parameters = [parameters] if isinstance(parameters, Tensor) else list(parameters)
+    by_id = dict(zip(map(id, parameters), parameters))
+    return [g for g in [p.grad for p in by_id.values()] if g is not None]
 
 
 def get_total_norm(tensors: Union[Tensor, Iterable[Tensor]], norm_type: float = 2.0,
@@ -117,7 +118,7 @@ def get_total_norm(tensors: Union[Tensor, Iterable[Tensor]], norm_type: float = 
     tensors = _checked("get_total_norm", tensors)
     if not tensors:
         return torch.tensor(0.0)
-    norm = ops.grad_norm([_storage_order(t.detach()) for t in tensors], tensors[0].device)
+    norm = ops.grad_norm(ops.HostList(_storage_order(tensors)), tensors[0].device)
     if error_if_nonfinite:
         _raise_if_nonfinite(norm)
     return norm
@@ -130,18 +131,19 @@ def _raise_if_nonfinite(norm: Tensor) -> None:
 
 
 def _scale_in_place(what: str, grads: List[Tensor], launch) -> Optional[Tensor]:
-    """Runs launch(contiguous tensors) over the gradients; those that are not dense (slices of a
+    """Runs launch(list of contiguous tensors) over the gradients; those that are not dense (slices of a
     larger buffer) are scaled in a copy and copied back."""
-    for g in grads:
+    held = _storage_order(grads)
+    copied = [(g, h) for g, h in zip(grads, held) if g is not h]
+    for g, _ in copied:
         if any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
             raise ValueError(f"{what}: a gradient's elements share memory (an expanded tensor)")
-    held = [_storage_order(g.detach()) for g in grads]
-    _refuse_overlap(what, held, held)
-    out = launch(held)
-    for g, h in zip(grads, held):
-        if h.data_ptr() != g.data_ptr():
-            with torch.no_grad():
-                g.copy_(h)
+    listed = ops.HostList(held)
+    _refuse_overlap(what, listed, listed)
+    out = launch(listed)
+    with torch.no_grad():
+        for g, h in copied:
+            g.copy_(h)
     torch.autograd.graph.increment_version(grads)
     return out
 
@@ -182,7 +184,7 @@ def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float
         return torch.tensor(0.0)
     dev = grads[0].device
     if error_if_nonfinite:
-        norm = ops.grad_norm([_storage_order(g.detach()) for g in grads], dev)
+        norm = ops.grad_norm(ops.HostList(_storage_order(grads)), dev)
         _raise_if_nonfinite(norm)
         _scale_in_place(what, grads, lambda t: ops.grad_scale(t, t, norm, max_norm, dev))
         return norm
@@ -205,13 +207,15 @@ def clipped_grads(grads: Sequence[Tensor], max_norm: float, out: Sequence[Tensor
     for g, o in zip(grads, out):
         if o.shape != g.shape:
             raise ValueError(f"{what}: output {tuple(o.shape)} for a gradient {tuple(g.shape)}")
-        if o.dtype not in (g.dtype, torch.float32):
-            raise TypeError(f"{what}: output dtype {o.dtype} for a gradient of {g.dtype}")
-        if not o.is_contiguous():
-            raise ValueError(f"{what}: outputs must be contiguous")
+    for got, want in {(o.dtype, g.dtype) for g, o in zip(grads, out)}:
+        if got not in (want, torch.float32):
+            raise TypeError(f"{what}: output dtype {got} for a gradient of {want}")
+    if not all([o.is_contiguous() for o in out]):
+        raise ValueError(f"{what}: outputs must be contiguous")
     _lib.require_gpu(what, grads[0], out[0])
-    src = [g.detach() if g.is_contiguous() else g.detach().contiguous() for g in grads]
-    _refuse_overlap(what, out, src)
-    norm = ops.grad_clip(src, out, max_norm, grads[0].device)
+    src = [g if g.is_contiguous() else g.detach().contiguous() for g in grads]
+    src_list, out_list = ops.HostList(src), ops.HostList(out)
+    _refuse_overlap(what, out_list, src_list)
+    norm = ops.grad_clip(src_list, out_list, max_norm, grads[0].device)
     torch.autograd.graph.increment_version(out)
     return norm

@@ -12,6 +12,7 @@ import ctypes
 
 from typing import Optional, Tuple
 
+import numpy as np
 import torch
 from torch import Tensor
 
@@ -525,55 +526,100 @@ def swiglu_backward(dout: Tensor, gate: Tensor, up: Tensor) -> Tuple[Tensor, Ten
 
 
 # ---------------------------------------------------------------------------
+# Token embedding
+# ---------------------------------------------------------------------------
+
+def embedding_forward(ids: Tensor, weight: Tensor, ldw: int, scale: float) -> Tensor:
+    """scale * weight[ids] for contiguous int64 ids [N]: [N, H] in the weight's dtype."""
+    dev = _lib.require_gpu("embedding", ids, weight)
+    n, (v, h) = ids.shape[0], weight.shape
+    out = torch.empty((n, h), dtype=weight.dtype, device=dev)
+    with _lib.on_device(dev):
+        check(_lib.load().ts_embedding_fwd(
+            ptr(ids), n, ptr(weight), ldw, _lib.dtype_code(weight, "embedding"), v, h, scale,
+            ptr(out), h, _lib.stream_handle(dev)), "ts_embedding_fwd")
+    return out
+
+
+def embedding_backward(ids: Tensor, dout2d: Tensor, ldd: int, rows: int, scale: float,
+                       padding_idx: int = -1) -> Tensor:
+    """The dense gradient [rows, H] of embedding_forward's weight (padding_idx -1: none)."""
+    dev = _lib.require_gpu("embedding backward", ids, dout2d)
+    n, h = dout2d.shape
+    if ids.shape[0] != n:
+        raise ValueError(f"embedding backward: {ids.shape[0]} ids for {n} rows")
+    lib = _lib.load()
+    grad = torch.empty((rows, h), dtype=dout2d.dtype, device=dev)
+    wsb = int(lib.ts_embedding_bwd_workspace_size(n, rows, h))
+    ws = torch.empty((wsb,), dtype=torch.uint8, device=dev)
+    with _lib.on_device(dev):
+        check(lib.ts_embedding_bwd(
+            ptr(ids), n, ptr(dout2d), ldd, _lib.dtype_code(dout2d, "embedding backward"), rows, h,
+            scale, padding_idx, ptr(grad), ptr(ws), wsb, _lib.stream_handle(dev)),
+            "ts_embedding_bwd")
+    return grad
+
+
+# ---------------------------------------------------------------------------
 # Global gradient norm and clipping
 # ---------------------------------------------------------------------------
 
-def _host_lists(tensors, outs=None):
-    """The C ABI's host lists of contiguous tensors: pointers, element counts, dtype codes (and
-    the outputs' pointers and codes)."""
-    n = len(tensors)
-    code = _lib.DTYPE_CODE
-    lists = [(ctypes.c_void_p * n)(*[t.data_ptr() for t in tensors]),
-             (ctypes.c_int64 * n)(*[t.numel() for t in tensors]),
-             (ctypes.c_int32 * n)(*[code[t.dtype] for t in tensors])]
-    if outs is not None:
-        lists += [(ctypes.c_void_p * n)(*[t.data_ptr() for t in outs]),
-                  (ctypes.c_int32 * n)(*[code[t.dtype] for t in outs])]
-    return lists
+class HostList:
+    """Contiguous tensors as the C ABI takes a list of them: host arrays of pointers, element
+    counts and dtype codes."""
+
+    def __init__(self, tensors):
+        self.count = len(tensors)
+        self.ptr = np.array([t.data_ptr() for t in tensors], dtype=np.uint64)
+        self.numel = np.array([t.numel() for t in tensors], dtype=np.int64)
+        dtypes = [t.dtype for t in tensors]
+        if dtypes and dtypes.count(dtypes[0]) == self.count:
+            self.code = np.full(self.count, _lib.DTYPE_CODE[dtypes[0]], dtype=np.int32)
+        else:
+            self.code = np.array([_lib.DTYPE_CODE[d] for d in dtypes], dtype=np.int32)
+
+    def end(self) -> np.ndarray:
+        """One past each tensor's last address (the pointer itself for empty ones)."""
+        return self.ptr + (self.numel << np.where(self.code == _lib.TS_F32, 2, 1)).astype(np.uint64)
 
 
-def grad_norm(tensors, dev: torch.device) -> Tensor:
-    """The 2-norm of all values of contiguous tensors on `dev`: a 0-dim fp32 tensor."""
+def _host(a: np.ndarray) -> ctypes.c_void_p:
+    """A host array as a pointer; the array must outlive the call."""
+    return ctypes.c_void_p(a.ctypes.data)
+
+
+def grad_norm(grads: HostList, dev: torch.device) -> Tensor:
+    """The 2-norm of all values of the tensors, which are on `dev`: a 0-dim fp32 tensor."""
     lib = _lib.load()
-    n = len(tensors)
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    wsb = int(lib.ts_grad_norm_workspace_size(n))
+    wsb = int(lib.ts_grad_norm_workspace_size(grads.count))
     ws = torch.empty((wsb,), dtype=torch.uint8, device=dev)
-    src, numel, dt = _host_lists(tensors)
     with _lib.on_device(dev):
-        check(lib.ts_grad_norm(src, numel, dt, n, ptr(norm), ptr(ws), wsb,
-                               _lib.stream_handle(dev)), "ts_grad_norm")
+        check(lib.ts_grad_norm(_host(grads.ptr), _host(grads.numel), _host(grads.code),
+                               grads.count, ptr(norm), ptr(ws), wsb, _lib.stream_handle(dev)),
+              "ts_grad_norm")
     return norm
 
 
-def grad_scale(tensors, outs, norm: Tensor, max_norm: float, dev: torch.device) -> None:
-    """outs = tensors * min(1, max_norm / (norm + 1e-6)); norm a 0-dim fp32 tensor on `dev`."""
-    lib = _lib.load()
-    src, numel, dt, dst, ddt = _host_lists(tensors, outs)
+def grad_scale(grads: HostList, outs: HostList, norm: Tensor, max_norm: float,
+               dev: torch.device) -> None:
+    """outs = grads * min(1, max_norm / (norm + 1e-6)); norm a 0-dim fp32 tensor on `dev`."""
     with _lib.on_device(dev):
-        check(lib.ts_grad_scale(src, dst, numel, dt, ddt, len(tensors), ptr(norm), max_norm,
-                                _lib.stream_handle(dev)), "ts_grad_scale")
+        check(_lib.load().ts_grad_scale(
+            _host(grads.ptr), _host(outs.ptr), _host(grads.numel), _host(grads.code),
+            _host(outs.code), grads.count, ptr(norm), max_norm, _lib.stream_handle(dev)),
+            "ts_grad_scale")
 
 
-def grad_clip(tensors, outs, max_norm: float, dev: torch.device) -> Tensor:
+def grad_clip(grads: HostList, outs: HostList, max_norm: float, dev: torch.device) -> Tensor:
     """grad_norm, then grad_scale by it; returns the norm."""
     lib = _lib.load()
-    n = len(tensors)
     norm = torch.empty((), dtype=torch.float32, device=dev)
-    wsb = int(lib.ts_grad_norm_workspace_size(n))
+    wsb = int(lib.ts_grad_norm_workspace_size(grads.count))
     ws = torch.empty((wsb,), dtype=torch.uint8, device=dev)
-    src, numel, dt, dst, ddt = _host_lists(tensors, outs)
     with _lib.on_device(dev):
-        check(lib.ts_grad_clip(src, dst, numel, dt, ddt, n, max_norm, ptr(norm), ptr(ws), wsb,
-                               _lib.stream_handle(dev)), "ts_grad_clip")
+        check(lib.ts_grad_clip(
+            _host(grads.ptr), _host(outs.ptr), _host(grads.numel), _host(grads.code),
+            _host(outs.code), grads.count, max_norm, ptr(norm), ptr(ws), wsb,
+            _lib.stream_handle(dev)), "ts_grad_clip")
     return norm
