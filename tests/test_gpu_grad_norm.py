@@ -79,7 +79,7 @@ def test_many_tensors(gpu, count):
 
 def test_norm_formed_in_a_launch_of_its_own(gpu):
     # more partial sums than the scaling's workgroups add up themselves: full launches of 3 types
-    per = 64 * 1024 * 2049
+    per = 16 * 1024 * 2049
     ts = [torch.full((per // 4,), 1e-3, device=gpu),
           torch.full((per // 2,), 1e-3, device=gpu, dtype=BF),
           torch.full((per // 2 + 1,), 1e-3, device=gpu, dtype=F16)]

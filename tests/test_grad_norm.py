@@ -152,12 +152,12 @@ int main() {
         std::vector<int64_t> numel(count);
         std::vector<int32_t> end(count);
         int64_t chunks = 0;
-        const int64_t per = kGradChunkBytes / elt;
+        const int64_t per = grad_chunk(elt, rep % 2 ? kGradNormPieces : kGradScalePieces);
         for (int i = 0; i < count; ++i) {
           r = r * 1664525u + 1013904223u;
           const int64_t edge[] = {1, per - 1, per, per + 1, 3 * per, (int64_t)(r >> 12) + 1};
           numel[i] = edge[r % 6];
-          chunks += grad_chunks(numel[i], elt);
+          chunks += grad_chunks(numel[i], per);
           end[i] = (int32_t)chunks;
         }
         // every chunk belongs to one tensor and holds at least one of its values; together
@@ -184,7 +184,7 @@ int main() {
       }
     fails += most * kGradGrid > grad_norm_parts(count);
   }
-  fails += grad_chunks(0, 2) != 0 || grad_norm_parts(0) < 1;
+  fails += grad_chunks(0, 2048) != 0 || grad_norm_parts(0) < 1;
   std::printf("%d failures\n", fails);
   return fails != 0;
 }

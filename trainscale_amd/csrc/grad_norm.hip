@@ -23,11 +23,12 @@ namespace {
 
 using namespace ts;
 
-constexpr int kThreads = 256;
+constexpr int kThreads = ts_plan::kGradThreads;
 constexpr int kGrid = ts_plan::kGradGrid;
 constexpr int kTensors = ts_plan::kGradTensors;
-// 16-byte vectors each thread has in flight
-constexpr int kVecs = 4;
+// 16-byte vectors each thread has in flight: those of a chunk
+constexpr int kNormVecs = ts_plan::kGradNormPieces;
+constexpr int kScaleVecs = ts_plan::kGradScalePieces;
 
 struct Table {
   const void* src[kTensors];
@@ -75,7 +76,7 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void grad_squares(Table tab, int count, int chunks,
                                                          double* __restrict__ partial) {
   constexpr int V = Elt<T>::kVec;
-  constexpr int64_t kChunk = ts_plan::kGradChunkBytes / sizeof(T);
+  constexpr int64_t kChunk = ts_plan::grad_chunk(sizeof(T), kNormVecs);
   __shared__ double lds[kThreads / kWave];
   double acc = 0.;
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
@@ -85,19 +86,20 @@ __global__ __launch_bounds__(kThreads) void grad_squares(Table tab, int count, i
     const int64_t left = tab.numel[t] - first;
     const int n = (int)(left < kChunk ? left : kChunk);
     const int nvec = n / V;
-    int v = threadIdx.x;
-    for (; v + (kVecs - 1) * kThreads < nvec; v += kVecs * kThreads) {
-      u32x4 q[kVecs];
+    if (n == kChunk) {
+      u32x4 q[kNormVecs];
 #pragma unroll
-      for (int k = 0; k < kVecs; ++k) q[k] = ld16_any_stream(x + (v + k * kThreads) * V);
+      for (int k = 0; k < kNormVecs; ++k)
+        q[k] = ld16_any_stream(x + (threadIdx.x + k * kThreads) * V);
 #pragma unroll
-      for (int k = 0; k < kVecs; ++k) {
+      for (int k = 0; k < kNormVecs; ++k) {
         float f[V];
         Elt<T>::unpack(q[k], f);
         acc += vec_squares<V>(f);
       }
+      continue;
     }
-    for (; v < nvec; v += kThreads) {
+    for (int v = threadIdx.x; v < nvec; v += kThreads) {
       float f[V];
       Elt<T>::unpack(ld16_any_stream(x + v * V), f);
       acc += vec_squares<V>(f);
@@ -113,9 +115,9 @@ __global__ __launch_bounds__(kThreads) void grad_squares(Table tab, int count, i
 }
 
 // The partial sums' total, in the same order in every workgroup that asks for it. The scaling's
-// workgroups form it themselves, which saves a launch between the two passes; past kOwnParts
-// partial sums (over 256 tensors or so) a launch of its own forms the norm once.
-constexpr int kOwnParts = 2 * kGrid;
+// workgroups form it themselves while it is short, which saves a launch between the two passes;
+// past kOwnParts partial sums (8 MB of gradients in one launch) a launch of its own forms the norm.
+constexpr int kOwnParts = 512;
 constexpr int kFinalThreads = 1024;
 
 template <int kT>
@@ -140,28 +142,38 @@ __device__ inline float clip_coef(double norm, float max_norm) {
   return c >= 1. ? 1.f : (float)c;
 }
 
-template <typename T, typename D>
-__device__ inline void scale_vec(const T* x, D* o, float coef) {
-  constexpr int V = Elt<T>::kVec;
-  float f[V];
-  Elt<T>::unpack(ld16_any_stream(x), f);
+// N elements of T at any element address: 16 bytes, or 8 for 16-bit gradients that go to fp32,
+// so that every lane of a wave stores 16 bytes next to its neighbour's.
+typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
+template <typename T, int N>
+struct Piece {
+  u32x4 q;
+  __device__ inline void load(const T* x) {
+    if constexpr (N == Elt<T>::kVec) {
+      q = ld16_any_stream(x);
+    } else {
+      const u32x2_any h = __builtin_nontemporal_load(reinterpret_cast<const u32x2_any*>(x));
+      q = u32x4{h[0], h[1], 0u, 0u};
+    }
+  }
+  __device__ inline void unpack(float (&f)[N]) const {
+    float all[Elt<T>::kVec];
+    Elt<T>::unpack(q, all);
 #pragma unroll
-  for (int i = 0; i < V; ++i) f[i] *= coef;
-#pragma unroll
-  for (int h = 0; h < V / Elt<D>::kVec; ++h)
-    st16_any_stream(o + h * Elt<D>::kVec, Elt<D>::pack(f + h * Elt<D>::kVec));
-}
+    for (int i = 0; i < N; ++i) f[i] = all[i];
+  }
+};
 
 // The norm comes from `partial` (nparts > 0; workgroup 0 of the first launch writes it to
-// norm_out) or from *norm_in. The chunks run from the last to the first: what the norm's pass
-// read last is what the last-level cache still holds.
+// norm_out) or from *norm_in.
 template <typename T, typename D>
 __global__ __launch_bounds__(kThreads) void grad_scale(Table tab, int count, int chunks,
                                                        const double* __restrict__ partial,
                                                        int nparts, const float* norm_in,
-                                                       float* norm_out, float max_norm) {
-  constexpr int V = Elt<T>::kVec;
-  constexpr int64_t kChunk = ts_plan::kGradChunkBytes / sizeof(T);
+                                                       float* norm_out, float max_norm,
+                                                       int in_place) {
+  constexpr int V = Elt<D>::kVec;
+  constexpr int64_t kChunk = ts_plan::grad_chunk(sizeof(D), kScaleVecs);
   __shared__ double lds[kThreads / kWave];
   double norm;
   if (nparts > 0) {
@@ -171,20 +183,35 @@ __global__ __launch_bounds__(kThreads) void grad_scale(Table tab, int count, int
     norm = (double)*norm_in;
   }
   const float coef = clip_coef(norm, max_norm);
-  for (int i = blockIdx.x; i < chunks; i += gridDim.x) {
-    const int c = chunks - 1 - i;
-    const int t = find_tensor(tab, count, c);
-    if (coef == 1.f && tab.src[t] == tab.dst[t]) continue;  // in place and unchanged
-    const int64_t first = (int64_t)(c - (t ? tab.chunk_end[t - 1] : 0)) * kChunk;
-    const T* x = static_cast<const T*>(tab.src[t]) + first;
-    D* o = static_cast<D*>(tab.dst[t]) + first;
-    const int64_t left = tab.numel[t] - first;
-    const int n = (int)(left < kChunk ? left : kChunk);
-    const int nvec = n / V;
-    for (int v = threadIdx.x; v < nvec; v += kThreads) scale_vec(x + v * V, o + v * V, coef);
-    const int e = nvec * V + threadIdx.x;
-    if (e < n) Elt<D>::store1(o + e, Elt<T>::load1(x + e) * coef);
+  if (coef == 1.f && in_place) return;  // every gradient stays as it is
+  const int c = blockIdx.x;
+  const int t = find_tensor(tab, count, c);
+  if (coef == 1.f && tab.src[t] == tab.dst[t]) return;
+  const int64_t first = (int64_t)(c - (t ? tab.chunk_end[t - 1] : 0)) * kChunk;
+  const T* x = static_cast<const T*>(tab.src[t]) + first;
+  D* o = static_cast<D*>(tab.dst[t]) + first;
+  const int64_t left = tab.numel[t] - first;
+  const int n = (int)(left < kChunk ? left : kChunk);
+  const int nvec = n / V;
+  Piece<T, V> q[kScaleVecs];
+#pragma unroll
+  for (int k = 0; k < kScaleVecs; ++k) {
+    const int v = threadIdx.x + k * kThreads;
+    if (v < nvec) q[k].load(x + v * V);
   }
+#pragma unroll
+  for (int k = 0; k < kScaleVecs; ++k) {
+    const int v = threadIdx.x + k * kThreads;
+    if (v < nvec) {
+      float f[V];
+      q[k].unpack(f);
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] *= coef;
+      st16_any_stream(o + v * V, Elt<D>::pack(f));
+    }
+  }
+  const int e = nvec * V + threadIdx.x;
+  if (e < n) Elt<D>::store1(o + e, Elt<T>::load1(x + e) * coef);
 }
 
 // ---------------------------------------------------------------------------
@@ -226,12 +253,20 @@ ts_status check_lists(const char* what, const Lists& l, bool dst) {
         (dst && reinterpret_cast<uintptr_t>(l.dst[i]) % dsize != 0))
       return fail(TS_ERR_INVALID_ARGUMENT, "%s: tensor %lld is not aligned to its elements", what,
                   (long long)i);
-    const int64_t c = ts_plan::grad_chunks(l.numel[i], (int)size);
+    // the shorter of the two kernels' chunks
+    const int64_t c = ts_plan::grad_chunks(l.numel[i], ts_plan::grad_chunk(4, 2));
     if (c > ts_plan::kGradMaxChunks - chunks)
       return fail(TS_ERR_SHAPE, "%s: tensors too large", what);
     chunks += c;
   }
   return TS_OK;
+}
+
+int64_t norm_chunk(int32_t t) {
+  return ts_plan::grad_chunk((int)ts_host::dtype_size((ts_dtype)t), kNormVecs);
+}
+int64_t scale_chunk(int32_t t) {
+  return ts_plan::grad_chunk((int)ts_host::dtype_size((ts_dtype)t), kScaleVecs);
 }
 
 // Calls f(table, tensors, chunks, dtype, dst dtype) for groups of up to kTensors tensors of one
@@ -254,7 +289,7 @@ ts_status for_groups(const Lists& l, bool dst, F f) {
       if (i == l.count) break;
       if (l.dtype[i] != pairs[p][0] || (dst && l.dst_dtype[i] != pairs[p][1]) || l.numel[i] == 0)
         continue;
-      chunks += ts_plan::grad_chunks(l.numel[i], (int)ts_host::dtype_size((ts_dtype)l.dtype[i]));
+      chunks += ts_plan::grad_chunks(l.numel[i], dst ? scale_chunk(pairs[p][1]) : norm_chunk(pairs[p][0]));
       tab.src[n] = l.src[i];
       tab.dst[n] = dst ? l.dst[i] : nullptr;
       tab.numel[n] = l.numel[i];
@@ -265,13 +300,11 @@ ts_status for_groups(const Lists& l, bool dst, F f) {
   return TS_OK;
 }
 
-unsigned grid_for(int chunks) { return (unsigned)(chunks < kGrid ? chunks : kGrid); }
-
 ts_status launch_squares(const Lists& l, double* partial, int64_t capacity, int* nparts,
                          hipStream_t st) {
   *nparts = 0;
   return for_groups(l, false, [&](const Table& tab, int n, int chunks, int32_t t, int32_t) {
-    const unsigned g = grid_for(chunks);
+    const unsigned g = (unsigned)(chunks < kGrid ? chunks : kGrid);
     if (*nparts + (int64_t)g > capacity)
       return ts_host::fail(TS_ERR_WORKSPACE, "grad_norm: workspace too small");
     double* out = partial + *nparts;
@@ -294,10 +327,12 @@ ts_status launch_squares(const Lists& l, double* partial, int64_t capacity, int*
 ts_status launch_scale(const Lists& l, const double* partial, int nparts, const float* norm_in,
                        float* norm_out, float max_norm, hipStream_t st) {
   return for_groups(l, true, [&](const Table& tab, int n, int chunks, int32_t t, int32_t d) {
-    const dim3 grid(grid_for(chunks)), block(kThreads);
+    const dim3 grid((unsigned)chunks), block(kThreads);
+    int in_place = 1;
+    for (int i = 0; i < n; ++i) in_place &= tab.src[i] == tab.dst[i];
 #define TS_SCALE(T, D)                                                                         \
   hipLaunchKernelGGL((grad_scale<T, D>), grid, block, 0, st, tab, n, chunks, partial, nparts, \
-                     norm_in, norm_out, max_norm)
+                     norm_in, norm_out, max_norm, in_place)
     if (t == TS_F32) {
       TS_SCALE(float, float);
     } else if (t == TS_BF16) {

@@ -494,17 +494,21 @@ TS_HOST_DEVICE inline RopeElems rope_elems(int j, int width, int half, bool inte
 
 // ---------------------------------------------------------------------------
 // Global gradient norm and clipping (grad_norm.hip): the tensors of a launch are cut into
-// chunks of kGradChunkBytes (of the gradients), numbered through; chunk_end[t] is the number of
+// chunks of a workgroup's step, numbered through; chunk_end[t] is the number of
 // chunks of tensors 0 .. t.
 // ---------------------------------------------------------------------------
-constexpr int kGradTensors = 128;               // tensors of one launch
-constexpr int kGradGrid = 2048;                 // most workgroups of a launch: 8 a CU
-constexpr int64_t kGradChunkBytes = 64 * 1024;
-constexpr int64_t kGradMaxChunks = 1ll << 30;   // 64 TiB of gradients
+constexpr int kGradTensors = 128;  // tensors of one launch
+constexpr int kGradThreads = 256;
+constexpr int kGradGrid = 2048;    // most workgroups of a norm launch: 8 a CU
+constexpr int64_t kGradMaxChunks = 1ll << 30;
 
-TS_HOST_DEVICE inline int64_t grad_chunks(int64_t numel, int elt) {
-  const int64_t per = kGradChunkBytes / elt;
-  return numel / per + (numel % per != 0);
+// Elements of a chunk: `pieces` 16-byte vectors a thread of the type of `elt` bytes.
+TS_HOST_DEVICE constexpr int64_t grad_chunk(int elt, int pieces) {
+  return (int64_t)kGradThreads * pieces * (16 / elt);
+}
+constexpr int kGradNormPieces = 4, kGradScalePieces = 2;
+TS_HOST_DEVICE inline int64_t grad_chunks(int64_t numel, int64_t chunk) {
+  return numel / chunk + (numel % chunk != 0);
 }
 // The tensor that chunk c belongs to (c < end[count - 1]; no tensor is empty).
 template <typename A>
