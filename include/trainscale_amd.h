@@ -151,6 +151,46 @@ ts_status ts_rmsnorm_bwd_noalloc(const void* dy, int64_t lddy,
                                  int64_t rows, int64_t cols, ts_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* Norms before and after a block, with its gate and residual                */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * h = residual_scale * x + g * (y * ry) * (weight_offset + post),  n = h * rh * (weight_offset + pre)
+ * with ry = 1 / sqrt(mean(y^2) + eps), rh = 1 / sqrt(mean(h^2) + eps): y is a block's output, x
+ * the residual stream, n the next block's input. fp32 arithmetic; h and n are rounded once, n
+ * comes from the unrounded h.
+ * y, x, n, h: [rows, cols] of dtype with row strides ldy, ldx, ldn, ldh; any element-aligned
+ * address. post, pre: [cols] of w_dtype (dtype or TS_F32). gate: NULL (g = 1, gate_groups 1) or
+ * [gate_groups, cols] of gate_dtype (dtype or TS_F32), row r taking gate row
+ * r / (rows / gate_groups); gate_groups divides rows. rstd_y, rstd_h: [rows] fp32, written (for
+ * the backward). cols at most 32768 bytes of dtype.
+ */
+ts_status ts_sandwich_norm_fwd(const void* y, int64_t ldy, const void* x, int64_t ldx,
+                               ts_dtype dtype, const void* post, const void* pre,
+                               ts_dtype w_dtype, const void* gate, ts_dtype gate_dtype,
+                               int64_t gate_groups, void* n, int64_t ldn, void* h, int64_t ldh,
+                               float* rstd_y, float* rstd_h, int64_t rows, int64_t cols,
+                               float residual_scale, float weight_offset, float eps,
+                               ts_stream_t stream);
+
+/* Bytes of workspace ts_sandwich_norm_bwd needs when a parameter's gradient is asked for. */
+size_t ts_sandwich_norm_bwd_workspace_size(int64_t rows, int64_t cols, int64_t gate_groups);
+
+/*
+ * Gradients of the above from dn and dh (either may be NULL: zeros): dy and dx ([rows, cols]),
+ * dpost and dpre ([cols] of w_dtype), dgate ([gate_groups, cols] of gate_dtype); each may be
+ * NULL to skip it. y, x, the parameters and rstd are the forward's. The parameters' sums are
+ * fp32 in a fixed order. Workspace: 16-byte aligned.
+ */
+ts_status ts_sandwich_norm_bwd(
+    const void* dn, int64_t lddn, const void* dh, int64_t lddh, const void* y, int64_t ldy,
+    const void* x, int64_t ldx, ts_dtype dtype, const void* post, const void* pre,
+    ts_dtype w_dtype, const void* gate, ts_dtype gate_dtype, int64_t gate_groups,
+    const float* rstd_y, const float* rstd_h, void* dy, int64_t lddy, void* dx, int64_t lddx,
+    void* dpost, void* dpre, void* dgate, int64_t rows, int64_t cols, float residual_scale,
+    float weight_offset, void* workspace, size_t workspace_bytes, ts_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* SwiGLU                                                                    */
 /* ------------------------------------------------------------------------ */
 

@@ -119,6 +119,11 @@ __device__ inline u32x4 ld16_stream(const T* p) {
 // alignment, and the element-aligned vector type makes the compiler keep them whole.
 typedef u32x4 u32x4_any __attribute__((aligned(2)));
 template <typename T>
+__device__ inline u32x4 ld16_any(const T* p) {
+  const u32x4 v = *reinterpret_cast<const u32x4_any*>(p);
+  return v;
+}
+template <typename T>
 __device__ inline u32x4 ld16_any_stream(const T* p) {
   return __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
 }

@@ -625,4 +625,62 @@ inline int embed_fwd_lanes(int64_t parts) {
   return parts <= 8 ? 8 : parts <= 32 ? 32 : parts <= 128 ? 128 : 256;
 }
 
+// ---------------------------------------------------------------------------
+// Norms before and after a block (sandwich_norm.hip): a row of `parts` 16-byte vectors (the last
+// one may be partial) is owned by tpr threads, kv vectors each; rpb rows a workgroup.
+// ---------------------------------------------------------------------------
+constexpr int kSandwichMaxParts = 2048;
+constexpr int kSandwichReduceCols = 16;
+inline int64_t sandwich_max_cols(int elt) { return (int64_t)kSandwichMaxParts * (16 / elt); }
+
+struct SandwichPlan {
+  int tpr, kv, rpb;
+};
+// Two vectors a thread of each of the two inputs where the row allows it.
+inline SandwichPlan sandwich_fwd_plan(int parts) {
+  SandwichPlan p{0, 0, 0};
+  if (parts <= 64) { p.tpr = 64; p.kv = 1; }
+  else if (parts <= 128) { p.tpr = 64; p.kv = 2; }
+  else if (parts <= 256) { p.tpr = 128; p.kv = 2; }
+  else if (parts <= 512) { p.tpr = 256; p.kv = 2; }
+  else if (parts <= 1024) { p.tpr = 512; p.kv = 2; }
+  else { p.tpr = 512; p.kv = 4; }
+  p.rpb = p.tpr > 256 ? 1 : 256 / p.tpr;
+  return p;
+}
+
+// One vector a thread of each of the four inputs where the row allows it.
+struct SandwichBwdPlan {
+  SandwichPlan row;
+  int64_t per_group, steps;  // workgroups of a gate's group, steps of rpb rows of each
+};
+inline SandwichBwdPlan sandwich_bwd_plan(int64_t rows, int64_t groups, int64_t cols, int V) {
+  SandwichBwdPlan b{{0, 1, 0}, 0, 0};
+  const int64_t parts = (cols + V - 1) / V;
+  if (parts <= 64) b.row.tpr = 64;
+  else if (parts <= 128) b.row.tpr = 128;
+  else if (parts <= 256) b.row.tpr = 256;
+  else if (parts <= 512) b.row.tpr = 512;
+  else if (parts <= 1024) b.row.tpr = 1024;
+  else { b.row.tpr = 512; b.row.kv = 4; }
+  b.row.rpb = b.row.tpr > 512 ? 1 : 512 / b.row.tpr;
+  const int64_t sets = (rows / groups + b.row.rpb - 1) / b.row.rpb;  // of rpb rows, of a group
+  const int64_t target = (kBwdGridTarget + groups - 1) / groups;
+  b.per_group = sets < target ? sets : target;
+  b.steps = (sets + b.per_group - 1) / b.per_group;
+  b.per_group = (sets + b.steps - 1) / b.steps;
+  return b;
+}
+// Bytes for the partial rows (two a workgroup) and the groups' sums, for any type of the data.
+inline int64_t sandwich_workspace(int64_t rows, int64_t groups, int64_t cols) {
+  int64_t most = 0;
+  for (int V : {4, 8}) {
+    const int64_t ldp = (cols + V - 1) / V * V;
+    const SandwichBwdPlan b = sandwich_bwd_plan(rows, groups, cols, V);
+    const int64_t n = (2 * groups * b.per_group + (groups > 1 ? 2 * groups : 0)) * ldp * 4;
+    most = n > most ? n : most;
+  }
+  return most;
+}
+
 }  // namespace ts_plan

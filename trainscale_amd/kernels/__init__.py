@@ -24,10 +24,13 @@ from .grad_kernels import (
 from .layernorm_kernels import (
     FusedAddRMSLayerNormFunction,
     FusedRMSNorm,
+    FusedSandwichRMSNorm,
+    FusedSandwichRMSNormFunction,
     RMSLayerNormFunction,
     RMSNorm,
     fast_rms_layernorm,
     fused_add_rms_layernorm,
+    fused_sandwich_rms_layernorm,
     rms_layernorm,
 )
 from .rope_kernels import (
@@ -61,6 +64,9 @@ __all__ = [
     "FusedAddRMSLayerNormFunction",
     "fused_add_rms_layernorm",
     "FusedRMSNorm",
+    "FusedSandwichRMSNormFunction",
+    "fused_sandwich_rms_layernorm",
+    "FusedSandwichRMSNorm",
     "Fast_RoPE",
     "Fast_RoPE_Embedding",
     "FusedRoPEQKFunction",

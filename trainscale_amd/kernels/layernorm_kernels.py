@@ -18,6 +18,11 @@ Reference (``data_pipeline/trainer/``):
   gradient arriving at ``residual_out`` is not added and the weight gets no
   gradient (the reference's backward returns None for it).
 
+Not in the reference: ``FusedSandwichRMSNormFunction``, ``fused_sandwich_rms_layernorm`` and the
+``FusedSandwichRMSNorm`` module, the boundary between two blocks of models that normalise before
+and after each block: the norm of a block's output, its gate, the residual sum and the next
+block's norm in one pass, with every gradient.
+
 LayerNorm/Welford and dropout+RMS are not part of this layer.
 """
 from __future__ import annotations
@@ -40,6 +45,9 @@ __all__ = [
     "FusedAddRMSLayerNormFunction",
     "fused_add_rms_layernorm",
     "FusedRMSNorm",
+    "FusedSandwichRMSNormFunction",
+    "fused_sandwich_rms_layernorm",
+    "FusedSandwichRMSNorm",
     "DEFAULT_EPS_RMS",
 ]
 
@@ -179,3 +187,123 @@ class FusedRMSNorm(nn.Module):
 
     def extra_repr(self) -> str:
         return f"{self.hidden_size}, eps={self.eps}"
+
+
+def _gate_rows(gate: Tensor, X: Tensor) -> Tensor:
+    """A gate that broadcasts over X as [groups, H], group g covering equal runs of X's rows."""
+    shape, lead = tuple(gate.shape), tuple(X.shape[:-1])
+    if not shape or shape[-1] != X.shape[-1]:
+        raise ValueError(f"fused_sandwich_rms_layernorm: gate {shape} for X {tuple(X.shape)}")
+    if len(shape) > 1:
+        # the leading dimensions of X, then ones: the rows of a group are neighbours
+        own = len(shape) == X.dim()
+        k = 0
+        while own and k < len(lead) and shape[k] == lead[k]:
+            k += 1
+        if not own or any(n != 1 for n in shape[k:-1]):
+            raise ValueError(f"fused_sandwich_rms_layernorm: gate {shape} for X {tuple(X.shape)}: "
+                             "expected [H], or X's leading dimensions followed by ones and H")
+    return gate.reshape(-1, shape[-1]).contiguous()
+
+
+class FusedSandwichRMSNormFunction(torch.autograd.Function):
+    """forward(X, residual, post_weight, pre_weight, gate, eps, residual_scale, weight_offset) ->
+    (Y, residual_out); differentiable in the five tensors."""
+
+    @staticmethod
+    def forward(ctx, X: Tensor, residual: Tensor, post_weight: Tensor, pre_weight: Tensor,
+                gate: Optional[Tensor] = None, eps: float = DEFAULT_EPS_RMS,
+                residual_scale: float = 1.0, weight_offset: float = 0.0) -> Tuple[Tensor, Tensor]:
+        if residual.shape != X.shape:
+            raise ValueError(f"fused_sandwich_rms_layernorm: residual {tuple(residual.shape)} != "
+                             f"X {tuple(X.shape)}")
+        g2d = None if gate is None else _gate_rows(gate, X)
+        y2d, ldy = ops.as_rows(X)
+        x2d, ldx = ops.as_rows(residual)
+        post, pre = post_weight.contiguous(), pre_weight.contiguous()
+        n, h, ry, rh = ops.sandwich_norm_forward(y2d, ldy, x2d, ldx, post, pre, g2d,
+                                                 residual_scale, weight_offset, eps)
+        ctx.save_for_backward(y2d, x2d, post, pre, g2d, ry, rh)
+        ctx.set_materialize_grads(False)
+        ctx.cfg = (X.shape, ldy, ldx, None if gate is None else gate.shape, residual_scale,
+                   weight_offset)
+        return n.view(X.shape), h.view(X.shape)
+
+    @staticmethod
+    def backward(ctx, dn: Optional[Tensor], dh: Optional[Tensor]):
+        if dn is None and dh is None:
+            return (None,) * 8
+        y2d, x2d, post, pre, g2d, ry, rh = ctx.saved_tensors
+        shape, ldy, ldx, gate_shape, residual_scale, weight_offset = ctx.cfg
+        if y2d.shape[0] == 0:
+            return (*[None if t is None or not need else torch.zeros(s, dtype=t.dtype,
+                                                                      device=t.device)
+                      for t, need, s in zip((y2d, x2d, post, pre, g2d), ctx.needs_input_grad,
+                                            (shape, shape, post.shape, pre.shape, gate_shape))],
+                    None, None, None)
+        (dn, lddn), (dh, lddh) = [(None, 0) if d is None else ops.as_rows(d) for d in (dn, dh)]
+        dy, dx, dpost, dpre, dgate = ops.sandwich_norm_backward(
+            dn, lddn, dh, lddh, y2d, ldy, x2d, ldx, post, pre, g2d, ry, rh, residual_scale,
+            weight_offset, ctx.needs_input_grad[:5])
+        return (None if dy is None else dy.view(shape), None if dx is None else dx.view(shape),
+                dpost, dpre, None if dgate is None else dgate.view(gate_shape), None, None, None)
+
+
+def fused_sandwich_rms_layernorm(X: Tensor, residual: Tensor, post_weight: Tensor,
+                                 pre_weight: Tensor, gate: Optional[Tensor] = None,
+                                 eps: float = DEFAULT_EPS_RMS, residual_scale: float = 1.0,
+                                 weight_offset: float = 0.0) -> Tuple[Tensor, Tensor]:
+    """The boundary between two blocks with norms before and after each: X is a block's output,
+    residual the stream beside it.
+
+        residual_out = residual_scale * residual + gate * RMSNorm(X; post_weight)
+        Y            = RMSNorm(residual_out; pre_weight)
+
+    Returns (Y, residual_out): the next block's input and the stream. RMSNorm(x; w) is
+    x * rstd * (weight_offset + w); weight_offset 1 is for weights kept as their difference from
+    1. gate: None, [H], or X's leading dimensions followed by ones and H ([B, 1, H] for X
+    [B, S, H]: one gate for each sequence). fp32 arithmetic; Y comes from the unrounded sum and
+    both results are rounded once. The weights share one dtype, X's or fp32; the gate has X's
+    dtype or fp32. Differentiable in X, residual, both weights and the gate. H is at most 16384
+    for 16-bit X, 8192 for fp32."""
+    return FusedSandwichRMSNormFunction.apply(X, residual, post_weight, pre_weight, gate,
+                                              float(eps), float(residual_scale),
+                                              float(weight_offset))
+
+
+class FusedSandwichRMSNorm(nn.Module):
+    """The norm after a block and the one before the next, with the residual sum between them
+    (``fused_sandwich_rms_layernorm``). layer_gate adds a learned gate of hidden_size channels,
+    initialised to gate_init."""
+
+    def __init__(self, hidden_size: int, eps: float = DEFAULT_EPS_RMS, weight_offset: float = 0.0,
+                 residual_scale: float = 1.0, layer_gate: bool = False, gate_init: float = 1.0,
+                 device: Optional[torch.device] = None, dtype: torch.dtype = torch.float32):
+        super().__init__()
+        self.hidden_size = hidden_size
+        self.eps = eps
+        self.weight_offset = weight_offset
+        self.residual_scale = residual_scale
+
+        def param(value):
+            return nn.Parameter(torch.full((hidden_size,), value, device=device, dtype=dtype))
+
+        self.post_weight = param(1.0 - weight_offset)
+        self.pre_weight = param(1.0 - weight_offset)
+        if layer_gate:
+            self.gate = param(gate_init)
+        else:
+            self.register_parameter("gate", None)
+
+    def forward(self, X: Tensor, residual: Tensor,
+                gate: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+        """gate: a conditioning gate, where the module has no learned one."""
+        if gate is not None and self.gate is not None:
+            raise ValueError("FusedSandwichRMSNorm: the module has a gate of its own")
+        return fused_sandwich_rms_layernorm(X, residual, self.post_weight, self.pre_weight,
+                                            self.gate if gate is None else gate, self.eps,
+                                            self.residual_scale, self.weight_offset)
+
+    def extra_repr(self) -> str:
+        return (f"{self.hidden_size}, eps={self.eps}, weight_offset={self.weight_offset}, "
+                f"residual_scale={self.residual_scale}")

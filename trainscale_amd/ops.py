@@ -128,6 +128,77 @@ def rmsnorm_backward(dy2d: Tensor, lddy: int, x2d: Tensor, ldx: int, weight: Opt
 
 
 # ---------------------------------------------------------------------------
+# Norms before and after a block
+# ---------------------------------------------------------------------------
+
+def _check_sandwich(y2d, x2d, post, pre, gate):
+    """Device and parameter dtype codes of one call; gate is None or [groups, cols]."""
+    dev = _lib.require_gpu("sandwich_norm", y2d, x2d, post, pre, gate)
+    rows, cols = y2d.shape
+    if x2d.shape != y2d.shape:
+        raise ValueError(f"sandwich_norm: residual {tuple(x2d.shape)} != block {tuple(y2d.shape)}")
+    if x2d.dtype != y2d.dtype:
+        raise TypeError(f"sandwich_norm: residual dtype {x2d.dtype} != block dtype {y2d.dtype}")
+    for name, w in (("post", post), ("pre", pre)):
+        if w.shape != (cols,):
+            raise ValueError(f"sandwich_norm: {name} weight {tuple(w.shape)} != ({cols},)")
+    if post.dtype != pre.dtype:
+        raise TypeError(f"sandwich_norm: weight dtypes {post.dtype} and {pre.dtype} differ")
+    g_code = _lib.dtype_code(gate, "sandwich_norm gate") if gate is not None else 0
+    return dev, _lib.dtype_code(post, "sandwich_norm weight"), g_code
+
+
+def sandwich_norm_forward(y2d: Tensor, ldy: int, x2d: Tensor, ldx: int, post: Tensor, pre: Tensor,
+                          gate: Optional[Tensor], residual_scale: float, weight_offset: float,
+                          eps: float) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    """Returns (n, h, rstd of y, rstd of h); parameters contiguous, gate None or [groups, cols]."""
+    dev, w_code, g_code = _check_sandwich(y2d, x2d, post, pre, gate)
+    rows, cols = y2d.shape
+    n = torch.empty((rows, cols), dtype=y2d.dtype, device=dev)
+    h = torch.empty((rows, cols), dtype=y2d.dtype, device=dev)
+    rstd = torch.empty((2, rows), dtype=torch.float32, device=dev)
+    if rows == 0:
+        return n, h, rstd[0], rstd[1]
+    with _lib.on_device(dev):
+        check(_lib.load().ts_sandwich_norm_fwd(
+            ptr(y2d), ldy, ptr(x2d), ldx, _lib.dtype_code(y2d, "sandwich_norm"), ptr(post),
+            ptr(pre), w_code, ptr(gate), g_code, 1 if gate is None else gate.shape[0], ptr(n),
+            cols, ptr(h), cols, ptr(rstd[0]), ptr(rstd[1]), rows, cols, residual_scale,
+            weight_offset, eps, _lib.stream_handle(dev)), "ts_sandwich_norm_fwd")
+    return n, h, rstd[0], rstd[1]
+
+
+def sandwich_norm_backward(dn: Optional[Tensor], lddn: int, dh: Optional[Tensor], lddh: int,
+                           y2d: Tensor, ldy: int, x2d: Tensor, ldx: int, post: Tensor,
+                           pre: Tensor, gate: Optional[Tensor], rstd_y: Tensor, rstd_h: Tensor,
+                           residual_scale: float, weight_offset: float,
+                           needs: Tuple[bool, bool, bool, bool, bool]):
+    """Gradients of (y, x, post, pre, gate), None where `needs` is false."""
+    dev, w_code, g_code = _check_sandwich(y2d, x2d, post, pre, gate)
+    rows, cols = y2d.shape
+    for name, d in (("n", dn), ("h", dh)):
+        if d is not None and (d.shape != y2d.shape or d.dtype != y2d.dtype):
+            raise ValueError(f"sandwich_norm: gradient of {name} is {tuple(d.shape)} {d.dtype}")
+    groups = 1 if gate is None else gate.shape[0]
+    like = (y2d, x2d, post, pre, gate)
+    out = [torch.empty(t.shape, dtype=t.dtype, device=dev) if need and t is not None else None
+           for t, need in zip(like, needs)]
+    lib = _lib.load()
+    ws, wsb = None, 0
+    if any(o is not None for o in out[2:]):
+        wsb = int(lib.ts_sandwich_norm_bwd_workspace_size(rows, cols, groups))
+        ws = torch.empty((wsb,), dtype=torch.uint8, device=dev)
+    with _lib.on_device(dev):
+        check(lib.ts_sandwich_norm_bwd(
+            ptr(dn), lddn, ptr(dh), lddh, ptr(y2d), ldy, ptr(x2d), ldx,
+            _lib.dtype_code(y2d, "sandwich_norm"), ptr(post), ptr(pre), w_code, ptr(gate), g_code,
+            groups, ptr(rstd_y), ptr(rstd_h), ptr(out[0]), cols, ptr(out[1]), cols, ptr(out[2]),
+            ptr(out[3]), ptr(out[4]), rows, cols, residual_scale, weight_offset, ptr(ws), wsb,
+            _lib.stream_handle(dev)), "ts_sandwich_norm_bwd")
+    return out
+
+
+# ---------------------------------------------------------------------------
 # RoPE
 # ---------------------------------------------------------------------------
 
