@@ -649,6 +649,59 @@ ts_status ts_embedding_bwd(const int64_t* ids, int64_t N, const void* dout, int6
                            size_t workspace_bytes, ts_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* Clipped policy loss                                                       */
+/* ------------------------------------------------------------------------ */
+
+enum { TS_POLICY_TOKEN = 0, TS_POLICY_SEQUENCE = 1, TS_POLICY_SUM = 2 };
+
+/*
+ * Inputs of the clipped policy loss over token log-probabilities, [rows, tokens] each (rows:
+ * sequences) with row strides in elements and unit column strides; any element-aligned address.
+ */
+typedef struct {
+  const void* logp; /* the policy's, of dtype */
+  int64_t ld_logp;
+  const void* old; /* the sampling policy's, of old_dtype; NULL: the policy's own values */
+  int64_t ld_old;
+  const void* ref; /* the reference's, of ref_dtype, for the KL term; NULL: none */
+  int64_t ld_ref;
+  const float* adv; /* advantages: [rows, tokens], or one a row (element row * ld_adv) */
+  int64_t ld_adv;
+  const uint8_t* mask; /* valid tokens: non-zero; NULL: all. Other tokens are not looked at */
+  int64_t ld_mask;
+  int64_t rows, tokens;
+  double clip_low, clip_high; /* ratio bounds 1 - clip_low, 1 + clip_high (clip_low >= 1: none) */
+  double kl_coef;
+  int32_t dtype, old_dtype, ref_dtype; /* ts_dtype; old and ref: dtype or TS_F32 */
+  int32_t adv_per_token;
+  int32_t reduction; /* TS_POLICY_* */
+} ts_policy_inputs;
+
+/* Bytes of workspace ts_policy_loss_fwd needs (0 for small batches), 8-byte aligned. */
+size_t ts_policy_loss_workspace_size(int64_t rows, int64_t tokens);
+
+/*
+ * With d = logp - old, r = exp(d), x = ref - logp, for every valid token:
+ *   policy = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A), kl = exp(x) - x - 1,
+ * and over them, with the reduction's weights w (TOKEN: 1 / valid tokens; SEQUENCE: 1 / (the
+ * row's valid tokens * rows that have any); SUM: 1):
+ *   policy_loss = sum w policy, kl = sum w kl, clip_fraction = sum w [clipped],
+ *   loss = policy_loss + kl_coef kl          (0-dim fp32 each; 0 without a valid token)
+ * weights: [rows] fp32, written for the backward (each row's w).
+ * The RL trainer's losses over these log-probs: rl_training.py:483-600.
+ */
+ts_status ts_policy_loss_fwd(const ts_policy_inputs* in, float* loss, float* policy_loss,
+                             float* kl, float* clip_fraction, float* weights, void* workspace,
+                             size_t workspace_bytes, ts_stream_t stream);
+
+/*
+ * dlogp = *dloss * w * ((clipped ? 0 : -r A) - kl_coef (exp(x) - 1)) in dtype, row stride
+ * ld_dlogp; exactly 0 for tokens that are not valid.
+ */
+ts_status ts_policy_loss_bwd(const ts_policy_inputs* in, const float* weights, const float* dloss,
+                             void* dlogp, int64_t ld_dlogp, ts_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* Global gradient norm and clipping                                         */
 /* ------------------------------------------------------------------------ */
 

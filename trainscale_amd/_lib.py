@@ -50,6 +50,16 @@ I32 = ctypes.c_int32
 F32 = ctypes.c_float
 SZ = ctypes.c_size_t
 
+class PolicyInputs(ctypes.Structure):
+    """ts_policy_inputs."""
+    _fields_ = [("logp", P), ("ld_logp", I64), ("old", P), ("ld_old", I64), ("ref", P),
+                ("ld_ref", I64), ("adv", P), ("ld_adv", I64), ("mask", P), ("ld_mask", I64),
+                ("rows", I64), ("tokens", I64), ("clip_low", ctypes.c_double),
+                ("clip_high", ctypes.c_double), ("kl_coef", ctypes.c_double), ("dtype", I32),
+                ("old_dtype", I32), ("ref_dtype", I32), ("adv_per_token", I32),
+                ("reduction", I32)]
+
+
 # argtypes of every exported entry point, in header order
 SIGNATURES = {
     "ts_last_error": ([], ctypes.c_char_p),
@@ -111,6 +121,9 @@ SIGNATURES = {
     "ts_embedding_fwd": ([P, I64, P, I64, I32, I64, I64, F32, P, I64, P], I32),
     "ts_embedding_bwd_workspace_size": ([I64, I64, I64], SZ),
     "ts_embedding_bwd": ([P, I64, P, I64, I32, I64, I64, F32, I64, P, P, SZ, P], I32),
+    "ts_policy_loss_workspace_size": ([I64, I64], SZ),
+    "ts_policy_loss_fwd": ([P, P, P, P, P, P, P, SZ, P], I32),
+    "ts_policy_loss_bwd": ([P, P, P, P, I64, P], I32),
     "ts_grad_norm_workspace_size": ([I64], SZ),
     "ts_grad_norm": ([P, P, P, I64, P, P, SZ, P], I32),
     "ts_grad_scale": ([P, P, P, P, P, I64, P, F32, P], I32),

@@ -683,4 +683,9 @@ inline int64_t sandwich_workspace(int64_t rows, int64_t groups, int64_t cols) {
   return most;
 }
 
+// Clipped policy loss (policy_loss.hip): tokens of one row that a wave takes, and the units up
+// to which one workgroup does the whole forward (4 rounds of its 16 waves).
+constexpr int kPolicyUnit = 512;
+constexpr int kPolicySmallUnits = 64;
+
 }  // namespace ts_plan

@@ -23,6 +23,31 @@ from .. import ops
 __all__ = ["ScaledEmbeddingFunction", "scaled_embedding", "ScaledEmbedding"]
 
 
+def _forward(input_ids: Tensor, weight: Tensor, scale: float, padding_idx: Optional[int]):
+    """(result, contiguous int64 ids, padding row or -1), after the checks of the arguments."""
+    if weight.dim() != 2:
+        raise ValueError(f"scaled_embedding: weight must be [V, H], got {tuple(weight.shape)}")
+    if input_ids.dtype is not torch.int64:
+        if input_ids.dtype is not torch.int32:
+            raise TypeError(f"scaled_embedding: ids must be int64 or int32, got {input_ids.dtype}")
+        input_ids = input_ids.to(torch.int64)
+    if not math.isfinite(scale):
+        raise ValueError(f"scaled_embedding: scale must be finite, got {scale}")
+    if padding_idx is None:
+        padding_idx = -1
+    else:
+        rows = weight.shape[0]
+        if not -rows <= padding_idx < rows:
+            raise ValueError(f"scaled_embedding: padding_idx {padding_idx} for {rows} rows")
+        padding_idx %= rows
+    ids = input_ids.contiguous()
+    if weight.is_contiguous():
+        w2d, ldw = weight, weight.shape[1]
+    else:
+        w2d, ldw = ops.as_rows(weight)
+    return ops.embedding_forward(ids, w2d, ldw, scale), ids, padding_idx
+
+
 class ScaledEmbeddingFunction(torch.autograd.Function):
     """forward(input_ids [...], weight [V, H], scale, padding_idx) -> [..., H]; backward gives the
     weight's gradient."""
@@ -30,23 +55,10 @@ class ScaledEmbeddingFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, input_ids: Tensor, weight: Tensor, scale: float = 1.0,
                 padding_idx: Optional[int] = None) -> Tensor:
-        if weight.dim() != 2:
-            raise ValueError(f"scaled_embedding: weight must be [V, H], got {tuple(weight.shape)}")
-        if input_ids.dtype not in (torch.int64, torch.int32):
-            raise TypeError(f"scaled_embedding: ids must be int64 or int32, got {input_ids.dtype}")
-        if not math.isfinite(scale):
-            raise ValueError(f"scaled_embedding: scale must be finite, got {scale}")
-        rows = weight.shape[0]
-        if padding_idx is not None:
-            if not -rows <= padding_idx < rows:
-                raise ValueError(f"scaled_embedding: padding_idx {padding_idx} for {rows} rows")
-            padding_idx %= rows
-        w2d, ldw = ops.as_rows(weight)
-        ids = input_ids.reshape(-1).to(torch.int64).contiguous()
-        out = ops.embedding_forward(ids, w2d, ldw, scale)
+        out, ids, padding_idx = _forward(input_ids, weight, scale, padding_idx)
         ctx.save_for_backward(ids)
-        ctx.cfg = (rows, scale, -1 if padding_idx is None else padding_idx)
-        return out.view(*input_ids.shape, weight.shape[1])
+        ctx.cfg = (weight.shape[0], scale, padding_idx)
+        return out
 
     @staticmethod
     def backward(ctx, dout: Tensor):
@@ -63,7 +75,9 @@ def scaled_embedding(input_ids: Tensor, weight: Tensor, scale: float = 1.0,
     """scale * weight[input_ids]: ids [...] int64 or int32, weight [V, H] fp32/bf16/fp16; the
     result is [..., H] in the weight's dtype, differentiable in weight. Tokens equal to
     padding_idx (negative counts from the end) get their row but give it no gradient."""
-    return ScaledEmbeddingFunction.apply(input_ids, weight, float(scale), padding_idx)
+    if weight.requires_grad and torch.is_grad_enabled():
+        return ScaledEmbeddingFunction.apply(input_ids, weight, float(scale), padding_idx)
+    return _forward(input_ids, weight, float(scale), padding_idx)[0]
 
 
 class ScaledEmbedding(nn.Module):

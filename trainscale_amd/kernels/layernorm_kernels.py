@@ -206,6 +206,21 @@ def _gate_rows(gate: Tensor, X: Tensor) -> Tensor:
     return gate.reshape(-1, shape[-1]).contiguous()
 
 
+def _sandwich_forward(X, residual, post_weight, pre_weight, gate, eps, residual_scale,
+                      weight_offset):
+    """The results and what the backward needs of one call: (n, h, saved tensors, strides)."""
+    if residual.shape != X.shape:
+        raise ValueError(f"fused_sandwich_rms_layernorm: residual {tuple(residual.shape)} != "
+                         f"X {tuple(X.shape)}")
+    g2d = None if gate is None else _gate_rows(gate, X)
+    y2d, ldy = ops.as_rows(X)
+    x2d, ldx = ops.as_rows(residual)
+    post, pre = post_weight.contiguous(), pre_weight.contiguous()
+    n, h, rstd = ops.sandwich_norm_forward(y2d, ldy, x2d, ldx, post, pre, g2d, residual_scale,
+                                           weight_offset, eps)
+    return n.view(X.shape), h.view(X.shape), (y2d, x2d, post, pre, g2d, rstd), (ldy, ldx)
+
+
 class FusedSandwichRMSNormFunction(torch.autograd.Function):
     """forward(X, residual, post_weight, pre_weight, gate, eps, residual_scale, weight_offset) ->
     (Y, residual_out); differentiable in the five tensors."""
@@ -214,27 +229,20 @@ class FusedSandwichRMSNormFunction(torch.autograd.Function):
     def forward(ctx, X: Tensor, residual: Tensor, post_weight: Tensor, pre_weight: Tensor,
                 gate: Optional[Tensor] = None, eps: float = DEFAULT_EPS_RMS,
                 residual_scale: float = 1.0, weight_offset: float = 0.0) -> Tuple[Tensor, Tensor]:
-        if residual.shape != X.shape:
-            raise ValueError(f"fused_sandwich_rms_layernorm: residual {tuple(residual.shape)} != "
-                             f"X {tuple(X.shape)}")
-        g2d = None if gate is None else _gate_rows(gate, X)
-        y2d, ldy = ops.as_rows(X)
-        x2d, ldx = ops.as_rows(residual)
-        post, pre = post_weight.contiguous(), pre_weight.contiguous()
-        n, h, ry, rh = ops.sandwich_norm_forward(y2d, ldy, x2d, ldx, post, pre, g2d,
-                                                 residual_scale, weight_offset, eps)
-        ctx.save_for_backward(y2d, x2d, post, pre, g2d, ry, rh)
+        n, h, saved, ld = _sandwich_forward(X, residual, post_weight, pre_weight, gate, eps,
+                                            residual_scale, weight_offset)
+        ctx.save_for_backward(*saved)
         ctx.set_materialize_grads(False)
-        ctx.cfg = (X.shape, ldy, ldx, None if gate is None else gate.shape, residual_scale,
+        ctx.cfg = (X.shape, ld, None if gate is None else gate.shape, residual_scale,
                    weight_offset)
-        return n.view(X.shape), h.view(X.shape)
+        return n, h
 
     @staticmethod
     def backward(ctx, dn: Optional[Tensor], dh: Optional[Tensor]):
         if dn is None and dh is None:
             return (None,) * 8
-        y2d, x2d, post, pre, g2d, ry, rh = ctx.saved_tensors
-        shape, ldy, ldx, gate_shape, residual_scale, weight_offset = ctx.cfg
+        y2d, x2d, post, pre, g2d, rstd = ctx.saved_tensors
+        shape, (ldy, ldx), gate_shape, residual_scale, weight_offset = ctx.cfg
         if y2d.shape[0] == 0:
             return (*[None if t is None or not need else torch.zeros(s, dtype=t.dtype,
                                                                       device=t.device)
@@ -243,7 +251,7 @@ class FusedSandwichRMSNormFunction(torch.autograd.Function):
                     None, None, None)
         (dn, lddn), (dh, lddh) = [(None, 0) if d is None else ops.as_rows(d) for d in (dn, dh)]
         dy, dx, dpost, dpre, dgate = ops.sandwich_norm_backward(
-            dn, lddn, dh, lddh, y2d, ldy, x2d, ldx, post, pre, g2d, ry, rh, residual_scale,
+            dn, lddn, dh, lddh, y2d, ldy, x2d, ldx, post, pre, g2d, rstd, residual_scale,
             weight_offset, ctx.needs_input_grad[:5])
         return (None if dy is None else dy.view(shape), None if dx is None else dx.view(shape),
                 dpost, dpre, None if dgate is None else dgate.view(gate_shape), None, None, None)
@@ -266,9 +274,11 @@ def fused_sandwich_rms_layernorm(X: Tensor, residual: Tensor, post_weight: Tenso
     both results are rounded once. The weights share one dtype, X's or fp32; the gate has X's
     dtype or fp32. Differentiable in X, residual, both weights and the gate. H is at most 16384
     for 16-bit X, 8192 for fp32."""
-    return FusedSandwichRMSNormFunction.apply(X, residual, post_weight, pre_weight, gate,
-                                              float(eps), float(residual_scale),
-                                              float(weight_offset))
+    args = (X, residual, post_weight, pre_weight, gate, float(eps), float(residual_scale),
+            float(weight_offset))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:5]):
+        return FusedSandwichRMSNormFunction.apply(*args)
+    return _sandwich_forward(*args)[:2]
 
 
 class FusedSandwichRMSNorm(nn.Module):

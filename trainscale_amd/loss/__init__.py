@@ -13,6 +13,8 @@ from torch import Tensor
 from .linear_ce import (FusedLinearCrossEntropyFunction, LinearCrossEntropyFunction,
                         SelectiveLogSoftmaxFunction, chunked_log_softmax,
                         fused_linear_cross_entropy, selective_log_softmax)
+from .policy_loss import (ClippedPolicyLoss, ClippedPolicyLossFunction, PolicyLoss,
+                          clipped_policy_loss)
 from .sota_losses import (
     ChunkedCrossEntropyLoss,
     CrossEntropyRowsFunction,
@@ -35,6 +37,10 @@ __all__ = [
     "chunked_log_softmax",
     "selective_log_softmax",
     "SelectiveLogSoftmaxFunction",
+    "PolicyLoss",
+    "ClippedPolicyLoss",
+    "ClippedPolicyLossFunction",
+    "clipped_policy_loss",
 ]
 
 

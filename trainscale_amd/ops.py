@@ -139,9 +139,9 @@ def _check_sandwich(y2d, x2d, post, pre, gate):
         raise ValueError(f"sandwich_norm: residual {tuple(x2d.shape)} != block {tuple(y2d.shape)}")
     if x2d.dtype != y2d.dtype:
         raise TypeError(f"sandwich_norm: residual dtype {x2d.dtype} != block dtype {y2d.dtype}")
-    for name, w in (("post", post), ("pre", pre)):
-        if w.shape != (cols,):
-            raise ValueError(f"sandwich_norm: {name} weight {tuple(w.shape)} != ({cols},)")
+    if post.shape != (cols,) or pre.shape != (cols,):
+        raise ValueError(f"sandwich_norm: weights {tuple(post.shape)} and {tuple(pre.shape)} != "
+                         f"({cols},)")
     if post.dtype != pre.dtype:
         raise TypeError(f"sandwich_norm: weight dtypes {post.dtype} and {pre.dtype} differ")
     g_code = _lib.dtype_code(gate, "sandwich_norm gate") if gate is not None else 0
@@ -150,28 +150,30 @@ def _check_sandwich(y2d, x2d, post, pre, gate):
 
 def sandwich_norm_forward(y2d: Tensor, ldy: int, x2d: Tensor, ldx: int, post: Tensor, pre: Tensor,
                           gate: Optional[Tensor], residual_scale: float, weight_offset: float,
-                          eps: float) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
-    """Returns (n, h, rstd of y, rstd of h); parameters contiguous, gate None or [groups, cols]."""
+                          eps: float) -> Tuple[Tensor, Tensor, Tensor]:
+    """Returns (n, h, rstd [2, rows] of y and of h); parameters contiguous, gate None or
+    [groups, cols]."""
     dev, w_code, g_code = _check_sandwich(y2d, x2d, post, pre, gate)
     rows, cols = y2d.shape
     n = torch.empty((rows, cols), dtype=y2d.dtype, device=dev)
     h = torch.empty((rows, cols), dtype=y2d.dtype, device=dev)
     rstd = torch.empty((2, rows), dtype=torch.float32, device=dev)
     if rows == 0:
-        return n, h, rstd[0], rstd[1]
+        return n, h, rstd
     with _lib.on_device(dev):
         check(_lib.load().ts_sandwich_norm_fwd(
-            ptr(y2d), ldy, ptr(x2d), ldx, _lib.dtype_code(y2d, "sandwich_norm"), ptr(post),
-            ptr(pre), w_code, ptr(gate), g_code, 1 if gate is None else gate.shape[0], ptr(n),
-            cols, ptr(h), cols, ptr(rstd[0]), ptr(rstd[1]), rows, cols, residual_scale,
+            y2d.data_ptr(), ldy, x2d.data_ptr(), ldx, _lib.dtype_code(y2d, "sandwich_norm"),
+            post.data_ptr(), pre.data_ptr(), w_code, ptr(gate), g_code,
+            1 if gate is None else gate.shape[0], n.data_ptr(), cols, h.data_ptr(), cols,
+            rstd.data_ptr(), rstd.data_ptr() + 4 * rows, rows, cols, residual_scale,
             weight_offset, eps, _lib.stream_handle(dev)), "ts_sandwich_norm_fwd")
-    return n, h, rstd[0], rstd[1]
+    return n, h, rstd
 
 
 def sandwich_norm_backward(dn: Optional[Tensor], lddn: int, dh: Optional[Tensor], lddh: int,
                            y2d: Tensor, ldy: int, x2d: Tensor, ldx: int, post: Tensor,
-                           pre: Tensor, gate: Optional[Tensor], rstd_y: Tensor, rstd_h: Tensor,
-                           residual_scale: float, weight_offset: float,
+                           pre: Tensor, gate: Optional[Tensor], rstd: Tensor, residual_scale: float,
+                           weight_offset: float,
                            needs: Tuple[bool, bool, bool, bool, bool]):
     """Gradients of (y, x, post, pre, gate), None where `needs` is false."""
     dev, w_code, g_code = _check_sandwich(y2d, x2d, post, pre, gate)
@@ -192,7 +194,7 @@ def sandwich_norm_backward(dn: Optional[Tensor], lddn: int, dh: Optional[Tensor]
         check(lib.ts_sandwich_norm_bwd(
             ptr(dn), lddn, ptr(dh), lddh, ptr(y2d), ldy, ptr(x2d), ldx,
             _lib.dtype_code(y2d, "sandwich_norm"), ptr(post), ptr(pre), w_code, ptr(gate), g_code,
-            groups, ptr(rstd_y), ptr(rstd_h), ptr(out[0]), cols, ptr(out[1]), cols, ptr(out[2]),
+            groups, rstd.data_ptr(), rstd.data_ptr() + 4 * rows, ptr(out[0]), cols, ptr(out[1]), cols, ptr(out[2]),
             ptr(out[3]), ptr(out[4]), rows, cols, residual_scale, weight_offset, ptr(ws), wsb,
             _lib.stream_handle(dev)), "ts_sandwich_norm_bwd")
     return out
@@ -601,14 +603,15 @@ def swiglu_backward(dout: Tensor, gate: Tensor, up: Tensor) -> Tuple[Tensor, Ten
 # ---------------------------------------------------------------------------
 
 def embedding_forward(ids: Tensor, weight: Tensor, ldw: int, scale: float) -> Tensor:
-    """scale * weight[ids] for contiguous int64 ids [N]: [N, H] in the weight's dtype."""
+    """scale * weight[ids] for contiguous int64 ids: [*ids.shape, H] in the weight's dtype."""
     dev = _lib.require_gpu("embedding", ids, weight)
-    n, (v, h) = ids.shape[0], weight.shape
-    out = torch.empty((n, h), dtype=weight.dtype, device=dev)
+    v, h = weight.shape
+    out = torch.empty((*ids.shape, h), dtype=weight.dtype, device=dev)
     with _lib.on_device(dev):
         check(_lib.load().ts_embedding_fwd(
-            ptr(ids), n, ptr(weight), ldw, _lib.dtype_code(weight, "embedding"), v, h, scale,
-            ptr(out), h, _lib.stream_handle(dev)), "ts_embedding_fwd")
+            ids.data_ptr(), ids.numel(), weight.data_ptr(), ldw,
+            _lib.dtype_code(weight, "embedding"), v, h, scale, out.data_ptr(), h,
+            _lib.stream_handle(dev)), "ts_embedding_fwd")
     return out
 
 
@@ -617,8 +620,8 @@ def embedding_backward(ids: Tensor, dout2d: Tensor, ldd: int, rows: int, scale: 
     """The dense gradient [rows, H] of embedding_forward's weight (padding_idx -1: none)."""
     dev = _lib.require_gpu("embedding backward", ids, dout2d)
     n, h = dout2d.shape
-    if ids.shape[0] != n:
-        raise ValueError(f"embedding backward: {ids.shape[0]} ids for {n} rows")
+    if ids.numel() != n:
+        raise ValueError(f"embedding backward: {ids.numel()} ids for {n} rows")
     lib = _lib.load()
     grad = torch.empty((rows, h), dtype=dout2d.dtype, device=dev)
     wsb = int(lib.ts_embedding_bwd_workspace_size(n, rows, h))
@@ -628,6 +631,63 @@ def embedding_backward(ids: Tensor, dout2d: Tensor, ldd: int, rows: int, scale: 
             ptr(ids), n, ptr(dout2d), ldd, _lib.dtype_code(dout2d, "embedding backward"), rows, h,
             scale, padding_idx, ptr(grad), ptr(ws), wsb, _lib.stream_handle(dev)),
             "ts_embedding_bwd")
+    return grad
+
+
+# ---------------------------------------------------------------------------
+# Clipped policy loss
+# ---------------------------------------------------------------------------
+
+POLICY_REDUCTIONS = {"token": 0, "sequence": 1, "sum": 2}
+
+
+def _field(t: Optional[Tensor], tokens: int) -> Tuple[int, int]:
+    """Pointer and row stride of a struct's tensor (NULL where there is none)."""
+    if t is None:
+        return 0, tokens
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else tokens
+
+
+def policy_inputs(logps: Tensor, old: Optional[Tensor], adv: Tensor, mask: Optional[Tensor],
+                  ref: Optional[Tensor], clip_low: float, clip_high: float, kl_coef: float,
+                  reduction: str) -> "_lib.PolicyInputs":
+    """The C struct over 2-D tensors with unit column strides (adv [B, T] or [B], fp32; mask one
+    byte a token). It holds pointers only: the tensors must outlive the launches."""
+    rows, tokens = logps.shape
+    code = _lib.DTYPE_CODE
+    own, most = code[logps.dtype], max(tokens, 1)
+    return _lib.PolicyInputs(
+        *_field(logps, most), *_field(old, most), *_field(ref, most), *_field(adv, most),
+        *_field(mask, most), rows, tokens, clip_low, clip_high, kl_coef, own,
+        own if old is None else code[old.dtype], own if ref is None else code[ref.dtype],
+        adv.dim() == 2, POLICY_REDUCTIONS[reduction])
+
+
+def policy_loss_forward(inputs: "_lib.PolicyInputs", dev: torch.device) -> Tuple[Tensor, ...]:
+    """(loss, policy loss, KL, clip fraction, row weights), fp32 on `dev`."""
+    lib = _lib.load()
+    # the results apart from one another: a caller may scale the loss in place
+    loss, policy, kl, clipped = [torch.empty((), dtype=torch.float32, device=dev) for _ in range(4)]
+    weights = torch.empty(inputs.rows, dtype=torch.float32, device=dev)
+    wsb = lib.ts_policy_loss_workspace_size(inputs.rows, inputs.tokens)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+    with _lib.on_device(dev):
+        check(lib.ts_policy_loss_fwd(
+            ctypes.byref(inputs), loss.data_ptr(), policy.data_ptr(), kl.data_ptr(),
+            clipped.data_ptr(), weights.data_ptr(), ptr(ws), wsb, _lib.stream_handle(dev)),
+            "ts_policy_loss_fwd")
+    return loss, policy, kl, clipped, weights
+
+
+def policy_loss_backward(inputs: "_lib.PolicyInputs", weights: Tensor, dloss: Tensor,
+                         dtype: torch.dtype) -> Tensor:
+    """The gradient of logps, [rows, tokens] of dtype; dloss a 0-dim fp32 tensor."""
+    dev = weights.device
+    grad = torch.empty((inputs.rows, inputs.tokens), dtype=dtype, device=dev)
+    with _lib.on_device(dev):
+        check(_lib.load().ts_policy_loss_bwd(
+            ctypes.byref(inputs), weights.data_ptr(), dloss.data_ptr(), grad.data_ptr(),
+            max(inputs.tokens, 1), _lib.stream_handle(dev)), "ts_policy_loss_bwd")
     return grad
 
 
