@@ -2,8 +2,8 @@
 
 Tolerances: the forward is one fp32 product rounded once more (fp32: 2^-24; 16-bit: half a step
 plus 2^-24). A gradient row of n tokens is an fp32 sum; its additions run through at most
-DEPTH = 2 * 31 tokens, 2 * 63 chunk sums, n / 1024 sums of sums and the 2 * 31 additions inside
-those, so it is off by at most (DEPTH + n / 1024) 2^-24 times the sum of the magnitudes, plus the
+DEPTH = 2 * 31 tokens, 2 * 63 chunk sums, n / 256 sums of sums and the 2 * 31 additions inside
+those, so it is off by at most (DEPTH + n / 256) 2^-24 times the sum of the magnitudes, plus the
 rounding of the scale's product (2^-24) and of the result.
 """
 import pytest
@@ -34,7 +34,7 @@ def grad64(ids, dout, rows, scale, padding=None):
 
 def check_grad(got, ids, dout, scale=1.0, padding=None):
     want, mag, n = grad64(ids, dout, got.shape[0], scale, padding)
-    tol = (DEPTH + n / 1024 + 1) * 2.0 ** -24 * mag + (half_step(got.dtype) + 2.0 ** -24) * want.abs()
+    tol = (DEPTH + n / 256 + 1) * 2.0 ** -24 * mag + (half_step(got.dtype) + 2.0 ** -24) * want.abs()
     tol += torch.finfo(got.dtype).smallest_normal * torch.finfo(got.dtype).eps
     bad = (got.double() - want).abs() > tol
     assert not bad.any(), (int(bad.sum()), bad.nonzero()[:5].tolist())

@@ -535,7 +535,8 @@ constexpr int kEmbedTile = 1024;         // keys of a sorting workgroup's step
 constexpr int64_t kEmbedMaxBlocks = 256;
 constexpr int64_t kEmbedMaxIndex = 0x7ffffffe;  // tokens and rows: 32-bit keys and positions
 // Neighbours of the sorted list whose sum is formed beforehand when they share an id.
-constexpr int kEmbedChunk = 32;
+constexpr int kEmbedChunk = 16;
+constexpr int64_t kEmbedFillBytes = 4096;  // cleared by one workgroup
 
 struct EmbedSort {
   int passes, bits;  // keys 0 .. V (V: no row) fit passes * bits bits
@@ -602,22 +603,6 @@ TS_HOST_DEVICE inline EmbedRun embed_run(int64_t s, int64_t e) {
     r.c1 = c1;
   }
   return r;
-}
-
-// Rows of the gradient: each workgroup takes `rows` groups of `slots` neighbouring rows, `groups`
-// apart. Few rows for a small vocabulary (8 workgroups a CU first), more for a large one.
-constexpr int kEmbedMaxRows = 128;  // rows of a workgroup
-struct EmbedRows {
-  int64_t groups;
-  int rows;
-};
-inline EmbedRows embed_rows(int64_t V, int slots) {
-  const int64_t all = (V + slots - 1) / slots;
-  int64_t rows = all / (256 * 8);
-  const int64_t most = kEmbedMaxRows / slots < 16 ? kEmbedMaxRows / slots : 16;
-  if (rows > most) rows = most;
-  if (rows < 1) rows = 1;
-  return EmbedRows{(all + rows - 1) / rows, (int)rows};
 }
 
 // Lanes that own a row of `parts` vectors in the forward.
