@@ -36,7 +36,7 @@ using namespace ts;
 template <typename T>
 __device__ inline u32x4 load_raw(const T* __restrict__ row, int v, int nvec, int tail) {
   constexpr int V = Elt<T>::kVec;
-  if (v < nvec) return ld16_any_stream(row + (int64_t)v * V);
+  if (v < nvec) return ld16_any(row + (int64_t)v * V);
   float f[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) f[i] = v == nvec && i < tail ? Elt<T>::load1(row + (int64_t)v * V + i) : 0.f;
@@ -132,7 +132,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void sandwich_fwd(
   constexpr int kBlock = TPR > 256 ? TPR : 256;
   __shared__ float red[2][1][kBlock / kWave];
   const int t = threadIdx.x % TPR;
-  const int64_t row = (int64_t)blockIdx.x * (kBlock / TPR) + threadIdx.x / TPR;
+  const int64_t row =
+      (int64_t)blockIdx.x * (kBlock / TPR) + __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);
   const bool valid = row < s.rows;
   const int64_t r = valid ? row : 0;
   u32x4 yq[KV], xq[KV];
@@ -204,43 +205,86 @@ __global__ __launch_bounds__(TPR > 512 ? TPR : 512) void sandwich_bwd(
   constexpr int kRpb = kBlock / TPR;
   __shared__ float red[2][3][kBlock / kWave];
   __shared__ float4 slots[kRpb > 1 ? kBlock * KV * V / 4 : 1];
-  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  const int t = threadIdx.x % TPR;
+  const int sub = __builtin_amdgcn_readfirstlane(threadIdx.x / TPR);  // a wave's: rows in SGPRs
   const int64_t group = blockIdx.x / per_group, p = blockIdx.x % per_group;
   const int64_t row0 = group * s.group_rows;
   const int64_t row1 = row0 + s.group_rows < s.rows ? row0 + s.group_rows : s.rows;
 
-  // u0 = g (o + post) and o + pre of this thread's columns
-  float u0[KV][V], wq[KV][V], acc_a[KV][V], acc_b[KV][V];
+  // u0 = g (o + post) and o + pre of this thread's columns, in registers, or in LDS where a thread
+  // has several vectors (the widest rows; registers would spill)
+  constexpr bool kHold = KV == 1;
+  __shared__ float4 pars[kHold ? 1 : 2 * KV * V / 4 * TPR];
+  float u0[V], wq[V], acc_a[KV][V], acc_b[KV][V];
 #pragma unroll
   for (int k = 0; k < KV; ++k) {
     float g[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) g[i] = 1.f;
-    load_param<T>(post, 0, s.cols, t + k * TPR, s.nvec, s.tail, u0[k]);
-    load_param<T>(pre, 0, s.cols, t + k * TPR, s.nvec, s.tail, wq[k]);
+    load_param<T>(post, 0, s.cols, t + k * TPR, s.nvec, s.tail, u0);
+    load_param<T>(pre, 0, s.cols, t + k * TPR, s.nvec, s.tail, wq);
     if (gate.p != nullptr) load_param<T>(gate, group, s.cols, t + k * TPR, s.nvec, s.tail, g);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      u0[k][i] = (u0[k][i] + s.offset) * g[i];
-      wq[k][i] += s.offset;
+      u0[i] = (u0[i] + s.offset) * g[i];
+      wq[i] += s.offset;
       acc_a[k][i] = acc_b[k][i] = 0.f;
     }
+    if constexpr (!kHold) {
+#pragma unroll
+      for (int q = 0; q < V / 4; ++q) {
+        pars[(2 * (k * (V / 4) + q)) * TPR + t] =
+            make_float4(u0[4 * q], u0[4 * q + 1], u0[4 * q + 2], u0[4 * q + 3]);
+        pars[(2 * (k * (V / 4) + q) + 1) * TPR + t] =
+            make_float4(wq[4 * q], wq[4 * q + 1], wq[4 * q + 2], wq[4 * q + 3]);
+      }
+    }
   }
-  for (int64_t st = 0; st < steps; ++st) {  // uniform over the workgroup
-    const int64_t at = row0 + (p + st * per_group) * kRpb + sub;
-    const bool valid = at < row1;
-    const int64_t r = valid ? at : row0;
-    u32x4 yq[KV], xq[KV], nq[KV], hq[KV];
+  auto params_of = [&](int k) {  // the thread's own entries: no barrier
+    if constexpr (!kHold) {
+#pragma unroll
+      for (int q = 0; q < V / 4; ++q) {
+        const float4 a = pars[(2 * (k * (V / 4) + q)) * TPR + t];
+        const float4 b = pars[(2 * (k * (V / 4) + q) + 1) * TPR + t];
+        u0[4 * q] = a.x, u0[4 * q + 1] = a.y, u0[4 * q + 2] = a.z, u0[4 * q + 3] = a.w;
+        wq[4 * q] = b.x, wq[4 * q + 1] = b.y, wq[4 * q + 2] = b.z, wq[4 * q + 3] = b.w;
+      }
+    }
+  };
+  u32x4 yn[KV], xn[KV], nn[KV], hn[KV];  // the next step's row
+  float ryn, rhn;
+  auto row_of = [&](int64_t st) { return row0 + (p + st * per_group) * kRpb + sub; };
+  auto issue = [&](int64_t st) {
+    const int64_t at = row_of(st), r = at < row1 ? at : row0;
     const u32x4 zero = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int k = 0; k < KV; ++k) {
       const int v = t + k * TPR;
-      yq[k] = load_raw(y.p + r * y.ld, v, s.nvec, s.tail);
-      xq[k] = load_raw(x.p + r * x.ld, v, s.nvec, s.tail);
-      nq[k] = dn.p != nullptr ? load_raw(dn.p + r * dn.ld, v, s.nvec, s.tail) : zero;
-      hq[k] = dh.p != nullptr ? load_raw(dh.p + r * dh.ld, v, s.nvec, s.tail) : zero;
+      yn[k] = load_raw(y.p + r * y.ld, v, s.nvec, s.tail);
+      xn[k] = load_raw(x.p + r * x.ld, v, s.nvec, s.tail);
+      nn[k] = dn.p != nullptr ? load_raw(dn.p + r * dn.ld, v, s.nvec, s.tail) : zero;
+      hn[k] = dh.p != nullptr ? load_raw(dh.p + r * dh.ld, v, s.nvec, s.tail) : zero;
     }
-    const float ry = ry_in[r], rh = rh_in[r];
+    ryn = ry_in[r];
+    rhn = rh_in[r];
+  };
+  // a row ahead where the registers allow it and two workgroups share a CU ([8192, 4096] bf16:
+  // 72.5 -> 69 us; workgroups of 1024 threads lose by it, 76 -> 82 us at [4095, 8192])
+  constexpr bool kAhead = KV == 1 && TPR <= 512;
+  if (kAhead) issue(0);
+  for (int64_t st = 0; st < steps; ++st) {  // uniform over the workgroup
+    const int64_t r = row_of(st);
+    const bool valid = r < row1;
+    if (!kAhead) issue(st);
+    u32x4 yq[KV], xq[KV], nq[KV], hq[KV];
+#pragma unroll
+    for (int k = 0; k < KV; ++k) {
+      yq[k] = yn[k];
+      xq[k] = xn[k];
+      nq[k] = nn[k];
+      hq[k] = hn[k];
+    }
+    const float ry = ryn, rh = rhn;
     float sum[3] = {0.f, 0.f, 0.f};  // e hhat, (dh + rh e) u, hhat u
 #pragma unroll
     for (int k = 0; k < KV; ++k) {
@@ -249,17 +293,19 @@ __global__ __launch_bounds__(TPR > 512 ? TPR : 512) void sandwich_bwd(
       Elt<T>::unpack(xq[k], xf);
       Elt<T>::unpack(nq[k], nf);
       Elt<T>::unpack(hq[k], df);
+      params_of(k);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float u = (yf[i] * ry) * u0[k][i];
+        const float u = (yf[i] * ry) * u0[i];
         const float hh = __builtin_fmaf(xf[i], s.scale, u) * rh;
-        const float e = nf[i] * wq[k][i];
+        const float e = nf[i] * wq[i];
         sum[0] = __builtin_fmaf(e, hh, sum[0]);
         sum[1] = __builtin_fmaf(__builtin_fmaf(rh, e, df[i]), u, sum[1]);
         sum[2] = __builtin_fmaf(hh, u, sum[2]);
       }
     }
     row_sums<TPR, kBlock>(sum, red[st & 1]);
+    if (kAhead) issue(st + 1);  // in flight while this row is finished (a row past the group: its first)
     const float c1 = sum[0] / s.fcols;
     const float c2 = (sum[1] - (rh * c1) * sum[2]) / s.fcols;
     // the vectors are unpacked again below: carried across the reduction as floats they would
@@ -275,15 +321,16 @@ __global__ __launch_bounds__(TPR > 512 ? TPR : 512) void sandwich_bwd(
         Elt<T>::unpack(xq[k], xf);
         Elt<T>::unpack(nq[k], nf);
         Elt<T>::unpack(hq[k], df);
+        params_of(k);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
           const float yh = yf[i] * ry;
-          const float hh = __builtin_fmaf(xf[i], s.scale, yh * u0[k][i]) * rh;
-          const float tt = df[i] + rh * (nf[i] * wq[k][i] - hh * c1);
+          const float hh = __builtin_fmaf(xf[i], s.scale, yh * u0[i]) * rh;
+          const float tt = df[i] + rh * (nf[i] * wq[i] - hh * c1);
           acc_a[k][i] = __builtin_fmaf(tt, yh, acc_a[k][i]);
           acc_b[k][i] = __builtin_fmaf(nf[i], hh, acc_b[k][i]);
           xf[i] = s.scale * tt;
-          yf[i] = ry * (tt * u0[k][i] - yh * c2);
+          yf[i] = ry * (tt * u0[i] - yh * c2);
         }
         if (dx.p != nullptr) store_part(dx.p + r * dx.ld, t + k * TPR, s.nvec, s.tail, xf);
         if (dy.p != nullptr) store_part(dy.p + r * dy.ld, t + k * TPR, s.nvec, s.tail, yf);
@@ -339,17 +386,19 @@ __global__ __launch_bounds__(TPR > 512 ? TPR : 512) void sandwich_bwd(
 // ---------------------------------------------------------------------------
 // Gradients of the parameters from the partial rows
 // ---------------------------------------------------------------------------
-constexpr int kCols = 16;  // columns of a workgroup: 4 quads by 64 row groups
+// Columns of a workgroup: 8 quads (128 bytes of a row) by 32 row groups.
+constexpr int kCols = 32;
+constexpr int kQuads = kCols / 4, kGroups = 256 / kQuads;
 static_assert(ts_plan::kSandwichReduceCols == kCols, "columns of a reducing workgroup");
 
 // Sum over rows i < nrows of the quad at rows + i * stride + c, in a fixed order; valid in the
-// first 4 threads (g == 0), one for each quad.
+// first kQuads threads (g == 0), one for each quad.
 __device__ inline float4 sum_rows(const float* __restrict__ rows, int64_t stride, int64_t nrows,
-                                  int64_t c, bool in, float4 (*red)[4]) {
-  const int cq = threadIdx.x & 3, g = threadIdx.x >> 2;
+                                  int64_t c, bool in, float4 (*red)[kQuads]) {
+  const int cq = threadIdx.x % kQuads, g = threadIdx.x / kQuads;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
   if (in) {
-    for (int64_t i = g; i < nrows; i += 64) {
+    for (int64_t i = g; i < nrows; i += kGroups) {
       const float4 v = *reinterpret_cast<const float4*>(rows + i * stride + c);
       a.x += v.x;
       a.y += v.y;
@@ -360,7 +409,7 @@ __device__ inline float4 sum_rows(const float* __restrict__ rows, int64_t stride
   red[g][cq] = a;
   __syncthreads();
 #pragma unroll
-  for (int h = 32; h >= 1; h >>= 1) {
+  for (int h = kGroups / 2; h >= 1; h >>= 1) {
     if (g < h) {
       const float4 o = red[g + h][cq];
       float4 m = red[g][cq];
@@ -398,14 +447,14 @@ __global__ __launch_bounds__(256) void sandwich_params(const float* __restrict__
                                                        void* dpre, void* dgate, int post_f32,
                                                        int pre_f32, int gate_f32,
                                                        float* __restrict__ mid) {
-  __shared__ float4 red[64][4];
+  __shared__ float4 red[kGroups][kQuads];
   const int64_t blocks_x = (ldp + kCols - 1) / kCols;
   const int64_t group = blockIdx.x / blocks_x / 2;
   const int which = (int)(blockIdx.x / blocks_x & 1);
-  const int64_t c = blockIdx.x % blocks_x * kCols + (threadIdx.x & 3) * 4;
+  const int64_t c = blockIdx.x % blocks_x * kCols + (threadIdx.x % kQuads) * 4;
   const float4 a = sum_rows(partial + (group * per_group * 2 + which) * ldp, 2 * ldp, per_group, c,
                             c < ldp, red);
-  if (threadIdx.x >= 4) return;
+  if (threadIdx.x >= kQuads) return;
   const float f[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -433,11 +482,11 @@ __global__ __launch_bounds__(256) void sandwich_params_groups(const float* __res
                                                               int64_t ldp, int64_t groups,
                                                               int cols, void* dpost, void* dpre,
                                                               int post_f32, int pre_f32) {
-  __shared__ float4 red[64][4];
-  const int64_t c = (int64_t)blockIdx.x * kCols + (threadIdx.x & 3) * 4;
+  __shared__ float4 red[kGroups][kQuads];
+  const int64_t c = (int64_t)blockIdx.x * kCols + (threadIdx.x % kQuads) * 4;
   const float4 a = sum_rows(mid + blockIdx.y * ldp, 2 * ldp, groups, c, c < ldp, red);
   void* out = blockIdx.y ? dpre : dpost;
-  if (threadIdx.x >= 4 || out == nullptr) return;
+  if (threadIdx.x >= kQuads || out == nullptr) return;
   const float f[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i)
