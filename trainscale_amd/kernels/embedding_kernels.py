@@ -17,6 +17,7 @@ from typing import Optional
 import torch
 import torch.nn as nn
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -61,6 +62,7 @@ class ScaledEmbeddingFunction(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout: Tensor):
         if not ctx.needs_input_grad[1]:
             return None, None, None, None

@@ -32,6 +32,7 @@ from typing import Optional, Tuple
 import torch
 import torch.nn as nn
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -217,8 +218,8 @@ def _sandwich_forward(X, residual, post_weight, pre_weight, gate, eps, residual_
     x2d, ldx = ops.as_rows(residual)
     post, pre = post_weight.contiguous(), pre_weight.contiguous()
     n, h, rstd = ops.sandwich_norm_forward(y2d, ldy, x2d, ldx, post, pre, g2d, residual_scale,
-                                           weight_offset, eps)
-    return n.view(X.shape), h.view(X.shape), (y2d, x2d, post, pre, g2d, rstd), (ldy, ldx)
+                                           weight_offset, eps, X.shape)
+    return n, h, (y2d, x2d, post, pre, g2d, rstd), (ldy, ldx)
 
 
 class FusedSandwichRMSNormFunction(torch.autograd.Function):
@@ -238,6 +239,7 @@ class FusedSandwichRMSNormFunction(torch.autograd.Function):
         return n, h
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dn: Optional[Tensor], dh: Optional[Tensor]):
         if dn is None and dh is None:
             return (None,) * 8
@@ -250,11 +252,9 @@ class FusedSandwichRMSNormFunction(torch.autograd.Function):
                                             (shape, shape, post.shape, pre.shape, gate_shape))],
                     None, None, None)
         (dn, lddn), (dh, lddh) = [(None, 0) if d is None else ops.as_rows(d) for d in (dn, dh)]
-        dy, dx, dpost, dpre, dgate = ops.sandwich_norm_backward(
+        return (*ops.sandwich_norm_backward(
             dn, lddn, dh, lddh, y2d, ldy, x2d, ldx, post, pre, g2d, rstd, residual_scale,
-            weight_offset, ctx.needs_input_grad[:5])
-        return (None if dy is None else dy.view(shape), None if dx is None else dx.view(shape),
-                dpost, dpre, None if dgate is None else dgate.view(gate_shape), None, None, None)
+            weight_offset, ctx.needs_input_grad, shape, gate_shape), None, None, None)
 
 
 def fused_sandwich_rms_layernorm(X: Tensor, residual: Tensor, post_weight: Tensor,

@@ -21,6 +21,7 @@ from typing import NamedTuple, Optional
 import torch
 import torch.nn as nn
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from .. import _lib, ops
 
@@ -106,6 +107,7 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
         return loss, policy, kl, clipped
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dloss: Optional[Tensor], *_unused):
         if dloss is None or not ctx.needs_input_grad[0]:
             return (None,) * 9

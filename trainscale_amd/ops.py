@@ -27,6 +27,8 @@ ROUND_TWICE = 1
 def as_rows(t: Tensor) -> Tuple[Tensor, int]:
     """[..., C] -> (2-D view or copy with unit column stride, row stride)."""
     c = t.shape[-1]
+    if c > 0 and t.is_contiguous():
+        return (t if t.dim() == 2 else t.view(-1, c)), c
     t2 = t.reshape(-1, c)
     if c > 1 and t2.stride(1) != 1:
         t2 = t2.contiguous()
@@ -150,53 +152,65 @@ def _check_sandwich(y2d, x2d, post, pre, gate):
 
 def sandwich_norm_forward(y2d: Tensor, ldy: int, x2d: Tensor, ldx: int, post: Tensor, pre: Tensor,
                           gate: Optional[Tensor], residual_scale: float, weight_offset: float,
-                          eps: float) -> Tuple[Tensor, Tensor, Tensor]:
-    """Returns (n, h, rstd [2, rows] of y and of h); parameters contiguous, gate None or
-    [groups, cols]."""
+                          eps: float, shape=None) -> Tuple[Tensor, Tensor, Tensor]:
+    """Returns (n, h, rstd [2, rows] of y and of h), n and h of `shape` (y2d's); parameters
+    contiguous, gate None or [groups, cols]."""
     dev, w_code, g_code = _check_sandwich(y2d, x2d, post, pre, gate)
     rows, cols = y2d.shape
-    n = torch.empty((rows, cols), dtype=y2d.dtype, device=dev)
-    h = torch.empty((rows, cols), dtype=y2d.dtype, device=dev)
+    n = torch.empty(shape or y2d.shape, dtype=y2d.dtype, device=dev)
+    h = torch.empty(shape or y2d.shape, dtype=y2d.dtype, device=dev)
     rstd = torch.empty((2, rows), dtype=torch.float32, device=dev)
     if rows == 0:
         return n, h, rstd
+    ry = rstd.data_ptr()
     with _lib.on_device(dev):
         check(_lib.load().ts_sandwich_norm_fwd(
-            y2d.data_ptr(), ldy, x2d.data_ptr(), ldx, _lib.dtype_code(y2d, "sandwich_norm"),
-            post.data_ptr(), pre.data_ptr(), w_code, ptr(gate), g_code,
-            1 if gate is None else gate.shape[0], n.data_ptr(), cols, h.data_ptr(), cols,
-            rstd.data_ptr(), rstd.data_ptr() + 4 * rows, rows, cols, residual_scale,
-            weight_offset, eps, _lib.stream_handle(dev)), "ts_sandwich_norm_fwd")
+            y2d.data_ptr(), ldy, x2d.data_ptr(), ldx, _lib.DTYPE_CODE[y2d.dtype],
+            post.data_ptr(), pre.data_ptr(), w_code, 0 if gate is None else gate.data_ptr(), g_code,
+            1 if gate is None else gate.shape[0], n.data_ptr(), cols, h.data_ptr(), cols, ry,
+            ry + 4 * rows, rows, cols, residual_scale, weight_offset, eps,
+            _lib.stream_handle(dev)), "ts_sandwich_norm_fwd")
     return n, h, rstd
 
 
 def sandwich_norm_backward(dn: Optional[Tensor], lddn: int, dh: Optional[Tensor], lddh: int,
                            y2d: Tensor, ldy: int, x2d: Tensor, ldx: int, post: Tensor,
-                           pre: Tensor, gate: Optional[Tensor], rstd: Tensor, residual_scale: float,
-                           weight_offset: float,
-                           needs: Tuple[bool, bool, bool, bool, bool]):
-    """Gradients of (y, x, post, pre, gate), None where `needs` is false."""
-    dev, w_code, g_code = _check_sandwich(y2d, x2d, post, pre, gate)
+                           pre: Tensor, gate: Optional[Tensor], rstd: Tensor,
+                           residual_scale: float, weight_offset: float,
+                           needs: Tuple[bool, bool, bool, bool, bool], shape=None,
+                           gate_shape=None) -> list:
+    """Gradients of (y, x, post, pre, gate), None where `needs` is false, of the shapes given
+    (else those of the arguments). The other arguments are the forward's."""
     rows, cols = y2d.shape
     for name, d in (("n", dn), ("h", dh)):
         if d is not None and (d.shape != y2d.shape or d.dtype != y2d.dtype):
             raise ValueError(f"sandwich_norm: gradient of {name} is {tuple(d.shape)} {d.dtype}")
-    groups = 1 if gate is None else gate.shape[0]
-    like = (y2d, x2d, post, pre, gate)
-    out = [torch.empty(t.shape, dtype=t.dtype, device=dev) if need and t is not None else None
-           for t, need in zip(like, needs)]
+    dev = _lib.require_gpu("sandwich_norm", dn, dh, y2d)
+    code = _lib.DTYPE_CODE
+    shape = shape or y2d.shape
+    out = [torch.empty(shape, dtype=y2d.dtype, device=dev) if needs[0] else None,
+           torch.empty(shape, dtype=y2d.dtype, device=dev) if needs[1] else None,
+           torch.empty(cols, dtype=post.dtype, device=dev) if needs[2] else None,
+           torch.empty(cols, dtype=pre.dtype, device=dev) if needs[3] else None, None]
+    groups, g_code, g_ptr = 1, 0, 0
+    if gate is not None:
+        groups, g_code, g_ptr = gate.shape[0], code[gate.dtype], gate.data_ptr()
+        if needs[4]:
+            out[4] = torch.empty(gate_shape or gate.shape, dtype=gate.dtype, device=dev)
     lib = _lib.load()
     ws, wsb = None, 0
-    if any(o is not None for o in out[2:]):
-        wsb = int(lib.ts_sandwich_norm_bwd_workspace_size(rows, cols, groups))
-        ws = torch.empty((wsb,), dtype=torch.uint8, device=dev)
+    if needs[2] or needs[3] or out[4] is not None:
+        wsb = lib.ts_sandwich_norm_bwd_workspace_size(rows, cols, groups)
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    at = [0 if t is None else t.data_ptr() for t in (dn, dh, *out, ws)]
+    ry = rstd.data_ptr()
     with _lib.on_device(dev):
         check(lib.ts_sandwich_norm_bwd(
-            ptr(dn), lddn, ptr(dh), lddh, ptr(y2d), ldy, ptr(x2d), ldx,
-            _lib.dtype_code(y2d, "sandwich_norm"), ptr(post), ptr(pre), w_code, ptr(gate), g_code,
-            groups, rstd.data_ptr(), rstd.data_ptr() + 4 * rows, ptr(out[0]), cols, ptr(out[1]), cols, ptr(out[2]),
-            ptr(out[3]), ptr(out[4]), rows, cols, residual_scale, weight_offset, ptr(ws), wsb,
-            _lib.stream_handle(dev)), "ts_sandwich_norm_bwd")
+            at[0], lddn, at[1], lddh, y2d.data_ptr(), ldy, x2d.data_ptr(), ldx, code[y2d.dtype],
+            post.data_ptr(), pre.data_ptr(), code[post.dtype], g_ptr, g_code, groups, ry,
+            ry + 4 * rows, at[2], cols, at[3], cols, at[4], at[5], at[6], rows, cols,
+            residual_scale, weight_offset, at[7], wsb, _lib.stream_handle(dev)),
+            "ts_sandwich_norm_bwd")
     return out
 
 

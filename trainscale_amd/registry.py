@@ -26,11 +26,12 @@ import torch.nn as nn
 
 import sys
 
+from .kernels.embedding_kernels import scaled_embedding
 from .kernels.fused_kernels import fast_rms_layernorm, swiglu_forward
 from .kernels.rope_kernels import RoPEConfig, RoPEScalingType, hf_apply_rotary_pos_emb
 
 __all__ = ["LAYER_PATCHES", "NORMS_WITH_OTHER_MATH", "register_layer_patch", "auto_patch_layernorm", "auto_patch_mlp",
-           "auto_patch_rope", "KernelPatcher", "patch_model"]
+           "auto_patch_rope", "auto_patch_embedding", "KernelPatcher", "patch_model"]
 
 LAYER_PATCHES: Dict[str, Callable[[nn.Module], None]] = {}
 
@@ -163,6 +164,25 @@ for _name in ("LlamaRotaryEmbedding", "LlamaLinearScalingRotaryEmbedding",
     register_layer_patch(_name, auto_patch_rope)
 
 
+def auto_patch_embedding(module: nn.Module) -> None:
+    """Routes an ``nn.Embedding`` through ``scaled_embedding``: the same rows, and a dense gradient
+    summed in fp32 in a fixed order. Modules that renormalise, weight the gradient by frequency
+    or ask for a sparse one keep their own forward."""
+    if module.max_norm is not None or module.scale_grad_by_freq or module.sparse:
+        return
+    original_forward = module.forward
+
+    def patched_forward(input):
+        weight = module.weight
+        if (not isinstance(input, torch.Tensor) or not input.is_cuda or not weight.is_cuda
+                or weight.dtype not in (torch.float32, torch.bfloat16, torch.float16)):
+            return original_forward(input)
+        return scaled_embedding(input, weight, padding_idx=module.padding_idx)
+
+    module.forward = patched_forward
+    module._trainscale_amd_patched = True
+
+
 class KernelPatcher:
     """Applies the registered layer patches to a model (registry/__init__.py:1331-1418).
 
@@ -170,12 +190,15 @@ class KernelPatcher:
     compatibility; this layer registers no attention or FP8 patches, so they
     select nothing. ``skip_inexact_norms`` (not in the reference) leaves the
     classes of NORMS_WITH_OTHER_MATH unpatched; by default they are patched, as
-    the reference patches them.
+    the reference patches them. ``patch_embedding`` (not in the reference, off by
+    default) patches modules of class ``nn.Embedding`` itself.
     """
 
     def __init__(self, patch_layernorm: bool = True, patch_mlp: bool = True,
                  patch_attention: bool = True, patch_rope: bool = True, patch_fp8: bool = False,
-                 verbose: bool = False, skip_inexact_norms: bool = False):
+                 verbose: bool = False, skip_inexact_norms: bool = False,
+                 patch_embedding: bool = False):
+        self.patch_embedding = patch_embedding
         self.skip_inexact_norms = skip_inexact_norms
         self.patch_layernorm = patch_layernorm
         self.patch_mlp = patch_mlp
@@ -189,6 +212,8 @@ class KernelPatcher:
         for name, module in model.named_modules():
             cls = module.__class__.__name__
             fn = LAYER_PATCHES.get(cls)
+            if fn is None and self.patch_embedding and type(module) is nn.Embedding:
+                fn = auto_patch_embedding
             if fn is None or getattr(module, "_trainscale_amd_patched", False):
                 continue
             if cls.endswith(("RMSNorm", "LayerNorm")):
