@@ -11,7 +11,7 @@
 // id, stably, so the tokens of every gradient row are one run of the sorted list: its sum is
 // formed and written once, without atomics on floats, in an order that depends on the ids alone.
 // The sort is a radix sort of (id, position) pairs by digits of up to 10 bits: ids below 2^20
-// take two passes (a histogram and a scatter each), up to kEmbedSmallTokens tokens one launch in
+// take two passes (a histogram and a scatter each); few tokens are sorted by one workgroup in
 // LDS. Padding and out-of-range ids get the key V, behind all rows.
 //
 // Most rows of a large vocabulary have no token. The whole gradient is cleared by a plain fill,
@@ -156,12 +156,12 @@ __device__ inline int block_exclusive(int v, int* lds) {
 
 // Ranks the wave's keys among equal digits of the wave, in their order: rank[r] for key r * 64 +
 // lane; cnt[digit] (the wave's own, cleared) ends as the digit's count.
-__device__ inline void wave_ranks(const uint32_t (&digit)[kKeysPerLane],
-                                  const bool (&valid)[kKeysPerLane], int bits, volatile int* cnt,
-                                  int (&rank)[kKeysPerLane]) {
+template <int kKeys>
+__device__ inline void wave_ranks(const uint32_t (&digit)[kKeys], const bool (&valid)[kKeys],
+                                  int bits, volatile int* cnt, int (&rank)[kKeys]) {
   const int lane = threadIdx.x & (kWave - 1);
 #pragma unroll
-  for (int r = 0; r < kKeysPerLane; ++r) {
+  for (int r = 0; r < kKeys; ++r) {
     const uint64_t m = same_digit(digit[r], bits, valid[r]);
     const int below = __popcll(m & ((1ull << lane) - 1));
     const int prev = valid[r] ? cnt[digit[r]] : 0;
@@ -172,9 +172,10 @@ __device__ inline void wave_ranks(const uint32_t (&digit)[kKeysPerLane],
   }
 }
 
-// Whole sort in one workgroup: N <= kSmallTokens.
-constexpr int kSmallThreads = 512;
-static_assert(ts_plan::kEmbedSmallTokens == kSmallThreads / kWave * kWaveKeys, "keys of a workgroup");
+// Whole sort in one workgroup, N <= kEmbedSmallTokens: the keys stay in registers, a pass moves
+// them through LDS.
+constexpr int kSmallThreads = 1024;
+constexpr int kSmallKeys = ts_plan::kEmbedSmallTokens / kSmallThreads;  // of a lane
 
 __global__ __launch_bounds__(kSmallThreads) void sort_small(const int64_t* __restrict__ ids, int N,
                                                             int64_t V, int64_t padding, int bits,
@@ -184,60 +185,63 @@ __global__ __launch_bounds__(kSmallThreads) void sort_small(const int64_t* __res
   __shared__ int cnt[kWaves][kMaxBins];
   __shared__ uint2 held[ts_plan::kEmbedSmallTokens];
   __shared__ int scan[kWaves];
+  static_assert(kMaxBins <= kSmallThreads, "a bin a thread");
   const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
   const int bins = 1 << bits;
-  constexpr int kPer = kMaxBins / kSmallThreads;  // bins of a thread
-  uint32_t key[kKeysPerLane], val[kKeysPerLane];
-  bool valid[kKeysPerLane];
+  // wave w holds keys [w * mine, (w + 1) * mine), 64 neighbours at a time: all waves have some
+  const int steps = (N + kSmallThreads - 1) / kSmallThreads;
+  uint32_t key[kSmallKeys], val[kSmallKeys];
+  bool valid[kSmallKeys];
+  auto index = [&](int r) { return (wid * steps + r) * kWave + lane; };
 #pragma unroll
-  for (int r = 0; r < kKeysPerLane; ++r) {
-    const int i = wid * kWaveKeys + r * kWave + lane;
-    valid[r] = i < N;
+  for (int r = 0; r < kSmallKeys; ++r) {
+    const int i = index(r);
+    valid[r] = r < steps && i < N;
     key[r] = valid[r] ? key_of(ids[i], V, padding) : 0;
     val[r] = (uint32_t)i;
   }
   for (int p = 0; p < passes; ++p) {
-    for (int i = threadIdx.x; i < kWaves * kMaxBins; i += kSmallThreads) (&cnt[0][0])[i] = 0;
-    __syncthreads();
-    uint32_t digit[kKeysPerLane];
-    int rank[kKeysPerLane];
 #pragma unroll
-    for (int r = 0; r < kKeysPerLane; ++r) digit[r] = (key[r] >> (p * bits)) & (uint32_t)(bins - 1);
+    for (int w = 0; w < kWaves; ++w)
+      if ((int)threadIdx.x < bins) cnt[w][threadIdx.x] = 0;
+    __syncthreads();
+    uint32_t digit[kSmallKeys];
+    int rank[kSmallKeys];
+#pragma unroll
+    for (int r = 0; r < kSmallKeys; ++r) digit[r] = (key[r] >> (p * bits)) & (uint32_t)(bins - 1);
     wave_ranks(digit, valid, bits, cnt[wid], rank);
     __syncthreads();
-    int mine = 0;
+    int c[kWaves], sum = 0;  // this thread's bin in every wave
 #pragma unroll
-    for (int k = 0; k < kPer; ++k)
-      for (int w = 0; w < kWaves; ++w) mine += cnt[w][threadIdx.x * kPer + k];
-    int at = block_exclusive<kSmallThreads>(mine, scan);
+    for (int w = 0; w < kWaves; ++w) {
+      c[w] = (int)threadIdx.x < bins ? cnt[w][threadIdx.x] : 0;
+      sum += c[w];
+    }
+    int at = block_exclusive<kSmallThreads>(sum, scan);
 #pragma unroll
-    for (int k = 0; k < kPer; ++k)
-      for (int w = 0; w < kWaves; ++w) {
-        const int c = cnt[w][threadIdx.x * kPer + k];
-        cnt[w][threadIdx.x * kPer + k] = at;
-        at += c;
-      }
+    for (int w = 0; w < kWaves; ++w) {
+      if ((int)threadIdx.x < bins) cnt[w][threadIdx.x] = at;
+      at += c[w];
+    }
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kKeysPerLane; ++r)
+    for (int r = 0; r < kSmallKeys; ++r)
       if (valid[r]) held[cnt[wid][digit[r]] + rank[r]] = make_uint2(key[r], val[r]);
     __syncthreads();
 #pragma unroll
-    for (int r = 0; r < kKeysPerLane; ++r) {
-      const int i = wid * kWaveKeys + r * kWave + lane;
+    for (int r = 0; r < kSmallKeys; ++r) {
       if (valid[r]) {
-        const uint2 kv = held[i];
+        const uint2 kv = held[index(r)];
         key[r] = kv.x;
         val[r] = kv.y;
       }
     }
   }
 #pragma unroll
-  for (int r = 0; r < kKeysPerLane; ++r) {
-    const int i = wid * kWaveKeys + r * kWave + lane;
+  for (int r = 0; r < kSmallKeys; ++r) {
     if (valid[r]) {
-      keys[i] = key[r];
-      vals[i] = val[r];
+      keys[index(r)] = key[r];
+      vals[index(r)] = val[r];
     }
   }
 }
