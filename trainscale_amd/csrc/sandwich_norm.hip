@@ -251,89 +251,68 @@ __global__ __launch_bounds__(TPR > 512 ? TPR : 512) void sandwich_bwd(
       }
     }
   };
-  u32x4 yn[KV], xn[KV], nn[KV], hn[KV];  // the next step's row
-  float ryn, rhn;
-  auto row_of = [&](int64_t st) { return row0 + (p + st * per_group) * kRpb + sub; };
-  auto issue = [&](int64_t st) {
-    const int64_t at = row_of(st), r = at < row1 ? at : row0;
+  for (int64_t st = 0; st < steps; ++st) {  // uniform over the workgroup
+    const int64_t at = row0 + (p + st * per_group) * kRpb + sub;
+    const bool valid = at < row1;
+    const int64_t r = valid ? at : row0;  // (past the group: its first row, for nothing)
+    u32x4 yq[KV], xq[KV], nq[KV], hq[KV];
     const u32x4 zero = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int k = 0; k < KV; ++k) {
       const int v = t + k * TPR;
-      yn[k] = load_raw(y.p + r * y.ld, v, s.nvec, s.tail);
-      xn[k] = load_raw(x.p + r * x.ld, v, s.nvec, s.tail);
-      nn[k] = dn.p != nullptr ? load_raw(dn.p + r * dn.ld, v, s.nvec, s.tail) : zero;
-      hn[k] = dh.p != nullptr ? load_raw(dh.p + r * dh.ld, v, s.nvec, s.tail) : zero;
+      yq[k] = load_raw(y.p + r * y.ld, v, s.nvec, s.tail);
+      xq[k] = load_raw(x.p + r * x.ld, v, s.nvec, s.tail);
+      nq[k] = dn.p != nullptr ? load_raw(dn.p + r * dn.ld, v, s.nvec, s.tail) : zero;
+      hq[k] = dh.p != nullptr ? load_raw(dh.p + r * dh.ld, v, s.nvec, s.tail) : zero;
     }
-    ryn = ry_in[r];
-    rhn = rh_in[r];
-  };
-  // a row ahead where the registers allow it and two workgroups share a CU ([8192, 4096] bf16:
-  // 72.5 -> 69 us; workgroups of 1024 threads lose by it, 76 -> 82 us at [4095, 8192])
-  constexpr bool kAhead = KV == 1 && TPR <= 512;
-  if (kAhead) issue(0);
-  for (int64_t st = 0; st < steps; ++st) {  // uniform over the workgroup
-    const int64_t r = row_of(st);
-    const bool valid = r < row1;
-    if (!kAhead) issue(st);
-    u32x4 yq[KV], xq[KV], nq[KV], hq[KV];
-#pragma unroll
-    for (int k = 0; k < KV; ++k) {
-      yq[k] = yn[k];
-      xq[k] = xn[k];
-      nq[k] = nn[k];
-      hq[k] = hn[k];
-    }
-    const float ry = ryn, rh = rhn;
+    const float ry = ry_in[r], rh = rh_in[r];
     float sum[3] = {0.f, 0.f, 0.f};  // e hhat, (dh + rh e) u, hhat u
+    // what the outputs need of the row, unpacked and scaled once: with each vector unpacked again
+    // after the reduction (fewer registers) the kernel issued 48 operations an element, 41 of its
+    // 70 us at [8192, 4096] bf16. Loading a row ahead does not help: 68 us against 66.
+    float yh[KV][V], hh[KV][V], d[KV][V];  // yhat, hhat, dh + rh e
 #pragma unroll
     for (int k = 0; k < KV; ++k) {
-      float yf[V], xf[V], nf[V], df[V];
-      Elt<T>::unpack(yq[k], yf);
+      float xf[V], nf[V];
+      Elt<T>::unpack(yq[k], yh[k]);
       Elt<T>::unpack(xq[k], xf);
       Elt<T>::unpack(nq[k], nf);
-      Elt<T>::unpack(hq[k], df);
+      Elt<T>::unpack(hq[k], d[k]);
       params_of(k);
 #pragma unroll
       for (int i = 0; i < V; ++i) {
-        const float u = (yf[i] * ry) * u0[i];
-        const float hh = __builtin_fmaf(xf[i], s.scale, u) * rh;
+        yh[k][i] *= ry;
+        const float u = yh[k][i] * u0[i];
+        hh[k][i] = __builtin_fmaf(xf[i], s.scale, u) * rh;
         const float e = nf[i] * wq[i];
-        sum[0] = __builtin_fmaf(e, hh, sum[0]);
-        sum[1] = __builtin_fmaf(__builtin_fmaf(rh, e, df[i]), u, sum[1]);
-        sum[2] = __builtin_fmaf(hh, u, sum[2]);
+        d[k][i] = __builtin_fmaf(rh, e, d[k][i]);
+        sum[0] = __builtin_fmaf(e, hh[k][i], sum[0]);
+        sum[1] = __builtin_fmaf(d[k][i], u, sum[1]);
+        sum[2] = __builtin_fmaf(hh[k][i], u, sum[2]);
+      }
+      if (valid) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc_b[k][i] = __builtin_fmaf(nf[i], hh[k][i], acc_b[k][i]);
       }
     }
     row_sums<TPR, kBlock>(sum, red[st & 1]);
-    if (kAhead) issue(st + 1);  // in flight while this row is finished (a row past the group: its first)
     const float c1 = sum[0] / s.fcols;
     const float c2 = (sum[1] - (rh * c1) * sum[2]) / s.fcols;
-    // the vectors are unpacked again below: carried across the reduction as floats they would
-    // take twice the registers
-#pragma unroll
-    for (int k = 0; k < KV; ++k)
-      asm volatile("" : "+v"(yq[k]), "+v"(xq[k]), "+v"(nq[k]), "+v"(hq[k]));
+    const float rc1 = rh * c1, rc2 = ry * c2;
     if (valid) {
 #pragma unroll
       for (int k = 0; k < KV; ++k) {
-        float yf[V], xf[V], nf[V], df[V];
-        Elt<T>::unpack(yq[k], yf);
-        Elt<T>::unpack(xq[k], xf);
-        Elt<T>::unpack(nq[k], nf);
-        Elt<T>::unpack(hq[k], df);
         params_of(k);
+        float o[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          const float yh = yf[i] * ry;
-          const float hh = __builtin_fmaf(xf[i], s.scale, yh * u0[i]) * rh;
-          const float tt = df[i] + rh * (nf[i] * wq[i] - hh * c1);
-          acc_a[k][i] = __builtin_fmaf(tt, yh, acc_a[k][i]);
-          acc_b[k][i] = __builtin_fmaf(nf[i], hh, acc_b[k][i]);
-          xf[i] = s.scale * tt;
-          yf[i] = ry * (tt * u0[i] - yh * c2);
+          d[k][i] = __builtin_fmaf(-hh[k][i], rc1, d[k][i]);  // t
+          acc_a[k][i] = __builtin_fmaf(d[k][i], yh[k][i], acc_a[k][i]);
+          o[i] = __builtin_fmaf(d[k][i] * u0[i], ry, -(yh[k][i] * rc2));
+          d[k][i] *= s.scale;
         }
-        if (dx.p != nullptr) store_part(dx.p + r * dx.ld, t + k * TPR, s.nvec, s.tail, xf);
-        if (dy.p != nullptr) store_part(dy.p + r * dy.ld, t + k * TPR, s.nvec, s.tail, yf);
+        if (dx.p != nullptr) store_part(dx.p + r * dx.ld, t + k * TPR, s.nvec, s.tail, d[k]);
+        if (dy.p != nullptr) store_part(dy.p + r * dy.ld, t + k * TPR, s.nvec, s.tail, o);
       }
     }
   }
