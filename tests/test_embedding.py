@@ -64,6 +64,8 @@ def test_python_refusals():
         scaled_embedding(ids, w)
     with pytest.raises(ValueError, match="weight must be"):
         scaled_embedding(ids, w[0])
+    with pytest.raises(ValueError, match="weight must be"):
+        scaled_embedding(ids, w[:, :0])
     with pytest.raises(TypeError, match="ids must be"):
         scaled_embedding(ids.float(), w)
     with pytest.raises(TypeError, match="ids must be"):

@@ -84,6 +84,10 @@ def test_forward_shapes_and_ids(gpu):
     assert same(scaled_embedding(ids, wide[:, 3:99]), wide[ids, 3:99])  # strided, unaligned rows
     assert same(scaled_embedding(ids, wide.t()[:, :50].contiguous().t()), wide[ids, :200])
     assert scaled_embedding(ids[:0], w).shape == (0, 96)
+    assert same(scaled_embedding(ids[3], w), w[ids[3]])  # one id without a dimension
+    wr = w.clone().requires_grad_()
+    (g,) = torch.autograd.grad(scaled_embedding(ids[3], wr), wr, w[1])
+    assert same(g[ids[3]], w[1]) and int(g.any(1).sum()) == 1
     bad = torch.tensor([-1, 50, 3, 1 << 40, -(1 << 40)], device=gpu)
     out = scaled_embedding(bad, w)
     assert bool(out[[0, 1, 3, 4]].isnan().all()) and same(out[2], w[3])

@@ -483,8 +483,11 @@ __global__ __launch_bounds__(kThreads) void embed_runs(
   constexpr int VE = Elt<T>::kVec;
   const int64_t i = (int64_t)(blockIdx.x / slices) * (kThreads / TPR) + threadIdx.x / TPR;
   if (i >= N) return;
-  const int v = (int)(blockIdx.x % slices) * TPR + threadIdx.x % TPR;
-  const bool mine = v < nvec + (tail > 0);
+  const int part = (int)(blockIdx.x % slices) * TPR + threadIdx.x % TPR;
+  const bool mine = part < nvec + (tail > 0);
+  // lanes behind the row's end read its first part for nothing: the wave stays whole where lanes
+  // read one another's tokens
+  const int v = mine ? part : 0;
   float acc[VE] = {};
   uint32_t key;
   int64_t e;
@@ -499,10 +502,9 @@ __global__ __launch_bounds__(kThreads) void embed_runs(
     e = other != 0 ? i - 1 + __builtin_ctzll(other) : run_end(keys, N, i + kWave - 1, key);
     if (ts_plan::embed_run(i, e).t0 == e && other != 0) {  // no whole chunk: these tokens alone
       const int n = (int)(e - i);
-      if (mine)
-        add_tokens<2>(dout, ldd,
-                      [=](int64_t a) { return (uint32_t)__builtin_amdgcn_readlane(t, (int)a + 1); },
-                      0, n, v, nvec, tail, acc);
+      add_tokens<2>(dout, ldd,
+                    [=](int64_t a) { return (uint32_t)__builtin_amdgcn_readlane(t, (int)a + 1); },
+                    0, n, v, nvec, tail, acc);
       done = true;
     }
   } else {
@@ -510,7 +512,6 @@ __global__ __launch_bounds__(kThreads) void embed_runs(
     if (key == none || (i > 0 && keys[i - 1] == key)) return;
     e = run_end(keys, N, i + 1, key);
   }
-  if (!mine) return;
   if (!done) {
     const ts_plan::EmbedRun run = ts_plan::embed_run(i, e);
     const auto token = [=](int64_t a) { return vals[a]; };
@@ -522,7 +523,7 @@ __global__ __launch_bounds__(kThreads) void embed_runs(
   }
 #pragma unroll
   for (int k = 0; k < VE; ++k) acc[k] *= scale;
-  store_part(grad + (int64_t)key * ((int64_t)nvec * VE + tail), v, nvec, tail, acc);
+  if (mine) store_part(grad + (int64_t)key * ((int64_t)nvec * VE + tail), v, nvec, tail, acc);
 }
 
 // ---------------------------------------------------------------------------

@@ -26,7 +26,7 @@ __all__ = ["ScaledEmbeddingFunction", "scaled_embedding", "ScaledEmbedding"]
 
 def _forward(input_ids: Tensor, weight: Tensor, scale: float, padding_idx: Optional[int]):
     """(result, contiguous int64 ids, padding row or -1), after the checks of the arguments."""
-    if weight.dim() != 2:
+    if weight.dim() != 2 or weight.shape[1] == 0:
         raise ValueError(f"scaled_embedding: weight must be [V, H], got {tuple(weight.shape)}")
     if input_ids.dtype is not torch.int64:
         if input_ids.dtype is not torch.int32:

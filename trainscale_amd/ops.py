@@ -28,7 +28,7 @@ def as_rows(t: Tensor) -> Tuple[Tensor, int]:
     """[..., C] -> (2-D view or copy with unit column stride, row stride)."""
     c = t.shape[-1]
     if c > 0 and t.is_contiguous():
-        return (t if t.dim() == 2 else t.view(-1, c)), c
+        return t.view(-1, c), c
     t2 = t.reshape(-1, c)
     if c > 1 and t2.stride(1) != 1:
         t2 = t2.contiguous()
