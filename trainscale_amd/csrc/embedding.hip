@@ -19,7 +19,8 @@
 // tokens of 128256 x 4096 bf16 took 249 us with one kernel over all rows (each looked up in the
 // sorted list, then zeroed or summed: the few sums hold up the stores behind them). The fill
 // waits for nothing and the sort occupies a few workgroups, so every launch of the sort carries
-// a share of the fill as further workgroups.
+// a share of the fill as further workgroups: 161 us in all for that gradient (6.5 TB/s), the sort
+// within it, then 33 to 48 us for the rows with tokens.
 //
 // Token frequencies are far from uniform (a frequent token, or one filler token in most places,
 // would leave one workgroup with thousands of rows), so runs are cut: wherever kEmbedChunk

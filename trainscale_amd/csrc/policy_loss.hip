@@ -6,8 +6,10 @@
 // weight: 1 / valid tokens ("token"), 1 / (valid tokens of the sequence * sequences that have
 // any) ("sequence"), or 1 ("sum").
 //
-// A token costs 13 to 17 bytes of reading in each direction and some 60 operations: memory-bound
-// for large batches, and bound by launches and host time for the usual ones. So: one pass over
+// A token costs up to 17 bytes of reading in each direction and some 60 operations: bound by
+// arithmetic and memory alike for large batches (512 x 8192 fp32 tokens: 24 us for the sums, 10
+// to join them, 15 for the backward, where the bytes alone take 8 and 11), and by launches and
+// host time for the usual ones (4 x 500 tokens: 10 and 5 us). So: one pass over
 // the tokens and one workgroup that joins its partial sums (up to kSmallUnits units: both in one
 // launch), one launch backward. A wave owns a unit of kUnit tokens of one row and reduces
 // without LDS or barrier; rows of few tokens and few rows of many tokens both spread over the
@@ -17,8 +19,8 @@
 //
 // Numerics: log ratios are differences in double (the inputs' difference is exact there), and a
 // token is clipped where d lies beyond log(1 + high) or log(1 - low), compared in double: no
-// rounding of exp decides it. exp(x) - x - 1 cancels near 0: a power series there. Sums in
-// double, in a fixed order.
+// rounding of exp decides it. The sums' terms are formed and added in double, in a fixed order;
+// the gradient's in fp32.
 #include <math.h>
 
 #include "common.hpp"
@@ -56,8 +58,8 @@ struct Args {
   int64_t ldm;
   int64_t rows, tokens, units_per_row, units;
   double log_high, log_low;  // log(1 + high), log(1 - low)
-  float high, low;           // 1 + high, 1 - low
-  float kl_coef;
+  double high, low;          // 1 + high, 1 - low
+  double kl_coef;
 };
 
 typedef uint32_t u32x2_any __attribute__((ext_vector_type(2), aligned(2)));
@@ -126,10 +128,58 @@ __device__ inline void load_tokens(const Args& a, int64_t row, int64_t i, int n,
   }
 }
 
-// exp(x) to about 1.5 units in the last place: 2^(x log2 e) with the product's rounding error put
-// back (the hardware's 2^p is good to one). Results below 2^-126 are 0.
+// A token's clip test, in double: beyond log(1 + high) or log(1 - low).
+__device__ inline bool is_clipped(const Args& a, double d, float adv) {
+  return (adv > 0.f && d > a.log_high) || (adv < 0.f && d < a.log_low);
+}
+
+// Forward: the terms of the sums in double. The policy's terms have either sign and nearly cancel
+// where the advantages are centred, so fp32's rounding of each would show in the loss (2e-6 of it
+// at 512 x 8192 tokens).
+//
+// exp(x) = 2^k exp(r), r = x - k ln 2: exp(r) - 1 - r = r^2 (1/2! + r/3! + ... + r^8/10!) for
+// |r| <= ln 2 / 2, whose next term is below 2^-41 of exp(r) - 1 - r. `rise2` is exp(x) - 1 - x,
+// which near 0 (k = 0) is that series itself, without cancellation.
+__device__ inline double exp_f64(double x, double& rise2) {
+  const double c = x < -800. ? -800. : x > 800. ? 800. : x;  // a NaN stays one
+  const double k = __builtin_rint(c * 1.4426950408889634);
+  double r = __builtin_fma(-k, 0.6931471805599453, c);
+  r = __builtin_fma(-k, 2.3190468138462996e-17, r);
+  double s = 1. / 3628800.;
+  s = __builtin_fma(s, r, 1. / 362880.);
+  s = __builtin_fma(s, r, 1. / 40320.);
+  s = __builtin_fma(s, r, 1. / 5040.);
+  s = __builtin_fma(s, r, 1. / 720.);
+  s = __builtin_fma(s, r, 1. / 120.);
+  s = __builtin_fma(s, r, 1. / 24.);
+  s = __builtin_fma(s, r, 1. / 6.);
+  s = __builtin_fma(s, r, 0.5);
+  s *= r * r;
+  const double e = __builtin_ldexp(1. + (r + s), (int)k);
+  rise2 = k == 0. ? s : (e - 1.) - x;
+  return e;
+}
+
+struct Terms {
+  double policy, kl;
+  bool clipped;
+};
+__device__ inline Terms token_terms(const Args& a, float lp, float old, float ref, float adv) {
+  Terms t;
+  double rise2;
+  const double d = a.old.p != nullptr ? (double)lp - (double)old : 0.;
+  t.clipped = is_clipped(a, d, adv);
+  const double r = t.clipped ? (adv > 0.f ? a.high : a.low) : exp_f64(d, rise2);
+  t.policy = -(r * (double)adv);
+  t.kl = 0.;
+  if (a.ref.p != nullptr) exp_f64((double)ref - (double)lp, t.kl);
+  return t;
+}
+
+// Backward, in fp32: exp(x) to about 1.5 units in the last place, 2^(x log2 e) with the product's
+// rounding error put back (the hardware's 2^p is good to one). Results below 2^-126 are 0.
 constexpr float kLog2eLow = 1.925963033e-8f;  // log2 e - (float)log2 e
-__device__ inline float exp_f(float x) {
+__device__ inline float exp_f32(float x) {
   const float p = x * kLog2e;
   float low = __builtin_fmaf(x, kLog2eLow, __builtin_fmaf(x, kLog2e, -p));
   low = fabsf(p) < 1e4f ? low * kLn2 : 0.f;  // an infinity's error is no number
@@ -137,9 +187,9 @@ __device__ inline float exp_f(float x) {
   return __builtin_fmaf(e, low, e);
 }
 
-// exp(x) - x - 1. Below 1/2 the series x^2 (1/2! + x/3! + ... + x^7/9!), whose next term is
-// below 2^-29 of the sum; above, the difference loses at most two bits. rise: exp(x) - 1.
-__device__ inline float exp_rise(float x, float& rise) {
+// exp(x) - 1. Below 1/2 the series x + x^2/2! + ... + x^9/9!, whose next term is below 2^-29 of
+// the sum; above, the difference loses at most two bits.
+__device__ inline float expm1_f32(float x) {
   float s = 2.75573192e-6f;  // 1/9!
   s = __builtin_fmaf(s, x, 2.48015873e-5f);
   s = __builtin_fmaf(s, x, 1.98412698e-4f);
@@ -148,32 +198,16 @@ __device__ inline float exp_rise(float x, float& rise) {
   s = __builtin_fmaf(s, x, 4.16666667e-2f);
   s = __builtin_fmaf(s, x, 1.66666667e-1f);
   s = __builtin_fmaf(s, x, 0.5f);
-  const float em1 = exp_f(x) - 1.f;
-  const bool small = fabsf(x) < 0.5f;
-  const float k = small ? (x * x) * s : em1 - x;
-  rise = small ? x + k : em1;
-  return k;
+  return fabsf(x) < 0.5f ? __builtin_fmaf(x * x, s, x) : exp_f32(x) - 1.f;
 }
 
-struct Terms {
-  float policy, kl, grad;
-  bool clipped;
-};
-__device__ inline Terms token_terms(const Args& a, float lp, float old, float ref, float adv) {
-  Terms t;
+// d(policy + kl_coef kl) / d logp of a token.
+__device__ inline float token_grad(const Args& a, float lp, float old, float ref, float adv) {
   const double d = a.old.p != nullptr ? (double)lp - (double)old : 0.;
-  t.clipped = (adv > 0.f && d > a.log_high) || (adv < 0.f && d < a.log_low);
-  const float ra = exp_f((float)d) * adv;
-  t.policy = t.clipped ? -((adv > 0.f ? a.high : a.low) * adv) : -ra;
-  t.grad = t.clipped ? 0.f : -ra;
-  t.kl = 0.f;
-  if (a.ref.p != nullptr) {
-    const float x = (float)((double)ref - (double)lp);
-    float rise;
-    t.kl = exp_rise(x, rise);
-    if (a.kl_coef != 0.f) t.grad = __builtin_fmaf(-a.kl_coef, rise, t.grad);
-  }
-  return t;
+  float g = is_clipped(a, d, adv) ? 0.f : -(exp_f32((float)d) * adv);
+  if (a.kl_coef != 0.)
+    g = __builtin_fmaf(-(float)a.kl_coef, expm1_f32((float)((double)ref - (double)lp)), g);
+  return g;
 }
 
 __device__ inline double wave_sum_f64(double v) {
@@ -209,8 +243,8 @@ __device__ inline Unit unit_sums(const Args& a, int64_t u) {
     for (int j = 0; j < kPer; ++j) {
       if ((t[s].valid >> j) & 1) {
         const Terms e = token_terms(a, t[s].lp[j], t[s].old[j], t[s].ref[j], t[s].adv[j]);
-        sum.policy += (double)e.policy;
-        sum.kl += (double)e.kl;
+        sum.policy += e.policy;
+        sum.kl += e.kl;
         sum.clipped += e.clipped ? 1 : 0;
         ++sum.count;
       }
@@ -286,7 +320,7 @@ __device__ inline void join_units(const Unit* units, const Args& a, const Outs& 
     *o.policy = (float)(all[0] * scale);
     *o.kl = (float)(all[1] * scale);
     *o.clipped = (float)(all[2] * scale);
-    *o.loss = (float)((all[0] + (double)a.kl_coef * all[1]) * scale);
+    *o.loss = (float)((all[0] + a.kl_coef * all[1]) * scale);
   }
   if (sub == 0)
     for (int64_t row = row0; row < a.rows; row += step)  // the thread's own weights
@@ -343,7 +377,7 @@ __global__ __launch_bounds__(kThreads) void policy_bwd(Args a, const float* __re
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       if ((t[s].valid >> j) & 1)
-        g[j] = token_terms(a, t[s].lp[j], t[s].old[j], t[s].ref[j], t[s].adv[j]).grad * w;
+        g[j] = token_grad(a, t[s].lp[j], t[s].old[j], t[s].ref[j], t[s].adv[j]) * w;
     }
     T* out = grad + row * ldg + first + s * kWave * kPer;
     if (n[s] == kPer) {
@@ -423,9 +457,9 @@ ts_status make_args(const char* what, const ts_policy_inputs* in, Args* a) {
   a->ldm = in->ld_mask;
   a->log_high = log1p(in->clip_high);
   a->log_low = in->clip_low < 1. ? log1p(-in->clip_low) : -INFINITY;
-  a->high = (float)(1. + in->clip_high);
-  a->low = (float)(1. - in->clip_low);
-  a->kl_coef = (float)in->kl_coef;
+  a->high = 1. + in->clip_high;
+  a->low = 1. - in->clip_low;
+  a->kl_coef = in->kl_coef;
   return TS_OK;
 }
 
