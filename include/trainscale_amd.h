@@ -163,7 +163,7 @@ ts_status ts_rmsnorm_bwd_noalloc(const void* dy, int64_t lddy,
  * address. post, pre: [cols] of w_dtype (dtype or TS_F32). gate: NULL (g = 1, gate_groups 1) or
  * [gate_groups, cols] of gate_dtype (dtype or TS_F32), row r taking gate row
  * r / (rows / gate_groups); gate_groups divides rows. rstd_y, rstd_h: [rows] fp32, written (for
- * the backward). cols at most 32768 bytes of dtype.
+ * the backward). cols at most 32768 bytes of dtype. No output overlaps an input.
  */
 ts_status ts_sandwich_norm_fwd(const void* y, int64_t ldy, const void* x, int64_t ldx,
                                ts_dtype dtype, const void* post, const void* pre,
@@ -179,8 +179,8 @@ size_t ts_sandwich_norm_bwd_workspace_size(int64_t rows, int64_t cols, int64_t g
 /*
  * Gradients of the above from dn and dh (either may be NULL: zeros): dy and dx ([rows, cols]),
  * dpost and dpre ([cols] of w_dtype), dgate ([gate_groups, cols] of gate_dtype); each may be
- * NULL to skip it. y, x, the parameters and rstd are the forward's. The parameters' sums are
- * fp32 in a fixed order. Workspace: 16-byte aligned.
+ * NULL to skip it. y, x, the parameters and rstd are the forward's; no output overlaps an input.
+ * The parameters' sums are fp32 in a fixed order. Workspace: 16-byte aligned.
  */
 ts_status ts_sandwich_norm_bwd(
     const void* dn, int64_t lddn, const void* dh, int64_t lddh, const void* y, int64_t ldy,
@@ -632,12 +632,12 @@ ts_status ts_embedding_fwd(const int64_t* ids, int64_t N, const void* weight, in
                            ts_dtype dtype, int64_t V, int64_t H, float scale, void* out,
                            int64_t ldo, ts_stream_t stream);
 
-/* Bytes of workspace ts_embedding_bwd needs (0 for sizes it refuses): about 16 N + H N / 8. */
+/* Bytes of workspace ts_embedding_bwd needs (0 for sizes it refuses): about 16 N + H N / 3. */
 size_t ts_embedding_bwd_workspace_size(int64_t N, int64_t V, int64_t H);
 
 /*
  * grad_weight[v, :] = scale * sum over n with ids[n] = v of dout[n, :], for every v in [0, V)
- * (rows without a token are written as zeros): the tokens are sorted by id, each row is summed
+ * (rows without a token are zeros): the tokens are sorted by id, each row is summed
  * in fp32 in an order that the ids alone fix and rounded once. Tokens whose id is padding_idx
  * or outside [0, V) contribute nothing (a padding_idx outside [0, V): none).
  * dout: [N, H] of dtype, row stride ldd; grad_weight: [V, H] of dtype, contiguous. N and V at

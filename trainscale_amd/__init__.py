@@ -7,6 +7,14 @@ in ``libtrainscale_amd.so`` (C ABI: ``include/trainscale_amd.h``):
 * RoPE forward/backward incl. packed ``position_ids`` (``kernels.apply_rope*``)
 * vocabulary cross-entropy forward/backward (``kernels.fast_cross_entropy_loss``,
   ``loss.ChunkedCrossEntropyLoss``, ``loss.FusedCrossEntropyLoss``, ``loss.CrossEntropyLoss``)
+
+and, for what a policy-gradient step runs around the model:
+
+* token embedding with its dense gradient (``kernels.scaled_embedding``)
+* norms before and after a block with its gate and residual
+  (``kernels.fused_sandwich_rms_layernorm``)
+* the clipped policy loss with a KL term (``loss.clipped_policy_loss``)
+* the global gradient norm and clipping (``kernels.clip_grad_norm_``, ``kernels.clipped_grads``)
 """
 from . import _lib
 

@@ -539,7 +539,8 @@ ts_status fwd_typed(const int64_t* ids, int64_t N, const void* w, int64_t ldw, i
   const int tpr = ts_plan::embed_fwd_lanes(parts);
   const int slices = (parts + tpr - 1) / tpr;
   const int64_t per = kThreads / tpr, blocks = (N + per - 1) / per * slices;
-  if (blocks > 0x7fffffff) return ts_host::fail(TS_ERR_SHAPE, "embedding_fwd: too many tokens");
+  if (blocks > ts_plan::max_blocks(kThreads))
+    return ts_host::fail(TS_ERR_SHAPE, "embedding_fwd: too many tokens");
 #define TS_FWD(R)                                                                             \
   hipLaunchKernelGGL((embed_fwd<T, R>), dim3((unsigned)blocks), dim3(kThreads), 0, st, ids, N, \
                      static_cast<const T*>(w), ldw, V, nvec, tail, slices, scale, static_cast<T*>(out), \
@@ -636,7 +637,8 @@ ts_status bwd_shaped(const BwdArgs& a, hipStream_t st) {
   const int64_t grad_bytes = a.V * a.H * (int64_t)sizeof(T);
   const int64_t runs = (a.N + kSlots - 1) / kSlots * slices;
   const int64_t b1 = (c1 + kSlots - 1) / kSlots * slices, b2 = (c2 + kSlots - 1) / kSlots * slices;
-  if (runs > 0x7fffffff || grad_bytes / ts_plan::kEmbedFillBytes > 0x7fffff00)
+  if (runs > ts_plan::max_blocks(kThreads) ||
+      grad_bytes / ts_plan::kEmbedFillBytes > ts_plan::max_blocks(kThreads) - 1024)
     return ts_host::fail(TS_ERR_SHAPE, "embedding_bwd: tensor too large");
   const uint32_t *keys, *vals;
   const ts_status s = launch_sort(a, w, grad_bytes, &keys, &vals, st);

@@ -189,34 +189,35 @@ __global__ __launch_bounds__(kThreads) void grad_scale(Table tab, int count, int
   }
   const float coef = clip_coef(norm, max_norm);
   if (coef == 1.f && in_place) return;  // every gradient stays as it is
-  const int c = blockIdx.x;
-  const int t = find_tensor(tab, count, c);
-  if (coef == 1.f && tab.src[t] == tab.dst[t]) return;
-  const int64_t first = (int64_t)(c - (t ? tab.chunk_end[t - 1] : 0)) * kChunk;
-  const T* x = static_cast<const T*>(tab.src[t]) + first;
-  D* o = static_cast<D*>(tab.dst[t]) + first;
-  const int64_t left = tab.numel[t] - first;
-  const int n = (int)(left < kChunk ? left : kChunk);
-  const int nvec = n / V;
-  Piece<T, V> q[kScaleVecs];
+  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {  // one chunk, but for 64 GB and more
+    const int t = find_tensor(tab, count, c);
+    if (coef == 1.f && tab.src[t] == tab.dst[t]) continue;
+    const int64_t first = (int64_t)(c - (t ? tab.chunk_end[t - 1] : 0)) * kChunk;
+    const T* x = static_cast<const T*>(tab.src[t]) + first;
+    D* o = static_cast<D*>(tab.dst[t]) + first;
+    const int64_t left = tab.numel[t] - first;
+    const int n = (int)(left < kChunk ? left : kChunk);
+    const int nvec = n / V;
+    Piece<T, V> q[kScaleVecs];
 #pragma unroll
-  for (int k = 0; k < kScaleVecs; ++k) {
-    const int v = threadIdx.x + k * kThreads;
-    if (v < nvec) q[k].load(x + v * V);
-  }
-#pragma unroll
-  for (int k = 0; k < kScaleVecs; ++k) {
-    const int v = threadIdx.x + k * kThreads;
-    if (v < nvec) {
-      float f[V];
-      q[k].unpack(f);
-#pragma unroll
-      for (int j = 0; j < V; ++j) f[j] *= coef;
-      st16_any_stream(o + v * V, Elt<D>::pack(f));
+    for (int k = 0; k < kScaleVecs; ++k) {
+      const int v = threadIdx.x + k * kThreads;
+      if (v < nvec) q[k].load(x + v * V);
     }
+#pragma unroll
+    for (int k = 0; k < kScaleVecs; ++k) {
+      const int v = threadIdx.x + k * kThreads;
+      if (v < nvec) {
+        float f[V];
+        q[k].unpack(f);
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[j] *= coef;
+        st16_any_stream(o + v * V, Elt<D>::pack(f));
+      }
+    }
+    const int e = nvec * V + threadIdx.x;
+    if (e < n) Elt<D>::store1(o + e, Elt<T>::load1(x + e) * coef);
   }
-  const int e = nvec * V + threadIdx.x;
-  if (e < n) Elt<D>::store1(o + e, Elt<T>::load1(x + e) * coef);
 }
 
 // ---------------------------------------------------------------------------
@@ -332,7 +333,8 @@ ts_status launch_squares(const Lists& l, double* partial, int64_t capacity, int*
 ts_status launch_scale(const Lists& l, const double* partial, int nparts, const float* norm_in,
                        float* norm_out, float max_norm, hipStream_t st) {
   return for_groups(l, true, [&](const Table& tab, int n, int chunks, int32_t t, int32_t d) {
-    const dim3 grid((unsigned)chunks), block(kThreads);
+    const dim3 grid((unsigned)(chunks < ts_plan::kGradScaleGrid ? chunks : ts_plan::kGradScaleGrid)),
+        block(kThreads);
     int in_place = 1;
     for (int i = 0; i < n; ++i) in_place &= tab.src[i] == tab.dst[i];
 #define TS_SCALE(T, D)                                                                         \

@@ -492,6 +492,10 @@ TS_HOST_DEVICE inline RopeElems rope_elems(int j, int width, int half, bool inte
   return interleaved ? RopeElems{j * width, -1} : RopeElems{j * width, half + j * width};
 }
 
+// Most workgroups of `threads` threads that one launch takes: a dispatch counts its threads in 32
+// bits.
+TS_HOST_DEVICE constexpr int64_t max_blocks(int threads) { return 0xffffffffll / threads; }
+
 // ---------------------------------------------------------------------------
 // Global gradient norm and clipping (grad_norm.hip): the tensors of a launch are cut into
 // chunks of a workgroup's step, numbered through; chunk_end[t] is the number of
@@ -500,6 +504,7 @@ TS_HOST_DEVICE inline RopeElems rope_elems(int j, int width, int half, bool inte
 constexpr int kGradTensors = 128;  // tensors of one launch
 constexpr int kGradThreads = 256;
 constexpr int kGradGrid = 2048;    // most workgroups of a norm launch: 8 a CU
+constexpr int kGradScaleGrid = 1 << 23;  // most workgroups of a scaling launch
 constexpr int64_t kGradMaxChunks = 1ll << 30;
 
 // Elements of a chunk: `pieces` 16-byte vectors a thread of the type of `elt` bytes.

@@ -36,6 +36,7 @@ constexpr int kPer = 4;                              // neighbouring tokens of a
 constexpr int kUnit = ts_plan::kPolicyUnit;          // tokens of a wave
 constexpr int kSteps = kUnit / (kWave * kPer);
 constexpr int kSmallUnits = ts_plan::kPolicySmallUnits;
+constexpr int64_t kMaxUnits = ts_plan::max_blocks(kThreads) * (kThreads / kWave);
 static_assert(kSteps * kWave * kPer == kUnit, "a unit is whole steps");
 
 struct Unit {
@@ -429,7 +430,7 @@ ts_status make_args(const char* what, const ts_policy_inputs* in, Args* a) {
   a->rows = in->rows;
   a->tokens = in->tokens;
   a->units_per_row = (in->tokens + kUnit - 1) / kUnit;
-  if (in->tokens > 0x7fffffff || (in->rows > 0 && a->units_per_row > 0x7fffffff / in->rows))
+  if (in->tokens > 0x7fffffff || (in->rows > 0 && a->units_per_row > kMaxUnits / in->rows))
     return fail(TS_ERR_SHAPE, "%s: too many tokens", what);
   a->units = a->units_per_row * in->rows;
   if (a->units > 0) {
@@ -468,7 +469,7 @@ ts_status make_args(const char* what, const ts_policy_inputs* in, Args* a) {
 extern "C" size_t ts_policy_loss_workspace_size(int64_t rows, int64_t tokens) {
   if (rows <= 0 || tokens <= 0) return 0;
   const int64_t per = (tokens + kUnit - 1) / kUnit;
-  if (tokens > 0x7fffffff || per > 0x7fffffff / rows || per * rows <= kSmallUnits) return 0;
+  if (tokens > 0x7fffffff || per > kMaxUnits / rows || per * rows <= kSmallUnits) return 0;
   return (size_t)(per * rows) * sizeof(Unit);
 }
 

@@ -509,7 +509,8 @@ ts_status fwd_typed(const Call& c, void* n, int64_t ldn, void* h, int64_t ldh, f
   const Shape s = shape_of<T>(c);
   const ts_plan::SandwichPlan p = ts_plan::sandwich_fwd_plan(s.nvec + (s.tail > 0));
   const int64_t blocks = (c.rows + p.rpb - 1) / p.rpb;
-  if (blocks > 0x7fffffff) return ts_host::fail(TS_ERR_SHAPE, "sandwich_norm_fwd: too many rows");
+  if (blocks > ts_plan::max_blocks(p.tpr > 256 ? p.tpr : 256))
+    return ts_host::fail(TS_ERR_SHAPE, "sandwich_norm_fwd: too many rows");
   const Io<const T> y{static_cast<const T*>(c.y), c.ldy}, x{static_cast<const T*>(c.x), c.ldx};
   const Io<T> no{static_cast<T*>(n), ldn}, ho{static_cast<T*>(h), ldh};
 #define TS_FWD(R, K)                                                                              \
@@ -539,7 +540,8 @@ ts_status bwd_typed(const Call& c, const float* ry, const float* rh, void* dy, i
   const int64_t ldp = (int64_t)parts * Elt<T>::kVec;
   const int64_t blocks = c.groups * p.per_group;
   const int64_t reduce = (ldp + kCols - 1) / kCols * c.groups * 2;
-  if (blocks > 0x7fffffff || reduce > 0x7fffffff)
+  if (blocks > ts_plan::max_blocks(p.row.tpr > 512 ? p.row.tpr : 512) ||
+      reduce > ts_plan::max_blocks(256))
     return ts_host::fail(TS_ERR_SHAPE, "sandwich_norm_bwd: too many groups");
   const Io<const T> dn{static_cast<const T*>(c.dn), c.lddn}, dh{static_cast<const T*>(c.dh), c.lddh},
       y{static_cast<const T*>(c.y), c.ldy}, x{static_cast<const T*>(c.x), c.ldx};

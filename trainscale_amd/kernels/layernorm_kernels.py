@@ -270,7 +270,8 @@ def fused_sandwich_rms_layernorm(X: Tensor, residual: Tensor, post_weight: Tenso
     Returns (Y, residual_out): the next block's input and the stream. RMSNorm(x; w) is
     x * rstd * (weight_offset + w); weight_offset 1 is for weights kept as their difference from
     1. gate: None, [H], or X's leading dimensions followed by ones and H ([B, 1, H] for X
-    [B, S, H]: one gate for each sequence). fp32 arithmetic; Y comes from the unrounded sum and
+    [B, S, H]: one gate for each sequence; the backward holds four fp32 rows of H for each gate
+    row, so a gate for every token is possible but costly). fp32 arithmetic; Y comes from the unrounded sum and
     both results are rounded once. The weights share one dtype, X's or fp32; the gate has X's
     dtype or fp32. Differentiable in X, residual, both weights and the gate. H is at most 16384
     for 16-bit X, 8192 for fp32."""
