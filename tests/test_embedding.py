@@ -95,13 +95,13 @@ using namespace ts_plan;
 static int fails = 0;
 #define CHECK(c, ...) do { if (!(c)) { if (fails++ < 20) { std::printf(__VA_ARGS__); std::printf("\n"); } } } while (0)
 int main() {
-  for (long long N : {0ll, 1ll, 31ll, 32ll, 2048ll, 2049ll, 4096ll, 4097ll, 16384ll, 262144ll, 262145ll, 1000003ll, (long long)kEmbedMaxIndex})
+  for (long long N : {0ll, 1ll, 31ll, 32ll, 2048ll, 2049ll, 8192ll, 8193ll, 16384ll, 262144ll, 262145ll, 1000003ll, (long long)kEmbedMaxIndex})
     for (long long V : {1ll, 2ll, 1023ll, 1024ll, 50257ll, 128256ll, (1ll << 20) - 1, 1ll << 20, (long long)kEmbedMaxIndex}) {
       const EmbedSort p = embed_sort(N, V);
       CHECK(p.bits >= 1 && p.bits <= kEmbedMaxBits, "bits");
       CHECK(p.passes * p.bits >= 63 - __builtin_clzll(V) + 1, "keys 0 .. V do not fit");
       CHECK((p.passes - 1) * p.bits < 32, "shift");
-      CHECK((p.blocks == 0) == (N <= kEmbedSmallTokens), "one workgroup holds them");
+      CHECK((p.blocks == 0) == (N <= kEmbedSmallTokens), "placed by counting");
       if (p.blocks > 0) {
         CHECK(p.blocks >= 1 && p.blocks <= kEmbedMaxBlocks && p.len % kEmbedTile == 0, "blocks");
         CHECK(p.blocks * p.len >= N && (p.blocks - 1) * p.len < N, "blocks do not cover");
@@ -119,6 +119,14 @@ int main() {
         for (long long o : {w.vals[0], w.keys[1], w.vals[1], w.table, w.sums1, w.sums2})
           CHECK(o % 16 == 0, "alignment");
       }
+    }
+  // placing by counting: the groups share the whole list in eights, the last own keys fit
+  for (int groups : {8, 16, 32})
+    for (int N = 1; N <= kEmbedSmallTokens; ++N) {
+      const EmbedRanks r = embed_ranks(N, groups);
+      const int own = 256 / groups;
+      CHECK(r.len % 8 == 0 && r.len > 0 && r.padded == groups * r.len, "len");
+      CHECK(r.padded >= (N + own - 1) / own * own && r.padded <= kEmbedSmallTokens, "padding of %d", N);
     }
   // a run's pieces: every token once, whole chunks and whole chunks of chunks inside the run
   const long long C = kEmbedChunk;

@@ -97,7 +97,8 @@ BWD = [(1, 1, 1, "random"), (1, 5, 8, "random"), (31, 3, 64, "same"), (32, 3, 64
        (33, 40, 72, "few"), (64, 9, 130, "few"), (1024, 1000, 96, "skewed"),
        (2047, 13, 100, "few"), (2048, 2000, 40, "random"), (2049, 2000, 40, "random"),
        (2049, 6, 264, "same"), (5000, 30, 1000, "few"), (8191, 50257, 64, "skewed"),
-       (4096, 50257, 72, "random"), (4097, 3000, 72, "few"), (5000, 70000, 2048, "skewed"),
+       (8192, 50257, 72, "random"), (8193, 3000, 72, "few"),
+       (63, 30, 8, "few"), (65, 30, 8, "few"), (4097, 3000, 72, "few"), (8191, 1, 40, "same"), (5000, 70000, 2048, "skewed"),
        (6001, (1 << 20) + 5, 64, "random"), (16384, 3000, 520, "skewed"), (4500, 1 << 20, 8, "random"), (70000, 17, 9, "few"),
        (300001, 1025, 3, "skewed"), (300000, 2, 8, "same"), (4096, 4096, 2056, "sorted"),
        (2500, 300, 4097, "skewed")]

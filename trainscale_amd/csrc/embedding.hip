@@ -11,8 +11,8 @@
 // id, stably, so the tokens of every gradient row are one run of the sorted list: its sum is
 // formed and written once, without atomics on floats, in an order that depends on the ids alone.
 // The sort is a radix sort of (id, position) pairs by digits of up to 10 bits: ids below 2^20
-// take two passes (a histogram and a scatter each); few tokens are sorted by one workgroup in
-// LDS. Padding and out-of-range ids get the key V, behind all rows.
+// take two passes (a histogram and a scatter each). Up to kEmbedSmallTokens tokens are placed by
+// counting, in one launch. Padding and out-of-range ids get the key V, behind all rows.
 //
 // Most rows of a large vocabulary have no token. The whole gradient is cleared by a plain fill,
 // which runs at the card's write rate, and the rows with tokens are written over it: 16384
@@ -99,17 +99,13 @@ struct Fill {
   uint8_t* p;
   int64_t bytes;
 };
-constexpr int kFillVecs = ts_plan::kEmbedFillBytes / (16 * kThreads);
+constexpr int kFillBytes = 16 * kThreads;  // of a workgroup
 
-// Workgroup `block` of those that fill (kThreads threads).
+// Workgroup `block` of those that fill, a vector a thread: the fastest fill found (four vectors a
+// thread 5.8 TB/s, one 6.5; workgroups of 1024 threads 6.1).
 __device__ inline void fill_zero(const Fill& f, int64_t block) {
-  const int64_t at = block * ts_plan::kEmbedFillBytes;
-  const int64_t nvec = f.bytes / 16;
-#pragma unroll
-  for (int k = 0; k < kFillVecs; ++k) {
-    const int64_t v = at / 16 + k * kThreads + threadIdx.x;
-    if (v < nvec) st16_any_stream(f.p + v * 16, u32x4{0u, 0u, 0u, 0u});
-  }
+  const int64_t nvec = f.bytes / 16, v = block * kThreads + threadIdx.x;
+  if (v < nvec) st16_any_stream(f.p + v * 16, u32x4{0u, 0u, 0u, 0u});
   // the last bytes, in elements of two
   const int64_t e = nvec * 16 + threadIdx.x * 2;
   if (block == 0 && e < f.bytes) *reinterpret_cast<uint16_t*>(f.p + e) = 0;
@@ -157,12 +153,12 @@ __device__ inline int block_exclusive(int v, int* lds) {
 
 // Ranks the wave's keys among equal digits of the wave, in their order: rank[r] for key r * 64 +
 // lane; cnt[digit] (the wave's own, cleared) ends as the digit's count.
-template <int kKeys>
-__device__ inline void wave_ranks(const uint32_t (&digit)[kKeys], const bool (&valid)[kKeys],
-                                  int bits, volatile int* cnt, int (&rank)[kKeys]) {
+__device__ inline void wave_ranks(const uint32_t (&digit)[kKeysPerLane],
+                                  const bool (&valid)[kKeysPerLane], int bits, volatile int* cnt,
+                                  int (&rank)[kKeysPerLane]) {
   const int lane = threadIdx.x & (kWave - 1);
 #pragma unroll
-  for (int r = 0; r < kKeys; ++r) {
+  for (int r = 0; r < kKeysPerLane; ++r) {
     const uint64_t m = same_digit(digit[r], bits, valid[r]);
     const int below = __popcll(m & ((1ull << lane) - 1));
     const int prev = valid[r] ? cnt[digit[r]] : 0;
@@ -173,78 +169,51 @@ __device__ inline void wave_ranks(const uint32_t (&digit)[kKeys], const bool (&v
   }
 }
 
-// Whole sort in one workgroup, N <= kEmbedSmallTokens: the keys stay in registers, a pass moves
-// them through LDS.
-constexpr int kSmallThreads = 1024;
-constexpr int kSmallKeys = ts_plan::kEmbedSmallTokens / kSmallThreads;  // of a lane
+// Up to kEmbedSmallTokens tokens, one launch: a key's place is the number of smaller keys and of
+// equal ones before it. Workgroup b < blocks places the keys [b kRankKeys, (b + 1) kRankKeys): its
+// lanes form groups of kRankKeys, a key a lane, and the groups share the list, which each
+// workgroup holds in LDS, and add their counts up. 67 million comparisons for 8192 keys, two
+// operations each, beside the whole of the gradient's fill, which the other workgroups do. 16
+// keys a workgroup: with 32 the counting ends late (8192 tokens, 65 MB of gradient: 26 us with
+// 16, 35 with 32), with 8 too many workgroups load the list (33).
+constexpr int kRankKeys = 16;
+constexpr int kRankGroups = kThreads / kRankKeys;
 
-__global__ __launch_bounds__(kSmallThreads) void sort_small(const int64_t* __restrict__ ids, int N,
-                                                            int64_t V, int64_t padding, int bits,
-                                                            int passes, uint32_t* __restrict__ keys,
-                                                            uint32_t* __restrict__ vals) {
-  constexpr int kWaves = kSmallThreads / kWave;
-  __shared__ int cnt[kWaves][kMaxBins];
-  __shared__ uint2 held[ts_plan::kEmbedSmallTokens];
-  __shared__ int scan[kWaves];
-  static_assert(kMaxBins <= kSmallThreads, "a bin a thread");
-  const int lane = threadIdx.x & (kWave - 1), wid = threadIdx.x / kWave;
-  const int bins = 1 << bits;
-  // wave w holds keys [w * mine, (w + 1) * mine), 64 neighbours at a time: all waves have some
-  const int steps = (N + kSmallThreads - 1) / kSmallThreads;
-  uint32_t key[kSmallKeys], val[kSmallKeys];
-  bool valid[kSmallKeys];
-  auto index = [&](int r) { return (wid * steps + r) * kWave + lane; };
-#pragma unroll
-  for (int r = 0; r < kSmallKeys; ++r) {
-    const int i = index(r);
-    valid[r] = r < steps && i < N;
-    key[r] = valid[r] ? key_of(ids[i], V, padding) : 0;
-    val[r] = (uint32_t)i;
+__global__ __launch_bounds__(kThreads) void sort_ranks(const int64_t* __restrict__ ids, int N,
+                                                       int64_t V, int64_t padding,
+                                                       uint32_t* __restrict__ keys,
+                                                       uint32_t* __restrict__ vals, int blocks,
+                                                       Fill fill) {
+  extern __shared__ __attribute__((aligned(16))) uint32_t key[];  // the padded list
+  __shared__ int counts[kRankGroups][kRankKeys];
+  if ((int)blockIdx.x >= blocks) return fill_zero(fill, (int)blockIdx.x - blocks);
+  const ts_plan::EmbedRanks p = ts_plan::embed_ranks(N, kRankGroups);
+  // behind the list: no key is as large
+  for (int i = threadIdx.x; i < p.padded; i += kThreads)
+    key[i] = i < N ? key_of(ids[i], V, padding) : ~0u;
+  __syncthreads();
+  const int lane = threadIdx.x % kRankKeys, group = threadIdx.x / kRankKeys;
+  const int own = (int)blockIdx.x * kRankKeys, i = own + lane;
+  const uint32_t k = key[i];
+  int count = 0;
+  for (int j = group * p.len; j < (group + 1) * p.len; j += 8) {
+    // before the workgroup's own keys equal ones count (own and len: multiples of 8)
+    const uint32_t t = k + (j < own ? 1u : 0u);
+    const uint4 q = *reinterpret_cast<const uint4*>(key + j);
+    const uint4 r = *reinterpret_cast<const uint4*>(key + j + 4);
+    count += (q.x < t) + (q.y < t) + (q.z < t) + (q.w < t);
+    count += (r.x < t) + (r.y < t) + (r.z < t) + (r.w < t);
   }
-  for (int p = 0; p < passes; ++p) {
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w)
-      if ((int)threadIdx.x < bins) cnt[w][threadIdx.x] = 0;
-    __syncthreads();
-    uint32_t digit[kSmallKeys];
-    int rank[kSmallKeys];
-#pragma unroll
-    for (int r = 0; r < kSmallKeys; ++r) digit[r] = (key[r] >> (p * bits)) & (uint32_t)(bins - 1);
-    wave_ranks(digit, valid, bits, cnt[wid], rank);
-    __syncthreads();
-    int c[kWaves], sum = 0;  // this thread's bin in every wave
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      c[w] = (int)threadIdx.x < bins ? cnt[w][threadIdx.x] : 0;
-      sum += c[w];
-    }
-    int at = block_exclusive<kSmallThreads>(sum, scan);
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      if ((int)threadIdx.x < bins) cnt[w][threadIdx.x] = at;
-      at += c[w];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kSmallKeys; ++r)
-      if (valid[r]) held[cnt[wid][digit[r]] + rank[r]] = make_uint2(key[r], val[r]);
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < kSmallKeys; ++r) {
-      if (valid[r]) {
-        const uint2 kv = held[index(r)];
-        key[r] = kv.x;
-        val[r] = kv.y;
-      }
-    }
-  }
-#pragma unroll
-  for (int r = 0; r < kSmallKeys; ++r) {
-    if (valid[r]) {
-      keys[index(r)] = key[r];
-      vals[index(r)] = val[r];
-    }
-  }
+  counts[group][lane] = count;
+  __syncthreads();
+  if (group != 0 || i >= N) return;
+  int at = 0;
+#pragma unroll 4
+  for (int g = 0; g < kRankGroups; ++g) at += counts[g][lane];
+#pragma unroll 4
+  for (int j = 0; j < kRankKeys; ++j) at += j < lane && key[own + j] == k;
+  keys[at] = k;
+  vals[at] = (uint32_t)i;
 }
 
 // One pass over many workgroups: workgroup b < blocks owns keys [b * len, (b + 1) * len), those
@@ -566,18 +535,13 @@ struct BwdArgs {
 
 // The next of `left` shares of the gradient's fill.
 Fill next_fill(uint8_t** p, int64_t* bytes, int left) {
-  int64_t n = *bytes;
-  if (left > 1) {
-    n = n / left / ts_plan::kEmbedFillBytes * ts_plan::kEmbedFillBytes;
-  }
+  const int64_t n = left > 1 ? *bytes / left / kFillBytes * kFillBytes : *bytes;
   const Fill f{*p, n};
   *p += n;
   *bytes -= n;
   return f;
 }
-int64_t fill_blocks(const Fill& f) {
-  return (f.bytes + ts_plan::kEmbedFillBytes - 1) / ts_plan::kEmbedFillBytes;
-}
+int64_t fill_blocks(const Fill& f) { return (f.bytes + kFillBytes - 1) / kFillBytes; }
 
 // Clears the gradient and sorts the tokens; *keys and *vals are where the sorted pairs end up.
 ts_status launch_sort(const BwdArgs& a, const ts_plan::EmbedWorkspace& w, int64_t grad_bytes,
@@ -590,13 +554,19 @@ ts_status launch_sort(const BwdArgs& a, const ts_plan::EmbedWorkspace& w, int64_
   *keys = k[0];
   *vals = v[0];
   uint8_t* to_fill = static_cast<uint8_t*>(a.grad);
-  if (p.blocks == 0) {
+  if (a.N == 0) {
     const Fill f{to_fill, grad_bytes};
     hipLaunchKernelGGL(embed_fill, dim3((unsigned)fill_blocks(f)), dim3(kThreads), 0, st, f);
-    if (a.N > 0)
-      hipLaunchKernelGGL(sort_small, dim3(1), dim3(kSmallThreads), 0, st, a.ids, (int)a.N, a.V,
-                         a.padding, p.bits, p.passes, k[0], v[0]);
-    return ts_host::check_launch("sort_small");
+    return ts_host::check_launch("embed_fill");
+  }
+  if (p.blocks == 0) {
+    const Fill f{to_fill, grad_bytes};
+    const int list = ts_plan::embed_ranks((int)a.N, kRankGroups).padded;
+    const int ranks = (int)((a.N + kRankKeys - 1) / kRankKeys);
+    hipLaunchKernelGGL(sort_ranks, dim3((unsigned)(ranks + fill_blocks(f))),
+                       dim3(kThreads), 4 * (size_t)list, st, a.ids, (int)a.N, a.V, a.padding,
+                       k[0], v[0], ranks, f);
+    return ts_host::check_launch("sort_ranks");
   }
   int* table = reinterpret_cast<int*>(a.ws + w.table);
   const int blocks = (int)p.blocks;
@@ -638,7 +608,7 @@ ts_status bwd_shaped(const BwdArgs& a, hipStream_t st) {
   const int64_t runs = (a.N + kSlots - 1) / kSlots * slices;
   const int64_t b1 = (c1 + kSlots - 1) / kSlots * slices, b2 = (c2 + kSlots - 1) / kSlots * slices;
   if (runs > ts_plan::max_blocks(kThreads) ||
-      grad_bytes / ts_plan::kEmbedFillBytes > ts_plan::max_blocks(kThreads) - 1024)
+      grad_bytes / kFillBytes > ts_plan::max_blocks(kThreads) - 1024)
     return ts_host::fail(TS_ERR_SHAPE, "embedding_bwd: tensor too large");
   const uint32_t *keys, *vals;
   const ts_status s = launch_sort(a, w, grad_bytes, &keys, &vals, st);
