@@ -13,7 +13,7 @@ import math
 import pytest
 import torch
 
-from helpers import BF, F16, F32, Guarded, flat, same
+from helpers import BF, F16, F32, Guarded, flat, same, saved_elsewhere
 from trainscale_amd import _lib, ops
 from trainscale_amd.loss import (ClippedPolicyLoss, chunked_log_softmax, clipped_policy_loss,
                                  selective_log_softmax)
@@ -302,3 +302,34 @@ def test_on_the_layers_log_probs(gpu):
     lp2 = selective_log_softmax(logits, ids, out_dtype=F32)
     (gl,) = torch.autograd.grad(clipped_policy_loss(lp2, old, adv).loss, logits)
     assert gl.shape == logits.shape and bool(gl.any())
+
+
+@pytest.mark.parametrize("how", ["moved", "checkpoint"])
+def test_saved_tensors_elsewhere(gpu, how):
+    from torch.utils.checkpoint import checkpoint
+    args = inputs(gpu, 6, 777, F32)
+    lp, rest = args[0].detach(), args[1:]
+
+    def loss(x):
+        # every operand is formed here: only what is saved keeps it
+        old, adv, mask, ref = [t.clone() for t in rest]
+        return clipped_policy_loss(x * 1.5, old, adv, mask, ref, 0.2, 0.28, 0.04, "sequence").loss
+
+    def grad(call):
+        x = lp.clone().requires_grad_()
+        out = call(x)
+        # the allocator's free blocks of these sizes are used again
+        held = [torch.full_like(lp, float("nan")) for _ in range(8)]
+        (g,) = torch.autograd.grad(out, x)
+        del held
+        return g
+
+    want = grad(loss)
+    if how == "checkpoint":
+        got = grad(lambda x: checkpoint(loss, x, use_reentrant=False))
+    else:
+        def moved(x):
+            with saved_elsewhere():
+                return loss(x)
+        got = grad(moved)
+    assert torch.isfinite(want).all() and same(got, want)

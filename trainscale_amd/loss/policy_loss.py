@@ -99,9 +99,8 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
         dev = _lib.require_gpu("clipped_policy_loss", lp, old, adv, mask, ref)
         inputs = ops.policy_inputs(lp, old, adv, mask, ref, clip_low, clip_high, kl_coef, reduction)
         loss, policy, kl, clipped, weights = ops.policy_loss_forward(inputs, dev)
-        # the struct points into these tensors: it is valid as long as they are saved
         ctx.save_for_backward(lp, old, adv, mask, ref, weights)
-        ctx.inputs = inputs
+        ctx.cfg = (clip_low, clip_high, kl_coef, reduction)
         ctx.mark_non_differentiable(policy, kl, clipped)
         ctx.set_materialize_grads(False)
         return loss, policy, kl, clipped
@@ -111,9 +110,11 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
     def backward(ctx, dloss: Optional[Tensor], *_unused):
         if dloss is None or not ctx.needs_input_grad[0]:
             return (None,) * 9
-        # (raises if an input was changed in place since, or if the graph was freed)
-        lp, _, _, _, _, weights = ctx.saved_tensors
-        grad = ops.policy_loss_backward(ctx.inputs, weights, dloss, lp.dtype)
+        # hooks on saved tensors may give them back elsewhere, with other strides
+        *saved, weights = ctx.saved_tensors
+        lp, old, adv, mask, ref = [t if t is None or t.dim() == 1 else _rows(t) for t in saved]
+        inputs = ops.policy_inputs(lp, old, adv, mask, ref, *ctx.cfg)
+        grad = ops.policy_loss_backward(inputs, weights, dloss, lp.dtype)
         return (grad, *(None,) * 8)
 
 
