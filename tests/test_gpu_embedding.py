@@ -9,7 +9,7 @@ rounding of the scale's product (2^-24) and of the result.
 import pytest
 import torch
 
-from helpers import BF, F16, F32, Guarded, flat, same
+from helpers import BF, F16, F32, Guarded, flat, same, saved_elsewhere
 from trainscale_amd import _lib
 from trainscale_amd.kernels import ScaledEmbedding, scaled_embedding
 
@@ -220,3 +220,12 @@ def test_module_stream_and_graph(gpu):
         torch.cuda.synchronize()
         (g3,) = torch.autograd.grad(m(sids), m.weight, sd)
         assert same(g2, g3) and same(out, m(sids)), rep
+
+
+def test_saved_ids_elsewhere(gpu):
+    ids, w, d = inputs(gpu, 600, 50, 96, BF, "skewed")
+    w.requires_grad_()
+    want = torch.autograd.grad(scaled_embedding(ids.view(20, 30), w), w, d.view(20, 30, 96))[0]
+    with saved_elsewhere():
+        out = scaled_embedding(ids.view(20, 30).clone(), w)
+    assert same(want, torch.autograd.grad(out, w, d.view(20, 30, 96))[0])

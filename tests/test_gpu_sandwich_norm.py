@@ -10,10 +10,12 @@ row slots, 8 partial rows, 6 in the tree; more rows are counted), so it is off b
 K = 6 (66 + 35 k) + 60 + rows / 512 times u times the same quantity formed from magnitudes
 (every difference a sum). 16-bit results add half a step of their type.
 """
+import contextlib
+
 import pytest
 import torch
 
-from helpers import BF, F16, F32, Guarded, flat, same
+from helpers import BF, F16, F32, Guarded, flat, same, saved_elsewhere
 from trainscale_amd import _lib
 from trainscale_amd.kernels import (FusedSandwichRMSNorm, fused_add_rms_layernorm,
                                     fused_sandwich_rms_layernorm)
@@ -297,3 +299,19 @@ def test_stream_and_graph(gpu):
         assert all(same(p, q) for p, q in zip(outs, ref)), rep
         if rep == 0:
             assert all(same(p, q) for p, q in zip(first, ref))
+
+
+@pytest.mark.parametrize("width", [256, 263])
+def test_saved_tensors_elsewhere(gpu, width):
+    y, x, post, pre, gate, dn, dh = inputs(gpu, (4, 50, 256), BF, BF, "batch", BF, 0.0, 21)
+    base = [torch.cat([t, t[..., :width - 256]], -1) for t in (y, x)]  # rows of a wider buffer
+
+    def grads(hooks):
+        leaves = [t.detach().requires_grad_() for t in (*base, post, pre, gate)]
+        with hooks:
+            n, h = fused_sandwich_rms_layernorm(leaves[0][..., :256], leaves[1][..., :256],
+                                                *leaves[2:], EPS)
+        return torch.autograd.grad([n, h], leaves, [dn, dh])
+
+    want, got = grads(contextlib.nullcontext()), grads(saved_elsewhere())
+    assert all(same(a, b) for a, b in zip(want, got))

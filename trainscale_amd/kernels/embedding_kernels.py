@@ -66,7 +66,7 @@ class ScaledEmbeddingFunction(torch.autograd.Function):
     def backward(ctx, dout: Tensor):
         if not ctx.needs_input_grad[1]:
             return None, None, None, None
-        (ids,) = ctx.saved_tensors
+        ids = ctx.saved_tensors[0].contiguous()  # hooks may give it back with other strides
         rows, scale, padding_idx = ctx.cfg
         d2d, ldd = ops.as_rows(dout)
         return None, ops.embedding_backward(ids, d2d, ldd, rows, scale, padding_idx), None, None

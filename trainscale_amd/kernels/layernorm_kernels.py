@@ -209,7 +209,7 @@ def _gate_rows(gate: Tensor, X: Tensor) -> Tensor:
 
 def _sandwich_forward(X, residual, post_weight, pre_weight, gate, eps, residual_scale,
                       weight_offset):
-    """The results and what the backward needs of one call: (n, h, saved tensors, strides)."""
+    """The results and what the backward needs of one call: (n, h, saved tensors)."""
     if residual.shape != X.shape:
         raise ValueError(f"fused_sandwich_rms_layernorm: residual {tuple(residual.shape)} != "
                          f"X {tuple(X.shape)}")
@@ -219,7 +219,7 @@ def _sandwich_forward(X, residual, post_weight, pre_weight, gate, eps, residual_
     post, pre = post_weight.contiguous(), pre_weight.contiguous()
     n, h, rstd = ops.sandwich_norm_forward(y2d, ldy, x2d, ldx, post, pre, g2d, residual_scale,
                                            weight_offset, eps, X.shape)
-    return n, h, (y2d, x2d, post, pre, g2d, rstd), (ldy, ldx)
+    return n, h, (y2d, x2d, post, pre, g2d, rstd)
 
 
 class FusedSandwichRMSNormFunction(torch.autograd.Function):
@@ -230,11 +230,11 @@ class FusedSandwichRMSNormFunction(torch.autograd.Function):
     def forward(ctx, X: Tensor, residual: Tensor, post_weight: Tensor, pre_weight: Tensor,
                 gate: Optional[Tensor] = None, eps: float = DEFAULT_EPS_RMS,
                 residual_scale: float = 1.0, weight_offset: float = 0.0) -> Tuple[Tensor, Tensor]:
-        n, h, saved, ld = _sandwich_forward(X, residual, post_weight, pre_weight, gate, eps,
-                                            residual_scale, weight_offset)
+        n, h, saved = _sandwich_forward(X, residual, post_weight, pre_weight, gate, eps,
+                                        residual_scale, weight_offset)
         ctx.save_for_backward(*saved)
         ctx.set_materialize_grads(False)
-        ctx.cfg = (X.shape, ld, None if gate is None else gate.shape, residual_scale,
+        ctx.cfg = (X.shape, None if gate is None else gate.shape, residual_scale,
                    weight_offset)
         return n, h
 
@@ -244,13 +244,17 @@ class FusedSandwichRMSNormFunction(torch.autograd.Function):
         if dn is None and dh is None:
             return (None,) * 8
         y2d, x2d, post, pre, g2d, rstd = ctx.saved_tensors
-        shape, (ldy, ldx), gate_shape, residual_scale, weight_offset = ctx.cfg
+        shape, gate_shape, residual_scale, weight_offset = ctx.cfg
         if y2d.shape[0] == 0:
             return (*[None if t is None or not need else torch.zeros(s, dtype=t.dtype,
                                                                       device=t.device)
                       for t, need, s in zip((y2d, x2d, post, pre, g2d), ctx.needs_input_grad,
                                             (shape, shape, post.shape, pre.shape, gate_shape))],
                     None, None, None)
+        # hooks on saved tensors may give them back with other strides
+        (y2d, ldy), (x2d, ldx) = ops.as_rows(y2d), ops.as_rows(x2d)
+        post, pre = post.contiguous(), pre.contiguous()
+        g2d = None if g2d is None else g2d.contiguous()
         (dn, lddn), (dh, lddh) = [(None, 0) if d is None else ops.as_rows(d) for d in (dn, dh)]
         return (*ops.sandwich_norm_backward(
             dn, lddn, dh, lddh, y2d, ldy, x2d, ldx, post, pre, g2d, rstd, residual_scale,

@@ -45,6 +45,11 @@ def _rows(t: Tensor) -> Tensor:
     return t
 
 
+def _places(tensors) -> list:
+    """Where the tensors' values lie."""
+    return [None if t is None else (t.data_ptr(), t.stride()) for t in tensors]
+
+
 def _logps(name: str, t: Tensor, logps: Tensor) -> Tensor:
     if t.shape != logps.shape:
         raise ValueError(f"clipped_policy_loss: {name} {tuple(t.shape)} != logps "
@@ -100,6 +105,8 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
         inputs = ops.policy_inputs(lp, old, adv, mask, ref, clip_low, clip_high, kl_coef, reduction)
         loss, policy, kl, clipped, weights = ops.policy_loss_forward(inputs, dev)
         ctx.save_for_backward(lp, old, adv, mask, ref, weights)
+        # the struct points into these tensors
+        ctx.inputs, ctx.places = inputs, _places((lp, old, adv, mask, ref))
         ctx.cfg = (clip_low, clip_high, kl_coef, reduction)
         ctx.mark_non_differentiable(policy, kl, clipped)
         ctx.set_materialize_grads(False)
@@ -110,11 +117,14 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
     def backward(ctx, dloss: Optional[Tensor], *_unused):
         if dloss is None or not ctx.needs_input_grad[0]:
             return (None,) * 9
-        # hooks on saved tensors may give them back elsewhere, with other strides
         *saved, weights = ctx.saved_tensors
-        lp, old, adv, mask, ref = [t if t is None or t.dim() == 1 else _rows(t) for t in saved]
-        inputs = ops.policy_inputs(lp, old, adv, mask, ref, *ctx.cfg)
-        grad = ops.policy_loss_backward(inputs, weights, dloss, lp.dtype)
+        inputs = ctx.inputs
+        if _places(saved) != ctx.places:
+            # hooks on saved tensors have given them back elsewhere or with other strides
+            saved = [t if t is None else t.contiguous() if t.dim() == 1 else _rows(t)
+                     for t in saved]
+            inputs = ops.policy_inputs(*saved, *ctx.cfg)
+        grad = ops.policy_loss_backward(inputs, weights, dloss, saved[0].dtype)
         return (grad, *(None,) * 8)
 
 

@@ -655,26 +655,21 @@ def embedding_backward(ids: Tensor, dout2d: Tensor, ldd: int, rows: int, scale: 
 POLICY_REDUCTIONS = {"token": 0, "sequence": 1, "sum": 2}
 
 
-def _field(t: Optional[Tensor], tokens: int) -> Tuple[int, int]:
-    """Pointer and row stride of a struct's tensor (NULL where there is none)."""
-    if t is None:
-        return 0, tokens
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else tokens
-
-
 def policy_inputs(logps: Tensor, old: Optional[Tensor], adv: Tensor, mask: Optional[Tensor],
                   ref: Optional[Tensor], clip_low: float, clip_high: float, kl_coef: float,
                   reduction: str) -> "_lib.PolicyInputs":
     """The C struct over 2-D tensors with unit column strides (adv [B, T] or [B], fp32; mask one
     byte a token). It holds pointers only: the tensors must outlive the launches."""
     rows, tokens = logps.shape
-    code = _lib.DTYPE_CODE
-    own, most = code[logps.dtype], max(tokens, 1)
-    return _lib.PolicyInputs(
-        *_field(logps, most), *_field(old, most), *_field(ref, most), *_field(adv, most),
-        *_field(mask, most), rows, tokens, clip_low, clip_high, kl_coef, own,
-        own if old is None else code[old.dtype], own if ref is None else code[ref.dtype],
-        adv.dim() == 2, POLICY_REDUCTIONS[reduction])
+    most = max(tokens, 1)
+    fields = []  # pointer and row stride of each, NULL where there is none
+    for t in (logps, old, ref, adv, mask):
+        fields += (0, most) if t is None else (t.data_ptr(), t.stride(0) if rows > 1 else most)
+    dtype = logps.dtype
+    own = _lib.DTYPE_CODE[dtype]
+    codes = [own if t is None or t.dtype is dtype else _lib.DTYPE_CODE[t.dtype] for t in (old, ref)]
+    return _lib.PolicyInputs(*fields, rows, tokens, clip_low, clip_high, kl_coef, own, *codes,
+                             adv.dim() == 2, POLICY_REDUCTIONS[reduction])
 
 
 def policy_loss_forward(inputs: "_lib.PolicyInputs", dev: torch.device) -> Tuple[Tensor, ...]:
