@@ -253,7 +253,7 @@ class FusedSandwichRMSNormFunction(torch.autograd.Function):
                     None, None, None)
         # hooks on saved tensors may give them back with other strides
         (y2d, ldy), (x2d, ldx) = ops.as_rows(y2d), ops.as_rows(x2d)
-        post, pre = post.contiguous(), pre.contiguous()
+        post, pre, rstd = post.contiguous(), pre.contiguous(), rstd.contiguous()
         g2d = None if g2d is None else g2d.contiguous()
         (dn, lddn), (dh, lddh) = [(None, 0) if d is None else ops.as_rows(d) for d in (dn, dh)]
         return (*ops.sandwich_norm_backward(

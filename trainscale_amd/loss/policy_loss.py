@@ -124,6 +124,7 @@ class ClippedPolicyLossFunction(torch.autograd.Function):
             saved = [t if t is None else t.contiguous() if t.dim() == 1 else _rows(t)
                      for t in saved]
             inputs = ops.policy_inputs(*saved, *ctx.cfg)
+            weights = weights.contiguous()
         grad = ops.policy_loss_backward(inputs, weights, dloss, saved[0].dtype)
         return (grad, *(None,) * 8)
 
