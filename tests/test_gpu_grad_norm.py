@@ -119,6 +119,14 @@ def test_norm_of_other_ranks(gpu):
         check_clipped(t, r, 1.0 / (8.0 + 1e-6))
 
 
+def test_norm_is_one_of_the_values(gpu):
+    t = make(gpu, [70001], [F32], seed=6)[0]
+    t[4321] = 8.0
+    ref = t.clone()
+    clip_grads_with_norm_(params_of([t]), 1.0, t[4321])
+    check_clipped(t, ref, 1.0 / (8.0 + 1e-6))
+
+
 @pytest.mark.parametrize("value,dtype", [(1e30, F32), (3e38, BF), (1e-30, F32), (1e-42, F32),
                                          (1e-40, BF), (6e-8, F16), (65504.0, F16)])
 def test_squares_beyond_fp32(gpu, value, dtype):

@@ -164,7 +164,13 @@ def clip_grads_with_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm:
         raise TypeError(f"{what}: total_norm must be a tensor of one value")
     _lib.require_gpu(what, grads[0], total_norm)
     norm = total_norm.detach().to(torch.float32).reshape(())
-    _scale_in_place(what, grads, lambda t: ops.grad_scale(t, t, norm, max_norm, dev))
+
+    def scale(listed: ops.HostList) -> None:
+        at = norm.data_ptr()
+        inside = ((listed.ptr <= at) & (at < listed.end())).any()  # one of the values to scale
+        ops.grad_scale(listed, listed, norm.clone() if inside else norm, max_norm, dev)
+
+    _scale_in_place(what, grads, scale)
 
 
 def clip_grad_norm_(parameters: Union[Tensor, Iterable[Tensor]], max_norm: float,
