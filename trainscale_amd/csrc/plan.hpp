@@ -637,7 +637,8 @@ inline int64_t sandwich_max_cols(int elt) { return (int64_t)kSandwichMaxParts * 
 struct SandwichPlan {
   int tpr, kv, rpb;
 };
-// Two vectors a thread of each of the two inputs where the row allows it.
+// Two vectors a thread of each of the two inputs where the row allows it: [8192, 4096] bf16 50 us
+// (one: 52, four: 53), [4095, 8192] 55 us (71, 57).
 inline SandwichPlan sandwich_fwd_plan(int parts) {
   SandwichPlan p{0, 0, 0};
   if (parts <= 64) { p.tpr = 64; p.kv = 1; }

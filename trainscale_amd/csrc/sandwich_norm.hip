@@ -156,6 +156,8 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void sandwich_fwd(
   row_sums<TPR, kBlock>(sum, red[0]);
   const float ry = rstd_of(sum[0], s);
   float hf[KV][V];
+  // (The weights loaded with the row instead of here: 55 us for 50 at [8192, 4096] bf16, their
+  // registers cost more than the round trip to L2 that they save.)
   sum[0] = 0.f;
 #pragma unroll
   for (int k = 0; k < KV; ++k) {
