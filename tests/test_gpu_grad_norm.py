@@ -188,6 +188,30 @@ def test_layouts(gpu):
         check_clipped(o, t, 0.1 / (n + 1e-6))
 
 
+@pytest.mark.parametrize("count", [2, 40, 200])
+def test_strided_gradients_over_several_launches(gpu, count):
+    # the copies of strided gradients are read by the last launches, while the first ones write
+    # their partial sums
+    def make_list():
+        g = torch.Generator(device=gpu).manual_seed(count)
+        ts = []
+        for k in range(count):
+            dtype = (F32, BF, F16)[k % 3]
+            t = torch.randn(300 + k, 57, device=gpu, generator=g).to(dtype)
+            ts.append(t[:, 5:40] if k % 4 else t)
+        return ts
+
+    ts = make_list()
+    want = norm64(ts)
+    for _ in range(3):
+        assert abs(float(get_total_norm(ts)) - want) <= NORM * want
+    ref = [t.clone() for t in ts]
+    n = clip_grad_norm_(params_of(ts), 1.0, error_if_nonfinite=True)
+    assert abs(float(n) - want) <= NORM * want
+    for t, r in zip(ts, ref):
+        check_clipped(t, r, 1.0 / (want + 1e-6))
+
+
 def test_same_parameter_and_shared_memory(gpu):
     t = torch.full((1000,), 1.0, device=gpu)
     p = params_of([t])[0]

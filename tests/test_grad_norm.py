@@ -3,6 +3,7 @@ points, and the cutting of tensors into chunks."""
 import ctypes
 import shutil
 import subprocess
+import weakref
 from pathlib import Path
 
 import pytest
@@ -135,6 +136,19 @@ def test_dense_and_overlap():
     check([torch.zeros(50), torch.zeros(50)], [a, a])  # read twice
     check([flat[:0], flat])
     check([torch.zeros(40), flat[60:]], [flat[:60].view(torch.bfloat16)[10:50], flat[:40]])
+
+
+def test_list_keeps_its_tensors():
+    # the copies of strided gradients have no other owner until the launches are queued
+    from trainscale_amd.kernels.grad_kernels import _storage_order
+    made = _storage_order([torch.zeros(4, 8)[:, :3]])
+    refs = [weakref.ref(t) for t in made]
+    held = HostList(made)
+    del made
+    assert all(r() is not None for r in refs)
+    assert [t.data_ptr() for t in held.tensors] == held.ptr.tolist()
+    del held
+    assert all(r() is None for r in refs)
 
 
 DRIVER = r"""

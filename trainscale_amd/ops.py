@@ -706,9 +706,11 @@ def policy_loss_backward(inputs: "_lib.PolicyInputs", weights: Tensor, dloss: Te
 
 class HostList:
     """Contiguous tensors as the C ABI takes a list of them: host arrays of pointers, element
-    counts and dtype codes."""
+    counts and dtype codes. It holds the tensors too: copies made for a call keep their memory
+    until the launches that read it are queued."""
 
     def __init__(self, tensors):
+        self.tensors = list(tensors)
         self.count = len(tensors)
         self.ptr = np.array([t.data_ptr() for t in tensors], dtype=np.uint64)
         self.numel = np.array([t.numel() for t in tensors], dtype=np.int64)
