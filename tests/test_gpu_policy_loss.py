@@ -333,3 +333,85 @@ def test_saved_tensors_elsewhere(gpu, how):
                 return loss(x)
         got = grad(moved)
     assert torch.isfinite(want).all() and same(got, want)
+
+
+# Log ratios whose exp leaves fp32's range, and infinite ones
+FAR = [0.25, 80.0, 88.0, 89.0, 95.0, 110.0, 800.0, math.inf, -80.0, -89.0, -800.0, -math.inf]
+
+
+def far_case(gpu, dtype, adv_of, beta, low, high, reduction, upstream):
+    """One far log ratio a row, among ordinary tokens: the loss's tensors and the gradient with
+    the definition's values in float64 (the policy's term of a token with A = 0 is 0 for any finite
+    difference; what is infinite follows float64's arithmetic)."""
+    b, t = len(FAR) * (2 if beta else 1), 7
+    g = torch.Generator(device=gpu).manual_seed(16)
+    lp = -torch.rand(b, t, device=gpu, generator=g)
+    old = (lp + 0.1 * torch.randn(b, t, device=gpu, generator=g)).to(dtype)
+    ref = (lp + 0.1 * torch.randn(b, t, device=gpu, generator=g)).to(dtype)
+    lp = lp.to(dtype)
+    lp[:, 3] = 0
+    old[:, 3] = ref[:, 3] = 0
+    old[:len(FAR), 3] = -torch.tensor(FAR, device=gpu).to(dtype)
+    if beta:
+        ref[len(FAR):, 3] = torch.tensor(FAR, device=gpu).to(dtype)
+    adv = torch.full((b,), float(adv_of), device=gpu)
+    lp.requires_grad_()
+    out = clipped_policy_loss(lp, old, adv, None, ref if beta else None, low, high, beta, reduction)
+    (grad,) = torch.autograd.grad(out.loss, lp, torch.tensor(upstream, device=gpu))
+
+    d, A = lp.detach().double() - old.double(), adv.double()[:, None]
+    r = d.exp()
+    clipped = ((A > 0) & (r > 1 + high)) | ((A < 0) & (r < 1 - low))
+    held = r.clamp(1 - low, 1 + high) if low < 1 else r.clamp(max=1 + high)
+    zero = (A == 0) & d.isfinite()
+    pol = torch.where(zero, 0.0, -torch.where(clipped, held, r) * A)
+    gpol = torch.where(zero | clipped, 0.0, -r * A)
+    x = ref.double() - lp.detach().double() if beta else torch.zeros_like(d)
+    rise = torch.expm1(x)
+    w = upstream * {"sum": 1.0, "token": 1.0 / (b * t), "sequence": 1.0 / (b * t)}[reduction]
+    want = w * (gpol - beta * rise if beta else gpol)
+    # |d| |r A| and |x| exp(x) are 0 in the limit of minus infinity, where exp gives an exact 0
+    e = abs(w) * (torch.where(gpol == 0, 0.0, (d.abs() + 3) * U * gpol.abs())
+                  + beta * (3 * U * rise.abs() + U * torch.where(x.isneginf(), 0.0, x.abs() * x.exp()))
+                  + 5 * U * (gpol.abs() + beta * rise.abs())
+                  # an exp below fp32's normal numbers becomes 0: up to 2^-126, times |A| in r A
+                  + 2.0 ** -126 * (1 + A.abs()))
+    fi = torch.finfo(dtype)
+    tol = e + fi.eps / 2 * (want.abs() + e) + fi.smallest_normal * fi.eps
+    rounded = want.to(dtype)  # infinities where the value leaves the type's range
+    ok = torch.where(rounded.isfinite(), (grad.double() - want).abs() <= tol,
+                     (grad == rounded) | (grad.isnan() & rounded.isnan()))
+    assert bool(ok.all()), [(k, grad[k].tolist(), want[k].tolist())
+                            for k in (~ok).any(1).nonzero()[:3, 0].tolist()]
+    return out, pol, torch.expm1(x) - x, rounded
+
+
+@pytest.mark.parametrize("dtype", [F32, BF, F16])
+@pytest.mark.parametrize("adv", [-1, 0, 1, -1e4])
+@pytest.mark.parametrize("beta", [0.0, 0.5])
+def test_exp_beyond_fp32(gpu, dtype, adv, beta):
+    finite = 0
+    for low, high in ((0.2, 0.2), (1.0, math.inf)):
+        for reduction, upstream in (("sum", 1.0), ("token", 1e-4), ("sequence", -1e-6)):
+            *_, want = far_case(gpu, dtype, adv, beta, low, high, reduction, upstream)
+            finite += int(want.isfinite().sum())
+            assert bool(want.isinf().any() or adv >= 0)
+    assert finite > 0
+
+
+def one_token(gpu, lp, old, adv, ref=None, **k):
+    lp, old, adv = [torch.tensor([[v]], device=gpu, dtype=F32) for v in (lp, old, adv)]
+    ref = None if ref is None else torch.tensor([[ref]], device=gpu, dtype=F32)
+    return clipped_policy_loss(lp, old, adv, None, ref, reduction="sum", **k)
+
+
+@pytest.mark.parametrize("d", FAR)
+def test_loss_of_far_tokens(gpu, d):
+    r = float(torch.tensor(d, dtype=torch.float64).exp())
+    for adv in (-1.0, 1.0):
+        got = one_token(gpu, 0.0, -d, adv)
+        want = -min(r * adv, min(max(r, 0.8), 1.2) * adv)
+        want = math.inf if want > 3.5e38 else want
+        assert float(got.loss) == want or abs(float(got.loss) - want) <= 2 * U * abs(want) + 2.0 ** -149
+    got = float(one_token(gpu, 0.0, -d, 0.0).loss)
+    assert got == 0.0 or (math.isinf(d) and math.isnan(got))

@@ -8,7 +8,7 @@
 //
 // A token costs up to 17 bytes of reading in each direction and some 60 operations: bound by
 // arithmetic and memory alike for large batches (512 x 8192 fp32 tokens: 24 us for the sums, 10
-// to join them, 15 for the backward, where the bytes alone take 8 and 11), and by launches and
+// to join them, 16 for the backward, where the bytes alone take 8 and 11), and by launches and
 // host time for the usual ones (4 x 500 tokens: 10 and 5 us). So: one pass over
 // the tokens and one workgroup that joins its partial sums (up to kSmallUnits units: both in one
 // launch), one launch backward. A wave owns a unit of kUnit tokens of one row and reduces
@@ -20,7 +20,9 @@
 // Numerics: log ratios are differences in double (the inputs' difference is exact there), and a
 // token is clipped where d lies beyond log(1 + high) or log(1 - low), compared in double: no
 // rounding of exp decides it. The sums' terms are formed and added in double, in a fixed order;
-// the gradient's in fp32.
+// the gradient's in fp32, and in double where that leaves fp32's range: a far token's exp may
+// overflow while its gradient, after the weight, does not. Without an advantage (A = 0) the policy's
+// term is 0 for any finite d.
 #include <math.h>
 
 #include "common.hpp"
@@ -134,6 +136,9 @@ __device__ inline bool is_clipped(const Args& a, double d, float adv) {
   return (adv > 0.f && d > a.log_high) || (adv < 0.f && d < a.log_low);
 }
 
+// Whether the policy's term is 0 whatever exp(d), which overflows for large d.
+__device__ inline bool is_zero(double d, float adv) { return adv == 0.f && fabs(d) < INFINITY; }
+
 // Forward: the terms of the sums in double. The policy's terms have either sign and nearly cancel
 // where the advantages are centred, so fp32's rounding of each would show in the loss (2e-6 of it
 // at 512 x 8192 tokens).
@@ -171,19 +176,21 @@ __device__ inline Terms token_terms(const Args& a, float lp, float old, float re
   const double d = a.old.p != nullptr ? (double)lp - (double)old : 0.;
   t.clipped = is_clipped(a, d, adv);
   const double r = t.clipped ? (adv > 0.f ? a.high : a.low) : exp_f64(d, rise2);
-  t.policy = -(r * (double)adv);
+  t.policy = is_zero(d, adv) ? 0. : -(r * (double)adv);
   t.kl = 0.;
   if (a.ref.p != nullptr) exp_f64((double)ref - (double)lp, t.kl);
   return t;
 }
 
 // Backward, in fp32: exp(x) to about 1.5 units in the last place, 2^(x log2 e) with the product's
-// rounding error put back (the hardware's 2^p is good to one). Results below 2^-126 are 0.
+// rounding error put back (the hardware's 2^p is good to one). Results below 2^-126 are 0; where
+// 2^p overflows the result is an infinity or a NaN (an infinity times the error), which the caller
+// forms again in double.
 constexpr float kLog2eLow = 1.925963033e-8f;  // log2 e - (float)log2 e
 __device__ inline float exp_f32(float x) {
   const float p = x * kLog2e;
   float low = __builtin_fmaf(x, kLog2eLow, __builtin_fmaf(x, kLog2e, -p));
-  low = fabsf(p) < 1e4f ? low * kLn2 : 0.f;  // an infinity's error is no number
+  low = fabsf(p) < 1e4f ? low * kLn2 : 0.f;  // minus infinity's error is no number
   const float e = fast_exp2(p);
   return __builtin_fmaf(e, low, e);
 }
@@ -202,13 +209,27 @@ __device__ inline float expm1_f32(float x) {
   return fabsf(x) < 0.5f ? __builtin_fmaf(x * x, s, x) : exp_f32(x) - 1.f;
 }
 
-// d(policy + kl_coef kl) / d logp of a token.
+// d(policy + kl_coef kl) / d logp of a token. Finite where every step stays in fp32's range.
 __device__ inline float token_grad(const Args& a, float lp, float old, float ref, float adv) {
   const double d = a.old.p != nullptr ? (double)lp - (double)old : 0.;
   float g = is_clipped(a, d, adv) ? 0.f : -(exp_f32((float)d) * adv);
   if (a.kl_coef != 0.)
     g = __builtin_fmaf(-(float)a.kl_coef, expm1_f32((float)((double)ref - (double)lp)), g);
   return g;
+}
+
+// The same in double, times the weight, rounded once.
+__device__ inline float token_grad_f64(const Args& a, float lp, float old, float ref, float adv,
+                                       double w) {
+  double rise2;
+  const double d = a.old.p != nullptr ? (double)lp - (double)old : 0.;
+  double g = 0.;
+  if (!is_clipped(a, d, adv) && !is_zero(d, adv)) g = -(exp_f64(d, rise2) * (double)adv);
+  if (a.kl_coef != 0.) {
+    const double x = (double)ref - (double)lp, e = exp_f64(x, rise2);
+    g -= a.kl_coef * (fabs(x) < 0.25 ? rise2 + x : e - 1.);
+  }
+  return (float)(g * w);
 }
 
 __device__ inline double wave_sum_f64(double v) {
@@ -362,7 +383,8 @@ __global__ __launch_bounds__(kThreads) void policy_bwd(Args a, const float* __re
   const int lane = threadIdx.x & (kWave - 1);
   const int64_t row = (uint32_t)u / (uint32_t)a.units_per_row;  // below 2^31
   const int64_t first = (u - row * a.units_per_row) * kUnit + lane * kPer;
-  const float w = weights[row] * *dloss;
+  const double w64 = (double)weights[row] * (double)*dloss;
+  const float w = (float)w64;
   Tokens t[kSteps];
   int n[kSteps];
 #pragma unroll
@@ -371,14 +393,17 @@ __global__ __launch_bounds__(kThreads) void policy_bwd(Args a, const float* __re
     n[s] = left >= kPer ? kPer : left > 0 ? (int)left : 0;
     if (n[s] > 0) load_tokens<T>(a, row, i, n[s], t[s]);
   }
+  float far = 0.f;  // a NaN once a gradient of this lane is none or infinite
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
     if (n[s] == 0) continue;
     float g[Elt<T>::kVec] = {};
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-      if ((t[s].valid >> j) & 1)
+      if ((t[s].valid >> j) & 1) {
         g[j] = token_grad(a, t[s].lp[j], t[s].old[j], t[s].ref[j], t[s].adv[j]) * w;
+        far = __builtin_fmaf(g[j], 0.f, far);
+      }
     }
     T* out = grad + row * ldg + first + s * kWave * kPer;
     if (n[s] == kPer) {
@@ -392,6 +417,21 @@ __global__ __launch_bounds__(kThreads) void policy_bwd(Args a, const float* __re
       for (int j = 0; j < kPer; ++j)
         if (j < n[s]) Elt<T>::store1(out + j, g[j]);
     }
+  }
+  // Rare: those are formed again in double, from the operands read again, and written over.
+  // (Behind the steps, where no operand is held any more: in them it took 8 registers more.)
+  if (far == 0.f) return;
+#pragma unroll 1
+  for (int k = 0; k < kSteps * kPer; ++k) {
+    const int64_t i = first + k / kPer * (kWave * kPer) + k % kPer;
+    T* out = grad + row * ldg + i;
+    if (i >= a.tokens || fabsf(Elt<T>::load1(out)) < INFINITY) continue;
+    float lp[kPer], old[kPer], ref[kPer];
+    load_rows<T>(a.logp, row, i, 1, lp);
+    if (a.old.p != nullptr) load_rows<T>(a.old, row, i, 1, old);
+    if (a.ref.p != nullptr) load_rows<T>(a.ref, row, i, 1, ref);
+    const float adv = a.adv[row * a.lda + (a.adv_per_token ? i : 0)];
+    Elt<T>::store1(out, token_grad_f64(a, lp[0], old[0], ref[0], adv, w64));
   }
 }
 
