@@ -415,3 +415,18 @@ def test_loss_of_far_tokens(gpu, d):
         assert float(got.loss) == want or abs(float(got.loss) - want) <= 2 * U * abs(want) + 2.0 ** -149
     got = float(one_token(gpu, 0.0, -d, 0.0).loss)
     assert got == 0.0 or (math.isinf(d) and math.isnan(got))
+
+
+@pytest.mark.parametrize("b,t", [(3, 50), (70, 600)])  # both forms of the forward
+@pytest.mark.parametrize("far", [-math.inf, 1e30])
+def test_infinite_kl_that_is_only_watched(gpu, b, t, far):
+    lp, old, adv, _, ref = inputs(gpu, b, t, F32, masked=False, seed=17)
+    ref[1, 7] = far
+    lp.requires_grad_()
+    out = clipped_policy_loss(lp, old, adv, None, ref, kl_coef=0.0)
+    assert float(out.kl) == math.inf
+    want = clipped_policy_loss(lp, old, adv, None, None)
+    assert math.isfinite(float(want.loss)) and same(out.loss, want.loss)
+    assert same(out.loss, out.policy_loss)
+    assert same(*[torch.autograd.grad(o.loss, lp)[0] for o in (out, want)])
+    assert float(clipped_policy_loss(lp, old, adv, None, ref, kl_coef=0.1).loss) == math.inf

@@ -342,7 +342,9 @@ __device__ inline void join_units(const Unit* units, const Args& a, const Outs& 
     *o.policy = (float)(all[0] * scale);
     *o.kl = (float)(all[1] * scale);
     *o.clipped = (float)(all[2] * scale);
-    *o.loss = (float)((all[0] + a.kl_coef * all[1]) * scale);
+    // (an infinite KL that is only watched stays out of the loss, as out of the gradient)
+    const double kl = a.kl_coef != 0. ? a.kl_coef * all[1] : 0.;
+    *o.loss = (float)((all[0] + kl) * scale);
   }
   if (sub == 0)
     for (int64_t row = row0; row < a.rows; row += step)  // the thread's own weights
