@@ -730,7 +730,9 @@ ts_status ts_grad_scale(const void* const* tensors, void* const* outs, const int
                         const float* norm, float max_norm, ts_stream_t stream);
 
 /*
- * Both at once: *norm = the tensors' norm, out = x * min(1, max_norm / (norm + 1e-6)).
+ * Both at once: *norm = the tensors' norm, out = x * min(1, max_norm / (*norm + 1e-6)), the same
+ * as ts_grad_norm and ts_grad_scale one after the other. A norm beyond fp32's range is infinite, and
+ * the factor 0.
  * Counterpart of the trainer's clip_grad_norm_ call (trainers/sota_trainer.py:2214-2245).
  */
 ts_status ts_grad_clip(const void* const* tensors, void* const* outs, const int64_t* numels,

@@ -145,6 +145,47 @@ def test_squares_beyond_fp32(gpu, value, dtype):
     check_clipped(out, t, min(1.0, 1.0 / (want + 1e-6)))
 
 
+@pytest.mark.parametrize("dtype", [F32, BF])
+@pytest.mark.parametrize("n", [5003, 1 << 23])  # few partial sums, and a launch of their own
+def test_norm_beyond_fp32(gpu, n, dtype):
+    def fresh():
+        t = torch.full((n,), 3e38, dtype=dtype, device=gpu)
+        t[::3] *= -0.5
+        t[7] = 1.0
+        return t
+
+    for kind in range(4):
+        t = fresh()
+        if kind == 0:
+            n_got = clip_grad_norm_(params_of([t]), 1.0)
+        elif kind == 1:
+            t2, t = t, torch.full((n,), float("nan"), device=gpu)
+            n_got = clipped_grads([t2], 1.0, [t])
+        elif kind == 2:
+            n_got = get_total_norm([t])
+            clip_grads_with_norm_(params_of([t]), 1.0, n_got)
+        else:
+            with pytest.raises(RuntimeError, match="non-finite"):
+                clip_grad_norm_(params_of([t]), 1.0, error_if_nonfinite=True)
+            assert same(t, fresh())
+            continue
+        assert float(n_got) == math.inf
+        assert not t.any(), kind  # x * (1 / inf), as torch's arithmetic has it
+
+
+@pytest.mark.parametrize("n", [70001, (1 << 22) + 5])
+def test_same_factor_on_every_path(gpu, n):
+    for seed in range(4):
+        src = make(gpu, [n, 333, n], [F32, BF, F16], seed=seed, std=1.0)
+        one, two, three = [[t.clone() for t in src] for _ in range(3)]
+        norm = clip_grad_norm_(params_of(one), 1.0)
+        clip_grads_with_norm_(params_of(two), 1.0, norm)
+        assert same(norm, clip_grad_norm_(params_of(three), 1.0, error_if_nonfinite=True))
+        assert same(norm, get_total_norm(src))
+        for a, b, c in zip(one, two, three):
+            assert same(a, b) and same(a, c)
+
+
 @pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
 @pytest.mark.parametrize("dtype", [F32, BF, F16])
 def test_nonfinite_as_torch(gpu, bad, dtype):

@@ -182,8 +182,11 @@ __global__ __launch_bounds__(kThreads) void grad_scale(Table tab, int count, int
   __shared__ double lds[kThreads / kWave];
   double norm;
   if (nparts > 0) {
-    norm = sqrt(total_squares<kThreads>(partial, nparts, lds));
-    if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
+    // rounded as the norm that is returned: the factor is the same whoever forms it, and 0 for
+    // norms beyond fp32's range
+    const float rounded = (float)sqrt(total_squares<kThreads>(partial, nparts, lds));
+    if (norm_out != nullptr && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = rounded;
+    norm = (double)rounded;
   } else {
     norm = (double)*norm_in;
   }
