@@ -330,3 +330,27 @@ def test_other_stream_and_graph(gpu):
         assert all(same(a, b) for a, b in zip(got, ts)), rep
         if rep == 0:
             assert same(n1, n3) and all(same(a, b) for a, b in zip(got, eager))
+
+
+def test_strided_gradients_beside_one_another(gpu):
+    buf = torch.randn(50, 90, device=gpu, generator=torch.Generator(device=gpu).manual_seed(4))
+    keep = buf.clone()
+
+    def parts(t):
+        return [t[:, :30], t[:20, 30:77], t[20:, 30:77:2], t[20:, 31:77:2], t[:, 80:]]
+
+    want = norm64(parts(keep))
+    n = clip_grad_norm_(params_of(parts(buf)), 1.0)
+    assert abs(float(n) - want) <= NORM * want
+    for t, r in zip(parts(buf), parts(keep)):
+        check_clipped(t, r, 1.0 / (want + 1e-6))
+    assert same(buf[:, 77:80], keep[:, 77:80])
+    now = buf.clone()
+    for grads in ([buf, buf[:, :4]], [buf[:, :6], buf[:, 3:9]], [buf[:, :4]] * 2,
+                  [buf.view(-1).as_strided((5, 5), (3, 1))]):
+        for call in (lambda p: clip_grad_norm_(p, 1e-3),
+                     lambda p: clip_grad_norm_(p, 1e-3, error_if_nonfinite=True),
+                     lambda p: clip_grads_with_norm_(p, 1e-3, torch.ones((), device=gpu))):
+            with pytest.raises(ValueError, match="share memory"):
+                call(params_of(grads))
+    assert same(buf, now)

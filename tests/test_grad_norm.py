@@ -12,7 +12,8 @@ import torch
 from trainscale_amd import _lib
 from trainscale_amd.kernels import (clip_grad_norm_, clip_grads_with_norm_, clipped_grads,
                                     get_total_norm)
-from trainscale_amd.kernels.grad_kernels import _is_dense, _refuse_overlap
+from trainscale_amd.kernels.grad_kernels import (_is_dense, _refuse_overlap,
+                                                 _refuse_strided_overlap, _share_memory)
 from trainscale_amd.ops import HostList
 
 TS_OK, INVALID, DTYPE, SHAPE, WORKSPACE = 0, -1, -2, -3, -4
@@ -136,6 +137,69 @@ def test_dense_and_overlap():
     check([torch.zeros(50), torch.zeros(50)], [a, a])  # read twice
     check([flat[:0], flat])
     check([torch.zeros(40), flat[60:]], [flat[:60].view(torch.bfloat16)[10:50], flat[:40]])
+
+
+def _strided_refused(grads):
+    try:
+        _refuse_strided_overlap("x", grads, [not (t.is_contiguous() or _is_dense(t)) for t in grads])
+    except ValueError as e:
+        assert "share memory" in str(e)
+        return True
+    return False
+
+
+def test_strided_gradients_that_share_memory():
+    buf = torch.zeros(12, 20)
+    for grads in ([buf, buf[:, :4]], [buf[:, :4], buf], [buf[:, :6], buf[:, 3:9]],
+                  [buf[2:, 5:], buf[:3, 5:9]], [buf[:, 3], buf[4:6, 2:5]],
+                  [buf[:, ::2], buf[:, 1:9]], [buf[:, ::2], buf[:, ::3]],
+                  [buf.t()[3:7], buf[:, 6:8]], [buf[:, :4]] * 2,
+                  [buf[:, 4:9], buf.view(torch.bfloat16)[3:5, 17:19]],
+                  [torch.zeros(5).expand(3, 5)], [torch.zeros(40).as_strided((4, 4), (3, 1))],
+                  [torch.zeros(40).as_strided((4, 4), (4, 4))],
+                  [torch.zeros(40).as_strided((3, 3, 2), (9, 4, 2))]):
+        if grads[-1].stride() == (9, 4, 2):  # odd, but its elements are apart
+            assert not _strided_refused(grads)
+        else:
+            assert _strided_refused(grads), [t.stride() for t in grads]
+    for grads in ([buf[:, :6], buf[:, 6:9], buf[:, 9:]], [buf[:, ::2], buf[:, 1::2]],
+                  [buf[:5, :6], buf[5:, :6], buf[:, 6:]], [buf[:, 3], buf[:, 4:6], buf[:, 2]],
+                  [buf[:, :0], buf[:, :4]], [buf[:, 4:9], buf.view(torch.bfloat16)[:, :7]],
+                  [torch.zeros(2, 3, 8, 8)[:, :, 1:, ::3]],
+                  [torch.zeros(3, 300)[:, k:290:7] for k in range(7)]):
+        assert not _strided_refused(grads), [t.stride() for t in grads]
+
+
+def test_shared_memory_as_by_addresses():
+    # against the bytes written down one by one
+    gen = torch.Generator().manual_seed(3)
+    r = lambda lo, hi: int(torch.randint(lo, hi, (), generator=gen))
+    buf = torch.zeros(8000, dtype=torch.uint8)
+    base = buf.data_ptr()
+    found = set()
+    for _ in range(3000):
+        ts, places = [], []
+        for _ in range(2):
+            dtype = (torch.float32, torch.bfloat16)[r(0, 2)]
+            flat = buf.view(dtype)
+            shape = [r(1, 5) for _ in range(r(1, 4))]
+            strides = [r(1, 30) for _ in shape]
+            if r(0, 2):
+                strides = [strides[0] * (3, 1, 9)[i] for i in range(len(shape))]
+            t = flat.as_strided(shape, strides, r(0, 60))
+            at = torch.zeros(shape, dtype=torch.int64) + t.data_ptr() - base
+            for k, st in enumerate(strides):
+                view = [1] * len(shape)
+                view[k] = shape[k]
+                at += (torch.arange(shape[k]) * st * t.element_size()).view(view)
+            ts.append(t)
+            places.append([p + i for p in at.reshape(-1).tolist() for i in range(t.element_size())])
+        own = len(set(places[0])) < len(places[0])
+        assert _share_memory(ts[0]) == own, (ts[0].shape, ts[0].stride())
+        both = not set(places[0]).isdisjoint(places[1])
+        assert _share_memory(*ts) == both
+        found.add((own, both))
+    assert len(found) == 4
 
 
 def test_list_keeps_its_tensors():

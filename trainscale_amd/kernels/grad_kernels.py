@@ -17,7 +17,7 @@ gradients next to 16-bit ones: one pass instead of a copy and a scaling.
 from __future__ import annotations
 
 import math
-from typing import Iterable, List, Optional, Sequence, Union
+from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
@@ -89,6 +89,77 @@ def _refuse_overlap(what: str, written: ops.HostList, read: ops.HostList) -> Non
         raise ValueError(f"{what}: gradients share memory: each must be written once")
 
 
+def _reaches(distance: int, ranges: List[Tuple[int, int, int]], other: bool) -> Optional[bool]:
+    """Whether distance = sum of d * stride with low <= d <= high for every (stride, low, high),
+    strides falling; `other`: by other d than 0 everywhere. None if there are too many ways."""
+    reach = [(0, 0)]  # what the strides behind k reach at least and at most
+    for stride, low, high in reversed(ranges):
+        reach.append((reach[-1][0] + stride * low, reach[-1][1] + stride * high))
+    reach.reverse()
+    tries, todo = 0, [(0, distance, not other)]
+    while todo:
+        k, left, counts = todo.pop()
+        if k == len(ranges):
+            if left == 0 and counts:
+                return True
+            continue
+        stride, low, high = ranges[k]
+        least, most = reach[k + 1]  # of left - d * stride
+        d = range(max(low, -((most - left) // stride)), min(high, (left - least) // stride) + 1)
+        tries += len(d)
+        if tries > 4096:
+            return None
+        todo += [(k + 1, left - i * stride, counts or i != 0) for i in d]
+    return False
+
+
+def _share_memory(a: Tensor, b: Optional[Tensor] = None) -> Optional[bool]:
+    """Whether a byte belongs to both tensors, or to two elements of a where b is None. Found by
+    their strides, one after the other: where strides nest, as those of slices do, each leaves one
+    or two ways open. None where there are too many ways to tell."""
+    size = a.element_size()
+    dims = [(st * size, n) for st, n in zip(a.stride(), a.shape) if n > 1]
+    if b is None and len({0, *[st for st, _ in dims]}) <= len(dims):
+        return True  # no stride, or two alike
+    # address of an element's byte: the tensor's plus those of its indices, bytes of stride 1
+    ranges = {}
+    for st, n in dims + [(1, size)]:
+        low, high = ranges.get(st, (0, 0))
+        ranges[st] = (low, high + n - 1)
+    other = a if b is None else b
+    size = other.element_size()
+    for st, n in [(st * size, n) for st, n in zip(other.stride(), other.shape)] + [(1, size)]:
+        low, high = ranges.get(st, (0, 0))
+        ranges[st] = (low - (n - 1), high)
+    return _reaches(other.data_ptr() - a.data_ptr(),
+                    sorted([(st, *r) for st, r in ranges.items() if st > 0], reverse=True),
+                    b is None)
+
+
+def _refuse_strided_overlap(what: str, grads: List[Tensor], strided: List[bool]) -> None:
+    """Raises if a gradient that is marked strided shares memory with itself or another one. Slices
+    of one buffer that lie beside each other do not, though their stretches of addresses meet."""
+    spans = []
+    for k, t in enumerate(grads):
+        if t.numel() > 0:
+            last = sum((n - 1) * st for st, n in zip(t.stride(), t.shape))
+            spans.append((t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size(), k))
+    still = []  # spans that reach behind the next one's start
+    for start, end, k in sorted(spans):
+        still = [s for s in still if s[1] > start]
+        pairs = [(grads[k], grads[s[2]]) for s in still if strided[k] or strided[s[2]]]
+        if strided[k]:
+            pairs.append((grads[k], None))
+        for a, b in pairs:
+            shared = _share_memory(a, b)
+            if shared is None:
+                raise ValueError(f"{what}: gradients of these strides may share memory: pass "
+                                 "contiguous ones")
+            if shared:
+                raise ValueError(f"{what}: gradients share memory: each must be written once")
+        still.append((start, end, k))
+
+
 def _max_norm(what: str, max_norm: float) -> float:
     max_norm = float(max_norm)
     if not max_norm >= 0:
@@ -134,16 +205,16 @@ def _scale_in_place(what: str, grads: List[Tensor], launch) -> Optional[Tensor]:
     """Runs launch(list of contiguous tensors) over the gradients; those that are not dense (slices of a
     larger buffer) are scaled in a copy and copied back."""
     held = _storage_order(grads)
-    copied = [(g, h) for g, h in zip(grads, held) if g is not h]
-    for g, _ in copied:
-        if any(st == 0 and n > 1 for st, n in zip(g.stride(), g.shape)):
-            raise ValueError(f"{what}: a gradient's elements share memory (an expanded tensor)")
+    strided = [g is not h for g, h in zip(grads, held)]
+    if True in strided:
+        _refuse_strided_overlap(what, grads, strided)
     listed = ops.HostList(held)
     _refuse_overlap(what, listed, listed)
     out = launch(listed)
     with torch.no_grad():
-        for g, h in copied:
-            g.copy_(h)
+        for g, h, copied in zip(grads, held, strided):
+            if copied:
+                g.copy_(h)
     torch.autograd.graph.increment_version(grads)
     return out
 
