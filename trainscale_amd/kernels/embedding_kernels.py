@@ -77,7 +77,7 @@ def scaled_embedding(input_ids: Tensor, weight: Tensor, scale: float = 1.0,
     """scale * weight[input_ids]: ids [...] int64 or int32, weight [V, H] fp32/bf16/fp16; the
     result is [..., H] in the weight's dtype, differentiable in weight. Tokens equal to
     padding_idx (negative counts from the end) get their row but give it no gradient."""
-    if weight.requires_grad and torch.is_grad_enabled():
+    if (weight.requires_grad and torch.is_grad_enabled()) or ops.in_forward_ad():
         return ScaledEmbeddingFunction.apply(input_ids, weight, float(scale), padding_idx)
     return _forward(input_ids, weight, float(scale), padding_idx)[0]
 

@@ -22,6 +22,7 @@ from typing import Iterable, List, Optional, Sequence, Tuple, Union
 import numpy as np
 import torch
 from torch import Tensor
+from torch.autograd.forward_ad import unpack_dual
 
 from .. import _lib, ops
 
@@ -48,6 +49,8 @@ def _checked(what: str, tensors: Union[Tensor, Iterable[Tensor]]) -> List[Tensor
         if not issubclass(cls, Tensor):
             raise TypeError(f"{what}: expected tensors, got {cls.__name__}")
         raise TypeError(f"{what}: {cls.__name__} is not supported: pass its local tensor")
+    if ops.in_forward_ad() and any(unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what}: forward-mode derivatives are not supported")
     if {t.layout for t in tensors} != {torch.strided}:
         raise TypeError(f"{what}: sparse gradients are not supported")
     for dtype in {t.dtype for t in tensors}:

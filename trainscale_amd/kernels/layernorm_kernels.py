@@ -281,7 +281,8 @@ def fused_sandwich_rms_layernorm(X: Tensor, residual: Tensor, post_weight: Tenso
     for 16-bit X, 8192 for fp32."""
     args = (X, residual, post_weight, pre_weight, gate, float(eps), float(residual_scale),
             float(weight_offset))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:5]):
+    if ops.in_forward_ad() or (torch.is_grad_enabled() and any(
+            t is not None and t.requires_grad for t in args[:5])):
         return FusedSandwichRMSNormFunction.apply(*args)
     return _sandwich_forward(*args)[:2]
 

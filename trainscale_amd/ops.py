@@ -15,6 +15,7 @@ from typing import Optional, Tuple
 import numpy as np
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import check, ptr
@@ -37,6 +38,13 @@ def as_rows(t: Tensor) -> Tuple[Tensor, int]:
         t2 = t2.contiguous()
         ld = c
     return t2, ld
+
+
+def in_forward_ad() -> bool:
+    """Whether a level of forward-mode differentiation is open, where tensors may have tangents. A
+    launch on a tensor's pointer drops its tangent; an autograd function, which has no forward-mode
+    derivative here, raises for it."""
+    return forward_ad._current_level >= 0
 
 
 def _norm_stride(t: Tensor, dim: int) -> int:
