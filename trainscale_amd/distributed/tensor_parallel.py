@@ -102,7 +102,6 @@ class VocabParallelCrossEntropyLoss(torch.autograd.Function):
         lse, loss = ops.ce_vocab_merge(stats_all, ex.rank if ex.world_size > 1 else 0, vp,
                                        label_smoothing)
         ctx.save_for_backward(x2d, t, lse)
-        ctx.ld = ld
         ctx.vocab_start = int(vocab_start)
         ctx.label_smoothing = float(label_smoothing)
         ctx.shape = logits.shape
@@ -111,8 +110,9 @@ class VocabParallelCrossEntropyLoss(torch.autograd.Function):
     @staticmethod
     def backward(ctx, grad_output: Tensor) -> Tuple[Optional[Tensor], None, None, None, None]:
         x2d, t, lse = ctx.saved_tensors
+        x2d, ld = ops.as_rows(x2d)
         n = x2d.shape[0]
-        grad = ops.ce_vocab_shard_backward(x2d, ctx.ld, t, lse, grad_output,
+        grad = ops.ce_vocab_shard_backward(x2d, ld, t, lse, grad_output,
                                            1.0 / max(n, 1), ctx.vocab_start,
                                            ctx.label_smoothing)
         return grad.view(ctx.shape), None, None, None, None

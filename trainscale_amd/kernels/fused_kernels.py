@@ -58,15 +58,14 @@ class Fast_RMS_LayerNorm(torch.autograd.Function):
         x2d, ldx = ops.as_rows(X)
         y, rstd = ops.rmsnorm_forward(x2d, ldx, weight, eps, ops.ROUND_ONCE)
         ctx.save_for_backward(x2d, weight, rstd)
-        ctx.ldx = ldx
         ctx.original_shape = original_shape
         return y.view(original_shape)
 
     @staticmethod
     def backward(ctx, dY: Tensor) -> Tuple[Optional[Tensor], Optional[Tensor], None]:
         x2d, weight, rstd = ctx.saved_tensors
-        dy2d, lddy = ops.as_rows(dY)
-        dx, dw = ops.rmsnorm_backward(dy2d, lddy, x2d, ctx.ldx, weight, rstd,
+        (x2d, ldx), (dy2d, lddy) = ops.as_rows(x2d), ops.as_rows(dY)
+        dx, dw = ops.rmsnorm_backward(dy2d, lddy, x2d, ldx, weight, rstd,
                                       need_dw=ctx.needs_input_grad[1])
         return dx.view(ctx.original_shape), dw, None
 
@@ -171,7 +170,6 @@ class Fast_CrossEntropyLoss(torch.autograd.Function):
         l2d, ld = ops.as_rows(logits)
         losses, lse = ops.ce_forward(l2d, ld, labels, -100, logit_scaling, logit_softcapping)
         ctx.save_for_backward(l2d, lse, labels)
-        ctx.ld = ld
         ctx.logit_softcapping = logit_softcapping
         ctx.logit_scaling = logit_scaling
         return losses
@@ -179,7 +177,8 @@ class Fast_CrossEntropyLoss(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dlosses: Tensor):
         l2d, lse, labels = ctx.saved_tensors
-        ops.ce_backward(l2d, ctx.ld, labels, lse, dlosses, l2d, ctx.ld,
+        l2d, ld = ops.as_rows(l2d)
+        ops.ce_backward(l2d, ld, labels, lse, dlosses, l2d, ld,
                         ignore_index=-100, logit_scale=ctx.logit_scaling,
                         softcap=ctx.logit_softcapping)
         return l2d, None, None, None

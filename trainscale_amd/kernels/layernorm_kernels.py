@@ -63,7 +63,6 @@ class RMSLayerNormFunction(torch.autograd.Function):
         x2d, ldx = ops.as_rows(X)
         y, rstd = ops.rmsnorm_forward(x2d, ldx, weight, eps, ops.ROUND_TWICE)
         ctx.save_for_backward(x2d, weight, rstd)
-        ctx.ldx = ldx
         ctx.orig_shape = orig_shape
         ctx.compute_weight_grad = compute_weight_grad
         return y.view(orig_shape)
@@ -71,9 +70,9 @@ class RMSLayerNormFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dY: Tensor) -> Tuple[Optional[Tensor], ...]:
         x2d, weight, rstd = ctx.saved_tensors
-        dy2d, lddy = ops.as_rows(dY)
+        (x2d, ldx), (dy2d, lddy) = ops.as_rows(x2d), ops.as_rows(dY)
         need_dw = bool(ctx.compute_weight_grad and weight is not None and weight.requires_grad)
-        dx, dw = ops.rmsnorm_backward(dy2d, lddy, x2d, ctx.ldx, weight, rstd, need_dw=need_dw)
+        dx, dw = ops.rmsnorm_backward(dy2d, lddy, x2d, ldx, weight, rstd, need_dw=need_dw)
         return dx.view(ctx.orig_shape), dw, None, None
 
 
@@ -92,15 +91,14 @@ class _RMSNormNoWeight(torch.autograd.Function):
         x2d, ldx = ops.as_rows(X)
         y, rstd = ops.rmsnorm_forward(x2d, ldx, None, eps, ops.ROUND_ONCE)
         ctx.save_for_backward(x2d, rstd)
-        ctx.ldx = ldx
         ctx.orig_shape = orig_shape
         return y.view(orig_shape)
 
     @staticmethod
     def backward(ctx, dY: Tensor):
         x2d, rstd = ctx.saved_tensors
-        dy2d, lddy = ops.as_rows(dY)
-        dx, _ = ops.rmsnorm_backward(dy2d, lddy, x2d, ctx.ldx, None, rstd, need_dw=False)
+        (x2d, ldx), (dy2d, lddy) = ops.as_rows(x2d), ops.as_rows(dY)
+        dx, _ = ops.rmsnorm_backward(dy2d, lddy, x2d, ldx, None, rstd, need_dw=False)
         return dx.view(ctx.orig_shape), None
 
 
@@ -156,8 +154,8 @@ class FusedAddRMSLayerNormFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dY: Tensor, _unused: Optional[Tensor]):
         h, weight, rstd = ctx.saved_tensors
-        dy2d, lddy = ops.as_rows(dY)
-        dx, _ = ops.rmsnorm_backward(dy2d, lddy, h, h.shape[1], weight, rstd, need_dw=False)
+        (h, ldh), (dy2d, lddy) = ops.as_rows(h), ops.as_rows(dY)
+        dx, _ = ops.rmsnorm_backward(dy2d, lddy, h, ldh, weight, rstd, need_dw=False)
         dx = dx.view(ctx.orig_shape)
         return dx, dx, None, None, None
 

@@ -600,13 +600,14 @@ class SelectiveLogSoftmaxFunction(torch.autograd.Function):
         ids = input_ids.reshape(-1)
         rows, lse = ops.ce_forward(l2d, ld, ids, _NO_IGNORE, scale, cap)
         ctx.save_for_backward(l2d, ids, lse)
-        ctx.cfg = (ld, scale, cap, logits.shape)
+        ctx.cfg = (scale, cap, logits.shape)
         return (-rows).to(out_dtype or logits.dtype).view(input_ids.shape)
 
     @staticmethod
     def backward(ctx, grad_out: Tensor):
         l2d, ids, lse = ctx.saved_tensors
-        ld, scale, cap, shape = ctx.cfg
+        l2d, ld = ops.as_rows(l2d)
+        scale, cap, shape = ctx.cfg
         grad = torch.empty((l2d.shape[0], l2d.shape[1]), dtype=l2d.dtype, device=l2d.device)
         # d(log-prob)/d(row loss) = -1
         dl = -grad_out.detach().float().reshape(-1)

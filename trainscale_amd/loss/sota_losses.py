@@ -54,7 +54,6 @@ class CrossEntropyRowsFunction(torch.autograd.Function):
         loss, lse = ops.ce_forward(l2d, ld, labels, ignore_index, logit_scale, softcap,
                                    label_smoothing)
         ctx.save_for_backward(l2d, labels, lse)
-        ctx.ld = ld
         ctx.cfg = (ignore_index, label_smoothing, logit_scale, softcap)
         ctx.shape = logits.shape
         return loss
@@ -62,9 +61,10 @@ class CrossEntropyRowsFunction(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dloss: Tensor):
         l2d, labels, lse = ctx.saved_tensors
+        l2d, ld = ops.as_rows(l2d)
         ignore_index, label_smoothing, logit_scale, softcap = ctx.cfg
         grad = torch.empty(l2d.shape, dtype=l2d.dtype, device=l2d.device)
-        ops.ce_backward(l2d, ctx.ld, labels, lse, dloss, grad, l2d.shape[1],
+        ops.ce_backward(l2d, ld, labels, lse, dloss, grad, l2d.shape[1],
                         ignore_index=ignore_index, logit_scale=logit_scale, softcap=softcap,
                         label_smoothing=label_smoothing)
         return grad.view(ctx.shape), None, None, None, None, None
@@ -188,7 +188,6 @@ class FusedCrossEntropyFunction(torch.autograd.Function):
         loss, lse = ops.ce_forward(l2d, ld, flat, ignore_index, 0.0, 0.0, label_smoothing)
         ctx.fused = False
         ctx.save_for_backward(l2d, flat, lse)
-        ctx.ld = ld
         return _reduced(loss, flat, ignore_index, reduction)
 
     @staticmethod
@@ -208,13 +207,14 @@ class FusedCrossEntropyFunction(torch.autograd.Function):
                 ops.rescale_(grad, grad_output, used, ctx.hint)
             return grad.view(ctx.shape), None, None, None, None, None
         l2d, labels, lse = ctx.saved_tensors
+        l2d, ld = ops.as_rows(l2d)
         n = l2d.shape[0]
         if reduction == "none":
             dloss = grad_output.float().reshape(-1)
         else:
             dloss = grad_output.float() * _row_weight(labels, ignore_index, reduction, n)
         grad = torch.empty(l2d.shape, dtype=l2d.dtype, device=l2d.device)
-        ops.ce_backward(l2d, ctx.ld, labels, lse, dloss, grad, l2d.shape[1],
+        ops.ce_backward(l2d, ld, labels, lse, dloss, grad, l2d.shape[1],
                         ignore_index=ignore_index, label_smoothing=label_smoothing)
         return grad.view(ctx.shape), None, None, None, None, None
 
