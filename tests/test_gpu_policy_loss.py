@@ -104,6 +104,12 @@ def test_shapes(gpu, b, t, dtype):
         run(inputs(gpu, b, t, dtype, per_token=i != 1, seed=b + t + i), reduction=reduction)
 
 
+@pytest.mark.parametrize("b,t", [(16, 512), (17, 512), (8, 513), (9, 513), (1, 8192), (1, 8193)])
+def test_around_the_one_launch_form(gpu, b, t):
+    for reduction in REDUCTIONS:
+        run(inputs(gpu, b, t, F32, seed=b), reduction=reduction)
+
+
 @pytest.mark.parametrize("per_token", [False, True])
 @pytest.mark.parametrize("ref", [False, True])
 @pytest.mark.parametrize("masked", [False, True])

@@ -56,6 +56,13 @@ def test_forward_validation(lib):
     assert f(ws=ctypes.c_void_p(0x1004)) == WORKSPACE
 
 
+def test_small_batches_need_no_workspace(lib):
+    # one round of the waves of one workgroup, 512 tokens of a row each
+    size = lib.ts_policy_loss_workspace_size
+    assert size(16, 512) == size(8, 513) == size(1, 8192) == size(5, 1025) == 0
+    assert size(17, 512) == 17 * 24 and size(9, 513) == 18 * 24 and size(1, 8193) == 17 * 24
+
+
 def test_backward_validation(lib):
     def f(weights=FAKE, dloss=FAKE, grad=FAKE, ld=100, **k):
         return lib.ts_policy_loss_bwd(ctypes.byref(inputs(**k)), weights, dloss, grad, ld, None)

@@ -688,9 +688,14 @@ inline int64_t sandwich_workspace(int64_t rows, int64_t groups, int64_t cols) {
   return most;
 }
 
-// Clipped policy loss (policy_loss.hip): tokens of one row that a wave takes, and the units up
-// to which one workgroup does the whole forward (4 rounds of its 16 waves).
+// Clipped policy loss (policy_loss.hip): tokens of one row that a wave takes. The forward, fp32 with
+// a reference, at 512 x 8192, 128 x 512 and 4 x 500 tokens: 31.2, 12.4 and 10.3 us; units of 256
+// 36.1, 10.7 and 9.5, of 1024 33.6, 12.9 and 12.0.
 constexpr int kPolicyUnit = 512;
-constexpr int kPolicySmallUnits = 64;
+// Units up to which one workgroup of 16 waves does the whole forward, in one launch and without a
+// workspace: 4 units 10.3 us against 11.9 in two launches, 8 units 11.2 and 12.2, 16 units 13.8 and
+// 12.3, where the second launch and the workspace cost the host more than that; a second round of
+// the waves is slower (24 units 16.3 and 12.2, 64 units 35.4 and 12.4).
+constexpr int kPolicySmallUnits = 16;
 
 }  // namespace ts_plan
