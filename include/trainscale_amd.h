@@ -682,7 +682,8 @@ size_t ts_policy_loss_workspace_size(int64_t rows, int64_t tokens);
 
 /*
  * With d = logp - old, r = exp(d), x = ref - logp, for every valid token:
- *   policy = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A), kl = exp(x) - x - 1,
+ *   policy = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A), kl = exp(x) - x - 1
+ * (with A = 0, policy is 0 for any finite d; with kl_coef = 0, kl is no part of the loss),
  * and over them, with the reduction's weights w (TOKEN: 1 / valid tokens; SEQUENCE: 1 / (the
  * row's valid tokens * rows that have any); SUM: 1):
  *   policy_loss = sum w policy, kl = sum w kl, clip_fraction = sum w [clipped],
@@ -696,7 +697,8 @@ ts_status ts_policy_loss_fwd(const ts_policy_inputs* in, float* loss, float* pol
 
 /*
  * dlogp = *dloss * w * ((clipped ? 0 : -r A) - kl_coef (exp(x) - 1)) in dtype, row stride
- * ld_dlogp; exactly 0 for tokens that are not valid.
+ * ld_dlogp; exactly 0 for tokens that are not valid. Infinite only where the product is: an exp
+ * beyond fp32's range is formed, and weighted, in double.
  */
 ts_status ts_policy_loss_bwd(const ts_policy_inputs* in, const float* weights, const float* dloss,
                              void* dlogp, int64_t ld_dlogp, ts_stream_t stream);

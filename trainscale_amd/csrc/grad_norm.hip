@@ -122,6 +122,8 @@ __global__ __launch_bounds__(kThreads) void grad_squares(Table tab, int count, i
 // The partial sums' total, in the same order in every workgroup that asks for it. The scaling's
 // workgroups form it themselves while it is short, which saves a launch between the two passes;
 // past kOwnParts partial sums (8 MB of gradients in one launch) a launch of its own forms the norm.
+// In place below the limit, bf16: 1 partial sum 4.0 us against 5.9 with the launch, 128 5.1 and 6.7,
+// 512 6.6 and 7.1, 1024 8.4 and 8.0, 4096 23.5 and 17.0.
 constexpr int kOwnParts = 512;
 constexpr int kFinalThreads = 1024;
 

@@ -535,8 +535,9 @@ inline int64_t grad_norm_parts(int64_t count) {
 // Embedding gradient by sorted tokens (embedding.hip)
 // ---------------------------------------------------------------------------
 constexpr int kEmbedMaxBits = 10;        // of a radix digit
-// Placed by counting, in one launch (the radix sort's four: 8192 tokens and 65 MB of gradient
-// 26 us against 33, 1 GB 177 against 185). The counting is quadratic.
+// Placed by counting, which is quadratic, in one launch, against the radix sort's four. The whole
+// gradient of 65 MB: 300 tokens 21.0 us and 29.7, 4096 39.2 and 47.3, 8192 51.3 and 50.8, 12288 71.0
+// and 58.4; of 1 GB: 300 tokens 166 and 168, 8192 180 and 186, 12288 204 and 192.
 constexpr int kEmbedSmallTokens = 8192;
 constexpr int kEmbedTile = 1024;         // keys of a sorting workgroup's step
 constexpr int64_t kEmbedMaxBlocks = 256;

@@ -20,11 +20,11 @@
 // dy out): [8192, 4096] bf16 50 us (5.3 TB/s) and 65 us (6.2 TB/s) + 7 us for the parameters' sums;
 // [4095, 8192] 55 and 75 us, where one workgroup of 1024 threads fills a CU and no other computes
 // while it waits. Inputs are read through the caches, where what the layer before has written may
-// still be (both directions 6 to 8 us faster than streaming loads when it is). A row is owned by TPR threads (whole waves), KV 16-byte vectors each, and stays in
-// registers between its reductions and its outputs. The backward's workgroups walk rows of one
-// group a fixed distance apart and keep t yhat and dn hhat of their columns in fp32 registers;
-// one partial row each per workgroup, summed in a fixed order afterwards, so the parameters'
-// gradients do not depend on timing.
+// still be (both directions 6 to 8 us faster than streaming loads when it is). A row is owned by
+// TPR threads (whole waves), KV 16-byte vectors each, and stays in registers between its reductions
+// and its outputs. The backward's workgroups walk rows of one group a fixed distance apart and keep
+// t yhat and dn hhat of their columns in fp32 registers; one partial row each per workgroup, summed
+// in a fixed order afterwards, so the parameters' gradients do not depend on timing.
 //
 // Rows of any length and address: vectors are loaded at element alignment, the elements behind
 // the last whole vector by one lane.
