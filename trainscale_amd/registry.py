@@ -25,6 +25,7 @@ import torch
 import torch.nn as nn
 
 import sys
+import types
 
 from .kernels.embedding_kernels import scaled_embedding
 from .kernels.fused_kernels import fast_rms_layernorm, swiglu_forward
@@ -41,21 +42,28 @@ def register_layer_patch(class_name: str, patch_fn: Callable[[nn.Module], None])
     LAYER_PATCHES[class_name] = patch_fn
 
 
+def _patch_forward(module: nn.Module, forward: Callable) -> None:
+    """Makes forward(module, ...) the module's forward. Both it and the module's own, kept as
+    ``_trainscale_amd_forward``, are bound methods: a deep copy of the module gets them bound to
+    itself and runs on its own parameters."""
+    module._trainscale_amd_forward = module.forward
+    module.forward = types.MethodType(forward, module)
+    module._trainscale_amd_patched = True
+
+
 def auto_patch_layernorm(module: nn.Module) -> None:
     """Routes an RMSNorm module's forward to the gfx950 kernel (registry/__init__.py:1033-1054)."""
-    original_forward = module.forward
     eps = getattr(module, "eps", getattr(module, "variance_epsilon", 1e-6))
 
-    def patched_forward(hidden_states):
-        weight = getattr(module, "weight", None)
+    def patched_forward(self, hidden_states):
+        weight = getattr(self, "weight", None)
         if (not isinstance(hidden_states, torch.Tensor) or weight is None
                 or not isinstance(weight, torch.Tensor) or not hidden_states.is_cuda
                 or not weight.is_cuda):
-            return original_forward(hidden_states)
+            return self._trainscale_amd_forward(hidden_states)
         return fast_rms_layernorm(hidden_states, weight, eps)
 
-    module.forward = patched_forward
-    module._trainscale_amd_patched = True
+    _patch_forward(module, patched_forward)
 
 
 for _name in ("LlamaRMSNorm", "Qwen2RMSNorm", "Qwen3RMSNorm", "GemmaRMSNorm", "Gemma2RMSNorm",
@@ -86,15 +94,13 @@ def auto_patch_mlp(module: nn.Module) -> None:
     if not (hasattr(module, "gate_proj") and hasattr(module, "up_proj")
             and hasattr(module, "down_proj")):
         return
-    original_forward = module.forward
 
-    def patched_forward(x):
+    def patched_forward(self, x):
         if not isinstance(x, torch.Tensor) or not x.is_cuda:
-            return original_forward(x)
-        return module.down_proj(swiglu_forward(module.gate_proj(x), module.up_proj(x)))
+            return self._trainscale_amd_forward(x)
+        return self.down_proj(swiglu_forward(self.gate_proj(x), self.up_proj(x)))
 
-    module.forward = patched_forward
-    module._trainscale_amd_patched = True
+    _patch_forward(module, patched_forward)
 
 
 for _name in ("LlamaMLP", "Qwen2MLP", "Qwen3MLP", "MistralMLP", "MixtralBlockSparseTop2MLP",
@@ -170,17 +176,15 @@ def auto_patch_embedding(module: nn.Module) -> None:
     or ask for a sparse one keep their own forward."""
     if module.max_norm is not None or module.scale_grad_by_freq or module.sparse:
         return
-    original_forward = module.forward
 
-    def patched_forward(input):
-        weight = module.weight
+    def patched_forward(self, input):
+        weight = self.weight
         if (not isinstance(input, torch.Tensor) or not input.is_cuda or not weight.is_cuda
                 or weight.dtype not in (torch.float32, torch.bfloat16, torch.float16)):
-            return original_forward(input)
-        return scaled_embedding(input, weight, padding_idx=module.padding_idx)
+            return self._trainscale_amd_forward(input)
+        return scaled_embedding(input, weight, padding_idx=self.padding_idx)
 
-    module.forward = patched_forward
-    module._trainscale_amd_patched = True
+    _patch_forward(module, patched_forward)
 
 
 class KernelPatcher:
