@@ -170,6 +170,13 @@ def test_strided_gradients_that_share_memory():
         assert not _strided_refused(grads), [t.stride() for t in grads]
 
 
+def test_interleaved_slices_of_wide_rows():
+    wide = torch.zeros(6, 12000)
+    assert not _strided_refused([wide[:, ::2], wide[:, 1::4], wide[:, 3::4]])
+    assert _strided_refused([wide[:, ::2], wide[:, 1::4], wide[:, 3::4], wide[5:, 11999]])
+    assert _strided_refused([wide[:, ::2], wide[:, 1::3]])
+
+
 def test_shared_memory_as_by_addresses():
     # against the bytes written down one by one
     gen = torch.Generator().manual_seed(3)

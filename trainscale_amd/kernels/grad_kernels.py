@@ -110,7 +110,7 @@ def _reaches(distance: int, ranges: List[Tuple[int, int, int]], other: bool) -> 
         least, most = reach[k + 1]  # of left - d * stride
         d = range(max(low, -((most - left) // stride)), min(high, (left - least) // stride) + 1)
         tries += len(d)
-        if tries > 4096:
+        if tries > 1 << 16:
             return None
         todo += [(k + 1, left - i * stride, counts or i != 0) for i in d]
     return False
