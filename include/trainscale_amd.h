@@ -620,6 +620,61 @@ ts_status ts_rescale_inplace(void* x, int64_t n, ts_dtype dtype, const float* no
                              const float* used, float* hint_out, ts_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
+/* Gated feed-forward block                                                  */
+/* ------------------------------------------------------------------------ */
+
+enum {
+  TS_ACT_SILU = 0,      /* g / (1 + exp(-g)) */
+  TS_ACT_GELU = 1,      /* g Phi(g), by the error function */
+  TS_ACT_GELU_TANH = 2, /* its tanh form */
+  TS_ACT_RELU = 3
+};
+
+/*
+ * Operands of the block, all of one 16-bit dtype (TS_BF16 or TS_F16), row-major with row strides
+ * in elements: 16-byte aligned, strides and H, F, O multiples of 8 and at most 2^21.
+ */
+typedef struct {
+  const void* x; /* [N, H] */
+  int64_t ldx;
+  const void* w_gate; /* [F, H] */
+  int64_t ld_gate;
+  const void* w_up; /* [F, H] */
+  int64_t ld_up;
+  const void* w_down; /* [O, F]; NULL: the block ends with the gated product */
+  int64_t ld_down;
+  int64_t N, H, F, O;
+  int32_t activation; /* TS_ACT_* */
+  int32_t dtype;
+} ts_gated_mlp_args;
+
+/* Bytes of workspace (O = 0 without w_down); the forward's may be 0. 16-byte aligned. */
+size_t ts_gated_mlp_fwd_workspace_size(int64_t N, int64_t H, int64_t F, int64_t O);
+size_t ts_gated_mlp_bwd_workspace_size(int64_t N, int64_t H, int64_t F, int64_t O);
+
+/*
+ * g = x w_gate^T, u = x w_up^T, act = activation(g) * u, out = act w_down^T: fp32 sums, act and
+ * out rounded once each (out is formed from the rounded act). act: [N, F], out: [N, O] (NULL
+ * without w_down), both contiguous. gate and up, [N, F] each, receive the rounded g and u for the
+ * backward; NULL both: not kept. The three products share their launches' order of sums for a
+ * given shape, so results repeat bit for bit.
+ * Counterpart of the MLP patch's three products and SwiGLU (registry/__init__.py:1080-1091).
+ */
+ts_status ts_gated_mlp_fwd(const ts_gated_mlp_args* args, void* gate, void* up, void* act,
+                           void* out, void* workspace, size_t workspace_bytes,
+                           ts_stream_t stream);
+
+/*
+ * Gradients from dout ([N, O], or [N, F] without w_down, row stride ld_dout) and what the forward
+ * kept, each contiguous in dtype and skipped where NULL: dx [N, H], dw_gate and dw_up [F, H],
+ * dw_down [O, F]. The gradients of g and u are rounded to dtype between the products. N > 0.
+ */
+ts_status ts_gated_mlp_bwd(const ts_gated_mlp_args* args, const void* gate, const void* up,
+                           const void* act, const void* dout, int64_t ld_dout, void* dx,
+                           void* dw_gate, void* dw_up, void* dw_down, void* workspace,
+                           size_t workspace_bytes, ts_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
 /* Token embedding                                                           */
 /* ------------------------------------------------------------------------ */
 

@@ -60,6 +60,13 @@ class PolicyInputs(ctypes.Structure):
                 ("reduction", I32)]
 
 
+class GatedMLPArgs(ctypes.Structure):
+    """ts_gated_mlp_args."""
+    _fields_ = [("x", P), ("ldx", I64), ("w_gate", P), ("ld_gate", I64), ("w_up", P),
+                ("ld_up", I64), ("w_down", P), ("ld_down", I64), ("N", I64), ("H", I64),
+                ("F", I64), ("O", I64), ("activation", I32), ("dtype", I32)]
+
+
 # argtypes of every exported entry point, in header order
 SIGNATURES = {
     "ts_last_error": ([], ctypes.c_char_p),
@@ -118,6 +125,10 @@ SIGNATURES = {
     "ts_swiglu_fwd": ([P, P, P, I64, I32, P], I32),
     "ts_swiglu_bwd": ([P, P, P, P, P, I64, I32, P], I32),
     "ts_rescale_inplace": ([P, I64, I32, P, P, P, P], I32),
+    "ts_gated_mlp_fwd_workspace_size": ([I64, I64, I64, I64], SZ),
+    "ts_gated_mlp_bwd_workspace_size": ([I64, I64, I64, I64], SZ),
+    "ts_gated_mlp_fwd": ([P, P, P, P, P, P, SZ, P], I32),
+    "ts_gated_mlp_bwd": ([P, P, P, P, P, I64, P, P, P, P, P, SZ, P], I32),
     "ts_embedding_fwd": ([P, I64, P, I64, I32, I64, I64, F32, P, I64, P], I32),
     "ts_embedding_bwd_workspace_size": ([I64, I64, I64], SZ),
     "ts_embedding_bwd": ([P, I64, P, I64, I32, I64, I64, F32, I64, P, P, SZ, P], I32),

@@ -1,0 +1,651 @@
+// Gated feed-forward block for gfx950, forward and backward:
+//   g = x Wg^T, u = x Wu^T, a = act(g) * u, y = a Wd^T          (x [N, H], Wg and Wu [F, H], Wd [O, F])
+//   da = dy Wd, dg = da u act'(g), du = da act(g)
+//   dx = dg Wg + du Wu, dWg = dg^T x, dWu = du^T x, dWd = dy^T a
+// act: silu g s(g); gelu g Phi(g); its tanh form g s(2 sqrt(2/pi) (g + 0.044715 g^3)); relu, with
+// s(z) = 1 / (1 + e^-z). Without Wd, y = a.
+//
+// Products run on the MFMA core (gemm.hpp), 16-bit operands and fp32 sums. Nothing is transposed
+// in memory: the backward reads the same weights as MN-major operands. What is fused:
+//   * Both projections are one product: a workgroup's 256 columns are the same 128 columns of g
+//     and of u, so that a lane holds g and u of one element and forms a in registers; x is read
+//     once for both. g and u are written (rounded) only where a backward will need them.
+//   * da never reaches memory: the epilogue of dy Wd reads g and u and writes dg and du.
+//   * dx sums both products in one accumulation (K is the concatenation of dg and du), and
+//     dx, dWg, dWu and dWd, which are independent, share one grid.
+// a is rounded to 16 bits between the products, as dg and du are: MFMA operands are 16-bit.
+#include <math.h>
+
+#include "common.hpp"
+#include "gemm.hpp"
+#include "plan.hpp"
+
+namespace {
+
+using namespace ts;
+using ts_gemm::AccOf;
+using ts_gemm::Cfg;
+using ts_gemm::f32x4;
+using ts_gemm::kKMajor;
+using ts_gemm::kMNMajor;
+using ts_gemm::wide_col;
+using ts_gemm::widen;
+
+// ---------------------------------------------------------------------------
+// Activations. Each keeps NaN, and the relative accuracy of small values of either sign.
+// ---------------------------------------------------------------------------
+__device__ inline float sigmoid_f(float z) {
+  return __builtin_amdgcn_rcpf(1.f + fast_exp2(-z * kLog2e));
+}
+
+constexpr float kGeluK = 0.7978845608028654f;   // sqrt(2 / pi)
+constexpr float kGeluC = 0.044715f;
+constexpr float kSqrtHalf = 0.7071067811865476f;
+constexpr float kInvSqrt2Pi = 0.3989422804014327f;
+// Beyond this the tanh form is g or 0 in fp32; its polynomial would overflow far out.
+constexpr float kGeluFar = 30.f;
+
+template <int kAct>
+__device__ inline float act_f(float g) {
+  if constexpr (kAct == TS_ACT_SILU) {
+    return g * sigmoid_f(g);
+  } else if constexpr (kAct == TS_ACT_GELU) {
+    return 0.5f * g * erfcf(-kSqrtHalf * g);
+  } else if constexpr (kAct == TS_ACT_GELU_TANH) {
+    const float c = fabsf(g) > kGeluFar ? copysignf(kGeluFar, g) : g;
+    return g * sigmoid_f(2.f * kGeluK * c * (1.f + kGeluC * c * c));
+  } else {
+    return g < 0.f ? 0.f : g;
+  }
+}
+
+// act(g), and its derivative in d.
+template <int kAct>
+__device__ inline float act_d(float g, float& d) {
+  if constexpr (kAct == TS_ACT_SILU) {
+    const float s = sigmoid_f(g);
+    d = s * (1.f + g * (1.f - s));
+    return g * s;
+  } else if constexpr (kAct == TS_ACT_GELU) {
+    const float cdf = 0.5f * erfcf(-kSqrtHalf * g);
+    d = cdf + g * kInvSqrt2Pi * fast_exp2(-0.5f * kLog2e * g * g);
+    return g * cdf;
+  } else if constexpr (kAct == TS_ACT_GELU_TANH) {
+    const float c = fabsf(g) > kGeluFar ? copysignf(kGeluFar, g) : g;
+    const float s = sigmoid_f(2.f * kGeluK * c * (1.f + kGeluC * c * c));
+    d = s + c * s * (1.f - s) * 2.f * kGeluK * (1.f + 3.f * kGeluC * c * c);
+    return g * s;
+  } else {
+    d = g > 0.f ? 1.f : g == g ? 0.f : g;
+    return g < 0.f ? 0.f : g;
+  }
+}
+
+// Calls f with the activation as a compile-time constant (a uniform branch).
+template <typename F>
+__device__ inline void with_act(int act, F&& f) {
+  switch (act) {
+    case TS_ACT_SILU: f(std::integral_constant<int, TS_ACT_SILU>()); break;
+    case TS_ACT_GELU: f(std::integral_constant<int, TS_ACT_GELU>()); break;
+    case TS_ACT_GELU_TANH: f(std::integral_constant<int, TS_ACT_GELU_TANH>()); break;
+    default: f(std::integral_constant<int, TS_ACT_RELU>()); break;
+  }
+}
+
+// Two 16-bit roundings in one register, and back.
+template <typename T>
+__device__ inline uint32_t pack2(float lo, float hi) {
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  const t2 v = {(T)lo, (T)hi};
+  return __builtin_bit_cast(uint32_t, v);
+}
+template <typename T>
+__device__ inline void unpack2(uint32_t p, float& lo, float& hi) {
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  const t2 v = __builtin_bit_cast(t2, p);
+  lo = (float)v[0];
+  hi = (float)v[1];
+}
+
+// ---------------------------------------------------------------------------
+// Products on 256 x 256 (kW 8) or 128 x 128 (kW 4) tiles
+// ---------------------------------------------------------------------------
+
+// C [M, N] = sum over the segments s of A_s [M, K] B_s [N, K]^T. Row strides are those of a
+// K-major operand's rows, or between consecutive k of an MN-major one.
+struct Product {
+  const __bf16* A[2];  // 16-bit elements of the kernel's type
+  const __bf16* B[2];
+  int64_t lda, ldb[2];
+  int64_t M, N, K;
+  int32_t segs;
+  int32_t splits;  // slots the segments' joint K (segs * K) is cut into, 1: whole
+  int64_t kper;    // k per slot
+  void* C;         // [M, N], contiguous
+  float* part;     // [splits][M][N] where splits > 1
+};
+
+struct Gated {  // what the gated epilogues read and write, [N, F] contiguous each
+  void* g;
+  void* u;
+  void* a;
+  void* dg;
+  void* du;
+  int32_t act;
+};
+
+enum Epi : int {
+  kEpiStore = 0,     // C, or a slot's fp32 partial
+  kEpiGatedFwd = 1,  // the columns are pairs of g and u: writes a, and g and u where given
+  kEpiGatedBwd = 2   // the product is da: reads g and u, writes dg and du
+};
+
+// The lanes' 16-byte pieces of rows of a [M, N] matrix in the accumulators' order.
+template <int kW, typename F>
+__device__ inline void epi_store(const AccOf<kW>& acc, int64_t M, int64_t N, int64_t gm0,
+                                 int64_t nb, F&& store) {
+  const int g = (threadIdx.x & 63) >> 4;
+#pragma unroll
+  for (int i = 0; i < Cfg<kW>::kTI; ++i) {
+    const int64_t gm = gm0 + 16 * i;
+#pragma unroll
+    for (int p = 0; p < Cfg<kW>::kTJ / 2; ++p) {
+      const int64_t gc = nb + wide_col(p, g);
+      store(acc.t[i][2 * p], acc.t[i][2 * p + 1], gm, gc, gm < M && gc < N);
+    }
+  }
+}
+
+template <typename T, int kEpi, int kMA, int kMB, int kW>
+__device__ inline void product_tile(const Product& a, const Gated& e, int64_t bid, uint8_t* smem) {
+  using C = Cfg<kW>;
+  constexpr bool kPair = kEpi == kEpiGatedFwd;
+  constexpr int kBN = kPair ? C::kBM / 2 : C::kBM;  // columns of C that the tile covers
+  const int64_t MT = (a.M + C::kBM - 1) / C::kBM;
+  const int64_t NT = (a.N + kBN - 1) / kBN;
+  int64_t slot, mt, nt;
+  ts_plan::gemm_piece_of(bid, MT, NT, a.splits, slot, mt, nt);
+  const int64_t m0 = mt * C::kBM, n0 = nt * kBN;
+  const int wid = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int wm = wid >> 1, wn = wid & 1;
+  AccOf<kW> acc;
+  ts_gemm::clear<kW>(acc);
+  if constexpr (kPair) {
+    const ts_gemm::OpLoader<kKMajor, kW> la(a.A[0], a.lda, a.M, m0);
+    const ts_gemm::PairLoader<kW> lb(a.B[0], a.ldb[0], a.B[1], a.ldb[1], a.N, n0);
+    ts_gemm::mainloop_acc<kKMajor, kKMajor, kW, T>(la, lb, a.K, wn * (C::CW / 2),
+                                                   C::kBM / 2 + wn * (C::CW / 2), smem, acc);
+  } else {
+    // dx alone has two segments (dg and du, each its own weight)
+    constexpr int kSegs = kEpi == kEpiStore && kMA == kKMajor && kMB == kMNMajor ? 2 : 1;
+    const int64_t lo = slot * a.kper;  // of the joint K
+    int64_t left = kSegs * a.K - lo < a.kper ? kSegs * a.K - lo : a.kper;
+    int64_t k0 = lo;
+#pragma unroll 1
+    for (int s = 0; s < kSegs; ++s) {
+      const int64_t n = kSegs == 1 || a.K - k0 > left ? left : a.K - k0;
+      if (kSegs == 1 || n > 0) {     // uniform
+        const __bf16* A = a.A[s] + (kMA == kKMajor ? k0 : k0 * a.lda);
+        const __bf16* B = a.B[s] + (kMB == kKMajor ? k0 : k0 * a.ldb[s]);
+        const ts_gemm::OpLoader<kMA, kW> la(A, a.lda, a.M, m0);
+        const ts_gemm::OpLoader<kMB, kW> lb(B, a.ldb[s], a.N, n0);
+        ts_gemm::mainloop_acc<kMA, kMB, kW, T>(la, lb, n, wn * C::CW, wn * C::CW + C::CW / 2,
+                                               smem, acc);
+        left -= n;
+        k0 += n;
+        if (kSegs > 1) __syncthreads();  // the operands' tiles in LDS are free again
+      }
+      k0 -= a.K;
+    }
+  }
+  const int64_t gm0 = m0 + wm * C::RW + (lane & 15);  // this lane's row of row block i: gm0 + 16 i
+  const int g4 = lane >> 4;
+  if constexpr (kEpi == kEpiStore) {
+    const int64_t nb = n0 + wn * C::CW;
+    if (a.splits > 1) {
+      float* P = a.part + slot * a.M * a.N;
+#pragma unroll
+      for (int i = 0; i < C::kTI; ++i)
+#pragma unroll
+        for (int j = 0; j < C::kTJ; ++j) {
+          const int64_t gm = gm0 + 16 * i, gc = nb + j * 16 + g4 * 4;
+          if (gm < a.M && gc < a.N) *reinterpret_cast<f32x4*>(P + gm * a.N + gc) = acc.t[i][j];
+        }
+    } else {
+      T* out = static_cast<T*>(a.C);
+      epi_store<kW>(acc, a.M, a.N, gm0, nb,
+                    [&](const f32x4& x, const f32x4& y, int64_t gm, int64_t gc, bool in) {
+                      const u32x4 v = widen(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]),
+                                            pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]));
+                      if (in) st16(out + gm * a.N + gc, v);
+                    });
+    }
+  } else if constexpr (kEpi == kEpiGatedFwd) {
+    // column tiles 0 .. kHJ - 1 are g, the others u of the same columns
+    const int64_t nb = n0 + wn * (C::CW / 2);
+    T* G = static_cast<T*>(e.g);
+    T* U = static_cast<T*>(e.u);
+    T* O = static_cast<T*>(e.a);
+    auto rows = [&](const f32x4 (&t)[C::kTI][C::kTJ], int j0, T* out) {
+#pragma unroll
+      for (int i = 0; i < C::kTI; ++i)
+#pragma unroll
+        for (int p = 0; p < C::kHJ / 2; ++p) {
+          const int64_t gm = gm0 + 16 * i, gc = nb + wide_col(p, g4);
+          const f32x4 x = t[i][j0 + 2 * p], y = t[i][j0 + 2 * p + 1];
+          const u32x4 v = widen(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]),
+                                pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]));
+          if (gm < a.M && gc < a.N) st16(out + gm * a.N + gc, v);
+        }
+    };
+    if (G != nullptr) {
+      rows(acc.t, 0, G);
+      rows(acc.t, C::kHJ, U);
+    }
+    with_act(e.act, [&](auto act) {
+#pragma unroll
+      for (int i = 0; i < C::kTI; ++i)
+#pragma unroll
+        for (int j = 0; j < C::kHJ; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            acc.t[i][j][q] = act_f<decltype(act)::value>(acc.t[i][j][q]) * acc.t[i][C::kHJ + j][q];
+    });
+    rows(acc.t, 0, O);
+  } else {
+    const int64_t nb = n0 + wn * C::CW;
+    const T* G = static_cast<const T*>(e.g);
+    const T* U = static_cast<const T*>(e.u);
+    T* DG = static_cast<T*>(e.dg);
+    T* DU = static_cast<T*>(e.du);
+    with_act(e.act, [&](auto act) {
+#pragma unroll
+      for (int i = 0; i < C::kTI; ++i) {
+        const int64_t gm = gm0 + 16 * i;
+        // a row block's old values are loaded before the first is used
+        u32x4 qg[C::kTJ / 2], qu[C::kTJ / 2];
+#pragma unroll
+        for (int p = 0; p < C::kTJ / 2; ++p) {
+          const int64_t gc = nb + wide_col(p, g4);
+          const bool in = gm < a.M && gc < a.N;
+          qg[p] = in ? ld16(G + gm * a.N + gc) : u32x4{0u, 0u, 0u, 0u};
+          qu[p] = in ? ld16(U + gm * a.N + gc) : u32x4{0u, 0u, 0u, 0u};
+        }
+#pragma unroll
+        for (int p = 0; p < C::kTJ / 2; ++p) {
+          const int64_t gc = nb + wide_col(p, g4);
+          // back to the accumulators' layout
+          const u32x4 vg = widen(qg[p][0], qg[p][1], qg[p][2], qg[p][3]);
+          const u32x4 vu = widen(qu[p][0], qu[p][1], qu[p][2], qu[p][3]);
+          uint32_t pg[4], pu[4];
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const f32x4 da = acc.t[i][2 * p + h / 2];
+            float g[2], u[2], t, d, og[2], ou[2];
+            unpack2<T>(vg[h], g[0], g[1]);
+            unpack2<T>(vu[h], u[0], u[1]);
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+              const float x = da[2 * (h & 1) + b];
+              t = act_d<decltype(act)::value>(g[b], d);
+              og[b] = x * u[b] * d;
+              ou[b] = x * t;
+            }
+            pg[h] = pack2<T>(og[0], og[1]);
+            pu[h] = pack2<T>(ou[0], ou[1]);
+          }
+          const u32x4 wg = widen(pg[0], pg[1], pg[2], pg[3]);
+          const u32x4 wu = widen(pu[0], pu[1], pu[2], pu[3]);
+          if (gm < a.M && gc < a.N) {
+            st16(DG + gm * a.N + gc, wg);
+            st16(DU + gm * a.N + gc, wu);
+          }
+        }
+      }
+    });
+  }
+}
+
+template <typename T, int kEpi, int kMA, int kMB, int kW>
+__global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void mlp_product(const Product a, const Gated e) {
+  __shared__ __attribute__((aligned(16))) uint8_t smem[Cfg<kW>::kLdsBytes];
+  product_tile<T, kEpi, kMA, kMB, kW>(a, e, blockIdx.x, smem);
+}
+
+// dx and the weights' gradients in one grid: they are independent, and the tiles of one fill the
+// CUs that another leaves.
+struct Grads {
+  Product dx;     // pieces 0 .. end[0]
+  Product dw[3];  // dWg, dWu, dWd: up to end[1], end[2], end[3]
+  int64_t end[4];
+};
+
+template <typename T, int kW>
+__global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void mlp_grads(const Grads a) {
+  __shared__ __attribute__((aligned(16))) uint8_t smem[Cfg<kW>::kLdsBytes];
+  const int64_t bid = blockIdx.x;
+  const Gated none{};
+  if (bid < a.end[0]) {
+    product_tile<T, kEpiStore, kKMajor, kMNMajor, kW>(a.dx, none, bid, smem);
+  } else {
+    const int w = bid < a.end[1] ? 0 : bid < a.end[2] ? 1 : 2;
+    product_tile<T, kEpiStore, kMNMajor, kMNMajor, kW>(a.dw[w], none, bid - a.end[w], smem);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Partials of a split K, added in slot order and rounded once
+// ---------------------------------------------------------------------------
+struct SumJobs {
+  const float* part[4];
+  void* out[4];
+  int64_t quads[4];  // elements / 4
+  int32_t splits[4];
+  int64_t end[4];    // workgroups up to and with this job
+};
+constexpr int kSumUnroll = 8;
+
+template <typename T>
+__global__ __launch_bounds__(256) void mlp_sum_slots(const SumJobs s) {
+  const int64_t bid = blockIdx.x;
+  int j = 0;
+  while (j < 3 && bid >= s.end[j]) ++j;
+  const int64_t i = (bid - (j ? s.end[j - 1] : 0)) * 256 + threadIdx.x;
+  const int64_t n = s.quads[j];
+  if (i >= n) return;
+  const f32x4* p = reinterpret_cast<const f32x4*>(s.part[j]);
+  f32x4 sum{0.f, 0.f, 0.f, 0.f};
+  for (int p0 = 0; p0 < s.splits[j]; p0 += kSumUnroll) {
+    f32x4 v[kSumUnroll];
+#pragma unroll
+    for (int q = 0; q < kSumUnroll; ++q)
+      v[q] = p0 + q < s.splits[j] ? p[(p0 + q) * n + i] : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < kSumUnroll; ++q) sum += v[q];
+  }
+  static_cast<uint2*>(s.out[j])[i] = make_uint2(pack2<T>(sum[0], sum[1]), pack2<T>(sum[2], sum[3]));
+}
+
+// ---------------------------------------------------------------------------
+// Without the down projection: dg and du of da = dy, element by element
+// ---------------------------------------------------------------------------
+template <typename T>
+__global__ __launch_bounds__(256) void mlp_gate_bwd(const T* __restrict__ da, int64_t ldd,
+                                                    const T* __restrict__ g,
+                                                    const T* __restrict__ u, T* __restrict__ dg,
+                                                    T* __restrict__ du, int64_t nvec, int64_t F8,
+                                                    int act) {
+  const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (v >= nvec) return;
+  const int64_t r = v / F8;
+  const u32x4 qd = ld16_any_stream(da + r * ldd + (v - r * F8) * 8);
+  const u32x4 qg = ld16_stream(g + v * 8), qu = ld16_stream(u + v * 8);
+  float d[8], G[8], U[8];
+  Elt<T>::unpack(qd, d);
+  Elt<T>::unpack(qg, G);
+  Elt<T>::unpack(qu, U);
+  with_act(act, [&](auto a) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float dt;
+      const float t = act_d<decltype(a)::value>(G[i], dt);
+      G[i] = d[i] * U[i] * dt;
+      U[i] = d[i] * t;
+    }
+  });
+  st16(dg + v * 8, Elt<T>::pack(G));
+  st16(du + v * 8, Elt<T>::pack(U));
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+ts_plan::MlpShape shape_of(const ts_gated_mlp_args& a) {
+  return ts_plan::MlpShape{a.N, a.H, a.F, a.w_down != nullptr ? a.O : 0};
+}
+
+constexpr int64_t kMaxDim = (int64_t)1 << 21;  // 32-bit offsets inside a tile
+
+ts_status check_args(const char* who, const ts_gated_mlp_args* a) {
+  using ts_host::fail;
+  if (a == nullptr) return fail(TS_ERR_INVALID_ARGUMENT, "%s: NULL arguments", who);
+  if (a->dtype != TS_BF16 && a->dtype != TS_F16)
+    return fail(TS_ERR_UNSUPPORTED_DTYPE, "%s: dtype must be bf16 or fp16", who);
+  if (a->activation < TS_ACT_SILU || a->activation > TS_ACT_RELU)
+    return fail(TS_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", who, (int)a->activation);
+  const bool down = a->w_down != nullptr;
+  if (a->N < 0 || a->H <= 0 || a->F <= 0 || (down && a->O <= 0))
+    return fail(TS_ERR_SHAPE, "%s: bad shape N=%lld H=%lld F=%lld O=%lld", who, (long long)a->N,
+                (long long)a->H, (long long)a->F, (long long)a->O);
+  if (a->H % 8 || a->F % 8 || (down && a->O % 8))
+    return fail(TS_ERR_SHAPE, "%s: H, F and O must be multiples of 8", who);
+  if (a->H > kMaxDim || a->F > kMaxDim || (down && a->O > kMaxDim) ||
+      a->N > ((int64_t)1 << 31))
+    return fail(TS_ERR_SHAPE, "%s: more than 2^21 features or 2^31 rows", who);
+  if (a->ldx < a->H || a->ld_gate < a->H || a->ld_up < a->H || (down && a->ld_down < a->F))
+    return fail(TS_ERR_SHAPE, "%s: row stride shorter than a row", who);
+  if (a->ldx % 8 || a->ld_gate % 8 || a->ld_up % 8 || (down && a->ld_down % 8))
+    return fail(TS_ERR_SHAPE, "%s: row strides must be multiples of 8", who);
+  if (a->ldx > kMaxDim || a->ld_gate > kMaxDim || a->ld_up > kMaxDim ||
+      (down && a->ld_down > kMaxDim))
+    return fail(TS_ERR_SHAPE, "%s: row strides above 2^21", who);
+  if (a->N > 0 && (a->x == nullptr || a->w_gate == nullptr || a->w_up == nullptr))
+    return fail(TS_ERR_INVALID_ARGUMENT, "%s: NULL operand", who);
+  if (!ts_host::aligned16(a->x) || !ts_host::aligned16(a->w_gate) ||
+      !ts_host::aligned16(a->w_up) || !ts_host::aligned16(a->w_down))
+    return fail(TS_ERR_INVALID_ARGUMENT, "%s: operands must be 16-byte aligned", who);
+  return TS_OK;
+}
+
+template <typename T>
+const __bf16* raw(const T* p) { return reinterpret_cast<const __bf16*>(p); }
+const __bf16* raw(const void* p) { return static_cast<const __bf16*>(p); }
+
+Product product(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N,
+                int64_t K, void* C) {
+  Product p{};
+  p.A[0] = p.A[1] = raw(A);
+  p.B[0] = p.B[1] = raw(B);
+  p.lda = lda;
+  p.ldb[0] = p.ldb[1] = ldb;
+  p.M = M;
+  p.N = N;
+  p.K = K;
+  p.segs = 1;
+  p.splits = 1;
+  p.kper = K;
+  p.C = C;
+  return p;
+}
+
+void set_split(Product& p, const ts_plan::KSplit& k, float* part) {
+  p.splits = (int32_t)k.splits;
+  p.kper = k.splits > 1 ? k.kper : p.segs * p.K;
+  p.part = part;
+}
+
+template <typename T, int kEpi, int kMA, int kMB>
+ts_status launch_product(const Product& p, const Gated& e, int waves, hipStream_t st,
+                         const char* name) {
+  const int64_t tiles = ts_plan::mlp_tiles(p.M, p.N, waves, kEpi == kEpiGatedFwd) * p.splits;
+  if (tiles <= 0) return TS_OK;
+  if (tiles > 0x7fffffffLL) return ts_host::fail(TS_ERR_SHAPE, "%s: too many tiles", name);
+  if (waves == 8)
+    hipLaunchKernelGGL((mlp_product<T, kEpi, kMA, kMB, 8>), dim3((unsigned)tiles), dim3(512), 0,
+                       st, p, e);
+  else
+    hipLaunchKernelGGL((mlp_product<T, kEpi, kMA, kMB, 4>), dim3((unsigned)tiles), dim3(256), 0,
+                       st, p, e);
+  return ts_host::check_launch(name);
+}
+
+void add_job(SumJobs& s, int& n, const Product& p) {
+  if (p.C == nullptr || p.splits <= 1) return;
+  s.part[n] = p.part;
+  s.out[n] = p.C;
+  s.quads[n] = p.M * p.N / 4;
+  s.splits[n] = p.splits;
+  s.end[n] = (n ? s.end[n - 1] : 0) + (s.quads[n] + 255) / 256;
+  ++n;
+}
+
+template <typename T>
+ts_status launch_sums(SumJobs& s, int n, hipStream_t st) {
+  if (n == 0) return TS_OK;
+  const int64_t blocks = s.end[n - 1];
+  for (int j = n; j < 4; ++j) s.end[j] = blocks;
+  if (blocks > 0x7fffffffLL) return ts_host::fail(TS_ERR_SHAPE, "mlp_sum_slots: too large");
+  hipLaunchKernelGGL(mlp_sum_slots<T>, dim3((unsigned)blocks), dim3(256), 0, st, s);
+  return ts_host::check_launch("mlp_sum_slots");
+}
+
+#define TS_TRY(x)                  \
+  do {                             \
+    const ts_status s_ = (x);      \
+    if (s_ != TS_OK) return s_;    \
+  } while (0)
+
+template <typename T>
+ts_status fwd_typed(const ts_gated_mlp_args& a, void* gate, void* up, void* act, void* out,
+                    void* ws, hipStream_t st) {
+  const ts_plan::MlpPlan pl = ts_plan::mlp_plan(shape_of(a));
+  Product p = product(a.x, a.ldx, a.w_gate, a.ld_gate, a.N, a.F, a.H, nullptr);
+  p.B[1] = raw(a.w_up);
+  p.ldb[1] = a.ld_up;
+  const Gated e{gate, up, act, nullptr, nullptr, a.activation};
+  TS_TRY((launch_product<T, kEpiGatedFwd, kKMajor, kKMajor>(p, e, pl.up_waves, st, "mlp_gated")));
+  if (out == nullptr) return TS_OK;
+  Product d = product(act, a.F, a.w_down, a.ld_down, a.N, a.O, a.F, out);
+  set_split(d, pl.down, static_cast<float*>(ws));
+  TS_TRY((launch_product<T, kEpiStore, kKMajor, kKMajor>(d, e, pl.down_waves, st, "mlp_down")));
+  SumJobs s{};
+  int n = 0;
+  add_job(s, n, d);
+  return launch_sums<T>(s, n, st);
+}
+
+template <typename T, int kW>
+ts_status launch_grads(const Grads& g, hipStream_t st) {
+  if (g.end[3] <= 0) return TS_OK;
+  if (g.end[3] > 0x7fffffffLL) return ts_host::fail(TS_ERR_SHAPE, "mlp_grads: too many tiles");
+  hipLaunchKernelGGL((mlp_grads<T, kW>), dim3((unsigned)g.end[3]), dim3(64 * kW), 0, st, g);
+  return ts_host::check_launch("mlp_grads");
+}
+
+template <typename T>
+ts_status bwd_typed(const ts_gated_mlp_args& a, const void* gate, const void* up, const void* act,
+                    const void* dout, int64_t ldd, void* dx, void* dwg, void* dwu, void* dwd,
+                    uint8_t* ws, hipStream_t st) {
+  const ts_plan::MlpShape sh = shape_of(a);
+  const ts_plan::MlpPlan pl = ts_plan::mlp_plan(sh);
+  const ts_plan::MlpBwdWorkspace w = ts_plan::mlp_bwd_workspace(sh);
+  void* dg = ws + w.dg;
+  void* du = ws + w.du;
+  const bool inner = dx != nullptr || dwg != nullptr || dwu != nullptr;
+  if (inner && a.w_down != nullptr) {
+    const Product p = product(dout, ldd, a.w_down, a.ld_down, a.N, a.F, a.O, nullptr);
+    const Gated e{const_cast<void*>(gate), const_cast<void*>(up), nullptr, dg, du, a.activation};
+    TS_TRY((launch_product<T, kEpiGatedBwd, kKMajor, kMNMajor>(p, e, pl.da_waves, st,
+                                                               "mlp_gated_bwd")));
+  } else if (inner) {
+    const int64_t nvec = a.N * a.F / 8, blocks = (nvec + 255) / 256;
+    if (blocks > 0x7fffffffLL) return ts_host::fail(TS_ERR_SHAPE, "mlp_gate_bwd: too large");
+    hipLaunchKernelGGL(mlp_gate_bwd<T>, dim3((unsigned)blocks), dim3(256), 0, st,
+                       static_cast<const T*>(dout), ldd, static_cast<const T*>(gate),
+                       static_cast<const T*>(up), static_cast<T*>(dg), static_cast<T*>(du), nvec,
+                       a.F / 8, (int)a.activation);
+    TS_TRY(ts_host::check_launch("mlp_gate_bwd"));
+  }
+  Grads g{};
+  g.dx = product(dg, a.F, a.w_gate, a.ld_gate, a.N, a.H, a.F, dx);
+  g.dx.A[1] = raw(du);
+  g.dx.B[1] = raw(a.w_up);
+  g.dx.ldb[1] = a.ld_up;
+  g.dx.segs = 2;
+  g.dw[0] = product(dg, a.F, a.x, a.ldx, a.F, a.H, a.N, dwg);
+  g.dw[1] = product(du, a.F, a.x, a.ldx, a.F, a.H, a.N, dwu);
+  g.dw[2] = product(dout, ldd, act, a.F, a.O, a.F, a.N, dwd);
+  set_split(g.dx, pl.dx, reinterpret_cast<float*>(ws + w.dx));
+  for (int i = 0; i < 3; ++i)
+    set_split(g.dw[i], i < 2 ? pl.dw : pl.dwd, reinterpret_cast<float*>(ws + w.dw[i]));
+  SumJobs s{};
+  int n = 0;
+  int64_t end = 0;
+  for (int i = 0; i < 4; ++i) {
+    const Product& p = i == 0 ? g.dx : g.dw[i - 1];
+    if (p.C != nullptr) end += ts_plan::mlp_tiles(p.M, p.N, pl.grad_waves, false) * p.splits;
+    g.end[i] = end;
+    add_job(s, n, p);
+  }
+  TS_TRY((pl.grad_waves == 8 ? launch_grads<T, 8>(g, st) : launch_grads<T, 4>(g, st)));
+  return launch_sums<T>(s, n, st);
+}
+
+}  // namespace
+
+extern "C" size_t ts_gated_mlp_fwd_workspace_size(int64_t N, int64_t H, int64_t F, int64_t O) {
+  if (N <= 0 || H <= 0 || F <= 0 || O < 0) return 0;
+  return (size_t)ts_plan::mlp_fwd_workspace(ts_plan::MlpShape{N, H, F, O});
+}
+
+extern "C" size_t ts_gated_mlp_bwd_workspace_size(int64_t N, int64_t H, int64_t F, int64_t O) {
+  if (N <= 0 || H <= 0 || F <= 0 || O < 0) return 0;
+  return (size_t)ts_plan::mlp_bwd_workspace(ts_plan::MlpShape{N, H, F, O}).total;
+}
+
+extern "C" ts_status ts_gated_mlp_fwd(const ts_gated_mlp_args* args, void* gate, void* up,
+                                      void* act, void* out, void* workspace,
+                                      size_t workspace_bytes, ts_stream_t stream) {
+  using ts_host::fail;
+  TS_TRY(check_args("gated_mlp_fwd", args));
+  if (args->N == 0) return TS_OK;
+  if (act == nullptr || (out == nullptr) != (args->w_down == nullptr))
+    return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_fwd: out goes with w_down, act is needed");
+  if ((gate == nullptr) != (up == nullptr))
+    return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_fwd: gate and up are kept together");
+  if (!ts_host::aligned16(gate) || !ts_host::aligned16(up) || !ts_host::aligned16(act) ||
+      !ts_host::aligned16(out) || !ts_host::aligned16(workspace))
+    return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_fwd: outputs must be 16-byte aligned");
+  const size_t need = (size_t)ts_plan::mlp_fwd_workspace(shape_of(*args));
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
+    return fail(TS_ERR_WORKSPACE, "gated_mlp_fwd: workspace of %zu bytes, need %zu",
+                workspace_bytes, need);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  return args->dtype == TS_BF16 ? fwd_typed<__bf16>(*args, gate, up, act, out, workspace, st)
+                                : fwd_typed<_Float16>(*args, gate, up, act, out, workspace, st);
+}
+
+extern "C" ts_status ts_gated_mlp_bwd(const ts_gated_mlp_args* args, const void* gate,
+                                      const void* up, const void* act, const void* dout,
+                                      int64_t ld_dout, void* dx, void* dw_gate, void* dw_up,
+                                      void* dw_down, void* workspace, size_t workspace_bytes,
+                                      ts_stream_t stream) {
+  using ts_host::fail;
+  TS_TRY(check_args("gated_mlp_bwd", args));
+  if (args->N == 0) return fail(TS_ERR_SHAPE, "gated_mlp_bwd: no rows (the gradients are zeros)");
+  const bool down = args->w_down != nullptr;
+  if (gate == nullptr || up == nullptr || dout == nullptr || (down && act == nullptr))
+    return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_bwd: NULL operand");
+  if (!down && dw_down != nullptr)
+    return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_bwd: dw_down without w_down");
+  const int64_t cols = down ? args->O : args->F;
+  if (ld_dout < cols || ld_dout % 8 || ld_dout > kMaxDim)
+    return fail(TS_ERR_SHAPE, "gated_mlp_bwd: bad row stride of dout");
+  for (const void* p : {gate, up, act, dout, (const void*)dx, (const void*)dw_gate,
+                        (const void*)dw_up, (const void*)dw_down, (const void*)workspace})
+    if (!ts_host::aligned16(p))
+      return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_bwd: buffers must be 16-byte aligned");
+  const size_t need = (size_t)ts_plan::mlp_bwd_workspace(shape_of(*args)).total;
+  if (workspace == nullptr || workspace_bytes < need)
+    return fail(TS_ERR_WORKSPACE, "gated_mlp_bwd: workspace of %zu bytes, need %zu",
+                workspace_bytes, need);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  return args->dtype == TS_BF16
+             ? bwd_typed<__bf16>(*args, gate, up, act, dout, ld_dout, dx, dw_gate, dw_up, dw_down,
+                                 ws, st)
+             : bwd_typed<_Float16>(*args, gate, up, act, dout, ld_dout, dx, dw_gate, dw_up,
+                                   dw_down, ws, st);
+}

@@ -38,6 +38,9 @@ using ts_gemm::Acc;
 using ts_gemm::BM;
 using ts_gemm::BN;
 using ts_gemm::f32x4;
+using ts_gemm::swap_rows;
+using ts_gemm::wide_col;
+using ts_gemm::widen;
 
 enum EpiMode : int {
   kEpiLogits = 0,     // bf16 C + row statistics
@@ -107,28 +110,6 @@ __device__ inline uint32_t pack2(float lo, float hi) {
 }
 __device__ inline float lo_f(uint32_t p) { return __builtin_bit_cast(float, p << 16); }
 __device__ inline float hi_f(uint32_t p) { return __builtin_bit_cast(float, p & 0xffff0000u); }
-
-// Exchanges the odd 16-lane rows of x with the even ones of y.
-__device__ inline void swap_rows(uint32_t& x, uint32_t& y) {
-  typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
-  const u32x2_t r =
-      __builtin_bit_cast(u32x2_t, __builtin_amdgcn_permlane16_swap(x, y, false, false));
-  x = r[0];
-  y = r[1];
-}
-
-// Rows of the epilogue in registers. Of 16 x 16 tile j of a row block, lane l holds row
-// l % 16 and columns 16 j + 4 g + e (g = l / 16, e < 4), in bf16 two packed registers. Two
-// tiles of 8-byte pieces become one 16-byte piece of 8 consecutive columns by swapping lane
-// rows: afterwards lane group g holds columns 8 * (g / 2) .. + 8 of tile 2p + g % 2, and the
-// four groups of a row 64 consecutive bytes of C. The exchange is its own inverse.
-__device__ inline u32x4 widen(uint32_t x0, uint32_t x1, uint32_t y0, uint32_t y1) {
-  swap_rows(x0, y0);
-  swap_rows(x1, y1);
-  return u32x4{x0, x1, y0, y1};
-}
-// Column, within the wave's 128, of the piece p < 4 that lane group g holds after widen.
-__device__ inline int wide_col(int p, int g) { return (2 * p + (g & 1)) * 16 + (g >> 1) * 8; }
 
 // Maximum and sum over the four lanes that share a row (l % 16); every lane gets the result.
 __device__ inline float groups_max(float v) {

@@ -363,6 +363,56 @@ inline int64_t hidden_split_bytes_any_shape(int64_t M) {
 }
 
 // ---------------------------------------------------------------------------
+// Gated feed-forward block: x [N, H], two weights [F, H], one [O, F] (O = 0: none).
+// ---------------------------------------------------------------------------
+struct MlpShape {
+  int64_t N, H, F, O;
+};
+// Tiles of an [M, N] result on 32 * waves squared tiles; a pair of products' (pair) cover half
+// the columns each.
+inline int64_t mlp_tiles(int64_t M, int64_t N, int waves, bool pair) {
+  const int64_t bm = 32 * waves, bn = pair ? bm / 2 : bm;
+  return ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
+}
+struct MlpPlan {
+  int up_waves, down_waves, da_waves, grad_waves;
+  KSplit down, dx, dw, dwd;
+};
+inline MlpPlan mlp_plan(const MlpShape& s) {
+  const KSplit one{1, 0};
+  (void)s;
+  return MlpPlan{8, 8, 8, 8, one, one, one, one};
+}
+inline int64_t mlp_part_bytes(const KSplit& k, int64_t M, int64_t N) {
+  return k.splits > 1 ? k.splits * M * N * 4 : 0;
+}
+inline int64_t mlp_fwd_workspace(const MlpShape& s) {
+  return s.O > 0 ? mlp_part_bytes(mlp_plan(s).down, s.N, s.O) : 0;
+}
+// Byte offsets in the backward's workspace: dg and du, then the partials.
+struct MlpBwdWorkspace {
+  int64_t dg, du, dx, dw[3], total;
+};
+inline MlpBwdWorkspace mlp_bwd_workspace(const MlpShape& s) {
+  const MlpPlan p = mlp_plan(s);
+  MlpBwdWorkspace w{};
+  int64_t off = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = off;
+    off += (bytes + 255) / 256 * 256;
+    return o;
+  };
+  w.dg = take(2 * s.N * s.F);
+  w.du = take(2 * s.N * s.F);
+  w.dx = take(mlp_part_bytes(p.dx, s.N, s.H));
+  w.dw[0] = take(mlp_part_bytes(p.dw, s.F, s.H));
+  w.dw[1] = take(mlp_part_bytes(p.dw, s.F, s.H));
+  w.dw[2] = take(s.O > 0 ? mlp_part_bytes(p.dwd, s.O, s.F) : 0);
+  w.total = off;
+  return w;
+}
+
+// ---------------------------------------------------------------------------
 // Addressing of the streaming and row kernels. The kernels compute their
 // accesses with these functions, and tests/test_plan.py sweeps them with the
 // launch shapes the host computes: every access lies inside its tensor and

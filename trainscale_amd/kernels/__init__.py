@@ -33,6 +33,12 @@ from .layernorm_kernels import (
     fused_sandwich_rms_layernorm,
     rms_layernorm,
 )
+from .mlp_kernels import (
+    FusedGatedMLP,
+    GatedMLPFunction,
+    fused_gated_linear,
+    fused_gated_mlp,
+)
 from .rope_kernels import (
     Fast_RoPE_Embedding,
     FusedRoPEQKFunction,
@@ -54,6 +60,10 @@ __all__ = [
     "fast_cross_entropy_loss",
     "Fast_SwiGLU",
     "swiglu_forward",
+    "GatedMLPFunction",
+    "fused_gated_linear",
+    "fused_gated_mlp",
+    "FusedGatedMLP",
     "Fast_RMS_LayerNorm",
     "HipRMSNorm",
     "TritonRMSNorm",

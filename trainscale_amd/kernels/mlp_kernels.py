@@ -1,0 +1,138 @@
+"""Gated feed-forward block: both projections, the activation and the product in one kernel.
+
+``fused_gated_mlp(x, gate, up, down)`` is ``(act(x gate^T) * (x up^T)) down^T``, the block whose
+elementwise part alone is ``Fast_SwiGLU``; ``fused_gated_linear`` is the same without the down
+projection. Weights have ``nn.Linear``'s layout. bf16 and fp16; the sums are fp32, and what lies
+between the products (the gated product forward, the gradients of both projections backward) is
+rounded to the data type once, where the unfused block rounds g, u, act(g) and the product.
+
+The forward keeps x, the weights, both projections and the gated product for the backward:
+3 N F 16-bit values beside x. Without a gradient to compute only the gated product is formed.
+"""
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+import torch.nn as nn
+from torch import Tensor
+from torch.autograd.function import once_differentiable
+
+from .. import ops
+
+__all__ = ["ACTIVATIONS", "GatedMLPFunction", "fused_gated_linear", "fused_gated_mlp",
+           "FusedGatedMLP"]
+
+# activation -> TS_ACT_*
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
+
+
+def _check(x: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], activation: str) -> int:
+    what = "fused_gated_linear" if down is None else "fused_gated_mlp"
+    code = ACTIVATIONS.get(activation)
+    if code is None:
+        raise ValueError(f"{what}: unknown activation {activation!r} ({', '.join(ACTIVATIONS)})")
+    if x.dtype is not torch.bfloat16 and x.dtype is not torch.float16:
+        raise TypeError(f"{what}: x must be bfloat16 or float16, got {x.dtype}")
+    for name, t in (("gate", gate), ("up", up), ("down", down)):
+        if t is not None and t.dtype is not x.dtype:
+            raise TypeError(f"{what}: {name} weight dtype {t.dtype} != x dtype {x.dtype}")
+    if x.dim() < 1 or gate.dim() != 2 or gate.shape[1] != x.shape[-1] or 0 in gate.shape:
+        raise ValueError(f"{what}: gate weight {tuple(gate.shape)} for x {tuple(x.shape)}")
+    if up.shape != gate.shape:
+        raise ValueError(f"{what}: up weight {tuple(up.shape)} != gate weight "
+                         f"{tuple(gate.shape)}")
+    if down is not None and (down.dim() != 2 or down.shape[1] != gate.shape[0]
+                             or down.shape[0] == 0):
+        raise ValueError(f"{what}: down weight {tuple(down.shape)} for a gate weight "
+                         f"{tuple(gate.shape)}")
+    return code
+
+
+def _forward(x: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], activation: str,
+             keep: bool):
+    """(result, the activation's code, kept g, u and gated product or None)."""
+    code = _check(x, gate, up, down, activation)
+    cols = (gate if down is None else down).shape[0]
+    x2d = x.reshape(-1, x.shape[-1])
+    g, u, a, y = ops.gated_mlp_forward(x2d, gate, up, down, code, keep)
+    out = a if down is None else y
+    if out.shape[1] != cols:
+        out = out[:, :cols].contiguous()
+    return out.view(*x.shape[:-1], cols), code, (g, u, None if down is None else a)
+
+
+class GatedMLPFunction(torch.autograd.Function):
+    """forward(x [..., H], gate [F, H], up [F, H], down [O, F] or None, activation) -> [..., O] or
+    [..., F]; differentiable in the four tensors."""
+
+    @staticmethod
+    def forward(ctx, x: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor],
+                activation: str) -> Tensor:
+        out, ctx.code, kept = _forward(x, gate, up, down, activation, True)
+        ctx.save_for_backward(x, gate, up, down, *kept)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout: Tensor):
+        x, gate, up, down, g, u, a = ctx.saved_tensors
+        grads = ops.gated_mlp_backward(
+            x.reshape(-1, x.shape[-1]), gate, up, down, ctx.code, g, u, a,
+            dout.reshape(-1, dout.shape[-1]), ctx.needs_input_grad[:4])
+        if grads[0] is not None:
+            grads[0] = grads[0].view(x.shape)
+        return (*grads, None)
+
+
+def _apply(x: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor],
+           activation: str) -> Tensor:
+    if ops.in_forward_ad() or (torch.is_grad_enabled() and (
+            x.requires_grad or gate.requires_grad or up.requires_grad
+            or (down is not None and down.requires_grad))):
+        return GatedMLPFunction.apply(x, gate, up, down, activation)
+    return _forward(x, gate, up, down, activation, False)[0]
+
+
+def fused_gated_linear(x: Tensor, gate: Tensor, up: Tensor, activation: str = "silu") -> Tensor:
+    """act(x @ gate.T) * (x @ up.T): x [..., H], gate and up [F, H], all bf16 or all fp16; the
+    result is [..., F]. activation: "silu", "gelu" (the error function's form), "gelu_tanh" or
+    "relu". Differentiable in all three. Any sizes and strides; sizes or row strides that are not
+    multiples of 8, or rows that do not start at 16 bytes, cost a copy of that operand."""
+    return _apply(x, gate, up, None, activation)
+
+
+def fused_gated_mlp(x: Tensor, gate: Tensor, up: Tensor, down: Tensor,
+                    activation: str = "silu") -> Tensor:
+    """fused_gated_linear(x, gate, up, activation) @ down.T with down [O, F]: [..., O].
+    Differentiable in all four tensors, in one backward whose gradients of the projections never
+    exist unfused."""
+    return _apply(x, gate, up, down, activation)
+
+
+class FusedGatedMLP(nn.Module):
+    """A gated feed-forward block on ``fused_gated_mlp`` with the weights of three bias-free
+    ``nn.Linear`` layers, under their usual names and with their initialisation."""
+
+    def __init__(self, hidden_size: int, intermediate_size: int, activation: str = "silu",
+                 device: Optional[torch.device] = None, dtype: Optional[torch.dtype] = None):
+        super().__init__()
+        if activation not in ACTIVATIONS:
+            raise ValueError(f"FusedGatedMLP: unknown activation {activation!r}")
+        self.hidden_size = hidden_size
+        self.intermediate_size = intermediate_size
+        self.activation = activation
+
+        def linear(i, o):
+            return nn.Linear(i, o, bias=False, device=device, dtype=dtype)
+
+        self.gate_proj = linear(hidden_size, intermediate_size)
+        self.up_proj = linear(hidden_size, intermediate_size)
+        self.down_proj = linear(intermediate_size, hidden_size)
+
+    def forward(self, x: Tensor) -> Tensor:
+        return fused_gated_mlp(x, self.gate_proj.weight, self.up_proj.weight,
+                               self.down_proj.weight, self.activation)
+
+    def extra_repr(self) -> str:
+        return f"{self.hidden_size}, {self.intermediate_size}, activation={self.activation!r}"

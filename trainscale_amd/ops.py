@@ -621,6 +621,95 @@ def swiglu_backward(dout: Tensor, gate: Tensor, up: Tensor) -> Tuple[Tensor, Ten
 
 
 # ---------------------------------------------------------------------------
+# Gated feed-forward block
+# ---------------------------------------------------------------------------
+
+_MLP_MAX_LD = 1 << 21
+
+
+def _mlp_operand(t: Tensor, rows: int, cols: int) -> Tuple[Tensor, int]:
+    """A matrix and its row stride as the kernels take it ([rows, cols] with cols and the stride
+    multiples of 8, 16-byte aligned): t itself where it is one, else a copy padded with zeros."""
+    if t.shape[1] == cols and t.shape[0] == rows:
+        ld = t.stride(0) if rows > 1 else cols
+        if (t.stride(1) == 1 and ld >= cols and ld % 8 == 0 and ld <= _MLP_MAX_LD
+                and t.data_ptr() % 16 == 0):
+            return t, ld
+    c = torch.zeros((rows, cols), dtype=t.dtype, device=t.device) if t.shape != (
+        rows, cols) else torch.empty((rows, cols), dtype=t.dtype, device=t.device)
+    c[:t.shape[0], :t.shape[1]].copy_(t)
+    return c, cols
+
+
+def _mlp_args(x2d, gate, up, down, code):
+    """The kernels' arguments, and what keeps their memory alive."""
+    n, h = x2d.shape
+    f, o = gate.shape[0], 0 if down is None else down.shape[0]
+    h8, f8, o8 = (h + 7) & ~7, (f + 7) & ~7, (o + 7) & ~7
+    x, ldx = _mlp_operand(x2d, n, h8)
+    g, ldg = _mlp_operand(gate, f8, h8)
+    u, ldu = _mlp_operand(up, f8, h8)
+    d, ldd = (None, 0) if down is None else _mlp_operand(down, o8, f8)
+    args = _lib.GatedMLPArgs(x.data_ptr(), ldx, g.data_ptr(), ldg, u.data_ptr(), ldu,
+                             0 if d is None else d.data_ptr(), ldd, n, h8, f8, o8, code,
+                             _lib.DTYPE_CODE[x.dtype])
+    return args, (x, g, u, d)
+
+
+def gated_mlp_forward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], code: int,
+                      keep: bool):
+    """(g, u, gated product, result) with features rounded up to multiples of 8; g and u None
+    unless kept, the result None without a down weight."""
+    dev = _lib.require_gpu("gated_mlp", x2d, gate, up, down)
+    n = x2d.shape[0]
+    args, held = _mlp_args(x2d, gate, up, down, code)
+    new = lambda cols: torch.empty((n, cols), dtype=x2d.dtype, device=dev)
+    g, u = (new(args.F), new(args.F)) if keep else (None, None)
+    a, y = new(args.F), None if down is None else new(args.O)
+    if n == 0:
+        return g, u, a, y
+    lib = _lib.load()
+    wsb = lib.ts_gated_mlp_fwd_workspace_size(n, args.H, args.F, args.O)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+    with _lib.on_device(dev):
+        check(lib.ts_gated_mlp_fwd(ctypes.byref(args), ptr(g), ptr(u), a.data_ptr(), ptr(y),
+                                   ptr(ws), wsb, _lib.stream_handle(dev)), "ts_gated_mlp_fwd")
+    del held
+    return g, u, a, y
+
+
+def gated_mlp_backward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], code: int,
+                       g: Tensor, u: Tensor, a: Optional[Tensor], dout: Tensor, needs) -> list:
+    """Gradients of (x2d, gate, up, down), None where `needs` is false."""
+    dev = _lib.require_gpu("gated_mlp", x2d, gate, up, down, g, u, a, dout)
+    n = x2d.shape[0]
+    out = [None] * 4
+    leaves = (x2d, gate, up, down)
+    needs = [bool(k) and t is not None for k, t in zip(needs, leaves)]
+    if n == 0 or not any(needs):
+        return [torch.zeros(t.shape, dtype=t.dtype, device=dev) if k else None
+                for t, k in zip(leaves, needs)]
+    args, held = _mlp_args(x2d, gate, up, down, code)
+    cols = args.F if down is None else args.O
+    d, ldd = _mlp_operand(dout, n, cols)
+    shapes = ((n, args.H), (args.F, args.H), (args.F, args.H), (args.O, args.F))
+    out = [torch.empty(s, dtype=x2d.dtype, device=dev) if k else None
+           for s, k in zip(shapes, needs)]
+    g, u = g.contiguous(), u.contiguous()
+    a = None if a is None else a.contiguous()
+    lib = _lib.load()
+    wsb = lib.ts_gated_mlp_bwd_workspace_size(n, args.H, args.F, args.O)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    with _lib.on_device(dev):
+        check(lib.ts_gated_mlp_bwd(ctypes.byref(args), g.data_ptr(), u.data_ptr(), ptr(a),
+                                   d.data_ptr(), ldd, *[ptr(t) for t in out], ws.data_ptr(), wsb,
+                                   _lib.stream_handle(dev)), "ts_gated_mlp_bwd")
+    del held
+    return [t if t is None or t.shape == s.shape else t[:s.shape[0], :s.shape[1]].contiguous()
+            for t, s in zip(out, leaves)]
+
+
+# ---------------------------------------------------------------------------
 # Token embedding
 # ---------------------------------------------------------------------------
 
