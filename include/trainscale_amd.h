@@ -263,6 +263,36 @@ ts_status ts_rope_apply(const void* q_in, void* q_out,
                         int32_t interleaved, int32_t backward,
                         ts_stream_t stream);
 
+/*
+ * Rotary positions with several axes. Pair i of a head's first R elements (element i with
+ * i + R / 2, or 2i with 2i + 1 where interleaved) is turned by the angle pos[axis[i]] f(i), and the
+ * D - R elements behind them stay. q and k: [B, S, heads, D] of dtype, unit stride along D, any
+ * strides otherwise (elements; 0 on inputs is fine) and any element-aligned address; an output may
+ * be its input, and overlaps nothing else. Hq or Hk may be 0.
+ * position_ids: device int64, pos[a] of token (b, s) at a * pos_sa + b * pos_sb + s * pos_ss; any
+ * values.
+ * turns, axis: HOST arrays of R / 2 entries, read before the call returns. turns[i] is
+ * f(i) / (2 pi) modulo 1, times 2^64: with integer positions the fraction of a turn that a position
+ * makes is all that matters, and its 64-bit product with a position is exact modulo a turn.
+ * backward 1: the transpose rotation, of gradients. R / 2 at most 256, D and heads 4096.
+ */
+typedef struct {
+  const void* q_in;
+  void* q_out;
+  int64_t q_in_sb, q_in_ss, q_in_sh, q_out_sb, q_out_ss, q_out_sh;
+  const void* k_in;
+  void* k_out;
+  int64_t k_in_sb, k_in_ss, k_in_sh, k_out_sb, k_out_ss, k_out_sh;
+  int64_t Hq, Hk, B, S, D, R;
+  const int64_t* position_ids;
+  int64_t pos_sa, pos_sb, pos_ss;
+  const uint64_t* turns;
+  const int32_t* axis;
+  int32_t axes, dtype, interleaved, backward;
+} ts_rope_axes_args;
+
+ts_status ts_rope_axes(const ts_rope_axes_args* args, ts_stream_t stream);
+
 /* ------------------------------------------------------------------------ */
 /* Cross-entropy over the vocabulary                                         */
 /* ------------------------------------------------------------------------ */
@@ -673,6 +703,58 @@ ts_status ts_gated_mlp_bwd(const ts_gated_mlp_args* args, const void* gate, cons
                            const void* act, const void* dout, int64_t ld_dout, void* dx,
                            void* dw_gate, void* dw_up, void* dw_down, void* workspace,
                            size_t workspace_bytes, ts_stream_t stream);
+
+/* ------------------------------------------------------------------------ */
+/* Dropout from a counter-based generator                                    */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Philox 4x32-10 under key `seed`: counter (row * ceil(cols / 8) + column / 8, offset) gives the
+ * elements of that group of 8 columns 16 bits each (low half of word 0, its high half, word 1,
+ * ...). An element is dropped where its bits are below `drop`, and kept ones are multiplied by
+ * 65536 / (65536 - drop): the probability of dropping is drop / 65536 exactly. state, where it is
+ * not NULL, is a device array of (seed, offset) read in place of the two values when the kernels
+ * run: a captured graph takes its numbers from there.
+ */
+typedef struct {
+  uint64_t seed, offset;
+  const int64_t* state;
+  int32_t drop; /* 0 .. 65536 */
+} ts_dropout_rng;
+
+/*
+ * out = D(x), or residual + D(x) where residual is not NULL (fp32 arithmetic, rounded once);
+ * D(x) = 0 for a dropped element whatever its value. x, residual, out: [rows, cols] of dtype, any
+ * element-aligned address, row strides in elements. The same call on a gradient is the backward.
+ */
+ts_status ts_dropout_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr, void* out,
+                         int64_t ldo, ts_dtype dtype, int64_t rows, int64_t cols,
+                         const ts_dropout_rng* rng, ts_stream_t stream);
+
+/*
+ * h = residual + D(x) and y = h * rstd * weight, rstd = 1 / sqrt(mean(h^2) + eps): y from the
+ * unrounded h, both rounded once; rstd [rows] fp32. y and h contiguous. weight: [cols] of dtype
+ * or fp32; cols at most 16384.
+ * Counterpart of the dropout + RMSNorm kernel, kernels/layernorm_kernels.py:556.
+ */
+ts_status ts_dropout_add_rmsnorm_fwd(const void* x, int64_t ldx, const void* residual, int64_t ldr,
+                                     ts_dtype dtype, const void* weight, ts_dtype wdtype, void* y,
+                                     void* h, float* rstd, int64_t rows, int64_t cols, float eps,
+                                     const ts_dropout_rng* rng, ts_stream_t stream);
+
+/*
+ * From dy and dh (either may be NULL: no gradient there) and the forward's h and rstd:
+ *   t = dh + rstd (dy w - hat mean(dy w hat)), hat = h rstd;
+ *   dres = t, dx = D(t), dw = sum over rows of dy hat (in dw's fixed order),
+ * each contiguous and skipped where NULL. Workspace (for dw): 16-byte aligned.
+ */
+size_t ts_dropout_add_rmsnorm_bwd_workspace_size(int64_t rows, int64_t cols);
+ts_status ts_dropout_add_rmsnorm_bwd(const void* dy, int64_t lddy, const void* dh, int64_t lddh,
+                                     const void* h, int64_t ldh, ts_dtype dtype,
+                                     const void* weight, ts_dtype wdtype, const float* rstd,
+                                     void* dx, void* dres, void* dw, int64_t rows, int64_t cols,
+                                     const ts_dropout_rng* rng, void* workspace,
+                                     size_t workspace_bytes, ts_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* Token embedding                                                           */

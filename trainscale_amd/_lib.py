@@ -60,11 +60,29 @@ class PolicyInputs(ctypes.Structure):
                 ("reduction", I32)]
 
 
+class RopeAxesArgs(ctypes.Structure):
+    """ts_rope_axes_args."""
+    _fields_ = [("q_in", P), ("q_out", P), *[(f"q_{n}", I64) for n in (
+                    "in_sb", "in_ss", "in_sh", "out_sb", "out_ss", "out_sh")],
+                ("k_in", P), ("k_out", P), *[(f"k_{n}", I64) for n in (
+                    "in_sb", "in_ss", "in_sh", "out_sb", "out_ss", "out_sh")],
+                ("Hq", I64), ("Hk", I64), ("B", I64), ("S", I64), ("D", I64), ("R", I64),
+                ("position_ids", P), ("pos_sa", I64), ("pos_sb", I64), ("pos_ss", I64),
+                ("turns", P), ("axis", P), ("axes", I32), ("dtype", I32), ("interleaved", I32),
+                ("backward", I32)]
+
+
 class GatedMLPArgs(ctypes.Structure):
     """ts_gated_mlp_args."""
     _fields_ = [("x", P), ("ldx", I64), ("w_gate", P), ("ld_gate", I64), ("w_up", P),
                 ("ld_up", I64), ("w_down", P), ("ld_down", I64), ("N", I64), ("H", I64),
                 ("F", I64), ("O", I64), ("activation", I32), ("dtype", I32)]
+
+
+class DropoutRng(ctypes.Structure):
+    """ts_dropout_rng."""
+    _fields_ = [("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64), ("state", P),
+                ("drop", I32)]
 
 
 # argtypes of every exported entry point, in header order
@@ -92,6 +110,7 @@ SIGNATURES = {
          P, I64, I64, I64,                          # position_ids, strides, offset
          I32, I32, P],                              # interleaved, backward, stream
         I32),
+    "ts_rope_axes": ([P, P], I32),
     "ts_ce_fwd": ([P, I64, I32, P, I64, I64, I64, F32, F32, F32, P, P, P], I32),
     "ts_ce_bwd": ([P, I64, I32, P, P, P, I64, F32, P, I64, I32, I64, I64, I64, F32, F32, F32, P],
                   I32),
@@ -129,6 +148,12 @@ SIGNATURES = {
     "ts_gated_mlp_bwd_workspace_size": ([I64, I64, I64, I64], SZ),
     "ts_gated_mlp_fwd": ([P, P, P, P, P, P, SZ, P], I32),
     "ts_gated_mlp_bwd": ([P, P, P, P, P, I64, P, P, P, P, P, SZ, P], I32),
+    "ts_dropout_fwd": ([P, I64, P, I64, P, I64, I32, I64, I64, P, P], I32),
+    "ts_dropout_add_rmsnorm_fwd": ([P, I64, P, I64, I32, P, I32, P, P, P, I64, I64, F32, P, P],
+                                   I32),
+    "ts_dropout_add_rmsnorm_bwd_workspace_size": ([I64, I64], SZ),
+    "ts_dropout_add_rmsnorm_bwd": ([P, I64, P, I64, P, I64, I32, P, I32, P, P, P, P, I64, I64, P,
+                                    P, SZ, P], I32),
     "ts_embedding_fwd": ([P, I64, P, I64, I32, I64, I64, F32, P, I64, P], I32),
     "ts_embedding_bwd_workspace_size": ([I64, I64, I64], SZ),
     "ts_embedding_bwd": ([P, I64, P, I64, I32, I64, I64, F32, I64, P, P, SZ, P], I32),

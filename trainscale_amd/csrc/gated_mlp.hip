@@ -471,7 +471,8 @@ ts_status launch_product(const Product& p, const Gated& e, int waves, hipStream_
                          const char* name) {
   const int64_t tiles = ts_plan::mlp_tiles(p.M, p.N, waves, kEpi == kEpiGatedFwd) * p.splits;
   if (tiles <= 0) return TS_OK;
-  if (tiles > 0x7fffffffLL) return ts_host::fail(TS_ERR_SHAPE, "%s: too many tiles", name);
+  if (tiles > ts_plan::max_blocks(64 * waves))
+    return ts_host::fail(TS_ERR_SHAPE, "%s: too many tiles", name);
   if (waves == 8)
     hipLaunchKernelGGL((mlp_product<T, kEpi, kMA, kMB, 8>), dim3((unsigned)tiles), dim3(512), 0,
                        st, p, e);
@@ -496,7 +497,7 @@ ts_status launch_sums(SumJobs& s, int n, hipStream_t st) {
   if (n == 0) return TS_OK;
   const int64_t blocks = s.end[n - 1];
   for (int j = n; j < 4; ++j) s.end[j] = blocks;
-  if (blocks > 0x7fffffffLL) return ts_host::fail(TS_ERR_SHAPE, "mlp_sum_slots: too large");
+  if (blocks > ts_plan::max_blocks(256)) return ts_host::fail(TS_ERR_SHAPE, "mlp_sum_slots: too large");
   hipLaunchKernelGGL(mlp_sum_slots<T>, dim3((unsigned)blocks), dim3(256), 0, st, s);
   return ts_host::check_launch("mlp_sum_slots");
 }
@@ -529,7 +530,8 @@ ts_status fwd_typed(const ts_gated_mlp_args& a, void* gate, void* up, void* act,
 template <typename T, int kW>
 ts_status launch_grads(const Grads& g, hipStream_t st) {
   if (g.end[3] <= 0) return TS_OK;
-  if (g.end[3] > 0x7fffffffLL) return ts_host::fail(TS_ERR_SHAPE, "mlp_grads: too many tiles");
+  if (g.end[3] > ts_plan::max_blocks(64 * kW))
+    return ts_host::fail(TS_ERR_SHAPE, "mlp_grads: too many tiles");
   hipLaunchKernelGGL((mlp_grads<T, kW>), dim3((unsigned)g.end[3]), dim3(64 * kW), 0, st, g);
   return ts_host::check_launch("mlp_grads");
 }
@@ -551,7 +553,8 @@ ts_status bwd_typed(const ts_gated_mlp_args& a, const void* gate, const void* up
                                                                "mlp_gated_bwd")));
   } else if (inner) {
     const int64_t nvec = a.N * a.F / 8, blocks = (nvec + 255) / 256;
-    if (blocks > 0x7fffffffLL) return ts_host::fail(TS_ERR_SHAPE, "mlp_gate_bwd: too large");
+    if (blocks > ts_plan::max_blocks(256))
+      return ts_host::fail(TS_ERR_SHAPE, "mlp_gate_bwd: too large");
     hipLaunchKernelGGL(mlp_gate_bwd<T>, dim3((unsigned)blocks), dim3(256), 0, st,
                        static_cast<const T*>(dout), ldd, static_cast<const T*>(gate),
                        static_cast<const T*>(up), static_cast<T*>(dg), static_cast<T*>(du), nvec,

@@ -413,6 +413,33 @@ inline MlpBwdWorkspace mlp_bwd_workspace(const MlpShape& s) {
 }
 
 // ---------------------------------------------------------------------------
+// Dropout with the next norm: a row of `groups` groups of 8 columns on tpr threads of kv groups
+// each, `rows` rows a workgroup.
+// ---------------------------------------------------------------------------
+constexpr int64_t kDropNormMaxCols = 16384;
+struct DropNormPlan {
+  int tpr, kv, rows;
+};
+inline DropNormPlan drop_norm_plan(int64_t groups) {
+  if (groups <= 8) return DropNormPlan{8, 1, 32};
+  if (groups <= 32) return DropNormPlan{32, 1, 8};
+  if (groups <= 64) return DropNormPlan{64, 1, 4};
+  if (groups <= 128) return DropNormPlan{64, 2, 4};
+  if (groups <= 256) return DropNormPlan{256, 1, 1};
+  if (groups <= 512) return DropNormPlan{512, 1, 1};
+  if (groups <= 1024) return DropNormPlan{512, 2, 1};
+  if (groups <= 2048) return DropNormPlan{512, 4, 1};
+  return DropNormPlan{0, 0, 1};
+}
+// Workgroups of the backward, each of which writes a partial row of dw.
+constexpr int64_t kDropNormBwdGrid = 512;
+inline int64_t drop_norm_bwd_grid(int64_t rows, int64_t groups) {
+  const int64_t per = drop_norm_plan(groups).rows;
+  const int64_t steps = (rows + per - 1) / per;
+  return steps < kDropNormBwdGrid ? steps : kDropNormBwdGrid;
+}
+
+// ---------------------------------------------------------------------------
 // Addressing of the streaming and row kernels. The kernels compute their
 // accesses with these functions, and tests/test_plan.py sweeps them with the
 // launch shapes the host computes: every access lies inside its tensor and

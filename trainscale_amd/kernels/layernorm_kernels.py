@@ -23,7 +23,8 @@ Not in the reference: ``FusedSandwichRMSNormFunction``, ``fused_sandwich_rms_lay
 and after each block: the norm of a block's output, its gate, the residual sum and the next
 block's norm in one pass, with every gradient.
 
-LayerNorm/Welford and dropout+RMS are not part of this layer.
+LayerNorm/Welford is not part of this layer; dropout with the residual sum and RMSNorm is in
+``dropout_kernels``.
 """
 from __future__ import annotations
 

@@ -18,6 +18,10 @@ one rounding to the data dtype. Backward is the transpose rotation written to a
 new gradient tensor in one pass (the reference clones the gradient and then
 rotates it in place: two passes).
 
+Not in the reference: ``RopeAxes``, ``apply_rope_axes`` and ``MultiAxisRotaryEmbedding``, positions
+with several axes (time, height and width of images and video), in a kernel of their own
+(``ts_rope_axes``).
+
 Semantics kept from the reference: in-place forwards return the input tensor
 object modified in place. One difference: 1-D ``position_ids`` of length S are
 applied to every sequence of the batch (the reference's Triton path indexed a
@@ -25,6 +29,7 @@ applied to every sequence of the batch (the reference's Triton path indexed a
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from dataclasses import dataclass
 from enum import Enum, auto
@@ -33,6 +38,7 @@ from typing import Dict, List, Optional, Tuple, Union
 import torch
 import torch.nn as nn
 from torch import Tensor
+from torch.autograd.function import once_differentiable
 
 from .. import ops
 
@@ -53,6 +59,10 @@ __all__ = [
     "apply_rope_theta",
     "RotaryEmbedding",
     "hf_apply_rotary_pos_emb",
+    "RopeAxes",
+    "RopeAxesFunction",
+    "apply_rope_axes",
+    "MultiAxisRotaryEmbedding",
     "position_ids_from_cu_seqlens",
     "ROPE_GROUP_SIZE",
 ]
@@ -406,6 +416,179 @@ def hf_apply_rotary_pos_emb(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor,
         qo, ko = _HFTableRoPEFunction.apply(q.transpose(1, 2), k.transpose(1, 2), cos, sin)
         return qo.transpose(1, 2), ko.transpose(1, 2)
     return _HFTableRoPEFunction.apply(q, k, cos, sin)
+
+
+# ---------------------------------------------------------------------------
+# Several axes: time, height and width of images and video
+# ---------------------------------------------------------------------------
+
+# floor(2^192 / (2 pi))
+_INV_2PI_192 = 0x28BE60DB9391054A7F09D5F47D4D377036D8A5664F10E410
+
+
+def _turns(freq: float) -> int:
+    """freq / (2 pi) modulo 1 in units of 2^-64, rounded."""
+    num, den = freq.as_integer_ratio()
+    return ((num * _INV_2PI_192 >> 127) // den + 1 >> 1) & (1 << 64) - 1
+
+
+class RopeAxes:
+    """How the pairs of a rotary embedding are shared out among position axes, and their
+    frequencies: the plan that ``apply_rope_axes`` takes, made once.
+
+    sections: pairs of each axis; their sum is half of the rotated elements of a head. Pair i turns
+    by position[axis(i)] * inv_freq[i]. layout:
+
+    * ``"blocks"``: one progression base**(-i / n) over the n pairs, in order sections[0] pairs of
+      axis 0, then sections[1] of axis 1, and so on;
+    * ``"interleaved"``: the same progression, pair i belonging to axis i mod A of A axes while i <
+      A * sections[i mod A], and to axis 0 otherwise;
+    * ``"separate"``: blocks whose every axis has a progression of its own, base**(-j / sections[a])
+      over its pairs (images: rows and columns alike).
+
+    inv_freq overrides the progression (fp32 or fp64 values, one a pair). interleaved pairs adjacent
+    elements instead of halves.
+    """
+
+    __slots__ = ("sections", "layout", "interleaved", "inv_freq", "axis", "_turns_c", "_axis_c")
+
+    def __init__(self, sections, layout: str = "blocks", base: float = 10000.0,
+                 inv_freq: Optional[Tensor] = None, interleaved: bool = False):
+        self.sections = tuple(int(n) for n in sections)
+        n, a = sum(self.sections), len(self.sections)
+        if not self.sections or min(self.sections) < 1 or n > 256 or a > 255:
+            raise ValueError(f"RopeAxes: sections {self.sections}: at least one axis, pairs on each "
+                             "and at most 256 in all")
+        blocks = [k for k, m in enumerate(self.sections) for _ in range(m)]
+        if layout in ("blocks", "separate"):
+            self.axis = tuple(blocks)
+        elif layout == "interleaved":
+            self.axis = tuple(i % a if i < a * self.sections[i % a] else 0 for i in range(n))
+            if tuple(self.axis.count(k) for k in range(a)) != self.sections:
+                raise ValueError(f"RopeAxes: sections {self.sections} do not interleave (the first "
+                                 "axis takes what the others leave)")
+        else:
+            raise ValueError(f"RopeAxes: unknown layout {layout!r} (blocks, interleaved, separate)")
+        if inv_freq is None:
+            inv_freq = torch.cat([_base_inv_freq(base, 2 * m, "cpu") for m in (
+                self.sections if layout == "separate" else (n,))])
+        inv_freq = inv_freq.detach().to("cpu", torch.float64).reshape(-1)
+        if inv_freq.shape[0] != n or not bool(torch.isfinite(inv_freq).all()):
+            raise ValueError(f"RopeAxes: {inv_freq.shape[0]} frequencies for {n} pairs (finite)")
+        self.layout = layout
+        self.interleaved = bool(interleaved)
+        self.inv_freq = inv_freq
+        self._turns_c = (ctypes.c_uint64 * n)(*[_turns(f) for f in inv_freq.tolist()])
+        self._axis_c = (ctypes.c_int32 * n)(*self.axis)
+
+    def __repr__(self) -> str:
+        return (f"RopeAxes({self.sections}, layout={self.layout!r}, "
+                f"interleaved={self.interleaved})")
+
+    def __reduce__(self):
+        return _rope_axes_again, (self.sections, self.layout, self.inv_freq, self.interleaved)
+
+
+def _rope_axes_again(sections, layout, inv_freq, interleaved) -> RopeAxes:
+    return RopeAxes(sections, layout, inv_freq=inv_freq, interleaved=interleaved)
+
+
+def _axes_positions(position_ids: Tensor, axes: int, batch: int, seq: int) -> Tensor:
+    """position_ids as an int64 [axes, B, S] view."""
+    if position_ids.dtype is not torch.int64:
+        if position_ids.dtype is not torch.int32:
+            raise TypeError(f"apply_rope_axes: position_ids must be int64 or int32, got "
+                            f"{position_ids.dtype}")
+        position_ids = position_ids.to(torch.int64)
+    shape = tuple(position_ids.shape)
+    if shape == (axes, seq):
+        position_ids = position_ids[:, None]
+    elif shape != (axes, 1, seq) and shape != (axes, batch, seq):
+        raise ValueError(f"apply_rope_axes: position_ids {shape} for {axes} axes, batch {batch} "
+                         f"and {seq} tokens")
+    return position_ids.expand(axes, batch, seq)
+
+
+def _rope_axes(plan: RopeAxes, pos: Tensor, q: Optional[Tensor], k: Optional[Tensor],
+               inplace: bool = False, backward: bool = False):
+    """The rotated q and k (either may be None), new contiguous tensors or the same ones."""
+    if inplace:
+        outs = (q, k)
+    else:
+        q, k = [t if t is None else ops._bshd(t, "apply_rope_axes") for t in (q, k)]
+        outs = [t if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+                for t in (q, k)]
+    if any(t is not None for t in (q, k)):
+        ops.rope_axes(q, outs[0], k, outs[1], pos, plan._turns_c, plan._axis_c,
+                      len(plan.sections), 2 * len(plan.axis), plan.interleaved, backward)
+    return outs[0], outs[1]
+
+
+class RopeAxesFunction(torch.autograd.Function):
+    """forward(q, k or None, position_ids [A, B, S], plan) -> (q, k rotated)."""
+
+    @staticmethod
+    def forward(ctx, q: Tensor, k: Optional[Tensor], pos: Tensor, plan: RopeAxes):
+        ctx.set_materialize_grads(False)
+        ctx.plan = plan
+        ctx.save_for_backward(pos)
+        return _rope_axes(plan, pos, q, k)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dq: Optional[Tensor], dk: Optional[Tensor]):
+        dq, dk = [d if need else None for d, need in zip((dq, dk), ctx.needs_input_grad)]
+        if dq is None and dk is None:
+            return None, None, None, None
+        return (*_rope_axes(ctx.plan, ctx.saved_tensors[0], dq, dk, backward=True), None, None)
+
+
+def apply_rope_axes(q: Tensor, k: Optional[Tensor], position_ids: Tensor, plan: RopeAxes,
+                    inplace: bool = False) -> Tuple[Tensor, Optional[Tensor]]:
+    """Rotary positions with several axes: q [B, S, Hq, D] and k [B, S, Hk, D] (or None) turned by
+    their tokens' positions along each axis of plan, position_ids [A, B, S], [A, 1, S] or [A, S]
+    (int64 or int32, any values: angles are exact to fp32's rounding however far). Elements past
+    plan's pairs stay. fp32 arithmetic, rounded once; returns new tensors, differentiable in q and
+    k. inplace writes into q and k instead, for calls that autograd does not record; their last
+    dimension must be contiguous."""
+    n = 2 * len(plan.axis)
+    for name, t in (("q", q), ("k", k)):
+        if t is None:
+            continue
+        if t.dim() != 4 or t.shape[-1] < n:
+            raise ValueError(f"apply_rope_axes: {name} {tuple(t.shape)}: expected [B, S, H, D], D at "
+                             f"least {n}")
+        if t.shape[:2] != q.shape[:2] or t.shape[3] != q.shape[3] or t.dtype is not q.dtype:
+            raise ValueError(f"apply_rope_axes: k {tuple(t.shape)} {t.dtype} for q "
+                             f"{tuple(q.shape)} {q.dtype}")
+    pos = _axes_positions(position_ids, len(plan.sections), q.shape[0], q.shape[1])
+    record = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
+    if inplace:
+        if record or ops.in_forward_ad():
+            raise ValueError("apply_rope_axes: inplace while gradients are recorded")
+        for t in (q, k):
+            if t is not None and t.shape[3] > 1 and t.stride(3) != 1:
+                raise ValueError("apply_rope_axes: inplace needs contiguous head dimensions")
+    elif record or ops.in_forward_ad():
+        return RopeAxesFunction.apply(q, k, pos, plan)
+    return _rope_axes(plan, pos, q, k, inplace)
+
+
+class MultiAxisRotaryEmbedding(nn.Module):
+    """``apply_rope_axes`` with a plan of its own; the arguments are ``RopeAxes``'s."""
+
+    def __init__(self, sections, layout: str = "blocks", base: float = 10000.0,
+                 inv_freq: Optional[Tensor] = None, interleaved: bool = False):
+        super().__init__()
+        self.plan = RopeAxes(sections, layout, base, inv_freq, interleaved)
+
+    def forward(self, q: Tensor, k: Optional[Tensor], position_ids: Tensor,
+                inplace: bool = False) -> Tuple[Tensor, Optional[Tensor]]:
+        return apply_rope_axes(q, k, position_ids, self.plan, inplace)
+
+    def extra_repr(self) -> str:
+        return (f"{self.plan.sections}, layout={self.plan.layout!r}, "
+                f"interleaved={self.plan.interleaved}")
 
 
 def position_ids_from_cu_seqlens(cu_seqlens, total: Optional[int] = None) -> Tensor:

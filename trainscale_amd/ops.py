@@ -332,6 +332,33 @@ def rope_apply(q_in: Optional[Tensor], q_out: Optional[Tensor],
     del inv_host
 
 
+def rope_axes(q_in: Optional[Tensor], q_out: Optional[Tensor], k_in: Optional[Tensor],
+              k_out: Optional[Tensor], position_ids: Tensor, turns, axis, axes: int, rotary: int,
+              interleaved: bool, backward: bool = False) -> None:
+    """Rotates q_in -> q_out and k_in -> k_out ([B, S, H, D], unit last stride; either pair may be
+    None; in == out is in place) at position_ids [axes, B, S] (int64, any strides). turns and axis
+    are ctypes arrays of rotary / 2 entries (ts_rope_axes)."""
+    ref = q_in if q_in is not None else k_in
+    dev = _lib.require_gpu("rope_axes", q_in, q_out, k_in, k_out, position_ids)
+    B, S, _, D = ref.shape
+
+    def side(i, o):
+        if i is None:
+            return (0,) * 8
+        si, so = i.stride(), o.stride()
+        return (i.data_ptr(), o.data_ptr(), si[0], si[1], si[2], so[0], so[1], so[2])
+
+    sp = position_ids.stride()
+    args = _lib.RopeAxesArgs(
+        *side(q_in, q_out), *side(k_in, k_out), 0 if q_in is None else q_in.shape[2],
+        0 if k_in is None else k_in.shape[2], B, S, D, rotary, position_ids.data_ptr(), sp[0],
+        sp[1], sp[2], ctypes.addressof(turns), ctypes.addressof(axis), axes,
+        _lib.dtype_code(ref, "rope_axes"), interleaved, backward)
+    with _lib.on_device(dev):
+        check(_lib.load().ts_rope_axes(ctypes.byref(args), _lib.stream_handle(dev)),
+              "ts_rope_axes")
+
+
 # ---------------------------------------------------------------------------
 # Cross-entropy
 # ---------------------------------------------------------------------------
@@ -707,6 +734,79 @@ def gated_mlp_backward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Ten
     del held
     return [t if t is None or t.shape == s.shape else t[:s.shape[0], :s.shape[1]].contiguous()
             for t, s in zip(out, leaves)]
+
+
+# ---------------------------------------------------------------------------
+# Dropout from a counter-based generator
+# ---------------------------------------------------------------------------
+
+def _rng_arg(rng, drop: int):
+    """ts_dropout_rng of (seed, offset) or of a device state."""
+    if isinstance(rng, Tensor):
+        return ctypes.byref(_lib.DropoutRng(0, 0, rng.data_ptr(), drop))
+    return ctypes.byref(_lib.DropoutRng(rng[0], rng[1], 0, drop))
+
+
+def dropout_forward(x2d: Tensor, ldx: int, res2d: Optional[Tensor], ldr: int, rng, drop: int,
+                    shape) -> Tensor:
+    """[residual +] dropout(x2d), of `shape`."""
+    dev = _lib.require_gpu("dropout", x2d, res2d, rng if isinstance(rng, Tensor) else None)
+    rows, cols = x2d.shape
+    out = torch.empty(shape, dtype=x2d.dtype, device=dev)
+    if out.numel() == 0:
+        return out
+    with _lib.on_device(dev):
+        check(_lib.load().ts_dropout_fwd(
+            x2d.data_ptr(), ldx, 0 if res2d is None else res2d.data_ptr(), ldr, out.data_ptr(),
+            cols, _lib.dtype_code(x2d, "dropout"), rows, cols, _rng_arg(rng, drop),
+            _lib.stream_handle(dev)), "ts_dropout_fwd")
+    return out
+
+
+def dropout_add_rmsnorm_forward(x2d: Tensor, ldx: int, res2d: Tensor, ldr: int, weight: Tensor,
+                                eps: float, rng, drop: int, shape
+                                ) -> Tuple[Tensor, Tensor, Tensor]:
+    """(y, h, rstd fp32 [rows]) of h = residual + dropout(x), y = RMSNorm(h); y and h of `shape`."""
+    dev = _lib.require_gpu("dropout_add_rmsnorm", x2d, res2d, weight,
+                           rng if isinstance(rng, Tensor) else None)
+    rows, cols = x2d.shape
+    y = torch.empty(shape, dtype=x2d.dtype, device=dev)
+    h = torch.empty(shape, dtype=x2d.dtype, device=dev)
+    rstd = torch.empty((rows,), dtype=torch.float32, device=dev)
+    if rows == 0:
+        return y, h, rstd
+    with _lib.on_device(dev):
+        check(_lib.load().ts_dropout_add_rmsnorm_fwd(
+            x2d.data_ptr(), ldx, res2d.data_ptr(), ldr, _lib.dtype_code(x2d, "dropout"),
+            weight.data_ptr(), _lib.dtype_code(weight, "dropout_add_rmsnorm weight"), y.data_ptr(),
+            h.data_ptr(), rstd.data_ptr(), rows, cols, eps, _rng_arg(rng, drop),
+            _lib.stream_handle(dev)), "ts_dropout_add_rmsnorm_fwd")
+    return y, h, rstd
+
+
+def dropout_add_rmsnorm_backward(dy: Optional[Tensor], lddy: int, dh: Optional[Tensor], lddh: int,
+                                 h2d: Tensor, ldh: int, weight: Tensor, rstd: Tensor, rng,
+                                 drop: int, needs, shape) -> list:
+    """Gradients of (x, residual, weight), None where `needs` is false, the first two of
+    `shape`."""
+    dev = _lib.require_gpu("dropout_add_rmsnorm", dy, dh, h2d, weight, rstd)
+    rows, cols = h2d.shape
+    out = [torch.empty(shape, dtype=h2d.dtype, device=dev) if needs[0] else None,
+           torch.empty(shape, dtype=h2d.dtype, device=dev) if needs[1] else None,
+           torch.empty((cols,), dtype=weight.dtype, device=dev) if needs[2] else None]
+    lib = _lib.load()
+    ws, wsb = None, 0
+    if needs[2]:
+        wsb = lib.ts_dropout_add_rmsnorm_bwd_workspace_size(rows, cols)
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    at = [0 if t is None else t.data_ptr() for t in (dy, dh, *out, ws)]
+    with _lib.on_device(dev):
+        check(lib.ts_dropout_add_rmsnorm_bwd(
+            at[0], lddy, at[1], lddh, h2d.data_ptr(), ldh, _lib.DTYPE_CODE[h2d.dtype],
+            weight.data_ptr(), _lib.DTYPE_CODE[weight.dtype], rstd.data_ptr(), at[2], at[3], at[4],
+            rows, cols, _rng_arg(rng, drop), at[5], wsb, _lib.stream_handle(dev)),
+            "ts_dropout_add_rmsnorm_bwd")
+    return out
 
 
 # ---------------------------------------------------------------------------
