@@ -336,6 +336,167 @@ void mlp_grads(const Grads a) {
 }
 
 // ---------------------------------------------------------------------------
+// Few rows (decoding): bound by reading the weights once. A workgroup owns 16 output features and
+// every row; its waves take k-blocks of 64 in turn. Each wave streams the 128-byte runs of its 16
+// weight rows (of both projections) and of x into a ring of its own in LDS, kDepth k-blocks ahead,
+// and never waits for another wave until their sums are added in LDS, in wave order, at the end.
+// The weights are the MFMAs' first operand, so a lane ends with four features of one row.
+// The eight lanes of a load into LDS that share a row read its 128 bytes whole, where a load into
+// MFMA operands takes 16 bytes of 16 rows at a time. Measured on MI355X, 16 rows, [14336, 4096] pair
+// and [4096, 14336] (352 MB, three sets in turn): registers 85 us, LDS 72 us, the weights past the
+// caches 66 us (5.3 TB/s; one row 62 us). 64 rows: registers 157 us, LDS 107 us, products on
+// 128 x 128 tiles with K in 12 slots 103 us, but 20 against 13 us at [2048, 768].
+// ---------------------------------------------------------------------------
+struct Few {
+  const __bf16* x;
+  int64_t ldx;
+  const __bf16* w[2];
+  int64_t ldw[2];
+  int64_t N, F, K;
+  void* g;
+  void* u;
+  void* out;
+  int32_t act;
+};
+
+// 16 rows from row r0 of a [rows, ld] matrix, for k-blocks in tiles of 16 x 128 bytes.
+struct FewTile {
+  ts_gemm::i32x4 rsrc;
+  uint32_t off[2];
+  uint32_t tail[2];  // off, or out of range where the last, short k-block has no such k
+};
+__device__ inline FewTile few_tile(const __bf16* p, int64_t ld, int64_t rows, int64_t r0,
+                                   int64_t K) {
+  FewTile t;
+  const int lane = threadIdx.x & 63;
+  int64_t valid = rows - r0;
+  if (valid > 16) valid = 16;
+  if (valid < 0) valid = 0;
+  t.rsrc = ts_gemm::make_rsrc(p + r0 * ld, (uint64_t)valid * (uint64_t)ld * 2);
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int row = u * 8 + (lane >> 3);
+    const int chunk = ts_gemm::swz(row, lane & 7);
+    t.off[u] = (uint32_t)(row * ld * 2 + chunk * 16);
+    t.tail[u] = K / ts_gemm::BK * ts_gemm::BK + chunk * 8 < K ? t.off[u] : ts_gemm::kOob;
+  }
+  return t;
+}
+template <int kAux>
+__device__ inline void few_issue(const FewTile& t, int64_t kb, bool last, uint8_t* lds) {
+#pragma unroll
+  for (int u = 0; u < 2; ++u)
+    ts_gemm::buffer_load_lds(t.rsrc, (ts_gemm::lds_ptr_t)(lds + u * 1024), 16,
+                             (int)(last ? t.tail[u] : t.off[u]), (int)(kb * 128), 0, kAux);
+}
+
+// kNT 16-row tiles of x. kStream: the weights are read past the caches.
+template <typename T, int kNT, bool kPair, bool kStream>
+__global__ __launch_bounds__(64 * ts_plan::kMlpFewWaves) void mlp_few(const Few a) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  constexpr int kP = kPair ? 2 : 1;
+  constexpr int kDepth = ts_plan::mlp_few_depth(kNT);
+  constexpr int kTiles = kP + kNT;
+  constexpr int kStage = kTiles * 2048;
+  const int lane = threadIdx.x & 63;
+  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int waves = blockDim.x >> 6;
+  const int64_t f0 = (int64_t)blockIdx.x * 16;
+  uint8_t* ring = smem + wid * (kDepth * kStage);
+  FewTile tile[kTiles];
+#pragma unroll
+  for (int p = 0; p < kP; ++p) tile[p] = few_tile(a.w[p], a.ldw[p], a.F, f0, a.K);
+#pragma unroll
+  for (int t = 0; t < kNT; ++t) tile[kP + t] = few_tile(a.x, a.ldx, a.N, t * 16, a.K);
+  f32x4 acc[kP][kNT];
+#pragma unroll
+  for (int p = 0; p < kP; ++p)
+#pragma unroll
+    for (int t = 0; t < kNT; ++t) acc[p][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int64_t blocks = (a.K + ts_gemm::BK - 1) / ts_gemm::BK;
+  const int64_t part = a.K % ts_gemm::BK != 0 ? blocks - 1 : blocks;  // the short block's index
+  auto issue = [&](int64_t kb, int slot) {
+#pragma unroll
+    for (int q = 0; q < kTiles; ++q) {
+      uint8_t* to = ring + slot * kStage + q * 2048;
+      if (q < kP && kStream) few_issue<kBufNt>(tile[q], kb, kb == part, to);
+      else few_issue<0>(tile[q], kb, kb == part, to);
+    }
+  };
+  const int64_t mine = wid < blocks ? (blocks - wid + waves - 1) / waves : 0;  // this wave's blocks
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d)
+    if (d < mine) issue(wid + (int64_t)d * waves, d);
+  int slot = 0;
+  for (int64_t n = 0; n < mine; ++n) {
+    // loads return in order: all but those of the blocks behind this one
+    const int64_t behind = mine - 1 - n;
+    static_assert(kDepth == 2 || kDepth == 3, "waits");
+    if (kDepth == 3 && behind >= 2) ts_gemm::wait_vmcnt<2 * 2 * kTiles>();
+    else if (behind >= 1) ts_gemm::wait_vmcnt<2 * kTiles>();
+    else ts_gemm::wait_vmcnt<0>();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    const uint8_t* s = ring + slot * kStage;
+    ts_gemm::bf16x8 w[kP][2], x[kNT][2];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+#pragma unroll
+      for (int p = 0; p < kP; ++p) ts_gemm::read_op_k<1>(s + p * 2048, 0, lane, ks, &w[p][ks]);
+#pragma unroll
+      for (int t = 0; t < kNT; ++t)
+        ts_gemm::read_op_k<1>(s + (kP + t) * 2048, 0, lane, ks, &x[t][ks]);
+    }
+    // read before the slot is filled again
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    if (n + kDepth < mine) issue(wid + (n + kDepth) * waves, slot);
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+#pragma unroll
+      for (int p = 0; p < kP; ++p)
+#pragma unroll
+        for (int t = 0; t < kNT; ++t)
+          acc[p][t] = ts_gemm::mfma<T>(w[p][ks], x[t][ks], acc[p][t]);
+    slot = slot + 1 == kDepth ? 0 : slot + 1;
+  }
+  __syncthreads();  // every wave is done with its ring
+  f32x4* sums = reinterpret_cast<f32x4*>(smem);  // [waves][kP][kNT][64]
+#pragma unroll
+  for (int p = 0; p < kP; ++p)
+#pragma unroll
+    for (int t = 0; t < kNT; ++t) sums[((wid * kP + p) * kNT + t) * 64 + lane] = acc[p][t];
+  __syncthreads();
+  for (int i = threadIdx.x; i < kNT * 64; i += blockDim.x) {
+    f32x4 s[kP];
+#pragma unroll
+    for (int p = 0; p < kP; ++p) {
+      s[p] = sums[p * kNT * 64 + i];
+      for (int v = 1; v < waves; ++v) s[p] += sums[(v * kP + p) * kNT * 64 + i];
+    }
+    const int64_t r = (i >> 6) * 16 + (i & 15), fo = f0 + ((i & 63) >> 4) * 4;
+    if (r >= a.N || fo >= a.F) continue;
+    const int64_t at = r * a.F + fo;
+    auto put = [&](void* o, const f32x4& v) {
+      *reinterpret_cast<uint2*>(static_cast<T*>(o) + at) =
+          make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    };
+    if constexpr (kPair) {
+      if (a.g != nullptr) {
+        put(a.g, s[0]);
+        put(a.u, s[1]);
+      }
+      with_act(a.act, [&](auto act) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) s[0][q] = act_f<decltype(act)::value>(s[0][q]) * s[1][q];
+      });
+    }
+    put(a.out, s[0]);
+  }
+}
+
+// ---------------------------------------------------------------------------
 // Partials of a split K, added in slot order and rounded once
 // ---------------------------------------------------------------------------
 struct SumJobs {
@@ -508,9 +669,44 @@ ts_status launch_sums(SumJobs& s, int n, hipStream_t st) {
     if (s_ != TS_OK) return s_;    \
   } while (0)
 
+template <typename T, int kNT, bool kPair>
+ts_status launch_few_rows(const Few& f, hipStream_t st) {
+  const int64_t blocks = (f.F + 15) / 16;
+  const int waves = ts_plan::mlp_few_waves(f.K);
+  const size_t lds =
+      (size_t)waves * ((kPair ? 2 : 1) + kNT) * ts_plan::mlp_few_depth(kNT) * 2048;
+  if (ts_plan::mlp_few_stream(f.F, f.K, kPair))
+    hipLaunchKernelGGL((mlp_few<T, kNT, kPair, true>), dim3((unsigned)blocks), dim3(64 * waves),
+                       lds, st, f);
+  else
+    hipLaunchKernelGGL((mlp_few<T, kNT, kPair, false>), dim3((unsigned)blocks), dim3(64 * waves),
+                       lds, st, f);
+  return ts_host::check_launch("mlp_few");
+}
+
+template <typename T, bool kPair>
+ts_status launch_few(const Few& f, hipStream_t st) {
+  if (f.N <= 16) return launch_few_rows<T, 1, kPair>(f, st);
+  if (f.N <= 32) return launch_few_rows<T, 2, kPair>(f, st);
+  if (f.N <= 48) return launch_few_rows<T, 3, kPair>(f, st);
+  return launch_few_rows<T, 4, kPair>(f, st);
+}
+
+template <typename T>
+ts_status fwd_few(const ts_gated_mlp_args& a, void* gate, void* up, void* act, void* out,
+                  hipStream_t st) {
+  TS_TRY((launch_few<T, true>(Few{raw(a.x), a.ldx, {raw(a.w_gate), raw(a.w_up)},
+                                  {a.ld_gate, a.ld_up}, a.N, a.F, a.H, gate, up, act,
+                                  a.activation}, st)));
+  if (out == nullptr) return TS_OK;
+  return launch_few<T, false>(Few{raw(act), a.F, {raw(a.w_down), nullptr}, {a.ld_down, 0}, a.N,
+                                  a.O, a.F, nullptr, nullptr, out, 0}, st);
+}
+
 template <typename T>
 ts_status fwd_typed(const ts_gated_mlp_args& a, void* gate, void* up, void* act, void* out,
                     void* ws, hipStream_t st) {
+  if (a.N <= ts_plan::kMlpFewRows) return fwd_few<T>(a, gate, up, act, out, st);
   const ts_plan::MlpPlan pl = ts_plan::mlp_plan(shape_of(a));
   Product p = product(a.x, a.ldx, a.w_gate, a.ld_gate, a.N, a.F, a.H, nullptr);
   p.B[1] = raw(a.w_up);

@@ -374,6 +374,25 @@ inline int64_t mlp_tiles(int64_t M, int64_t N, int waves, bool pair) {
   const int64_t bm = 32 * waves, bn = pair ? bm / 2 : bm;
   return ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
 }
+// Few rows (mlp_few): a workgroup of up to kMlpFewWaves waves for every 16 of F features, each with
+// a ring of k-blocks in LDS, 2 KiB for the 16 rows of each operand tile. Three k-blocks deep with
+// one tile of x, so that a CU holds two workgroups of a pair of projections (72 KiB); two with more
+// (up to 96 KiB). Measured on MI355X at H 4096, F 14336: 16 rows, depth 3 against 2, 72.5 and 74.4 us;
+// 32 rows 87.5 and 83.5; 4 waves against 2 and 8, 72.5, 82.4 and 76.4 us.
+constexpr int64_t kMlpFewRows = 64;
+constexpr int kMlpFewWaves = 4;
+TS_HOST_DEVICE constexpr int mlp_few_depth(int row_tiles) { return row_tiles == 1 ? 3 : 2; }
+inline int mlp_few_waves(int64_t K) {
+  const int64_t blocks = (K + kGemmBlockK - 1) / kGemmBlockK;
+  return (int)(blocks < kMlpFewWaves ? blocks : kMlpFewWaves);
+}
+// Weights of a launch above 64 MB are read past the caches: the last level's 256 MB would not keep
+// them, and their neighbours, until the next step, and not allocating there is faster (72.5 -> 66.4 us
+// at the sizes above). Weights that it may keep are read through it (H 2048, F 5632, three sets
+// in turn: 18.7 us, and 23.5 past the caches).
+inline bool mlp_few_stream(int64_t F, int64_t K, bool pair) {
+  return (pair ? 2 : 1) * F * K * 2 > ((int64_t)64 << 20);
+}
 struct MlpPlan {
   int up_waves, down_waves, da_waves, grad_waves;
   KSplit down, dx, dw, dwd;
