@@ -704,10 +704,9 @@ ts_status fwd_few(const ts_gated_mlp_args& a, void* gate, void* up, void* act, v
 }
 
 template <typename T>
-ts_status fwd_typed(const ts_gated_mlp_args& a, void* gate, void* up, void* act, void* out,
-                    void* ws, hipStream_t st) {
+ts_status fwd_typed(const ts_gated_mlp_args& a, const ts_plan::MlpFwdPlan& pl, void* gate,
+                    void* up, void* act, void* out, void* ws, hipStream_t st) {
   if (a.N <= ts_plan::kMlpFewRows) return fwd_few<T>(a, gate, up, act, out, st);
-  const ts_plan::MlpPlan pl = ts_plan::mlp_plan(shape_of(a));
   Product p = product(a.x, a.ldx, a.w_gate, a.ld_gate, a.N, a.F, a.H, nullptr);
   p.B[1] = raw(a.w_up);
   p.ldb[1] = a.ld_up;
@@ -733,12 +732,10 @@ ts_status launch_grads(const Grads& g, hipStream_t st) {
 }
 
 template <typename T>
-ts_status bwd_typed(const ts_gated_mlp_args& a, const void* gate, const void* up, const void* act,
-                    const void* dout, int64_t ldd, void* dx, void* dwg, void* dwu, void* dwd,
-                    uint8_t* ws, hipStream_t st) {
-  const ts_plan::MlpShape sh = shape_of(a);
-  const ts_plan::MlpPlan pl = ts_plan::mlp_plan(sh);
-  const ts_plan::MlpBwdWorkspace w = ts_plan::mlp_bwd_workspace(sh);
+ts_status bwd_typed(const ts_gated_mlp_args& a, const ts_plan::MlpBwdPlan& pl,
+                    const ts_plan::MlpBwdWorkspace& w, const void* gate, const void* up,
+                    const void* act, const void* dout, int64_t ldd, void* dx, void* dwg, void* dwu,
+                    void* dwd, uint8_t* ws, hipStream_t st) {
   void* dg = ws + w.dg;
   void* du = ws + w.du;
   const bool inner = dx != nullptr || dwg != nullptr || dwu != nullptr;
@@ -768,7 +765,7 @@ ts_status bwd_typed(const ts_gated_mlp_args& a, const void* gate, const void* up
   g.dw[2] = product(dout, ldd, act, a.F, a.O, a.F, a.N, dwd);
   set_split(g.dx, pl.dx, reinterpret_cast<float*>(ws + w.dx));
   for (int i = 0; i < 3; ++i)
-    set_split(g.dw[i], i < 2 ? pl.dw : pl.dwd, reinterpret_cast<float*>(ws + w.dw[i]));
+    set_split(g.dw[i], pl.dw, reinterpret_cast<float*>(ws + w.dw[i]));
   SumJobs s{};
   int n = 0;
   int64_t end = 0;
@@ -786,12 +783,14 @@ ts_status bwd_typed(const ts_gated_mlp_args& a, const void* gate, const void* up
 
 extern "C" size_t ts_gated_mlp_fwd_workspace_size(int64_t N, int64_t H, int64_t F, int64_t O) {
   if (N <= 0 || H <= 0 || F <= 0 || O < 0) return 0;
-  return (size_t)ts_plan::mlp_fwd_workspace(ts_plan::MlpShape{N, H, F, O});
+  const ts_plan::MlpShape s{N, H, F, O};
+  return (size_t)ts_plan::mlp_fwd_workspace(s, ts_plan::mlp_fwd_plan(s));
 }
 
 extern "C" size_t ts_gated_mlp_bwd_workspace_size(int64_t N, int64_t H, int64_t F, int64_t O) {
   if (N <= 0 || H <= 0 || F <= 0 || O < 0) return 0;
-  return (size_t)ts_plan::mlp_bwd_workspace(ts_plan::MlpShape{N, H, F, O}).total;
+  const ts_plan::MlpShape s{N, H, F, O};
+  return (size_t)ts_plan::mlp_bwd_workspace(s, ts_plan::mlp_bwd_plan(s)).total;
 }
 
 extern "C" ts_status ts_gated_mlp_fwd(const ts_gated_mlp_args* args, void* gate, void* up,
@@ -807,13 +806,16 @@ extern "C" ts_status ts_gated_mlp_fwd(const ts_gated_mlp_args* args, void* gate,
   if (!ts_host::aligned16(gate) || !ts_host::aligned16(up) || !ts_host::aligned16(act) ||
       !ts_host::aligned16(out) || !ts_host::aligned16(workspace))
     return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_fwd: outputs must be 16-byte aligned");
-  const size_t need = (size_t)ts_plan::mlp_fwd_workspace(shape_of(*args));
+  const ts_plan::MlpShape s = shape_of(*args);
+  const ts_plan::MlpFwdPlan pl = ts_plan::mlp_fwd_plan(s);
+  const size_t need = (size_t)ts_plan::mlp_fwd_workspace(s, pl);
   if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(TS_ERR_WORKSPACE, "gated_mlp_fwd: workspace of %zu bytes, need %zu",
                 workspace_bytes, need);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return args->dtype == TS_BF16 ? fwd_typed<__bf16>(*args, gate, up, act, out, workspace, st)
-                                : fwd_typed<_Float16>(*args, gate, up, act, out, workspace, st);
+  return args->dtype == TS_BF16
+             ? fwd_typed<__bf16>(*args, pl, gate, up, act, out, workspace, st)
+             : fwd_typed<_Float16>(*args, pl, gate, up, act, out, workspace, st);
 }
 
 extern "C" ts_status ts_gated_mlp_bwd(const ts_gated_mlp_args* args, const void* gate,
@@ -836,15 +838,18 @@ extern "C" ts_status ts_gated_mlp_bwd(const ts_gated_mlp_args* args, const void*
                         (const void*)dw_up, (const void*)dw_down, (const void*)workspace})
     if (!ts_host::aligned16(p))
       return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_bwd: buffers must be 16-byte aligned");
-  const size_t need = (size_t)ts_plan::mlp_bwd_workspace(shape_of(*args)).total;
+  const ts_plan::MlpShape s = shape_of(*args);
+  const ts_plan::MlpBwdPlan pl = ts_plan::mlp_bwd_plan(s);
+  const ts_plan::MlpBwdWorkspace w = ts_plan::mlp_bwd_workspace(s, pl);
+  const size_t need = (size_t)w.total;
   if (workspace == nullptr || workspace_bytes < need)
     return fail(TS_ERR_WORKSPACE, "gated_mlp_bwd: workspace of %zu bytes, need %zu",
                 workspace_bytes, need);
   hipStream_t st = static_cast<hipStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   return args->dtype == TS_BF16
-             ? bwd_typed<__bf16>(*args, gate, up, act, dout, ld_dout, dx, dw_gate, dw_up, dw_down,
-                                 ws, st)
-             : bwd_typed<_Float16>(*args, gate, up, act, dout, ld_dout, dx, dw_gate, dw_up,
+             ? bwd_typed<__bf16>(*args, pl, w, gate, up, act, dout, ld_dout, dx, dw_gate, dw_up,
+                                 dw_down, ws, st)
+             : bwd_typed<_Float16>(*args, pl, w, gate, up, act, dout, ld_dout, dx, dw_gate, dw_up,
                                    dw_down, ws, st);
 }

@@ -393,27 +393,137 @@ inline int mlp_few_waves(int64_t K) {
 inline bool mlp_few_stream(int64_t F, int64_t K, bool pair) {
   return (pair ? 2 : 1) * F * K * 2 > ((int64_t)64 << 20);
 }
-struct MlpPlan {
-  int up_waves, down_waves, da_waves, grad_waves;
-  KSplit down, dx, dw, dwd;
+struct MlpFwdPlan {
+  int up_waves, down_waves;  // 8: 256 x 256 tiles, 4: 128 x 128
+  KSplit down;
 };
-inline MlpPlan mlp_plan(const MlpShape& s) {
+struct MlpBwdPlan {
+  int da_waves, grad_waves;
+  KSplit dx, dw;  // dw: of all three weights
+};
+
+// Which tiles, and how many slots K is cut into, by an estimate of the time in microseconds (the
+// host's choice follows from the shape alone, so a shape's sums keep their order). Fitted to
+// MI355X: a k-block of a 256 x 256 tile takes 1.35 us in a launch of one tile a CU and 1.65 us while
+// the whole card is at its power limit, one of a 128 x 128 tile 0.5 us on half the card's CUs, 0.75 us
+// on all of them and 1.0 us beside another on its CU; a tile's start and epilogue 4 to 5 us; slots cost their partials' traffic and a launch. Measured
+// against 256 x 256 tiles without slots, N, H, F: 2045, 768, 2048 forward 68 -> 38 us, backward 120 ->
+// 66; 256, 2048, 5632 143 -> 41 and 296 -> 90; 100, 4096, 14336 399 -> 109 and 901 -> 245; at
+// 8192, 4096, 14336 128 x 128 tiles would take 14% longer.
+inline int64_t mlp_kblocks(int64_t K) { return (K + kGemmBlockK - 1) / kGemmBlockK; }
+inline double mlp_time(int64_t pieces, int64_t kblocks, int waves) {
+  if (waves == 8)
+    return (double)((pieces + 255) / 256) * (kblocks * (pieces <= 256 ? 1.35 : 1.65) + 5.0);
+  if (pieces <= 256) return kblocks * (pieces <= 128 ? 0.5 : 0.75) + 4.0;
+  return (double)((pieces + 511) / 512) * (kblocks * 1.0 + 5.0);
+}
+inline double mlp_slots_time(int64_t slots, int64_t M, int64_t N) {  // without the launch
+  return slots > 1 ? (double)(slots * M * N) * 8.0 / 4.5e6 : 0.0;
+}
+constexpr double kMlpSumLaunch = 4.0;
+constexpr int64_t kMlpSlotBytes = (int64_t)256 << 20;  // most partials of one product
+constexpr int64_t kMlpSlotBlocks = 4;                  // fewest k-blocks of a slot
+inline bool mlp_slots_ok(int64_t slots, int64_t M, int64_t N, int64_t K) {
+  return slots == 1 ||
+         (slots * kMlpSlotBlocks <= mlp_kblocks(K) && slots * M * N * 4 <= kMlpSlotBytes);
+}
+// K in `slots` slots of whole k-blocks, as many as are not empty.
+inline KSplit mlp_split(int64_t K, int64_t slots) {
+  KSplit k{slots, split_kper(K, slots)};
+  k.splits = (K + k.kper - 1) / k.kper;
+  return k;
+}
+
+// About when n1 pieces of length a, then n2 of length b, are done by m workers that take them in turn.
+inline double mlp_makespan(int64_t n1, double a, int64_t n2, double b, int64_t m) {
+  const int64_t r = n1 % m;              // workers free a piece later than the others
+  const double t0 = (double)(n1 / m) * a, t1 = r > 0 ? t0 + a : t0;
+  if (n2 == 0) return t1;
+  const double even = ((double)n2 * b + (double)(m - r) * t0 + (double)r * t1) / (double)m;
+  double best = 1e30;
+  for (int side = 0; side < 2; ++side) {  // the last piece ends with one of the two groups
+    const double start = side ? t1 : t0;
+    for (int k = 0; k < 4; ++k) {
+      const int64_t i = (int64_t)((even - start) / b) + k;
+      const double t = start + (double)i * b;
+      if (i < 1 || t < t1) continue;
+      const double done = (double)(m - r) * (double)(int64_t)((t - t0) / b + 1e-6) +
+                          (double)r * (double)(int64_t)((t - t1) / b + 1e-6);
+      if (done >= (double)n2 && t < best) best = t;
+    }
+  }
+  return best < 1e30 ? best : t1 + even;
+}
+
+inline int mlp_waves(int64_t M, int64_t N, int64_t K, bool pair) {
+  const int64_t kb = mlp_kblocks(K);
+  return mlp_time(mlp_tiles(M, N, 8, pair), kb, 8) <= mlp_time(mlp_tiles(M, N, 4, pair), kb, 4)
+             ? 8 : 4;
+}
+inline MlpFwdPlan mlp_fwd_plan(const MlpShape& s) {
   const KSplit one{1, 0};
-  (void)s;
-  return MlpPlan{8, 8, 8, 8, one, one, one, one};
+  MlpFwdPlan p{mlp_waves(s.N, s.F, s.H, true), 8, one};
+  if (s.O <= 0) return p;
+  double best = 1e30;
+  for (int waves = 8; waves >= 4; waves -= 4) {
+    const int64_t tiles = mlp_tiles(s.N, s.O, waves, false), kb = mlp_kblocks(s.F);
+    for (int64_t k = 1; k <= 16; k *= 2) {
+      if (!mlp_slots_ok(k, s.N, s.O, s.F)) break;
+      const double t = mlp_time(tiles * k, (kb + k - 1) / k, waves) +
+                       mlp_slots_time(k, s.N, s.O) + (k > 1 ? kMlpSumLaunch : 0.0);
+      if (t >= best) continue;
+      best = t;
+      p.down_waves = waves;
+      p.down = k > 1 ? mlp_split(s.F, k) : one;
+    }
+  }
+  return p;
+}
+inline MlpBwdPlan mlp_bwd_plan(const MlpShape& s) {
+  const KSplit one{1, 0};
+  MlpBwdPlan p{s.O > 0 ? mlp_waves(s.N, s.F, s.O, false) : 8, 8, one, one};
+  // dx [N, H] over 2 F, then dWg and dWu [F, H] and dWd [O, F] over N, in one grid
+  double best = 1e30;
+  const int64_t kx = mlp_kblocks(2 * s.F), kw = mlp_kblocks(s.N);
+  for (int waves = 8; waves >= 4; waves -= 4) {
+    const int64_t tx = mlp_tiles(s.N, s.H, waves, false);
+    const int64_t tw = 2 * mlp_tiles(s.F, s.H, waves, false) +
+                       (s.O > 0 ? mlp_tiles(s.O, s.F, waves, false) : 0);
+    for (int64_t x = 1; x <= 16; x *= 2) {
+      if (!mlp_slots_ok(x, s.N, s.H, 2 * s.F)) break;
+      for (int64_t w = 1; w <= 8; w *= 2) {
+        if (!mlp_slots_ok(w, s.F, s.H, s.N) ||
+            (s.O > 0 && !mlp_slots_ok(w, s.O, s.F, s.N)))
+          break;
+        const bool one_each = tx * x + tw * w <= kCus;
+        const double rate = waves == 8 ? (one_each ? 1.4 : 1.65) : (one_each ? 0.85 : 1.2);
+        double t = rate * mlp_makespan(tx * x, (double)((kx + x - 1) / x), tw * w,
+                                       (double)((kw + w - 1) / w),
+                                       waves == 8 || one_each ? kCus : 2 * kCus) +
+                   mlp_slots_time(x, s.N, s.H) + 2 * mlp_slots_time(w, s.F, s.H) +
+                   mlp_slots_time(w, s.O, s.F);
+        if (x > 1 || w > 1) t += kMlpSumLaunch;
+        if (t >= best) continue;
+        best = t;
+        p.grad_waves = waves;
+        p.dx = x > 1 ? mlp_split(2 * s.F, x) : one;
+        p.dw = w > 1 ? mlp_split(s.N, w) : one;
+      }
+    }
+  }
+  return p;
 }
 inline int64_t mlp_part_bytes(const KSplit& k, int64_t M, int64_t N) {
   return k.splits > 1 ? k.splits * M * N * 4 : 0;
 }
-inline int64_t mlp_fwd_workspace(const MlpShape& s) {
-  return s.O > 0 ? mlp_part_bytes(mlp_plan(s).down, s.N, s.O) : 0;
+inline int64_t mlp_fwd_workspace(const MlpShape& s, const MlpFwdPlan& p) {
+  return s.O > 0 && s.N > kMlpFewRows ? mlp_part_bytes(p.down, s.N, s.O) : 0;
 }
 // Byte offsets in the backward's workspace: dg and du, then the partials.
 struct MlpBwdWorkspace {
   int64_t dg, du, dx, dw[3], total;
 };
-inline MlpBwdWorkspace mlp_bwd_workspace(const MlpShape& s) {
-  const MlpPlan p = mlp_plan(s);
+inline MlpBwdWorkspace mlp_bwd_workspace(const MlpShape& s, const MlpBwdPlan& p) {
   MlpBwdWorkspace w{};
   int64_t off = 0;
   auto take = [&](int64_t bytes) {
@@ -426,7 +536,7 @@ inline MlpBwdWorkspace mlp_bwd_workspace(const MlpShape& s) {
   w.dx = take(mlp_part_bytes(p.dx, s.N, s.H));
   w.dw[0] = take(mlp_part_bytes(p.dw, s.F, s.H));
   w.dw[1] = take(mlp_part_bytes(p.dw, s.F, s.H));
-  w.dw[2] = take(s.O > 0 ? mlp_part_bytes(p.dwd, s.O, s.F) : 0);
+  w.dw[2] = take(s.O > 0 ? mlp_part_bytes(p.dw, s.O, s.F) : 0);
   w.total = off;
   return w;
 }
