@@ -223,11 +223,17 @@ def stream_handle(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+# the current device's index without torch.cuda's checks that the runtime is up (it is: a tensor
+# lives there), and one context that does nothing
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_no_switch = contextlib.nullcontext()
+
+
 def on_device(device: torch.device):
     """A context under which `device` is the current device, for a launch on its stream
     (a no-op context when it already is, the common case)."""
-    if device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
+    if device.index == _current_device():
+        return _no_switch
     return torch.cuda.device(device)
 
 

@@ -79,38 +79,35 @@ def _rows(t: Tensor) -> Tuple[Tensor, int]:
     return ops.as_rows(t if t.dim() else t.reshape(1))
 
 
-def _forward(x: Tensor, residual: Optional[Tensor], rng, drop: int) -> Tensor:
+def _forward(x: Tensor, residual: Optional[Tensor], rng, state: Optional[Tensor]) -> Tensor:
     if x.is_cuda and x.numel() == 0:
         return torch.empty(x.shape, dtype=x.dtype, device=x.device)
     x2d, ldx = _rows(x)
     r2d, ldr = (None, 0) if residual is None else _rows(residual)
-    return ops.dropout_forward(x2d, ldx, r2d, ldr, rng, drop, x.shape)
+    return ops.dropout_forward(x2d, ldx, r2d, ldr, rng, state, x.shape)
 
 
 class FusedDropoutFunction(torch.autograd.Function):
     """forward(x, residual or None, rng, drop) -> [residual +] dropout(x); differentiable in x and
-    residual."""
+    residual. rng is (seed, offset) or a device tensor, drop the 16-bit limit."""
 
     @staticmethod
     def forward(ctx, x: Tensor, residual: Optional[Tensor], rng, drop: int) -> Tensor:
-        ctx.drop = drop
-        if isinstance(rng, Tensor):
-            ctx.save_for_backward(rng)
-            ctx.rng = None
-        else:
-            ctx.rng = rng
-        return _forward(x, residual, rng, drop)
+        ctx.rng = ops.dropout_rng(rng, drop)
+        state = rng if isinstance(rng, Tensor) else None
+        if state is not None:
+            ctx.save_for_backward(state)
+        return _forward(x, residual, ctx.rng, state)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout: Tensor):
-        rng = ctx.rng if ctx.rng is not None else ctx.saved_tensors[0].contiguous()
-        dx = dres = None
-        if ctx.needs_input_grad[0]:
-            dx = _forward(dout, None, rng, ctx.drop) if ctx.drop else dout
-        if ctx.needs_input_grad[1]:
-            dres = dout
-        return dx, dres, None, None
+        dx = dout
+        if ctx.needs_input_grad[0] and ctx.rng.drop:
+            saved = ctx.saved_tensors
+            dx = _forward(dout, None, ctx.rng, saved[0].contiguous() if saved else None)
+        return (dx if ctx.needs_input_grad[0] else None,
+                dout if ctx.needs_input_grad[1] else None, None, None)
 
 
 def _dropout(what: str, x: Tensor, residual: Optional[Tensor], p: float, rng: RngLike,
@@ -122,7 +119,8 @@ def _dropout(what: str, x: Tensor, residual: Optional[Tensor], p: float, rng: Rn
     if ops.in_forward_ad() or (torch.is_grad_enabled() and (
             x.requires_grad or (residual is not None and residual.requires_grad))):
         return FusedDropoutFunction.apply(x, residual, rng, drop)
-    return _forward(x, residual, rng, drop)
+    return _forward(x, residual, ops.dropout_rng(rng, drop),
+                    rng if isinstance(rng, Tensor) else None)
 
 
 def fused_dropout(x: Tensor, p: float, rng: RngLike = None, training: bool = True) -> Tensor:
@@ -138,11 +136,11 @@ def fused_dropout_add(x: Tensor, residual: Tensor, p: float, rng: RngLike = None
     return _dropout("fused_dropout_add", x, residual, p, rng, training)
 
 
-def _norm_forward(x, residual, weight, eps, rng, drop):
+def _norm_forward(x, residual, weight, eps, rng, state):
     x2d, ldx = ops.as_rows(x)
     r2d, ldr = ops.as_rows(residual)
     w = weight.contiguous()
-    y, h, rstd = ops.dropout_add_rmsnorm_forward(x2d, ldx, r2d, ldr, w, eps, rng, drop, x.shape)
+    y, h, rstd = ops.dropout_add_rmsnorm_forward(x2d, ldx, r2d, ldr, w, eps, rng, state, x.shape)
     return y, h, w, rstd
 
 
@@ -153,10 +151,11 @@ class FusedDropoutAddRMSNormFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, residual: Tensor, weight: Tensor, eps: float, rng,
                 drop: int) -> Tuple[Tensor, Tensor]:
-        y, h, w, rstd = _norm_forward(x, residual, weight, eps, rng, drop)
+        ctx.rng = ops.dropout_rng(rng, drop)
+        state = rng if isinstance(rng, Tensor) else None
+        y, h, w, rstd = _norm_forward(x, residual, weight, eps, ctx.rng, state)
         ctx.set_materialize_grads(False)
-        ctx.drop, ctx.rng = drop, None if isinstance(rng, Tensor) else rng
-        ctx.save_for_backward(h, w, rstd, rng if isinstance(rng, Tensor) else None)
+        ctx.save_for_backward(h, w, rstd, state)
         return y, h
 
     @staticmethod
@@ -164,18 +163,17 @@ class FusedDropoutAddRMSNormFunction(torch.autograd.Function):
     def backward(ctx, dy: Optional[Tensor], dh: Optional[Tensor]):
         if dy is None and dh is None:
             return (None,) * 6
-        h, w, rstd, rng = ctx.saved_tensors
+        h, w, rstd, state = ctx.saved_tensors
         needs = ctx.needs_input_grad[:3]
         if h.numel() == 0:
             return (*[torch.zeros(s, dtype=t.dtype, device=t.device) if need else None
                       for need, s, t in zip(needs, (h.shape, h.shape, w.shape), (h, h, w))],
                     None, None, None)
-        rng = ctx.rng if rng is None else rng.contiguous()
         h2d, ldh = ops.as_rows(h)
         (dy, lddy), (dh, lddh) = [(None, 0) if d is None else ops.as_rows(d) for d in (dy, dh)]
         return (*ops.dropout_add_rmsnorm_backward(
-            dy, lddy, dh, lddh, h2d, ldh, w.contiguous(), rstd.contiguous(), rng, ctx.drop, needs,
-            h.shape), None, None, None)
+            dy, lddy, dh, lddh, h2d, ldh, w.contiguous(), rstd.contiguous(), ctx.rng,
+            None if state is None else state.contiguous(), needs, h.shape), None, None, None)
 
 
 def fused_dropout_add_rms_layernorm(x: Tensor, residual: Tensor, weight: Tensor, p: float,
@@ -201,7 +199,8 @@ def fused_dropout_add_rms_layernorm(x: Tensor, residual: Tensor, weight: Tensor,
                                and (x.requires_grad or residual.requires_grad
                                     or weight.requires_grad)):
         return FusedDropoutAddRMSNormFunction.apply(*args)
-    return _norm_forward(*args)[:2]
+    return _norm_forward(x, residual, weight, float(eps), ops.dropout_rng(rng, drop),
+                         rng if isinstance(rng, Tensor) else None)[:2]
 
 
 class FusedDropoutAddRMSNorm(nn.Module):

@@ -51,15 +51,13 @@ def _check(x: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], activati
 
 def _forward(x: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], activation: str,
              keep: bool):
-    """(result, the activation's code, kept g, u and gated product or None)."""
+    """(result, the activation's code, what the backward needs)."""
     code = _check(x, gate, up, down, activation)
     cols = (gate if down is None else down).shape[0]
-    x2d = x.reshape(-1, x.shape[-1])
-    g, u, a, y = ops.gated_mlp_forward(x2d, gate, up, down, code, keep)
-    out = a if down is None else y
+    kept, out = ops.gated_mlp_forward(x.reshape(-1, x.shape[-1]), gate, up, down, code, keep)
     if out.shape[1] != cols:
         out = out[:, :cols].contiguous()
-    return out.view(*x.shape[:-1], cols), code, (g, u, None if down is None else a)
+    return out.view(*x.shape[:-1], cols), code, kept
 
 
 class GatedMLPFunction(torch.autograd.Function):
@@ -70,16 +68,16 @@ class GatedMLPFunction(torch.autograd.Function):
     def forward(ctx, x: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor],
                 activation: str) -> Tensor:
         out, ctx.code, kept = _forward(x, gate, up, down, activation, True)
-        ctx.save_for_backward(x, gate, up, down, *kept)
+        ctx.save_for_backward(x, gate, up, down, kept)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout: Tensor):
-        x, gate, up, down, g, u, a = ctx.saved_tensors
+        x, gate, up, down, kept = ctx.saved_tensors
         grads = ops.gated_mlp_backward(
-            x.reshape(-1, x.shape[-1]), gate, up, down, ctx.code, g, u, a,
-            dout.reshape(-1, dout.shape[-1]), ctx.needs_input_grad[:4])
+            x.reshape(-1, x.shape[-1]), gate, up, down, ctx.code, kept,
+            dout.reshape(-1, dout.shape[-1]), ctx.needs_input_grad)
         if grads[0] is not None:
             grads[0] = grads[0].view(x.shape)
         return (*grads, None)

@@ -685,30 +685,35 @@ def _mlp_args(x2d, gate, up, down, code):
 
 def gated_mlp_forward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], code: int,
                       keep: bool):
-    """(g, u, gated product, result) with features rounded up to multiples of 8; g and u None
-    unless kept, the result None without a down weight."""
+    """(kept, result), features rounded up to multiples of 8: kept [., N, F] is g and u where
+    `keep`, then the gated product where it is not the result; None for nothing."""
     dev = _lib.require_gpu("gated_mlp", x2d, gate, up, down)
     n = x2d.shape[0]
     args, held = _mlp_args(x2d, gate, up, down, code)
-    new = lambda cols: torch.empty((n, cols), dtype=x2d.dtype, device=dev)
-    g, u = (new(args.F), new(args.F)) if keep else (None, None)
-    a, y = new(args.F), None if down is None else new(args.O)
+    f = args.F
+    inner = (2 if keep else 0) + (0 if down is None else 1)  # matrices that no caller sees
+    kept = torch.empty((inner, n, f), dtype=x2d.dtype, device=dev) if inner else None
+    out = torch.empty((n, f if down is None else args.O), dtype=x2d.dtype, device=dev)
     if n == 0:
-        return g, u, a, y
+        return kept, out
+    at = 0 if kept is None else kept.data_ptr()
+    step = 2 * n * f
+    g, u = (at, at + step) if keep else (0, 0)
+    a, y = (out.data_ptr(), 0) if down is None else (at + (2 * step if keep else 0), out.data_ptr())
     lib = _lib.load()
-    wsb = lib.ts_gated_mlp_fwd_workspace_size(n, args.H, args.F, args.O)
+    wsb = lib.ts_gated_mlp_fwd_workspace_size(n, args.H, f, args.O)
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
     with _lib.on_device(dev):
-        check(lib.ts_gated_mlp_fwd(ctypes.byref(args), ptr(g), ptr(u), a.data_ptr(), ptr(y),
-                                   ptr(ws), wsb, _lib.stream_handle(dev)), "ts_gated_mlp_fwd")
+        check(lib.ts_gated_mlp_fwd(ctypes.byref(args), g, u, a, y, ptr(ws), wsb,
+                                   _lib.stream_handle(dev)), "ts_gated_mlp_fwd")
     del held
-    return g, u, a, y
+    return kept, out
 
 
 def gated_mlp_backward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], code: int,
-                       g: Tensor, u: Tensor, a: Optional[Tensor], dout: Tensor, needs) -> list:
-    """Gradients of (x2d, gate, up, down), None where `needs` is false."""
-    dev = _lib.require_gpu("gated_mlp", x2d, gate, up, down, g, u, a, dout)
+                       kept: Tensor, dout: Tensor, needs) -> list:
+    """Gradients of (x2d, gate, up, down), None where `needs` is false; kept is the forward's."""
+    dev = _lib.require_gpu("gated_mlp", x2d, gate, up, down, kept, dout)
     n = x2d.shape[0]
     out = [None] * 4
     leaves = (x2d, gate, up, down)
@@ -722,15 +727,17 @@ def gated_mlp_backward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Ten
     shapes = ((n, args.H), (args.F, args.H), (args.F, args.H), (args.O, args.F))
     out = [torch.empty(s, dtype=x2d.dtype, device=dev) if k else None
            for s, k in zip(shapes, needs)]
-    g, u = g.contiguous(), u.contiguous()
-    a = None if a is None else a.contiguous()
+    kept = kept.contiguous()
+    at, step = kept.data_ptr(), 2 * n * args.F
     lib = _lib.load()
     wsb = lib.ts_gated_mlp_bwd_workspace_size(n, args.H, args.F, args.O)
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
     with _lib.on_device(dev):
-        check(lib.ts_gated_mlp_bwd(ctypes.byref(args), g.data_ptr(), u.data_ptr(), ptr(a),
-                                   d.data_ptr(), ldd, *[ptr(t) for t in out], ws.data_ptr(), wsb,
-                                   _lib.stream_handle(dev)), "ts_gated_mlp_bwd")
+        check(lib.ts_gated_mlp_bwd(ctypes.byref(args), at, at + step,
+                                   0 if down is None else at + 2 * step, d.data_ptr(), ldd,
+                                   *[0 if t is None else t.data_ptr() for t in out],
+                                   ws.data_ptr(), wsb, _lib.stream_handle(dev)),
+              "ts_gated_mlp_bwd")
     del held
     return [t if t is None or t.shape == s.shape else t[:s.shape[0], :s.shape[1]].contiguous()
             for t, s in zip(out, leaves)]
@@ -740,35 +747,37 @@ def gated_mlp_backward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Ten
 # Dropout from a counter-based generator
 # ---------------------------------------------------------------------------
 
-def _rng_arg(rng, drop: int):
-    """ts_dropout_rng of (seed, offset) or of a device state."""
-    if isinstance(rng, Tensor):
-        return ctypes.byref(_lib.DropoutRng(0, 0, rng.data_ptr(), drop))
-    return ctypes.byref(_lib.DropoutRng(rng[0], rng[1], 0, drop))
+def dropout_rng(rng, drop: int) -> "_lib.DropoutRng":
+    """ts_dropout_rng of (seed, offset); a device state's address is set where it is used."""
+    return (_lib.DropoutRng(0, 0, 0, drop) if isinstance(rng, Tensor)
+            else _lib.DropoutRng(rng[0], rng[1], 0, drop))
 
 
-def dropout_forward(x2d: Tensor, ldx: int, res2d: Optional[Tensor], ldr: int, rng, drop: int,
-                    shape) -> Tensor:
+def _rng_ref(rng: "_lib.DropoutRng", state: Optional[Tensor]):
+    if state is not None:
+        rng.state = state.data_ptr()
+    return ctypes.byref(rng)
+
+
+def dropout_forward(x2d: Tensor, ldx: int, res2d: Optional[Tensor], ldr: int,
+                    rng: "_lib.DropoutRng", state: Optional[Tensor], shape) -> Tensor:
     """[residual +] dropout(x2d), of `shape`."""
-    dev = _lib.require_gpu("dropout", x2d, res2d, rng if isinstance(rng, Tensor) else None)
+    dev = _lib.require_gpu("dropout", x2d, res2d, state)
     rows, cols = x2d.shape
     out = torch.empty(shape, dtype=x2d.dtype, device=dev)
-    if out.numel() == 0:
-        return out
     with _lib.on_device(dev):
         check(_lib.load().ts_dropout_fwd(
             x2d.data_ptr(), ldx, 0 if res2d is None else res2d.data_ptr(), ldr, out.data_ptr(),
-            cols, _lib.dtype_code(x2d, "dropout"), rows, cols, _rng_arg(rng, drop),
+            cols, _lib.dtype_code(x2d, "dropout"), rows, cols, _rng_ref(rng, state),
             _lib.stream_handle(dev)), "ts_dropout_fwd")
     return out
 
 
 def dropout_add_rmsnorm_forward(x2d: Tensor, ldx: int, res2d: Tensor, ldr: int, weight: Tensor,
-                                eps: float, rng, drop: int, shape
+                                eps: float, rng: "_lib.DropoutRng", state: Optional[Tensor], shape
                                 ) -> Tuple[Tensor, Tensor, Tensor]:
     """(y, h, rstd fp32 [rows]) of h = residual + dropout(x), y = RMSNorm(h); y and h of `shape`."""
-    dev = _lib.require_gpu("dropout_add_rmsnorm", x2d, res2d, weight,
-                           rng if isinstance(rng, Tensor) else None)
+    dev = _lib.require_gpu("dropout_add_rmsnorm", x2d, res2d, weight, state)
     rows, cols = x2d.shape
     y = torch.empty(shape, dtype=x2d.dtype, device=dev)
     h = torch.empty(shape, dtype=x2d.dtype, device=dev)
@@ -779,14 +788,15 @@ def dropout_add_rmsnorm_forward(x2d: Tensor, ldx: int, res2d: Tensor, ldr: int, 
         check(_lib.load().ts_dropout_add_rmsnorm_fwd(
             x2d.data_ptr(), ldx, res2d.data_ptr(), ldr, _lib.dtype_code(x2d, "dropout"),
             weight.data_ptr(), _lib.dtype_code(weight, "dropout_add_rmsnorm weight"), y.data_ptr(),
-            h.data_ptr(), rstd.data_ptr(), rows, cols, eps, _rng_arg(rng, drop),
+            h.data_ptr(), rstd.data_ptr(), rows, cols, eps, _rng_ref(rng, state),
             _lib.stream_handle(dev)), "ts_dropout_add_rmsnorm_fwd")
     return y, h, rstd
 
 
 def dropout_add_rmsnorm_backward(dy: Optional[Tensor], lddy: int, dh: Optional[Tensor], lddh: int,
-                                 h2d: Tensor, ldh: int, weight: Tensor, rstd: Tensor, rng,
-                                 drop: int, needs, shape) -> list:
+                                 h2d: Tensor, ldh: int, weight: Tensor, rstd: Tensor,
+                                 rng: "_lib.DropoutRng", state: Optional[Tensor], needs,
+                                 shape) -> list:
     """Gradients of (x, residual, weight), None where `needs` is false, the first two of
     `shape`."""
     dev = _lib.require_gpu("dropout_add_rmsnorm", dy, dh, h2d, weight, rstd)
@@ -804,7 +814,7 @@ def dropout_add_rmsnorm_backward(dy: Optional[Tensor], lddy: int, dh: Optional[T
         check(lib.ts_dropout_add_rmsnorm_bwd(
             at[0], lddy, at[1], lddh, h2d.data_ptr(), ldh, _lib.DTYPE_CODE[h2d.dtype],
             weight.data_ptr(), _lib.DTYPE_CODE[weight.dtype], rstd.data_ptr(), at[2], at[3], at[4],
-            rows, cols, _rng_arg(rng, drop), at[5], wsb, _lib.stream_handle(dev)),
+            rows, cols, _rng_ref(rng, state), at[5], wsb, _lib.stream_handle(dev)),
             "ts_dropout_add_rmsnorm_bwd")
     return out
 
