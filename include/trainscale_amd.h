@@ -685,12 +685,12 @@ size_t ts_gated_mlp_bwd_workspace_size(int64_t N, int64_t H, int64_t F, int64_t 
 /*
  * g = x w_gate^T, u = x w_up^T, act = activation(g) * u, out = act w_down^T: fp32 sums, act and
  * out rounded once each (out is formed from the rounded act). act: [N, F], out: [N, O] (NULL
- * without w_down), both contiguous. gate and up, [N, F] each, receive the rounded g and u for the
- * backward; NULL both: not kept. The three products share their launches' order of sums for a
- * given shape, so results repeat bit for bit.
+ * without w_down), both contiguous. keep_p and keep_q, [N, F] fp32 each, receive what the backward
+ * multiplies by, u * activation'(g) and activation(g); NULL both: no backward follows. A given
+ * shape's sums keep their order, so results repeat bit for bit.
  * Counterpart of the MLP patch's three products and SwiGLU (registry/__init__.py:1080-1091).
  */
-ts_status ts_gated_mlp_fwd(const ts_gated_mlp_args* args, void* gate, void* up, void* act,
+ts_status ts_gated_mlp_fwd(const ts_gated_mlp_args* args, float* keep_p, float* keep_q, void* act,
                            void* out, void* workspace, size_t workspace_bytes,
                            ts_stream_t stream);
 
@@ -699,10 +699,10 @@ ts_status ts_gated_mlp_fwd(const ts_gated_mlp_args* args, void* gate, void* up, 
  * kept, each contiguous in dtype and skipped where NULL: dx [N, H], dw_gate and dw_up [F, H],
  * dw_down [O, F]. The gradients of g and u are rounded to dtype between the products. N > 0.
  */
-ts_status ts_gated_mlp_bwd(const ts_gated_mlp_args* args, const void* gate, const void* up,
-                           const void* act, const void* dout, int64_t ld_dout, void* dx,
-                           void* dw_gate, void* dw_up, void* dw_down, void* workspace,
-                           size_t workspace_bytes, ts_stream_t stream);
+ts_status ts_gated_mlp_bwd(const ts_gated_mlp_args* args, const float* keep_p,
+                           const float* keep_q, const void* act, const void* dout,
+                           int64_t ld_dout, void* dx, void* dw_gate, void* dw_up, void* dw_down,
+                           void* workspace, size_t workspace_bytes, ts_stream_t stream);
 
 /* ------------------------------------------------------------------------ */
 /* Dropout from a counter-based generator                                    */

@@ -9,8 +9,11 @@
 // in memory: the backward reads the same weights as MN-major operands. What is fused:
 //   * Both projections are one product: a workgroup's 256 columns are the same 128 columns of g
 //     and of u, so that a lane holds g and u of one element and forms a in registers; x is read
-//     once for both. g and u are written (rounded) only where a backward will need them.
-//   * da never reaches memory: the epilogue of dy Wd reads g and u and writes dg and du.
+//     once for both. Where a backward will follow, the epilogue also writes what it multiplies da
+//     by, u act'(g) and act(g), in fp32: kept in 16 bits, g and u would add their roundings to
+//     those of dg and du (measured rms error of dx and the projections' gradients 1.76 of one bf16
+//     rounding against 1.41).
+//   * da never reaches memory: the epilogue of dy Wd reads the two factors and writes dg and du.
 //   * dx sums both products in one accumulation (K is the concatenation of dg and du), and
 //     dx, dWg, dWu and dWd, which are independent, share one grid.
 // a is rounded to 16 bits between the products, as dg and du are: MFMA operands are 16-bit.
@@ -45,20 +48,6 @@ constexpr float kInvSqrt2Pi = 0.3989422804014327f;
 // Beyond this the tanh form is g or 0 in fp32; its polynomial would overflow far out.
 constexpr float kGeluFar = 30.f;
 
-template <int kAct>
-__device__ inline float act_f(float g) {
-  if constexpr (kAct == TS_ACT_SILU) {
-    return g * sigmoid_f(g);
-  } else if constexpr (kAct == TS_ACT_GELU) {
-    return 0.5f * g * erfcf(-kSqrtHalf * g);
-  } else if constexpr (kAct == TS_ACT_GELU_TANH) {
-    const float c = fabsf(g) > kGeluFar ? copysignf(kGeluFar, g) : g;
-    return g * sigmoid_f(2.f * kGeluK * c * (1.f + kGeluC * c * c));
-  } else {
-    return g < 0.f ? 0.f : g;
-  }
-}
-
 // act(g), and its derivative in d.
 template <int kAct>
 __device__ inline float act_d(float g, float& d) {
@@ -92,19 +81,12 @@ __device__ inline void with_act(int act, F&& f) {
   }
 }
 
-// Two 16-bit roundings in one register, and back.
+// Two 16-bit roundings in one register.
 template <typename T>
 __device__ inline uint32_t pack2(float lo, float hi) {
   typedef T t2 __attribute__((ext_vector_type(2)));
   const t2 v = {(T)lo, (T)hi};
   return __builtin_bit_cast(uint32_t, v);
-}
-template <typename T>
-__device__ inline void unpack2(uint32_t p, float& lo, float& hi) {
-  typedef T t2 __attribute__((ext_vector_type(2)));
-  const t2 v = __builtin_bit_cast(t2, p);
-  lo = (float)v[0];
-  hi = (float)v[1];
 }
 
 // ---------------------------------------------------------------------------
@@ -126,8 +108,8 @@ struct Product {
 };
 
 struct Gated {  // what the gated epilogues read and write, [N, F] contiguous each
-  void* g;
-  void* u;
+  float* p;     // u act'(g), or NULL: not kept
+  float* q;     // act(g)
   void* a;
   void* dg;
   void* du;
@@ -136,8 +118,8 @@ struct Gated {  // what the gated epilogues read and write, [N, F] contiguous ea
 
 enum Epi : int {
   kEpiStore = 0,     // C, or a slot's fp32 partial
-  kEpiGatedFwd = 1,  // the columns are pairs of g and u: writes a, and g and u where given
-  kEpiGatedBwd = 2   // the product is da: reads g and u, writes dg and du
+  kEpiGatedFwd = 1,  // the columns are pairs of g and u: writes a, and p and q where given
+  kEpiGatedBwd = 2   // the product is da: reads p and q, writes dg and du
 };
 
 // The lanes' 16-byte pieces of rows of a [M, N] matrix in the accumulators' order.
@@ -223,86 +205,80 @@ __device__ inline void product_tile(const Product& a, const Gated& e, int64_t bi
   } else if constexpr (kEpi == kEpiGatedFwd) {
     // column tiles 0 .. kHJ - 1 are g, the others u of the same columns
     const int64_t nb = n0 + wn * (C::CW / 2);
-    T* G = static_cast<T*>(e.g);
-    T* U = static_cast<T*>(e.u);
     T* O = static_cast<T*>(e.a);
-    auto rows = [&](const f32x4 (&t)[C::kTI][C::kTJ], int j0, T* out) {
-#pragma unroll
-      for (int i = 0; i < C::kTI; ++i)
-#pragma unroll
-        for (int p = 0; p < C::kHJ / 2; ++p) {
-          const int64_t gm = gm0 + 16 * i, gc = nb + wide_col(p, g4);
-          const f32x4 x = t[i][j0 + 2 * p], y = t[i][j0 + 2 * p + 1];
-          const u32x4 v = widen(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]),
-                                pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]));
-          if (gm < a.M && gc < a.N) st16(out + gm * a.N + gc, v);
-        }
-    };
-    if (G != nullptr) {
-      rows(acc.t, 0, G);
-      rows(acc.t, C::kHJ, U);
-    }
-    with_act(e.act, [&](auto act) {
-#pragma unroll
-      for (int i = 0; i < C::kTI; ++i)
-#pragma unroll
-        for (int j = 0; j < C::kHJ; ++j)
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-            acc.t[i][j][q] = act_f<decltype(act)::value>(acc.t[i][j][q]) * acc.t[i][C::kHJ + j][q];
-    });
-    rows(acc.t, 0, O);
-  } else {
-    const int64_t nb = n0 + wn * C::CW;
-    const T* G = static_cast<const T*>(e.g);
-    const T* U = static_cast<const T*>(e.u);
-    T* DG = static_cast<T*>(e.dg);
-    T* DU = static_cast<T*>(e.du);
     with_act(e.act, [&](auto act) {
 #pragma unroll
       for (int i = 0; i < C::kTI; ++i) {
         const int64_t gm = gm0 + 16 * i;
-        // a row block's old values are loaded before the first is used
-        u32x4 qg[C::kTJ / 2], qu[C::kTJ / 2];
 #pragma unroll
-        for (int p = 0; p < C::kTJ / 2; ++p) {
-          const int64_t gc = nb + wide_col(p, g4);
-          const bool in = gm < a.M && gc < a.N;
-          qg[p] = in ? ld16(G + gm * a.N + gc) : u32x4{0u, 0u, 0u, 0u};
-          qu[p] = in ? ld16(U + gm * a.N + gc) : u32x4{0u, 0u, 0u, 0u};
-        }
+        for (int j = 0; j < C::kHJ; ++j) {
+          f32x4 p, q;
 #pragma unroll
-        for (int p = 0; p < C::kTJ / 2; ++p) {
-          const int64_t gc = nb + wide_col(p, g4);
-          // back to the accumulators' layout
-          const u32x4 vg = widen(qg[p][0], qg[p][1], qg[p][2], qg[p][3]);
-          const u32x4 vu = widen(qu[p][0], qu[p][1], qu[p][2], qu[p][3]);
-          uint32_t pg[4], pu[4];
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            const f32x4 da = acc.t[i][2 * p + h / 2];
-            float g[2], u[2], t, d, og[2], ou[2];
-            unpack2<T>(vg[h], g[0], g[1]);
-            unpack2<T>(vu[h], u[0], u[1]);
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-              const float x = da[2 * (h & 1) + b];
-              t = act_d<decltype(act)::value>(g[b], d);
-              og[b] = x * u[b] * d;
-              ou[b] = x * t;
-            }
-            pg[h] = pack2<T>(og[0], og[1]);
-            pu[h] = pack2<T>(ou[0], ou[1]);
+          for (int b = 0; b < 4; ++b) {
+            const float u = acc.t[i][C::kHJ + j][b];
+            float d;
+            q[b] = act_d<decltype(act)::value>(acc.t[i][j][b], d);
+            p[b] = u * d;
+            acc.t[i][j][b] = q[b] * u;
           }
-          const u32x4 wg = widen(pg[0], pg[1], pg[2], pg[3]);
-          const u32x4 wu = widen(pu[0], pu[1], pu[2], pu[3]);
-          if (gm < a.M && gc < a.N) {
-            st16(DG + gm * a.N + gc, wg);
-            st16(DU + gm * a.N + gc, wu);
+          const int64_t gc = nb + 16 * j + 4 * g4;
+          if (e.p != nullptr && gm < a.M && gc < a.N) {
+            *reinterpret_cast<f32x4*>(e.p + gm * a.N + gc) = p;
+            *reinterpret_cast<f32x4*>(e.q + gm * a.N + gc) = q;
           }
         }
       }
     });
+#pragma unroll
+    for (int i = 0; i < C::kTI; ++i)
+#pragma unroll
+      for (int p = 0; p < C::kHJ / 2; ++p) {
+        const int64_t gm = gm0 + 16 * i, gc = nb + wide_col(p, g4);
+        const f32x4 x = acc.t[i][2 * p], y = acc.t[i][2 * p + 1];
+        const u32x4 v = widen(pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3]), pack2<T>(y[0], y[1]),
+                              pack2<T>(y[2], y[3]));
+        if (gm < a.M && gc < a.N) st16(O + gm * a.N + gc, v);
+      }
+  } else {
+    const int64_t nb = n0 + wn * C::CW;
+    T* DG = static_cast<T*>(e.dg);
+    T* DU = static_cast<T*>(e.du);
+#pragma unroll
+    for (int i = 0; i < C::kTI; ++i) {
+      const int64_t gm = gm0 + 16 * i;
+      // the factors of half a row block are loaded before the first is used
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        f32x4 p[C::kHJ], q[C::kHJ];
+#pragma unroll
+        for (int j = 0; j < C::kHJ; ++j) {
+          const int64_t gc = nb + 16 * (h * C::kHJ + j) + 4 * g4;
+          const bool in = gm < a.M && gc < a.N;
+          p[j] = in ? *reinterpret_cast<const f32x4*>(e.p + gm * a.N + gc) : f32x4{0, 0, 0, 0};
+          q[j] = in ? *reinterpret_cast<const f32x4*>(e.q + gm * a.N + gc) : f32x4{0, 0, 0, 0};
+        }
+#pragma unroll
+        for (int j = 0; j < C::kHJ; ++j) {
+          const f32x4 da = acc.t[i][h * C::kHJ + j];
+          p[j] *= da;
+          q[j] *= da;
+        }
+#pragma unroll
+        for (int j = 0; j < C::kHJ; j += 2) {
+          const int64_t gc = nb + wide_col((h * C::kHJ + j) / 2, g4);
+          const u32x4 vg = widen(pack2<T>(p[j][0], p[j][1]), pack2<T>(p[j][2], p[j][3]),
+                                 pack2<T>(p[j + 1][0], p[j + 1][1]),
+                                 pack2<T>(p[j + 1][2], p[j + 1][3]));
+          const u32x4 vu = widen(pack2<T>(q[j][0], q[j][1]), pack2<T>(q[j][2], q[j][3]),
+                                 pack2<T>(q[j + 1][0], q[j + 1][1]),
+                                 pack2<T>(q[j + 1][2], q[j + 1][3]));
+          if (gm < a.M && gc < a.N) {
+            st16(DG + gm * a.N + gc, vg);
+            st16(DU + gm * a.N + gc, vu);
+          }
+        }
+      }
+    }
   }
 }
 
@@ -353,8 +329,8 @@ struct Few {
   const __bf16* w[2];
   int64_t ldw[2];
   int64_t N, F, K;
-  void* g;
-  void* u;
+  float* p;
+  float* q;
   void* out;
   int32_t act;
 };
@@ -478,21 +454,24 @@ __global__ __launch_bounds__(64 * ts_plan::kMlpFewWaves) void mlp_few(const Few 
     const int64_t r = (i >> 6) * 16 + (i & 15), fo = f0 + ((i & 63) >> 4) * 4;
     if (r >= a.N || fo >= a.F) continue;
     const int64_t at = r * a.F + fo;
-    auto put = [&](void* o, const f32x4& v) {
-      *reinterpret_cast<uint2*>(static_cast<T*>(o) + at) =
-          make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
-    };
     if constexpr (kPair) {
-      if (a.g != nullptr) {
-        put(a.g, s[0]);
-        put(a.u, s[1]);
-      }
+      f32x4 p, q;
       with_act(a.act, [&](auto act) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) s[0][q] = act_f<decltype(act)::value>(s[0][q]) * s[1][q];
+        for (int b = 0; b < 4; ++b) {
+          float d;
+          q[b] = act_d<decltype(act)::value>(s[0][b], d);
+          p[b] = s[1][b] * d;
+          s[0][b] = q[b] * s[1][b];
+        }
       });
+      if (a.p != nullptr) {
+        *reinterpret_cast<f32x4*>(a.p + at) = p;
+        *reinterpret_cast<f32x4*>(a.q + at) = q;
+      }
     }
-    put(a.out, s[0]);
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at) =
+        make_uint2(pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]));
   }
 }
 
@@ -534,30 +513,29 @@ __global__ __launch_bounds__(256) void mlp_sum_slots(const SumJobs s) {
 // ---------------------------------------------------------------------------
 template <typename T>
 __global__ __launch_bounds__(256) void mlp_gate_bwd(const T* __restrict__ da, int64_t ldd,
-                                                    const T* __restrict__ g,
-                                                    const T* __restrict__ u, T* __restrict__ dg,
-                                                    T* __restrict__ du, int64_t nvec, int64_t F8,
-                                                    int act) {
+                                                    const float* __restrict__ p,
+                                                    const float* __restrict__ q,
+                                                    T* __restrict__ dg, T* __restrict__ du,
+                                                    int64_t nvec, int64_t F8) {
   const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (v >= nvec) return;
   const int64_t r = v / F8;
-  const u32x4 qd = ld16_any_stream(da + r * ldd + (v - r * F8) * 8);
-  const u32x4 qg = ld16_stream(g + v * 8), qu = ld16_stream(u + v * 8);
-  float d[8], G[8], U[8];
+  const u32x4 qd = ld16_stream(da + r * ldd + (v - r * F8) * 8);
+  const u32x4 p0 = ld16_stream(p + v * 8), p1 = ld16_stream(p + v * 8 + 4);
+  const u32x4 q0 = ld16_stream(q + v * 8), q1 = ld16_stream(q + v * 8 + 4);
+  float d[8], P[8], Q[8];
   Elt<T>::unpack(qd, d);
-  Elt<T>::unpack(qg, G);
-  Elt<T>::unpack(qu, U);
-  with_act(act, [&](auto a) {
+  Elt<float>::unpack(p0, P);
+  Elt<float>::unpack(p1, P + 4);
+  Elt<float>::unpack(q0, Q);
+  Elt<float>::unpack(q1, Q + 4);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float dt;
-      const float t = act_d<decltype(a)::value>(G[i], dt);
-      G[i] = d[i] * U[i] * dt;
-      U[i] = d[i] * t;
-    }
-  });
-  st16(dg + v * 8, Elt<T>::pack(G));
-  st16(du + v * 8, Elt<T>::pack(U));
+  for (int i = 0; i < 8; ++i) {
+    P[i] *= d[i];
+    Q[i] *= d[i];
+  }
+  st16(dg + v * 8, Elt<T>::pack(P));
+  st16(du + v * 8, Elt<T>::pack(Q));
 }
 
 // ---------------------------------------------------------------------------
@@ -693,10 +671,10 @@ ts_status launch_few(const Few& f, hipStream_t st) {
 }
 
 template <typename T>
-ts_status fwd_few(const ts_gated_mlp_args& a, void* gate, void* up, void* act, void* out,
+ts_status fwd_few(const ts_gated_mlp_args& a, float* p, float* q, void* act, void* out,
                   hipStream_t st) {
   TS_TRY((launch_few<T, true>(Few{raw(a.x), a.ldx, {raw(a.w_gate), raw(a.w_up)},
-                                  {a.ld_gate, a.ld_up}, a.N, a.F, a.H, gate, up, act,
+                                  {a.ld_gate, a.ld_up}, a.N, a.F, a.H, p, q, act,
                                   a.activation}, st)));
   if (out == nullptr) return TS_OK;
   return launch_few<T, false>(Few{raw(act), a.F, {raw(a.w_down), nullptr}, {a.ld_down, 0}, a.N,
@@ -704,13 +682,13 @@ ts_status fwd_few(const ts_gated_mlp_args& a, void* gate, void* up, void* act, v
 }
 
 template <typename T>
-ts_status fwd_typed(const ts_gated_mlp_args& a, const ts_plan::MlpFwdPlan& pl, void* gate,
-                    void* up, void* act, void* out, void* ws, hipStream_t st) {
-  if (a.N <= ts_plan::kMlpFewRows) return fwd_few<T>(a, gate, up, act, out, st);
+ts_status fwd_typed(const ts_gated_mlp_args& a, const ts_plan::MlpFwdPlan& pl, float* keep_p,
+                    float* keep_q, void* act, void* out, void* ws, hipStream_t st) {
+  if (a.N <= ts_plan::kMlpFewRows) return fwd_few<T>(a, keep_p, keep_q, act, out, st);
   Product p = product(a.x, a.ldx, a.w_gate, a.ld_gate, a.N, a.F, a.H, nullptr);
   p.B[1] = raw(a.w_up);
   p.ldb[1] = a.ld_up;
-  const Gated e{gate, up, act, nullptr, nullptr, a.activation};
+  const Gated e{keep_p, keep_q, act, nullptr, nullptr, a.activation};
   TS_TRY((launch_product<T, kEpiGatedFwd, kKMajor, kKMajor>(p, e, pl.up_waves, st, "mlp_gated")));
   if (out == nullptr) return TS_OK;
   Product d = product(act, a.F, a.w_down, a.ld_down, a.N, a.O, a.F, out);
@@ -733,7 +711,7 @@ ts_status launch_grads(const Grads& g, hipStream_t st) {
 
 template <typename T>
 ts_status bwd_typed(const ts_gated_mlp_args& a, const ts_plan::MlpBwdPlan& pl,
-                    const ts_plan::MlpBwdWorkspace& w, const void* gate, const void* up,
+                    const ts_plan::MlpBwdWorkspace& w, const float* keep_p, const float* keep_q,
                     const void* act, const void* dout, int64_t ldd, void* dx, void* dwg, void* dwu,
                     void* dwd, uint8_t* ws, hipStream_t st) {
   void* dg = ws + w.dg;
@@ -741,7 +719,8 @@ ts_status bwd_typed(const ts_gated_mlp_args& a, const ts_plan::MlpBwdPlan& pl,
   const bool inner = dx != nullptr || dwg != nullptr || dwu != nullptr;
   if (inner && a.w_down != nullptr) {
     const Product p = product(dout, ldd, a.w_down, a.ld_down, a.N, a.F, a.O, nullptr);
-    const Gated e{const_cast<void*>(gate), const_cast<void*>(up), nullptr, dg, du, a.activation};
+    const Gated e{const_cast<float*>(keep_p), const_cast<float*>(keep_q), nullptr, dg, du,
+                  a.activation};
     TS_TRY((launch_product<T, kEpiGatedBwd, kKMajor, kMNMajor>(p, e, pl.da_waves, st,
                                                                "mlp_gated_bwd")));
   } else if (inner) {
@@ -749,9 +728,8 @@ ts_status bwd_typed(const ts_gated_mlp_args& a, const ts_plan::MlpBwdPlan& pl,
     if (blocks > ts_plan::max_blocks(256))
       return ts_host::fail(TS_ERR_SHAPE, "mlp_gate_bwd: too large");
     hipLaunchKernelGGL(mlp_gate_bwd<T>, dim3((unsigned)blocks), dim3(256), 0, st,
-                       static_cast<const T*>(dout), ldd, static_cast<const T*>(gate),
-                       static_cast<const T*>(up), static_cast<T*>(dg), static_cast<T*>(du), nvec,
-                       a.F / 8, (int)a.activation);
+                       static_cast<const T*>(dout), ldd, keep_p, keep_q, static_cast<T*>(dg),
+                       static_cast<T*>(du), nvec, a.F / 8);
     TS_TRY(ts_host::check_launch("mlp_gate_bwd"));
   }
   Grads g{};
@@ -793,17 +771,17 @@ extern "C" size_t ts_gated_mlp_bwd_workspace_size(int64_t N, int64_t H, int64_t 
   return (size_t)ts_plan::mlp_bwd_workspace(s, ts_plan::mlp_bwd_plan(s)).total;
 }
 
-extern "C" ts_status ts_gated_mlp_fwd(const ts_gated_mlp_args* args, void* gate, void* up,
-                                      void* act, void* out, void* workspace,
+extern "C" ts_status ts_gated_mlp_fwd(const ts_gated_mlp_args* args, float* keep_p,
+                                      float* keep_q, void* act, void* out, void* workspace,
                                       size_t workspace_bytes, ts_stream_t stream) {
   using ts_host::fail;
   TS_TRY(check_args("gated_mlp_fwd", args));
   if (args->N == 0) return TS_OK;
   if (act == nullptr || (out == nullptr) != (args->w_down == nullptr))
     return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_fwd: out goes with w_down, act is needed");
-  if ((gate == nullptr) != (up == nullptr))
-    return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_fwd: gate and up are kept together");
-  if (!ts_host::aligned16(gate) || !ts_host::aligned16(up) || !ts_host::aligned16(act) ||
+  if ((keep_p == nullptr) != (keep_q == nullptr))
+    return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_fwd: keep_p and keep_q go together");
+  if (!ts_host::aligned16(keep_p) || !ts_host::aligned16(keep_q) || !ts_host::aligned16(act) ||
       !ts_host::aligned16(out) || !ts_host::aligned16(workspace))
     return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_fwd: outputs must be 16-byte aligned");
   const ts_plan::MlpShape s = shape_of(*args);
@@ -814,12 +792,12 @@ extern "C" ts_status ts_gated_mlp_fwd(const ts_gated_mlp_args* args, void* gate,
                 workspace_bytes, need);
   hipStream_t st = static_cast<hipStream_t>(stream);
   return args->dtype == TS_BF16
-             ? fwd_typed<__bf16>(*args, pl, gate, up, act, out, workspace, st)
-             : fwd_typed<_Float16>(*args, pl, gate, up, act, out, workspace, st);
+             ? fwd_typed<__bf16>(*args, pl, keep_p, keep_q, act, out, workspace, st)
+             : fwd_typed<_Float16>(*args, pl, keep_p, keep_q, act, out, workspace, st);
 }
 
-extern "C" ts_status ts_gated_mlp_bwd(const ts_gated_mlp_args* args, const void* gate,
-                                      const void* up, const void* act, const void* dout,
+extern "C" ts_status ts_gated_mlp_bwd(const ts_gated_mlp_args* args, const float* keep_p,
+                                      const float* keep_q, const void* act, const void* dout,
                                       int64_t ld_dout, void* dx, void* dw_gate, void* dw_up,
                                       void* dw_down, void* workspace, size_t workspace_bytes,
                                       ts_stream_t stream) {
@@ -827,14 +805,14 @@ extern "C" ts_status ts_gated_mlp_bwd(const ts_gated_mlp_args* args, const void*
   TS_TRY(check_args("gated_mlp_bwd", args));
   if (args->N == 0) return fail(TS_ERR_SHAPE, "gated_mlp_bwd: no rows (the gradients are zeros)");
   const bool down = args->w_down != nullptr;
-  if (gate == nullptr || up == nullptr || dout == nullptr || (down && act == nullptr))
+  if (keep_p == nullptr || keep_q == nullptr || dout == nullptr || (down && act == nullptr))
     return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_bwd: NULL operand");
   if (!down && dw_down != nullptr)
     return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_bwd: dw_down without w_down");
   const int64_t cols = down ? args->O : args->F;
   if (ld_dout < cols || ld_dout % 8 || ld_dout > kMaxDim)
     return fail(TS_ERR_SHAPE, "gated_mlp_bwd: bad row stride of dout");
-  for (const void* p : {gate, up, act, dout, (const void*)dx, (const void*)dw_gate,
+  for (const void* p : {(const void*)keep_p, (const void*)keep_q, act, dout, (const void*)dx, (const void*)dw_gate,
                         (const void*)dw_up, (const void*)dw_down, (const void*)workspace})
     if (!ts_host::aligned16(p))
       return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_bwd: buffers must be 16-byte aligned");
@@ -848,8 +826,8 @@ extern "C" ts_status ts_gated_mlp_bwd(const ts_gated_mlp_args* args, const void*
   hipStream_t st = static_cast<hipStream_t>(stream);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   return args->dtype == TS_BF16
-             ? bwd_typed<__bf16>(*args, pl, w, gate, up, act, dout, ld_dout, dx, dw_gate, dw_up,
+             ? bwd_typed<__bf16>(*args, pl, w, keep_p, keep_q, act, dout, ld_dout, dx, dw_gate, dw_up,
                                  dw_down, ws, st)
-             : bwd_typed<_Float16>(*args, pl, w, gate, up, act, dout, ld_dout, dx, dw_gate, dw_up,
+             : bwd_typed<_Float16>(*args, pl, w, keep_p, keep_q, act, dout, ld_dout, dx, dw_gate, dw_up,
                                    dw_down, ws, st);
 }

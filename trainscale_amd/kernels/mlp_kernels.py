@@ -6,8 +6,9 @@ projection. Weights have ``nn.Linear``'s layout. bf16 and fp16; the sums are fp3
 between the products (the gated product forward, the gradients of both projections backward) is
 rounded to the data type once, where the unfused block rounds g, u, act(g) and the product.
 
-The forward keeps x, the weights, both projections and the gated product for the backward:
-3 N F 16-bit values beside x. Without a gradient to compute only the gated product is formed.
+Where a gradient will follow, the forward keeps x, the weights, the gated product and the two
+factors of the backward in fp32 (up * act'(gate) and act(gate)): 10 N F bytes, so that no rounding
+of the projections adds to the gradients'. Otherwise only the gated product is formed.
 """
 from __future__ import annotations
 

@@ -685,26 +685,28 @@ def _mlp_args(x2d, gate, up, down, code):
 
 def gated_mlp_forward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], code: int,
                       keep: bool):
-    """(kept, result), features rounded up to multiples of 8: kept [., N, F] is g and u where
-    `keep`, then the gated product where it is not the result; None for nothing."""
+    """(kept, result), features rounded up to multiples of 8. kept holds what the backward needs
+    (2 N F fp32 values, where `keep`) and then the gated product (N F values), where that is not
+    the result; None for nothing."""
     dev = _lib.require_gpu("gated_mlp", x2d, gate, up, down)
     n = x2d.shape[0]
     args, held = _mlp_args(x2d, gate, up, down, code)
     f = args.F
-    inner = (2 if keep else 0) + (0 if down is None else 1)  # matrices that no caller sees
+    # fp32 factors of the backward, then the 16-bit product, which takes half a matrix
+    inner = (4 if keep else 0) + (0 if down is None else 1)
     kept = torch.empty((inner, n, f), dtype=x2d.dtype, device=dev) if inner else None
     out = torch.empty((n, f if down is None else args.O), dtype=x2d.dtype, device=dev)
     if n == 0:
         return kept, out
     at = 0 if kept is None else kept.data_ptr()
-    step = 2 * n * f
-    g, u = (at, at + step) if keep else (0, 0)
+    step = 4 * n * f
+    p, q = (at, at + step) if keep else (0, 0)
     a, y = (out.data_ptr(), 0) if down is None else (at + (2 * step if keep else 0), out.data_ptr())
     lib = _lib.load()
     wsb = lib.ts_gated_mlp_fwd_workspace_size(n, args.H, f, args.O)
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
     with _lib.on_device(dev):
-        check(lib.ts_gated_mlp_fwd(ctypes.byref(args), g, u, a, y, ptr(ws), wsb,
+        check(lib.ts_gated_mlp_fwd(ctypes.byref(args), p, q, a, y, ptr(ws), wsb,
                                    _lib.stream_handle(dev)), "ts_gated_mlp_fwd")
     del held
     return kept, out
@@ -728,7 +730,7 @@ def gated_mlp_backward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Ten
     out = [torch.empty(s, dtype=x2d.dtype, device=dev) if k else None
            for s, k in zip(shapes, needs)]
     kept = kept.contiguous()
-    at, step = kept.data_ptr(), 2 * n * args.F
+    at, step = kept.data_ptr(), 4 * n * args.F
     lib = _lib.load()
     wsb = lib.ts_gated_mlp_bwd_workspace_size(n, args.H, args.F, args.O)
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
