@@ -5,8 +5,10 @@
 // act: silu g s(g); gelu g Phi(g); its tanh form g s(2 sqrt(2/pi) (g + 0.044715 g^3)); relu, with
 // s(z) = 1 / (1 + e^-z). Without Wd, y = a.
 //
-// Products run on the MFMA core (gemm.hpp), 16-bit operands and fp32 sums. Nothing is transposed
-// in memory: the backward reads the same weights as MN-major operands. What is fused:
+// Products run on the MFMA core (gemm.hpp), 16-bit operands and fp32 sums. The backward's operands
+// are transposes of what is in memory and are read in place, as MN-major operands: transposed copies
+// of the weights for da and dx were slower than that at every size (N 8190, H 8192, F 4096: backward
+// 2400 us in place, 2510 with copies). What is fused:
 //   * Both projections are one product: a workgroup's 256 columns are the same 128 columns of g
 //     and of u, so that a lane holds g and u of one element and forms a in registers; x is read
 //     once for both. Where a backward will follow, the epilogue also writes what it multiplies da
@@ -138,7 +140,7 @@ __device__ inline void epi_store(const AccOf<kW>& acc, int64_t M, int64_t N, int
   }
 }
 
-template <typename T, int kEpi, int kMA, int kMB, int kW>
+template <typename T, int kEpi, int kMA, int kMB, int kW, int kSegs>
 __device__ inline void product_tile(const Product& a, const Gated& e, int64_t bid, uint8_t* smem) {
   using C = Cfg<kW>;
   constexpr bool kPair = kEpi == kEpiGatedFwd;
@@ -158,8 +160,7 @@ __device__ inline void product_tile(const Product& a, const Gated& e, int64_t bi
     ts_gemm::mainloop_acc<kKMajor, kKMajor, kW, T>(la, lb, a.K, wn * (C::CW / 2),
                                                    C::kBM / 2 + wn * (C::CW / 2), smem, acc);
   } else {
-    // dx alone has two segments (dg and du, each its own weight)
-    constexpr int kSegs = kEpi == kEpiStore && kMA == kKMajor && kMB == kMNMajor ? 2 : 1;
+    // dx has two segments (dg and du, each its own weight)
     const int64_t lo = slot * a.kper;  // of the joint K
     int64_t left = kSegs * a.K - lo < a.kper ? kSegs * a.K - lo : a.kper;
     int64_t k0 = lo;
@@ -169,10 +170,8 @@ __device__ inline void product_tile(const Product& a, const Gated& e, int64_t bi
       if (kSegs == 1 || n > 0) {     // uniform
         const __bf16* A = a.A[s] + (kMA == kKMajor ? k0 : k0 * a.lda);
         const __bf16* B = a.B[s] + (kMB == kKMajor ? k0 : k0 * a.ldb[s]);
-        const ts_gemm::OpLoader<kMA, kW> la(A, a.lda, a.M, m0);
-        const ts_gemm::OpLoader<kMB, kW> lb(B, a.ldb[s], a.N, n0);
-        ts_gemm::mainloop_acc<kMA, kMB, kW, T>(la, lb, n, wn * C::CW, wn * C::CW + C::CW / 2,
-                                               smem, acc);
+        ts_gemm::mainloop_more<kMA, kMB, kW, T>(A, a.lda, a.M, B, a.ldb[s], a.N, n, m0, n0, smem,
+                                                acc);
         left -= n;
         k0 += n;
         if (kSegs > 1) __syncthreads();  // the operands' tiles in LDS are free again
@@ -243,39 +242,41 @@ __device__ inline void product_tile(const Product& a, const Gated& e, int64_t bi
     const int64_t nb = n0 + wn * C::CW;
     T* DG = static_cast<T*>(e.dg);
     T* DU = static_cast<T*>(e.du);
+    // Half a row block at a time, its factors loaded while the half before it is worked on.
+    constexpr int kSteps = 2 * C::kTI;
+    f32x4 p[2][C::kHJ], q[2][C::kHJ];
+    auto load = [&](int s) {
+      const int64_t gm = gm0 + 16 * (s / 2);
 #pragma unroll
-    for (int i = 0; i < C::kTI; ++i) {
-      const int64_t gm = gm0 + 16 * i;
-      // the factors of half a row block are loaded before the first is used
+      for (int j = 0; j < C::kHJ; ++j) {
+        const int64_t gc = nb + 16 * (s % 2 * C::kHJ + j) + 4 * g4;
+        const bool in = gm < a.M && gc < a.N;
+        p[s % 2][j] = in ? *reinterpret_cast<const f32x4*>(e.p + gm * a.N + gc) : f32x4{0, 0, 0, 0};
+        q[s % 2][j] = in ? *reinterpret_cast<const f32x4*>(e.q + gm * a.N + gc) : f32x4{0, 0, 0, 0};
+      }
+    };
+    load(0);
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        f32x4 p[C::kHJ], q[C::kHJ];
+    for (int s = 0; s < kSteps; ++s) {
+      if (s + 1 < kSteps) load(s + 1);
+      const int64_t gm = gm0 + 16 * (s / 2);
 #pragma unroll
-        for (int j = 0; j < C::kHJ; ++j) {
-          const int64_t gc = nb + 16 * (h * C::kHJ + j) + 4 * g4;
-          const bool in = gm < a.M && gc < a.N;
-          p[j] = in ? *reinterpret_cast<const f32x4*>(e.p + gm * a.N + gc) : f32x4{0, 0, 0, 0};
-          q[j] = in ? *reinterpret_cast<const f32x4*>(e.q + gm * a.N + gc) : f32x4{0, 0, 0, 0};
-        }
+      for (int j = 0; j < C::kHJ; ++j) {
+        const f32x4 da = acc.t[s / 2][s % 2 * C::kHJ + j];
+        p[s % 2][j] *= da;
+        q[s % 2][j] *= da;
+      }
 #pragma unroll
-        for (int j = 0; j < C::kHJ; ++j) {
-          const f32x4 da = acc.t[i][h * C::kHJ + j];
-          p[j] *= da;
-          q[j] *= da;
-        }
-#pragma unroll
-        for (int j = 0; j < C::kHJ; j += 2) {
-          const int64_t gc = nb + wide_col((h * C::kHJ + j) / 2, g4);
-          const u32x4 vg = widen(pack2<T>(p[j][0], p[j][1]), pack2<T>(p[j][2], p[j][3]),
-                                 pack2<T>(p[j + 1][0], p[j + 1][1]),
-                                 pack2<T>(p[j + 1][2], p[j + 1][3]));
-          const u32x4 vu = widen(pack2<T>(q[j][0], q[j][1]), pack2<T>(q[j][2], q[j][3]),
-                                 pack2<T>(q[j + 1][0], q[j + 1][1]),
-                                 pack2<T>(q[j + 1][2], q[j + 1][3]));
-          if (gm < a.M && gc < a.N) {
-            st16(DG + gm * a.N + gc, vg);
-            st16(DU + gm * a.N + gc, vu);
-          }
+      for (int j = 0; j < C::kHJ; j += 2) {
+        const int64_t gc = nb + wide_col((s % 2 * C::kHJ + j) / 2, g4);
+        const f32x4 p0 = p[s % 2][j], p1 = p[s % 2][j + 1], q0 = q[s % 2][j], q1 = q[s % 2][j + 1];
+        const u32x4 vg = widen(pack2<T>(p0[0], p0[1]), pack2<T>(p0[2], p0[3]),
+                               pack2<T>(p1[0], p1[1]), pack2<T>(p1[2], p1[3]));
+        const u32x4 vu = widen(pack2<T>(q0[0], q0[1]), pack2<T>(q0[2], q0[3]),
+                               pack2<T>(q1[0], q1[1]), pack2<T>(q1[2], q1[3]));
+        if (gm < a.M && gc < a.N) {
+          st16(DG + gm * a.N + gc, vg);
+          st16(DU + gm * a.N + gc, vu);
         }
       }
     }
@@ -286,7 +287,7 @@ template <typename T, int kEpi, int kMA, int kMB, int kW>
 __global__ __launch_bounds__(64 * kW) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void mlp_product(const Product a, const Gated e) {
   __shared__ __attribute__((aligned(16))) uint8_t smem[Cfg<kW>::kLdsBytes];
-  product_tile<T, kEpi, kMA, kMB, kW>(a, e, blockIdx.x, smem);
+  product_tile<T, kEpi, kMA, kMB, kW, 1>(a, e, blockIdx.x, smem);
 }
 
 // dx and the weights' gradients in one grid: they are independent, and the tiles of one fill the
@@ -304,10 +305,10 @@ void mlp_grads(const Grads a) {
   const int64_t bid = blockIdx.x;
   const Gated none{};
   if (bid < a.end[0]) {
-    product_tile<T, kEpiStore, kKMajor, kMNMajor, kW>(a.dx, none, bid, smem);
+    product_tile<T, kEpiStore, kKMajor, kMNMajor, kW, 2>(a.dx, none, bid, smem);
   } else {
     const int w = bid < a.end[1] ? 0 : bid < a.end[2] ? 1 : 2;
-    product_tile<T, kEpiStore, kMNMajor, kMNMajor, kW>(a.dw[w], none, bid - a.end[w], smem);
+    product_tile<T, kEpiStore, kMNMajor, kMNMajor, kW, 1>(a.dw[w], none, bid - a.end[w], smem);
   }
 }
 
@@ -578,8 +579,6 @@ ts_status check_args(const char* who, const ts_gated_mlp_args* a) {
   return TS_OK;
 }
 
-template <typename T>
-const __bf16* raw(const T* p) { return reinterpret_cast<const __bf16*>(p); }
 const __bf16* raw(const void* p) { return static_cast<const __bf16*>(p); }
 
 Product product(const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N,
@@ -703,9 +702,10 @@ ts_status fwd_typed(const ts_gated_mlp_args& a, const ts_plan::MlpFwdPlan& pl, f
 template <typename T, int kW>
 ts_status launch_grads(const Grads& g, hipStream_t st) {
   if (g.end[3] <= 0) return TS_OK;
-  if (g.end[3] > ts_plan::max_blocks(64 * kW))
+  if (g.end[3] > ts_plan::max_blocks(Cfg<kW>::kThreads))
     return ts_host::fail(TS_ERR_SHAPE, "mlp_grads: too many tiles");
-  hipLaunchKernelGGL((mlp_grads<T, kW>), dim3((unsigned)g.end[3]), dim3(64 * kW), 0, st, g);
+  hipLaunchKernelGGL((mlp_grads<T, kW>), dim3((unsigned)g.end[3]),
+                     dim3(Cfg<kW>::kThreads), 0, st, g);
   return ts_host::check_launch("mlp_grads");
 }
 
@@ -717,10 +717,11 @@ ts_status bwd_typed(const ts_gated_mlp_args& a, const ts_plan::MlpBwdPlan& pl,
   void* dg = ws + w.dg;
   void* du = ws + w.du;
   const bool inner = dx != nullptr || dwg != nullptr || dwu != nullptr;
-  if (inner && a.w_down != nullptr) {
-    const Product p = product(dout, ldd, a.w_down, a.ld_down, a.N, a.F, a.O, nullptr);
+  const bool down = a.w_down != nullptr;
+  if (inner && down) {
     const Gated e{const_cast<float*>(keep_p), const_cast<float*>(keep_q), nullptr, dg, du,
                   a.activation};
+    const Product p = product(dout, ldd, a.w_down, a.ld_down, a.N, a.F, a.O, nullptr);
     TS_TRY((launch_product<T, kEpiGatedBwd, kKMajor, kMNMajor>(p, e, pl.da_waves, st,
                                                                "mlp_gated_bwd")));
   } else if (inner) {
@@ -742,8 +743,7 @@ ts_status bwd_typed(const ts_gated_mlp_args& a, const ts_plan::MlpBwdPlan& pl,
   g.dw[1] = product(du, a.F, a.x, a.ldx, a.F, a.H, a.N, dwu);
   g.dw[2] = product(dout, ldd, act, a.F, a.O, a.F, a.N, dwd);
   set_split(g.dx, pl.dx, reinterpret_cast<float*>(ws + w.dx));
-  for (int i = 0; i < 3; ++i)
-    set_split(g.dw[i], pl.dw, reinterpret_cast<float*>(ws + w.dw[i]));
+  for (int i = 0; i < 3; ++i) set_split(g.dw[i], pl.dw, reinterpret_cast<float*>(ws + w.dw[i]));
   SumJobs s{};
   int n = 0;
   int64_t end = 0;

@@ -563,17 +563,28 @@ __device__ inline void clear(AccOf<kW>& acc) {
     for (int j = 0; j < Cfg<kW>::kTJ; ++j) acc.t[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 }
 
-// acc = the tile at (m0, n0) of A [M, K] B [N, K]^T.
-template <int kMA, int kMB, int kW, typename T = __bf16>
-__device__ inline void mainloop(const __bf16* __restrict__ A, int64_t lda, int64_t M,
-                                const __bf16* __restrict__ B, int64_t ldb, int64_t N, int64_t K,
-                                int64_t m0, int64_t n0, uint8_t* smem, AccOf<kW>& acc) {
+// acc += the tile at (m0, n0) of A [M, K] B [N, K]^T. The operands' restrict matters: without it hipcc
+// (ROCm 7.2) waits for every load into LDS (vmcnt(0)) before the first transposing read of a
+// k-block, and the prefetch is lost.
+template <int kMA, int kMB, int kW, typename T>
+__device__ inline void mainloop_more(const __bf16* __restrict__ A, int64_t lda, int64_t M,
+                                     const __bf16* __restrict__ B, int64_t ldb, int64_t N,
+                                     int64_t K, int64_t m0, int64_t n0, uint8_t* smem,
+                                     AccOf<kW>& acc) {
   const int wn = (threadIdx.x >> 6) & 1;
-  clear<kW>(acc);
   const OpLoader<kMA, kW> la(A, lda, M, m0);
   const OpLoader<kMB, kW> lb(B, ldb, N, n0);
   mainloop_acc<kMA, kMB, kW, T>(la, lb, K, wn * Cfg<kW>::CW, wn * Cfg<kW>::CW + Cfg<kW>::CW / 2,
                                 smem, acc);
+}
+
+// acc = the tile at (m0, n0) of A [M, K] B [N, K]^T.
+template <int kMA, int kMB, int kW>
+__device__ inline void mainloop(const __bf16* __restrict__ A, int64_t lda, int64_t M,
+                                const __bf16* __restrict__ B, int64_t ldb, int64_t N, int64_t K,
+                                int64_t m0, int64_t n0, uint8_t* smem, AccOf<kW>& acc) {
+  clear<kW>(acc);
+  mainloop_more<kMA, kMB, kW, __bf16>(A, lda, M, B, ldb, N, K, m0, n0, smem, acc);
 }
 
 }  // namespace ts_gemm

@@ -406,14 +406,17 @@ struct MlpBwdPlan {
 // host's choice follows from the shape alone, so a shape's sums keep their order). Fitted to
 // MI355X: a k-block of a 256 x 256 tile takes 1.35 us in a launch of one tile a CU and 1.65 us while
 // the whole card is at its power limit, one of a 128 x 128 tile 0.5 us on half the card's CUs, 0.75 us
-// on all of them and 1.0 us beside another on its CU; a tile's start and epilogue 4 to 5 us; slots cost their partials' traffic and a launch. Measured
-// against 256 x 256 tiles without slots, N, H, F: 2045, 768, 2048 forward 68 -> 38 us, backward 120 ->
-// 66; 256, 2048, 5632 143 -> 41 and 296 -> 90; 100, 4096, 14336 399 -> 109 and 901 -> 245; at
-// 8192, 4096, 14336 128 x 128 tiles would take 14% longer.
+// on all of them and 1.0 us beside another on its CU; a tile's start and epilogue 4 to 5 us, 13 us
+// where a large tile's epilogue also moves the backward's factors and no other workgroup's products
+// run beside it; slots cost their partials' traffic and a launch. Measured against 256 x 256 tiles
+// without slots, forward and backward, N, H, F: 2045, 768, 2048 71 -> 42 and 117 -> 62 us; 256, 2048,
+// 5632 147 -> 44 and 258 -> 72; 100, 4096, 14336 402 -> 110 and 734 -> 217; of 18 shapes tried, the
+// choice was within 15% of the best of all, mostly within 5%.
 inline int64_t mlp_kblocks(int64_t K) { return (K + kGemmBlockK - 1) / kGemmBlockK; }
-inline double mlp_time(int64_t pieces, int64_t kblocks, int waves) {
+inline double mlp_time(int64_t pieces, int64_t kblocks, int waves, bool gated = false) {
   if (waves == 8)
-    return (double)((pieces + 255) / 256) * (kblocks * (pieces <= 256 ? 1.35 : 1.65) + 5.0);
+    return (double)((pieces + 255) / 256) *
+           (kblocks * (pieces <= 256 ? 1.35 : 1.65) + (gated ? 13.0 : 5.0));
   if (pieces <= 256) return kblocks * (pieces <= 128 ? 0.5 : 0.75) + 4.0;
   return (double)((pieces + 511) / 512) * (kblocks * 1.0 + 5.0);
 }
@@ -455,14 +458,15 @@ inline double mlp_makespan(int64_t n1, double a, int64_t n2, double b, int64_t m
   return best < 1e30 ? best : t1 + even;
 }
 
-inline int mlp_waves(int64_t M, int64_t N, int64_t K, bool pair) {
+inline int mlp_gated_waves(int64_t M, int64_t N, int64_t K, bool pair) {
   const int64_t kb = mlp_kblocks(K);
-  return mlp_time(mlp_tiles(M, N, 8, pair), kb, 8) <= mlp_time(mlp_tiles(M, N, 4, pair), kb, 4)
+  return mlp_time(mlp_tiles(M, N, 8, pair), kb, 8, true) <=
+                 mlp_time(mlp_tiles(M, N, 4, pair), kb, 4, true)
              ? 8 : 4;
 }
 inline MlpFwdPlan mlp_fwd_plan(const MlpShape& s) {
   const KSplit one{1, 0};
-  MlpFwdPlan p{mlp_waves(s.N, s.F, s.H, true), 8, one};
+  MlpFwdPlan p{mlp_gated_waves(s.N, s.F, s.H, true), 8, one};
   if (s.O <= 0) return p;
   double best = 1e30;
   for (int waves = 8; waves >= 4; waves -= 4) {
@@ -481,7 +485,7 @@ inline MlpFwdPlan mlp_fwd_plan(const MlpShape& s) {
 }
 inline MlpBwdPlan mlp_bwd_plan(const MlpShape& s) {
   const KSplit one{1, 0};
-  MlpBwdPlan p{s.O > 0 ? mlp_waves(s.N, s.F, s.O, false) : 8, 8, one, one};
+  MlpBwdPlan p{s.O > 0 ? mlp_gated_waves(s.N, s.F, s.O, false) : 8, 8, one, one};
   // dx [N, H] over 2 F, then dWg and dWu [F, H] and dWd [O, F] over N, in one grid
   double best = 1e30;
   const int64_t kx = mlp_kblocks(2 * s.F), kw = mlp_kblocks(s.N);
@@ -495,13 +499,16 @@ inline MlpBwdPlan mlp_bwd_plan(const MlpShape& s) {
         if (!mlp_slots_ok(w, s.F, s.H, s.N) ||
             (s.O > 0 && !mlp_slots_ok(w, s.O, s.F, s.N)))
           break;
-        const bool one_each = tx * x + tw * w <= kCus;
-        const double rate = waves == 8 ? (one_each ? 1.4 : 1.65) : (one_each ? 0.85 : 1.2);
-        double t = rate * mlp_makespan(tx * x, (double)((kx + x - 1) / x), tw * w,
-                                       (double)((kw + w - 1) / w),
-                                       waves == 8 || one_each ? kCus : 2 * kCus) +
-                   mlp_slots_time(x, s.N, s.H) + 2 * mlp_slots_time(w, s.F, s.H) +
-                   mlp_slots_time(w, s.O, s.F);
+        const double ax = (double)((kx + x - 1) / x), aw = (double)((kw + w - 1) / w);
+        const double work = ((double)(tx * x) * ax + (double)(tw * w) * aw) / (2.0 * kCus);
+        const double longest = ax > aw ? ax : aw;
+        // 256 x 256 tiles take a CU each, in turn; of 128 x 128 tiles two share one, the longest
+        // going on alone at the end
+        double t = waves == 8 ? (tx * x + tw * w <= kCus ? 1.15 : 1.45) *
+                                    mlp_makespan(tx * x, ax, tw * w, aw, kCus)
+                              : (1.05 * work > 0.6 * longest ? 1.05 * work : 0.6 * longest);
+        t += mlp_slots_time(x, s.N, s.H) + 2 * mlp_slots_time(w, s.F, s.H) +
+             mlp_slots_time(w, s.O, s.F);
         if (x > 1 || w > 1) t += kMlpSumLaunch;
         if (t >= best) continue;
         best = t;

@@ -52,13 +52,13 @@ def _check(x: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], activati
 
 def _forward(x: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], activation: str,
              keep: bool):
-    """(result, the activation's code, what the backward needs)."""
+    """(result, the activation's code, the backward's factors, gated product)."""
     code = _check(x, gate, up, down, activation)
     cols = (gate if down is None else down).shape[0]
-    kept, out = ops.gated_mlp_forward(x.reshape(-1, x.shape[-1]), gate, up, down, code, keep)
+    factors, act, out = ops.gated_mlp_forward(x.reshape(-1, x.shape[-1]), gate, up, down, code, keep)
     if out.shape[1] != cols:
         out = out[:, :cols].contiguous()
-    return out.view(*x.shape[:-1], cols), code, kept
+    return out.view(*x.shape[:-1], cols), code, factors, act
 
 
 class GatedMLPFunction(torch.autograd.Function):
@@ -68,16 +68,16 @@ class GatedMLPFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor],
                 activation: str) -> Tensor:
-        out, ctx.code, kept = _forward(x, gate, up, down, activation, True)
-        ctx.save_for_backward(x, gate, up, down, kept)
+        out, ctx.code, factors, act = _forward(x, gate, up, down, activation, True)
+        ctx.save_for_backward(x, gate, up, down, factors, None if down is None else act)
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout: Tensor):
-        x, gate, up, down, kept = ctx.saved_tensors
+        x, gate, up, down, factors, act = ctx.saved_tensors
         grads = ops.gated_mlp_backward(
-            x.reshape(-1, x.shape[-1]), gate, up, down, ctx.code, kept,
+            x.reshape(-1, x.shape[-1]), gate, up, down, ctx.code, factors, act,
             dout.reshape(-1, dout.shape[-1]), ctx.needs_input_grad)
         if grads[0] is not None:
             grads[0] = grads[0].view(x.shape)

@@ -685,23 +685,20 @@ def _mlp_args(x2d, gate, up, down, code):
 
 def gated_mlp_forward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], code: int,
                       keep: bool):
-    """(kept, result), features rounded up to multiples of 8. kept holds what the backward needs
-    (2 N F fp32 values, where `keep`) and then the gated product (N F values), where that is not
-    the result; None for nothing."""
+    """(fp32 factors [2, N, F] of the backward or None, gated product, result), features rounded up
+    to multiples of 8; without a down weight the product is the result."""
     dev = _lib.require_gpu("gated_mlp", x2d, gate, up, down)
     n = x2d.shape[0]
     args, held = _mlp_args(x2d, gate, up, down, code)
     f = args.F
-    # fp32 factors of the backward, then the 16-bit product, which takes half a matrix
-    inner = (4 if keep else 0) + (0 if down is None else 1)
-    kept = torch.empty((inner, n, f), dtype=x2d.dtype, device=dev) if inner else None
-    out = torch.empty((n, f if down is None else args.O), dtype=x2d.dtype, device=dev)
+    factors = torch.empty((2, n, f), dtype=torch.float32, device=dev) if keep else None
+    act = torch.empty((n, f), dtype=x2d.dtype, device=dev)
+    out = act if down is None else torch.empty((n, args.O), dtype=x2d.dtype, device=dev)
     if n == 0:
-        return kept, out
-    at = 0 if kept is None else kept.data_ptr()
-    step = 4 * n * f
-    p, q = (at, at + step) if keep else (0, 0)
-    a, y = (out.data_ptr(), 0) if down is None else (at + (2 * step if keep else 0), out.data_ptr())
+        return factors, act, out
+    p = factors.data_ptr() if keep else 0
+    q = p + 4 * n * f if keep else 0
+    a, y = act.data_ptr(), 0 if down is None else out.data_ptr()
     lib = _lib.load()
     wsb = lib.ts_gated_mlp_fwd_workspace_size(n, args.H, f, args.O)
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
@@ -709,13 +706,14 @@ def gated_mlp_forward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Tens
         check(lib.ts_gated_mlp_fwd(ctypes.byref(args), p, q, a, y, ptr(ws), wsb,
                                    _lib.stream_handle(dev)), "ts_gated_mlp_fwd")
     del held
-    return kept, out
+    return factors, act, out
 
 
 def gated_mlp_backward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], code: int,
-                       kept: Tensor, dout: Tensor, needs) -> list:
-    """Gradients of (x2d, gate, up, down), None where `needs` is false; kept is the forward's."""
-    dev = _lib.require_gpu("gated_mlp", x2d, gate, up, down, kept, dout)
+                       factors: Tensor, act: Optional[Tensor], dout: Tensor, needs) -> list:
+    """Gradients of (x2d, gate, up, down), None where `needs` is false; factors and act are the
+    forward's."""
+    dev = _lib.require_gpu("gated_mlp", x2d, gate, up, down, factors, act, dout)
     n = x2d.shape[0]
     out = [None] * 4
     leaves = (x2d, gate, up, down)
@@ -729,14 +727,15 @@ def gated_mlp_backward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Ten
     shapes = ((n, args.H), (args.F, args.H), (args.F, args.H), (args.O, args.F))
     out = [torch.empty(s, dtype=x2d.dtype, device=dev) if k else None
            for s, k in zip(shapes, needs)]
-    kept = kept.contiguous()
-    at, step = kept.data_ptr(), 4 * n * args.F
+    factors = factors.contiguous()
+    act = None if act is None else act.contiguous()
+    at, step = factors.data_ptr(), 4 * n * args.F
     lib = _lib.load()
     wsb = lib.ts_gated_mlp_bwd_workspace_size(n, args.H, args.F, args.O)
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
     with _lib.on_device(dev):
         check(lib.ts_gated_mlp_bwd(ctypes.byref(args), at, at + step,
-                                   0 if down is None else at + 2 * step, d.data_ptr(), ldd,
+                                   0 if act is None else act.data_ptr(), d.data_ptr(), ldd,
                                    *[0 if t is None else t.data_ptr() for t in out],
                                    ws.data_ptr(), wsb, _lib.stream_handle(dev)),
               "ts_gated_mlp_bwd")
