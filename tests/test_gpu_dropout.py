@@ -155,6 +155,12 @@ def test_rows(gpu, rows, width):
     run_and_check(inputs(gpu, (rows, width), BF, BF, rows), 0.1)
 
 
+@pytest.mark.parametrize("rows,width,dtype", [(16391, 2048, BF), (65601, 512, F16),
+                                              (16400, 4090, BF), (16385, 1030, F32)])
+def test_many_rows(gpu, rows, width, dtype):
+    run_and_check(inputs(gpu, (rows, width), dtype, F32, rows), 0.1)
+
+
 @pytest.mark.parametrize("use", [(True, False), (False, True)])
 def test_one_result_used(gpu, use):
     run_and_check(inputs(gpu, (5, 9, 512), BF, F32, 5), 0.1, use)

@@ -567,12 +567,23 @@ inline DropNormPlan drop_norm_plan(int64_t groups) {
   if (groups <= 2048) return DropNormPlan{512, 4, 1};
   return DropNormPlan{0, 0, 1};
 }
-// Workgroups of the backward, each of which writes a partial row of dw.
-constexpr int64_t kDropNormBwdGrid = 512;
+// The backward's: 16-bit rows of 257 to 512 groups on half the threads, whose 16 registers of dw a
+// thread leave room for twice the workgroups a CU. At [16384, 4096] bf16 135 us against 145; with
+// fp32, whose groups are two loads, [4096, 4096] took 90 us against 83, and the forward at 4096 bf16
+// 96 against 89, so both keep one group a thread. Rows a workgroup are the forward's.
+inline DropNormPlan drop_norm_bwd_plan(int64_t groups, int elt_bytes) {
+  if (elt_bytes == 2 && groups > 256 && groups <= 512) return DropNormPlan{256, 2, 1};
+  return drop_norm_plan(groups);
+}
+// Workgroups of the backward, each of which writes a partial row of dw: 1024 where each still has 16
+// steps of rows, else 512. At 1024 / 512: [16384, 2048] bf16 71 / 100 us and [65536, 512] 67 / 95
+// (16 steps), [32768, 8192] 490 / 503 (32); [8191, 768] fp32 38 / 34 (2), [4096, 4096] 83 / 76 (4).
+// 2048 took 81 us at [16384, 2048] (8 steps).
 inline int64_t drop_norm_bwd_grid(int64_t rows, int64_t groups) {
   const int64_t per = drop_norm_plan(groups).rows;
   const int64_t steps = (rows + per - 1) / per;
-  return steps < kDropNormBwdGrid ? steps : kDropNormBwdGrid;
+  const int64_t most = steps >= 16 * 1024 ? 1024 : 512;
+  return steps < most ? steps : most;
 }
 
 // ---------------------------------------------------------------------------
