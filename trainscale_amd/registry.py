@@ -8,7 +8,8 @@ RMSNorm by ``fast_rms_layernorm`` and a gate/up/down MLP by
 ``down_proj(swiglu_forward(gate_proj(x), up_proj(x)))``, both on the gfx950
 kernels. The patched forward keeps calling the module's original forward for
 tensors that are not on a GPU (the module's own code, not a copy of the kernel
-math).
+math). ``auto_patch_fused_mlp`` (KernelPatcher(fuse_mlp=True)) takes the whole
+gated block, projections included.
 
 Rotary modules (``auto_patch_rope``, registry/__init__.py:1209-1282): the
 reference only records a RoPEConfig on the module. Here the patch also routes
@@ -29,10 +30,11 @@ import types
 
 from .kernels.embedding_kernels import scaled_embedding
 from .kernels.fused_kernels import fast_rms_layernorm, swiglu_forward
+from .kernels.mlp_kernels import fused_gated_mlp
 from .kernels.rope_kernels import RoPEConfig, RoPEScalingType, hf_apply_rotary_pos_emb
 
 __all__ = ["LAYER_PATCHES", "NORMS_WITH_OTHER_MATH", "register_layer_patch", "auto_patch_layernorm", "auto_patch_mlp",
-           "auto_patch_rope", "auto_patch_embedding", "KernelPatcher", "patch_model"]
+           "auto_patch_fused_mlp", "auto_patch_rope", "auto_patch_embedding", "KernelPatcher", "patch_model"]
 
 LAYER_PATCHES: Dict[str, Callable[[nn.Module], None]] = {}
 
@@ -106,6 +108,63 @@ def auto_patch_mlp(module: nn.Module) -> None:
 for _name in ("LlamaMLP", "Qwen2MLP", "Qwen3MLP", "MistralMLP", "MixtralBlockSparseTop2MLP",
               "Phi3MLP", "Phi4MLP"):
     register_layer_patch(_name, auto_patch_mlp)
+
+
+# activation modules and functions -> fused_gated_mlp's names; transformers' by class name
+_ACT_FUNCTIONS = ((torch.nn.functional.silu, "silu"), (torch.nn.functional.gelu, "gelu"),
+                  (torch.nn.functional.relu, "relu"), (torch.relu, "relu"))
+_ACT_CLASSES = {"SiLUActivation": "silu", "GELUActivation": "gelu", "GELUTanh": "gelu_tanh",
+                "PytorchGELUTanh": "gelu_tanh"}
+
+
+def _activation_of(module: nn.Module):
+    """The name of a gated block's activation, None where it is another's. Without an attribute it
+    is SiLU, which ``auto_patch_mlp`` puts in every registered block."""
+    act = getattr(module, "act_fn", getattr(module, "activation_fn", None))
+    if act is None:
+        return "silu"
+    if isinstance(act, nn.Module):
+        if act._forward_hooks or act._forward_pre_hooks or "forward" in vars(act):
+            return None
+        if type(act) in (nn.SiLU, nn.ReLU):
+            return "silu" if type(act) is nn.SiLU else "relu"
+        if type(act) is nn.GELU:
+            return "gelu" if act.approximate == "none" else "gelu_tanh"
+        return _ACT_CLASSES.get(type(act).__name__)
+    return next((name for f, name in _ACT_FUNCTIONS if act is f), None)
+
+
+def _plain_linear(layer) -> bool:
+    """Whether a projection is its weight's product and nothing else (no bias, adapter, hook,
+    parametrization, replaced forward or distributed weight)."""
+    return (type(layer) is nn.Linear and layer.bias is None and "forward" not in vars(layer)
+            and type(layer.weight) in (nn.Parameter, torch.Tensor)
+            and not (layer._forward_hooks or layer._forward_pre_hooks or layer._backward_hooks
+                     or layer._backward_pre_hooks))
+
+
+def auto_patch_fused_mlp(module: nn.Module) -> None:
+    """Routes a gate/up/down MLP through ``fused_gated_mlp``. Calls that are not the plain block in
+    bf16 or fp16 (a projection with a bias, an adapter or hooks, another activation, fp32, autocast
+    to another type, CPU tensors) keep the module's own forward; what a call is, is looked up at each
+    call, so adapters may come later."""
+    if not (hasattr(module, "gate_proj") and hasattr(module, "up_proj")
+            and hasattr(module, "down_proj")):
+        return
+
+    def patched_forward(self, x):
+        layers = (self.gate_proj, self.up_proj, self.down_proj)
+        act = _activation_of(self)
+        if (act is None or not isinstance(x, torch.Tensor) or not x.is_cuda
+                or x.dtype not in (torch.bfloat16, torch.float16)
+                or not all(_plain_linear(m) and m.weight.dtype is x.dtype
+                           and m.weight.device == x.device for m in layers)
+                or (torch.is_autocast_enabled("cuda")
+                    and torch.get_autocast_dtype("cuda") is not x.dtype)):
+            return self._trainscale_amd_forward(x)
+        return fused_gated_mlp(x, *(m.weight for m in layers), activation=act)
+
+    _patch_forward(module, patched_forward)
 
 
 _ROPE_TYPES = {"linear": RoPEScalingType.LINEAR, "ntk": RoPEScalingType.NTK,
@@ -195,14 +254,18 @@ class KernelPatcher:
     select nothing. ``skip_inexact_norms`` (not in the reference) leaves the
     classes of NORMS_WITH_OTHER_MATH unpatched; by default they are patched, as
     the reference patches them. ``patch_embedding`` (not in the reference, off by
-    default) patches modules of class ``nn.Embedding`` itself.
+    default) patches modules of class ``nn.Embedding`` itself. ``fuse_mlp`` (not in
+    the reference, off by default) patches the registered gate/up/down MLPs with
+    ``auto_patch_fused_mlp``, projections included, where ``auto_patch_mlp`` would
+    replace only their elementwise part.
     """
 
     def __init__(self, patch_layernorm: bool = True, patch_mlp: bool = True,
                  patch_attention: bool = True, patch_rope: bool = True, patch_fp8: bool = False,
                  verbose: bool = False, skip_inexact_norms: bool = False,
-                 patch_embedding: bool = False):
+                 patch_embedding: bool = False, fuse_mlp: bool = False):
         self.patch_embedding = patch_embedding
+        self.fuse_mlp = fuse_mlp
         self.skip_inexact_norms = skip_inexact_norms
         self.patch_layernorm = patch_layernorm
         self.patch_mlp = patch_mlp
@@ -231,6 +294,8 @@ class KernelPatcher:
             elif "Rotary" in cls:
                 if not self.patch_rope:
                     continue
+            if self.fuse_mlp and fn is auto_patch_mlp:
+                fn = auto_patch_fused_mlp
             fn(module)
             if getattr(module, "_trainscale_amd_patched", False):
                 self.patched_layers.append((name, cls))
