@@ -7,7 +7,7 @@ the root, rstd is off by (27 + 3 k) u, k = |M| / |h| in 2-norms being what cance
 product of three such factors: (40 + 4 k) u M rstd |w|. The backward reads the rounded h, so hat is
 off by eh = (half + (32 + 6 k) u) M rstd; its row mean c1 by mean |e| (eh + 50 u M rstd); t and dw as
 these propagate. dw adds a row for each step of a workgroup, its row slots, 32 partial rows a slice
-and 16 slices: (rows / 512 + 120) u of its magnitudes.
+and 32 slices: (rows / 512 + 120) u of its magnitudes.
 """
 import contextlib
 import copy
