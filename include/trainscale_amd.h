@@ -704,6 +704,22 @@ ts_status ts_gated_mlp_bwd(const ts_gated_mlp_args* args, const float* keep_p,
                            int64_t ld_dout, void* dx, void* dw_gate, void* dw_up, void* dw_down,
                            void* workspace, size_t workspace_bytes, ts_stream_t stream);
 
+/*
+ * Copies of up to 8 matrices of a 16-bit dtype in one launch, each into a contiguous, zero-padded
+ * one ([rows, cols] at most [dst_rows, dst_cols]) or out of one: for operands that the block's
+ * entry points above do not take as they are. Strides in elements, not negative; any
+ * element-aligned address. dst must not overlap any src.
+ */
+typedef struct {
+  const void* src;
+  int64_t row_stride, col_stride, rows, cols;
+  void* dst;
+  int64_t dst_rows, dst_cols;
+} ts_pad_job;
+
+ts_status ts_pad_matrices(const ts_pad_job* jobs, int32_t count, ts_dtype dtype,
+                          ts_stream_t stream);
+
 /* ------------------------------------------------------------------------ */
 /* Dropout from a counter-based generator                                    */
 /* ------------------------------------------------------------------------ */

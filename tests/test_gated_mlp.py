@@ -74,6 +74,27 @@ def test_workspace_sizes():
     assert lib.ts_gated_mlp_fwd_workspace_size(100, 64, 64, 0) == 0
 
 
+def test_pad_is_checked():
+    lib = _lib.load()
+
+    def pad(count=1, dtype=_lib.TS_BF16, jobs=True, **kw):
+        j = dict(src=FAKE, row_stride=4, col_stride=1, rows=2, cols=4, dst=FAKE, dst_rows=2,
+                 dst_cols=8)
+        return lib.ts_pad_matrices((_lib.PadJob * 9)(*[_lib.PadJob(**{**j, **kw})] * 9) if jobs
+                                   else None, count, dtype, None)
+
+    assert pad(0) == OK and pad(rows=0, dst_rows=0) == OK and pad(0, jobs=False) == OK
+    assert pad(9) == INVALID and pad(-1) == INVALID and pad(jobs=False) == INVALID
+    assert pad(dtype=_lib.TS_F32) == DTYPE
+    for kw in (dict(rows=3), dict(cols=9), dict(rows=-1), dict(cols=-1), dict(row_stride=-4),
+               dict(col_stride=-1), dict(dst_rows=1 << 41), dict(dst_rows=1 << 31),
+               dict(dst_rows=1 << 40, dst_cols=1 << 40)):
+        assert pad(**kw) == SHAPE, kw
+    for kw in (dict(src=None), dict(dst=None), dict(src=FAKE + 1), dict(dst=FAKE + 1)):
+        assert pad(**kw) == INVALID, kw
+    assert pad(8, dst_rows=1 << 25, dst_cols=1 << 8) == SHAPE  # together more than a launch
+
+
 BF = torch.bfloat16
 
 

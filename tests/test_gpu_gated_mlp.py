@@ -319,6 +319,24 @@ def test_nothing_outside_is_touched(gpu, n):
         assert same(t.t, got[k]), k
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_pad(gpu, dtype):
+    """Copies in one launch: of rows, of columns, of neither dense, of one repeated, of none."""
+    lib, r = _lib.load(), torch.Generator(device=gpu).manual_seed(1)
+    base = torch.randn(400, 401, device=gpu, generator=r).to(dtype)
+    views = [base[:67, 1:130], base[3:132, :5].t(), base[::3, ::2], base[:1].expand(70, 401),
+             base[:0, :8], base[5:6, 7:8], base[:65, :64].t(), base[2:66, 8:72]]
+    sizes = [(67, 136), (8, 136), (134, 201), (72, 408), (3, 8), (1, 1), (64, 65), (64, 64)]
+    outs = [Guarded(*s, s[1], dtype, gpu) for s in sizes]
+    jobs = [_lib.PadJob(v.data_ptr(), *v.stride(), *v.shape, o.p, *s)
+            for v, o, s in zip(views, outs, sizes)]
+    assert lib.ts_pad_matrices((_lib.PadJob * 8)(*jobs), 8, _lib.DTYPE_CODE[dtype],
+                               _lib.stream_handle(gpu)) == 0, _lib.last_error()
+    for v, o, s in zip(views, outs, sizes):
+        want = torch.nn.functional.pad(v, (0, s[1] - v.shape[1], 0, s[0] - v.shape[0]))
+        assert o.intact() and same(o.t, want), s
+
+
 def test_empty(gpu):
     _, wg, wu, wd, _ = inputs(gpu, 1, 16, 24, 8, BF, 1)
     leaf = [torch.empty(3, 0, 16, dtype=BF, device=gpu).requires_grad_()] + [

@@ -79,6 +79,12 @@ class GatedMLPArgs(ctypes.Structure):
                 ("F", I64), ("O", I64), ("activation", I32), ("dtype", I32)]
 
 
+class PadJob(ctypes.Structure):
+    """ts_pad_job."""
+    _fields_ = [("src", P), ("row_stride", I64), ("col_stride", I64), ("rows", I64),
+                ("cols", I64), ("dst", P), ("dst_rows", I64), ("dst_cols", I64)]
+
+
 class DropoutRng(ctypes.Structure):
     """ts_dropout_rng."""
     _fields_ = [("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64), ("state", P),
@@ -148,6 +154,7 @@ SIGNATURES = {
     "ts_gated_mlp_bwd_workspace_size": ([I64, I64, I64, I64], SZ),
     "ts_gated_mlp_fwd": ([P, P, P, P, P, P, SZ, P], I32),
     "ts_gated_mlp_bwd": ([P, P, P, P, P, I64, P, P, P, P, P, SZ, P], I32),
+    "ts_pad_matrices": ([P, I32, I32, P], I32),
     "ts_dropout_fwd": ([P, I64, P, I64, P, I64, I32, I64, I64, P, P], I32),
     "ts_dropout_add_rmsnorm_fwd": ([P, I64, P, I64, I32, P, I32, P, P, P, I64, I64, F32, P, P],
                                    I32),

@@ -56,8 +56,6 @@ def _forward(x: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], activa
     code = _check(x, gate, up, down, activation)
     cols = (gate if down is None else down).shape[0]
     factors, act, out = ops.gated_mlp_forward(x.reshape(-1, x.shape[-1]), gate, up, down, code, keep)
-    if out.shape[1] != cols:
-        out = out[:, :cols].contiguous()
     return out.view(*x.shape[:-1], cols), code, factors, act
 
 
@@ -97,7 +95,8 @@ def fused_gated_linear(x: Tensor, gate: Tensor, up: Tensor, activation: str = "s
     """act(x @ gate.T) * (x @ up.T): x [..., H], gate and up [F, H], all bf16 or all fp16; the
     result is [..., F]. activation: "silu", "gelu" (the error function's form), "gelu_tanh" or
     "relu". Differentiable in all three. Any sizes and strides; sizes or row strides that are not
-    multiples of 8, or rows that do not start at 16 bytes, cost a copy of that operand."""
+    multiples of 8, or rows that do not start at 16 bytes, cost a copy of that operand (one launch for
+    all of them)."""
     return _apply(x, gate, up, None, activation)
 
 

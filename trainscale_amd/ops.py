@@ -654,48 +654,88 @@ def swiglu_backward(dout: Tensor, gate: Tensor, up: Tensor) -> Tuple[Tensor, Ten
 _MLP_MAX_LD = 1 << 21
 
 
-def _mlp_operand(t: Tensor, rows: int, cols: int) -> Tuple[Tensor, int]:
-    """A matrix and its row stride as the kernels take it ([rows, cols] with cols and the stride
-    multiples of 8, 16-byte aligned): t itself where it is one, else a copy padded with zeros."""
-    if t.shape[1] == cols and t.shape[0] == rows:
-        ld = t.stride(0) if rows > 1 else cols
-        if (t.stride(1) == 1 and ld >= cols and ld % 8 == 0 and ld <= _MLP_MAX_LD
-                and t.data_ptr() % 16 == 0):
-            return t, ld
-    c = torch.zeros((rows, cols), dtype=t.dtype, device=t.device) if t.shape != (
-        rows, cols) else torch.empty((rows, cols), dtype=t.dtype, device=t.device)
-    c[:t.shape[0], :t.shape[1]].copy_(t)
-    return c, cols
+def _pad(jobs: list, dtype: torch.dtype, dev) -> None:
+    """Runs ts_pad_job tuples in one launch."""
+    with _lib.on_device(dev):
+        check(_lib.load().ts_pad_matrices(
+            (_lib.PadJob * len(jobs))(*jobs), len(jobs), _lib.DTYPE_CODE[dtype],
+            _lib.stream_handle(dev)), "ts_pad_matrices")
 
 
-def _mlp_args(x2d, gate, up, down, code):
-    """The kernels' arguments, and what keeps their memory alive."""
+def _mlp_operands(dev, *operands):
+    """[(address, row stride)] of (matrix or None, rows, cols) as the kernels take them ([rows, cols]
+    with cols and the stride multiples of 8, 16-byte aligned): the matrix itself where it is
+    one, else a copy padded with zeros; and the memory of the copies."""
+    out, jobs, total = [], [], 0
+    for t, rows, cols in operands:
+        if t is None:
+            out.append((0, 0))
+            continue
+        r, c = t.shape
+        s0, s1 = t.stride()
+        at, ld = t.data_ptr(), s0 if rows > 1 else cols
+        if not (c == cols and r == rows and s1 == 1 and ld >= cols and ld % 8 == 0
+                and ld <= _MLP_MAX_LD and at % 16 == 0):
+            jobs.append((len(out), (at, s0, s1, r, c, total, rows, cols)))
+            ld = cols
+            total += rows * cols * 2
+        out.append((at, ld))
+    if not jobs:
+        return out, None
+    dtype = operands[0][0].dtype
+    copies = torch.empty(total // 2, dtype=dtype, device=dev)
+    base = copies.data_ptr()
+    for i, j in jobs:
+        out[i] = (base + j[5], out[i][1])
+    _pad([(*j[:5], base + j[5], *j[6:]) for _, j in jobs], dtype, dev)
+    return out, copies
+
+
+def _crop(pairs, dev) -> list:
+    """Contiguous [:r, :c] of padded matrices, in one launch; those of the size asked for as they
+    are."""
+    out, jobs, dtype = [], [], None
+    for t, shape in pairs:
+        if t is not None and t.shape != shape:
+            dtype, whole = t.dtype, t
+            t = torch.empty(shape, dtype=dtype, device=dev)
+            jobs.append((whole.data_ptr(), whole.shape[1], 1, *shape, t.data_ptr(), *shape))
+        out.append(t)
+    if jobs:
+        _pad(jobs, dtype, dev)
+    return out
+
+
+def _mlp_args(dev, x2d, gate, up, down, code, *dout):
+    """The kernels' arguments, with dout's address and row stride, and the copies' memory."""
     n, h = x2d.shape
     f, o = gate.shape[0], 0 if down is None else down.shape[0]
     h8, f8, o8 = (h + 7) & ~7, (f + 7) & ~7, (o + 7) & ~7
-    x, ldx = _mlp_operand(x2d, n, h8)
-    g, ldg = _mlp_operand(gate, f8, h8)
-    u, ldu = _mlp_operand(up, f8, h8)
-    d, ldd = (None, 0) if down is None else _mlp_operand(down, o8, f8)
-    args = _lib.GatedMLPArgs(x.data_ptr(), ldx, g.data_ptr(), ldg, u.data_ptr(), ldu,
-                             0 if d is None else d.data_ptr(), ldd, n, h8, f8, o8, code,
-                             _lib.DTYPE_CODE[x.dtype])
-    return args, (x, g, u, d)
+    at, copies = _mlp_operands(dev, (x2d, n, h8), (gate, f8, h8), (up, f8, h8), (down, o8, f8),
+                               *[(d, n, o8 or f8) for d in dout])
+    (x, ldx), (g, ldg), (u, ldu), (d, ldd) = at[:4]
+    args = _lib.GatedMLPArgs(x, ldx, g, ldg, u, ldu, d, ldd, n, h8, f8, o8, code,
+                             _lib.DTYPE_CODE[x2d.dtype])
+    return args, at[4:], copies
 
 
 def gated_mlp_forward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], code: int,
                       keep: bool):
-    """(fp32 factors [2, N, F] of the backward or None, gated product, result), features rounded up
-    to multiples of 8; without a down weight the product is the result."""
+    """(fp32 factors [2, N, F] of the backward or None, gated product, result); F in the first two
+    rounded up to a multiple of 8. Without a down weight the product is the result too."""
     dev = _lib.require_gpu("gated_mlp", x2d, gate, up, down)
-    n = x2d.shape[0]
-    args, held = _mlp_args(x2d, gate, up, down, code)
+    n, last = x2d.shape[0], gate if down is None else down
+    cols = last.shape[0]
+    if n == 0:
+        f8 = (gate.shape[0] + 7) & ~7
+        new = [torch.empty((*s, c), dtype=t, device=dev) for s, c, t in (
+            ((2, 0), f8, torch.float32), ((0,), f8, x2d.dtype), ((0,), cols, x2d.dtype))]
+        return new[0] if keep else None, new[1], new[2]
+    args, _, copies = _mlp_args(dev, x2d, gate, up, down, code)
     f = args.F
     factors = torch.empty((2, n, f), dtype=torch.float32, device=dev) if keep else None
     act = torch.empty((n, f), dtype=x2d.dtype, device=dev)
     out = act if down is None else torch.empty((n, args.O), dtype=x2d.dtype, device=dev)
-    if n == 0:
-        return factors, act, out
     p = factors.data_ptr() if keep else 0
     q = p + 4 * n * f if keep else 0
     a, y = act.data_ptr(), 0 if down is None else out.data_ptr()
@@ -705,8 +745,8 @@ def gated_mlp_forward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Tens
     with _lib.on_device(dev):
         check(lib.ts_gated_mlp_fwd(ctypes.byref(args), p, q, a, y, ptr(ws), wsb,
                                    _lib.stream_handle(dev)), "ts_gated_mlp_fwd")
-    del held
-    return factors, act, out
+    del copies
+    return factors, act, _crop([(out, (n, cols))], dev)[0]
 
 
 def gated_mlp_backward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], code: int,
@@ -715,15 +755,12 @@ def gated_mlp_backward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Ten
     forward's."""
     dev = _lib.require_gpu("gated_mlp", x2d, gate, up, down, factors, act, dout)
     n = x2d.shape[0]
-    out = [None] * 4
     leaves = (x2d, gate, up, down)
     needs = [bool(k) and t is not None for k, t in zip(needs, leaves)]
     if n == 0 or not any(needs):
         return [torch.zeros(t.shape, dtype=t.dtype, device=dev) if k else None
                 for t, k in zip(leaves, needs)]
-    args, held = _mlp_args(x2d, gate, up, down, code)
-    cols = args.F if down is None else args.O
-    d, ldd = _mlp_operand(dout, n, cols)
+    args, ((d, ldd),), copies = _mlp_args(dev, x2d, gate, up, down, code, dout)
     shapes = ((n, args.H), (args.F, args.H), (args.F, args.H), (args.O, args.F))
     out = [torch.empty(s, dtype=x2d.dtype, device=dev) if k else None
            for s, k in zip(shapes, needs)]
@@ -735,13 +772,12 @@ def gated_mlp_backward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Ten
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
     with _lib.on_device(dev):
         check(lib.ts_gated_mlp_bwd(ctypes.byref(args), at, at + step,
-                                   0 if act is None else act.data_ptr(), d.data_ptr(), ldd,
+                                   0 if act is None else act.data_ptr(), d, ldd,
                                    *[0 if t is None else t.data_ptr() for t in out],
                                    ws.data_ptr(), wsb, _lib.stream_handle(dev)),
               "ts_gated_mlp_bwd")
-    del held
-    return [t if t is None or t.shape == s.shape else t[:s.shape[0], :s.shape[1]].contiguous()
-            for t, s in zip(out, leaves)]
+    del copies
+    return _crop([(t, None if s is None else s.shape) for t, s in zip(out, leaves)], dev)
 
 
 # ---------------------------------------------------------------------------
