@@ -6,10 +6,10 @@
 // Bound by HBM where the matrices are large, by the launch where they are small, so all of a call's
 // operands share one. A workgroup copies a 64 x 64 tile, 8 elements of the closer-strided dimension
 // to a lane, 16 bytes at any element address where that dimension is dense; a matrix stored column
-// by column is turned in LDS, so that both sides of it stay in 128-byte runs. Measured on MI355X, bf16:
-[8192, 4100] 36 us (3.8 TB/s; torch's fill and copy 35), [4096, 14336] stored by columns 39 us (6.1
-TB/s; torch's copy 233); the block's three operands and result at 34 x 168 x 145 28 us a forward,
-54 when each had a fill and a copy of its own.
+// by column is turned in LDS, so that both sides of it stay in 128-byte runs. Measured on MI355X,
+// bf16: [8192, 4100] 36 us (3.8 TB/s; torch's fill and copy 35), [4096, 14336] stored by columns 39 us
+// (6.1 TB/s; torch's copy 233); the gated block at 34 x 168 x 145 28 us a forward, 54 when each
+// operand had a fill and a copy of its own.
 #include "common.hpp"
 #include "plan.hpp"
 
