@@ -276,7 +276,7 @@ ts_status ts_rope_apply(const void* q_in, void* q_out,
  * makes is all that matters, and its 64-bit product with a position is exact modulo a turn.
  * backward 1: the transpose rotation, of gradients. R / 2 at most 256, D and heads 4096.
  */
-typedef struct {
+typedef struct ts_rope_axes_args {
   const void* q_in;
   void* q_out;
   int64_t q_in_sb, q_in_ss, q_in_sh, q_out_sb, q_out_ss, q_out_sh;
@@ -664,7 +664,7 @@ enum {
  * Operands of the block, all of one 16-bit dtype (TS_BF16 or TS_F16), row-major with row strides
  * in elements: 16-byte aligned, strides and H, F, O multiples of 8 and at most 2^21.
  */
-typedef struct {
+typedef struct ts_gated_mlp_args {
   const void* x; /* [N, H] */
   int64_t ldx;
   const void* w_gate; /* [F, H] */
@@ -710,7 +710,7 @@ ts_status ts_gated_mlp_bwd(const ts_gated_mlp_args* args, const float* keep_p,
  * entry points above do not take as they are. Strides in elements, not negative; any
  * element-aligned address. dst must not overlap any src.
  */
-typedef struct {
+typedef struct ts_pad_job {
   const void* src;
   int64_t row_stride, col_stride, rows, cols;
   void* dst;
@@ -732,7 +732,7 @@ ts_status ts_pad_matrices(const ts_pad_job* jobs, int32_t count, ts_dtype dtype,
  * not NULL, is a device array of (seed, offset) read in place of the two values when the kernels
  * run: a captured graph takes its numbers from there.
  */
-typedef struct {
+typedef struct ts_dropout_rng {
   uint64_t seed, offset;
   const int64_t* state;
   int32_t drop; /* 0 .. 65536 */
