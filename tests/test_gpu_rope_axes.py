@@ -185,6 +185,20 @@ def test_in_place(gpu):
     assert torch.isnan(buf[:, :, 4]).all() and torch.isnan(buf[:, :, 7]).all()
 
 
+def test_in_place_is_seen_by_autograd(gpu):
+    p = RopeAxes((16, 16))
+    q, _, pos, _, _ = inputs(gpu, 2, 9, 4, 0, 64, BF, 2, 8)
+    w = torch.ones_like(q, requires_grad=True)
+    y = w * q  # keeps q
+    apply_rope_axes(q, None, pos, p, inplace=True)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.sum().backward()
+    with torch.inference_mode():
+        t = q.clone()
+        want = apply_rope_axes(t, None, pos, p)[0]
+        assert same(apply_rope_axes(t, None, pos, p, inplace=True)[0], want)
+
+
 def test_only_one_gradient(gpu):
     p = RopeAxes((16, 16))
     q, k, pos, dq, dk = inputs(gpu, 2, 9, 4, 2, 64, BF, 2, 8)

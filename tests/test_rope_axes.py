@@ -117,6 +117,10 @@ def test_functions_refuse():
         apply_rope_axes(q.clone().requires_grad_(), k, pos, p, inplace=True)
     with pytest.raises(ValueError, match="contiguous head"):
         apply_rope_axes(q.transpose(2, 3).contiguous().transpose(2, 3), None, pos, p, inplace=True)
+    with pytest.raises(ValueError, match="expanded"):
+        apply_rope_axes(q[:, :, :1].expand_as(q), None, pos, p, inplace=True)
+    with pytest.raises(ValueError, match="same memory"):
+        apply_rope_axes(q, q[:, :, :1], pos, p, inplace=True)
     with pytest.raises(RuntimeError, match="no CPU fallback"):
         MultiAxisRotaryEmbedding((4, 4))(q, k, pos)
     assert _axes_positions(pos[:, 0], 2, 2, 3).shape == (2, 2, 3)

@@ -501,9 +501,11 @@ def _axes_positions(position_ids: Tensor, axes: int, batch: int, seq: int) -> Te
                             f"{position_ids.dtype}")
         position_ids = position_ids.to(torch.int64)
     shape = tuple(position_ids.shape)
+    if shape == (axes, batch, seq):
+        return position_ids
     if shape == (axes, seq):
         position_ids = position_ids[:, None]
-    elif shape != (axes, 1, seq) and shape != (axes, batch, seq):
+    elif shape != (axes, 1, seq):
         raise ValueError(f"apply_rope_axes: position_ids {shape} for {axes} axes, batch {batch} "
                          f"and {seq} tokens")
     return position_ids.expand(axes, batch, seq)
@@ -516,9 +518,9 @@ def _rope_axes(plan: RopeAxes, pos: Tensor, q: Optional[Tensor], k: Optional[Ten
         outs = (q, k)
     else:
         q, k = [t if t is None else ops._bshd(t, "apply_rope_axes") for t in (q, k)]
-        outs = [t if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+        outs = [t if t is None else torch.empty(*t.shape, dtype=t.dtype, device=t.device)
                 for t in (q, k)]
-    if any(t is not None for t in (q, k)):
+    if q is not None or k is not None:
         ops.rope_axes(q, outs[0], k, outs[1], pos, plan._turns_c, plan._axis_c,
                       len(plan.sections), 2 * len(plan.axis), plan.interleaved, backward)
     return outs[0], outs[1]
@@ -550,18 +552,18 @@ def apply_rope_axes(q: Tensor, k: Optional[Tensor], position_ids: Tensor, plan: 
     (int64 or int32, any values: angles are exact to fp32's rounding however far). Elements past
     plan's pairs stay. fp32 arithmetic, rounded once; returns new tensors, differentiable in q and
     k. inplace writes into q and k instead, for calls that autograd does not record; their last
-    dimension must be contiguous."""
+    dimension must be contiguous, and no two elements may share memory."""
     n = 2 * len(plan.axis)
-    for name, t in (("q", q), ("k", k)):
-        if t is None:
-            continue
-        if t.dim() != 4 or t.shape[-1] < n:
-            raise ValueError(f"apply_rope_axes: {name} {tuple(t.shape)}: expected [B, S, H, D], D at "
+    qs, ks = q.shape, None if k is None else k.shape
+    for name, t in (("q", qs), ("k", ks)):
+        if t is not None and (len(t) != 4 or t[3] < n):
+            raise ValueError(f"apply_rope_axes: {name} {tuple(t)}: expected [B, S, H, D], D at "
                              f"least {n}")
-        if t.shape[:2] != q.shape[:2] or t.shape[3] != q.shape[3] or t.dtype is not q.dtype:
-            raise ValueError(f"apply_rope_axes: k {tuple(t.shape)} {t.dtype} for q "
-                             f"{tuple(q.shape)} {q.dtype}")
-    pos = _axes_positions(position_ids, len(plan.sections), q.shape[0], q.shape[1])
+    batch, seq = qs[0], qs[1]
+    if k is not None and (ks[0] != batch or ks[1] != seq or ks[3] != qs[3]
+                          or k.dtype is not q.dtype):
+        raise ValueError(f"apply_rope_axes: k {tuple(ks)} {k.dtype} for q {tuple(qs)} {q.dtype}")
+    pos = _axes_positions(position_ids, len(plan.sections), batch, seq)
     record = torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))
     if inplace:
         if record or ops.in_forward_ad():
@@ -569,9 +571,18 @@ def apply_rope_axes(q: Tensor, k: Optional[Tensor], position_ids: Tensor, plan: 
         for t in (q, k):
             if t is not None and t.shape[3] > 1 and t.stride(3) != 1:
                 raise ValueError("apply_rope_axes: inplace needs contiguous head dimensions")
+            if t is not None and 0 in t.stride() and any(
+                    n > 1 and not s for n, s in zip(t.shape, t.stride())):
+                raise ValueError("apply_rope_axes: inplace on an expanded tensor")
+        if k is not None and k.numel() and q.data_ptr() == k.data_ptr():
+            raise ValueError("apply_rope_axes: inplace on q and k of the same memory")
+        out = _rope_axes(plan, pos, q, k, True)
+        torch.autograd.graph.increment_version(
+            [t for t in (q, k) if t is not None and not t.is_inference()])
+        return out
     elif record or ops.in_forward_ad():
         return RopeAxesFunction.apply(q, k, pos, plan)
-    return _rope_axes(plan, pos, q, k, inplace)
+    return _rope_axes(plan, pos, q, k)
 
 
 class MultiAxisRotaryEmbedding(nn.Module):
