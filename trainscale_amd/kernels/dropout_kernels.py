@@ -75,16 +75,14 @@ def _check_residual(what: str, x: Tensor, residual: Tensor) -> None:
         raise TypeError(f"{what}: residual dtype {residual.dtype} != x dtype {x.dtype}")
 
 
-def _rows(t: Tensor) -> Tuple[Tensor, int]:
-    return ops.as_rows(t if t.dim() else t.reshape(1))
-
-
 def _forward(x: Tensor, residual: Optional[Tensor], rng, state: Optional[Tensor]) -> Tensor:
+    shape = x.shape
     if x.is_cuda and x.numel() == 0:
-        return torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    x2d, ldx = _rows(x)
-    r2d, ldr = (None, 0) if residual is None else _rows(residual)
-    return ops.dropout_forward(x2d, ldx, r2d, ldr, rng, state, x.shape)
+        return torch.empty(shape, dtype=x.dtype, device=x.device)
+    cols = shape[-1] if shape else 1
+    x, ldx = ops.rows_at(x, cols)
+    residual, ldr = (None, 0) if residual is None else ops.rows_at(residual, cols)
+    return ops.dropout_forward(x, ldx, residual, ldr, rng, state, shape)
 
 
 class FusedDropoutFunction(torch.autograd.Function):
@@ -137,10 +135,10 @@ def fused_dropout_add(x: Tensor, residual: Tensor, p: float, rng: RngLike = None
 
 
 def _norm_forward(x, residual, weight, eps, rng, state):
-    x2d, ldx = ops.as_rows(x)
-    r2d, ldr = ops.as_rows(residual)
-    w = weight.contiguous()
-    y, h, rstd = ops.dropout_add_rmsnorm_forward(x2d, ldx, r2d, ldr, w, eps, rng, state, x.shape)
+    shape, w = x.shape, weight.contiguous()
+    x, ldx = ops.rows_at(x, shape[-1])
+    residual, ldr = ops.rows_at(residual, shape[-1])
+    y, h, rstd = ops.dropout_add_rmsnorm_forward(x, ldx, residual, ldr, w, eps, rng, state, shape)
     return y, h, w, rstd
 
 
@@ -169,11 +167,13 @@ class FusedDropoutAddRMSNormFunction(torch.autograd.Function):
             return (*[torch.zeros(s, dtype=t.dtype, device=t.device) if need else None
                       for need, s, t in zip(needs, (h.shape, h.shape, w.shape), (h, h, w))],
                     None, None, None)
-        h2d, ldh = ops.as_rows(h)
-        (dy, lddy), (dh, lddh) = [(None, 0) if d is None else ops.as_rows(d) for d in (dy, dh)]
+        shape, cols = h.shape, h.shape[-1]
+        h, ldh = ops.rows_at(h, cols)
+        (dy, lddy), (dh, lddh) = [(None, 0) if d is None else ops.rows_at(d, cols)
+                                  for d in (dy, dh)]
         return (*ops.dropout_add_rmsnorm_backward(
-            dy, lddy, dh, lddh, h2d, ldh, w.contiguous(), rstd.contiguous(), ctx.rng,
-            None if state is None else state.contiguous(), needs, h.shape), None, None, None)
+            dy, lddy, dh, lddh, h, ldh, w.contiguous(), rstd.contiguous(), ctx.rng,
+            None if state is None else state.contiguous(), needs, shape), None, None, None)
 
 
 def fused_dropout_add_rms_layernorm(x: Tensor, residual: Tensor, weight: Tensor, p: float,

@@ -33,30 +33,36 @@ def _check(x: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], activati
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise ValueError(f"{what}: unknown activation {activation!r} ({', '.join(ACTIVATIONS)})")
-    if x.dtype is not torch.bfloat16 and x.dtype is not torch.float16:
-        raise TypeError(f"{what}: x must be bfloat16 or float16, got {x.dtype}")
+    dtype = x.dtype
+    if dtype is not torch.bfloat16 and dtype is not torch.float16:
+        raise TypeError(f"{what}: x must be bfloat16 or float16, got {dtype}")
     for name, t in (("gate", gate), ("up", up), ("down", down)):
-        if t is not None and t.dtype is not x.dtype:
-            raise TypeError(f"{what}: {name} weight dtype {t.dtype} != x dtype {x.dtype}")
-    if x.dim() < 1 or gate.dim() != 2 or gate.shape[1] != x.shape[-1] or 0 in gate.shape:
-        raise ValueError(f"{what}: gate weight {tuple(gate.shape)} for x {tuple(x.shape)}")
-    if up.shape != gate.shape:
-        raise ValueError(f"{what}: up weight {tuple(up.shape)} != gate weight "
-                         f"{tuple(gate.shape)}")
-    if down is not None and (down.dim() != 2 or down.shape[1] != gate.shape[0]
-                             or down.shape[0] == 0):
-        raise ValueError(f"{what}: down weight {tuple(down.shape)} for a gate weight "
-                         f"{tuple(gate.shape)}")
+        if t is not None and t.dtype is not dtype:
+            raise TypeError(f"{what}: {name} weight dtype {t.dtype} != x dtype {dtype}")
+    xs, gs = x.shape, gate.shape
+    if len(xs) < 1 or len(gs) != 2 or gs[1] != xs[-1] or 0 in gs:
+        raise ValueError(f"{what}: gate weight {tuple(gs)} for x {tuple(xs)}")
+    if up.shape != gs:
+        raise ValueError(f"{what}: up weight {tuple(up.shape)} != gate weight {tuple(gs)}")
+    if down is not None:
+        ds = down.shape
+        if len(ds) != 2 or ds[1] != gs[0] or ds[0] == 0:
+            raise ValueError(f"{what}: down weight {tuple(ds)} for a gate weight {tuple(gs)}")
     return code
+
+
+def _2d(t: Tensor) -> Tensor:
+    return t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
 
 
 def _forward(x: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], activation: str,
              keep: bool):
     """(result, the activation's code, the backward's factors, gated product)."""
     code = _check(x, gate, up, down, activation)
-    cols = (gate if down is None else down).shape[0]
-    factors, act, out = ops.gated_mlp_forward(x.reshape(-1, x.shape[-1]), gate, up, down, code, keep)
-    return out.view(*x.shape[:-1], cols), code, factors, act
+    factors, act, out = ops.gated_mlp_forward(_2d(x), gate, up, down, code, keep)
+    if x.dim() != 2:
+        out = out.view(*x.shape[:-1], out.shape[1])
+    return out, code, factors, act
 
 
 class GatedMLPFunction(torch.autograd.Function):
@@ -75,9 +81,8 @@ class GatedMLPFunction(torch.autograd.Function):
     def backward(ctx, dout: Tensor):
         x, gate, up, down, factors, act = ctx.saved_tensors
         grads = ops.gated_mlp_backward(
-            x.reshape(-1, x.shape[-1]), gate, up, down, ctx.code, factors, act,
-            dout.reshape(-1, dout.shape[-1]), ctx.needs_input_grad)
-        if grads[0] is not None:
+            _2d(x), gate, up, down, ctx.code, factors, act, _2d(dout), ctx.needs_input_grad)
+        if grads[0] is not None and x.dim() != 2:
             grads[0] = grads[0].view(x.shape)
         return (*grads, None)
 

@@ -40,6 +40,11 @@ def as_rows(t: Tensor) -> Tuple[Tensor, int]:
     return t2, ld
 
 
+def rows_at(t: Tensor, cols: int) -> Tuple[Tensor, int]:
+    """as_rows for a launch that knows the sizes: a contiguous t is itself, not a view of it."""
+    return (t, cols) if t.is_contiguous() else as_rows(t)
+
+
 def in_forward_ad() -> bool:
     """Whether a level of forward-mode differentiation is open, where tensors may have tangents. A
     launch on a tensor's pointer drops its tangent; an autograd function, which has no forward-mode
@@ -698,7 +703,7 @@ def _crop(pairs, dev) -> list:
     for t, shape in pairs:
         if t is not None and t.shape != shape:
             dtype, whole = t.dtype, t
-            t = torch.empty(shape, dtype=dtype, device=dev)
+            t = torch.empty(*shape, dtype=dtype, device=dev)
             jobs.append((whole.data_ptr(), whole.shape[1], 1, *shape, t.data_ptr(), *shape))
         out.append(t)
     if jobs:
@@ -733,9 +738,9 @@ def gated_mlp_forward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Tens
         return new[0] if keep else None, new[1], new[2]
     args, _, copies = _mlp_args(dev, x2d, gate, up, down, code)
     f = args.F
-    factors = torch.empty((2, n, f), dtype=torch.float32, device=dev) if keep else None
-    act = torch.empty((n, f), dtype=x2d.dtype, device=dev)
-    out = act if down is None else torch.empty((n, args.O), dtype=x2d.dtype, device=dev)
+    factors = torch.empty(2, n, f, dtype=torch.float32, device=dev) if keep else None
+    act = torch.empty(n, f, dtype=x2d.dtype, device=dev)
+    out = act if down is None else torch.empty(n, args.O, dtype=x2d.dtype, device=dev)
     p = factors.data_ptr() if keep else 0
     q = p + 4 * n * f if keep else 0
     a, y = act.data_ptr(), 0 if down is None else out.data_ptr()
@@ -762,7 +767,7 @@ def gated_mlp_backward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Ten
                 for t, k in zip(leaves, needs)]
     args, ((d, ldd),), copies = _mlp_args(dev, x2d, gate, up, down, code, dout)
     shapes = ((n, args.H), (args.F, args.H), (args.F, args.H), (args.O, args.F))
-    out = [torch.empty(s, dtype=x2d.dtype, device=dev) if k else None
+    out = [torch.empty(*s, dtype=x2d.dtype, device=dev) if k else None
            for s, k in zip(shapes, needs)]
     factors = factors.contiguous()
     act = None if act is None else act.contiguous()
@@ -796,34 +801,37 @@ def _rng_ref(rng: "_lib.DropoutRng", state: Optional[Tensor]):
     return ctypes.byref(rng)
 
 
-def dropout_forward(x2d: Tensor, ldx: int, res2d: Optional[Tensor], ldr: int,
+def dropout_forward(x: Tensor, ldx: int, res: Optional[Tensor], ldr: int,
                     rng: "_lib.DropoutRng", state: Optional[Tensor], shape) -> Tensor:
-    """[residual +] dropout(x2d), of `shape`."""
-    dev = _lib.require_gpu("dropout", x2d, res2d, state)
-    rows, cols = x2d.shape
-    out = torch.empty(shape, dtype=x2d.dtype, device=dev)
+    """[residual +] dropout(x), of `shape`; x and res are its rows at strides of ldx and ldr."""
+    dev = _lib.require_gpu("dropout", x, res, state)
+    cols = shape[-1] if shape else 1
+    # sizes as separate arguments: torch takes 2 us more to read a tuple
+    out = torch.empty(*shape or ((),), dtype=x.dtype, device=dev)
     with _lib.on_device(dev):
         check(_lib.load().ts_dropout_fwd(
-            x2d.data_ptr(), ldx, 0 if res2d is None else res2d.data_ptr(), ldr, out.data_ptr(),
-            cols, _lib.dtype_code(x2d, "dropout"), rows, cols, _rng_ref(rng, state),
+            x.data_ptr(), ldx, 0 if res is None else res.data_ptr(), ldr, out.data_ptr(), cols,
+            _lib.dtype_code(x, "dropout"), x.numel() // cols, cols, _rng_ref(rng, state),
             _lib.stream_handle(dev)), "ts_dropout_fwd")
     return out
 
 
-def dropout_add_rmsnorm_forward(x2d: Tensor, ldx: int, res2d: Tensor, ldr: int, weight: Tensor,
+def dropout_add_rmsnorm_forward(x: Tensor, ldx: int, res: Tensor, ldr: int, weight: Tensor,
                                 eps: float, rng: "_lib.DropoutRng", state: Optional[Tensor], shape
                                 ) -> Tuple[Tensor, Tensor, Tensor]:
-    """(y, h, rstd fp32 [rows]) of h = residual + dropout(x), y = RMSNorm(h); y and h of `shape`."""
-    dev = _lib.require_gpu("dropout_add_rmsnorm", x2d, res2d, weight, state)
-    rows, cols = x2d.shape
-    y = torch.empty(shape, dtype=x2d.dtype, device=dev)
-    h = torch.empty(shape, dtype=x2d.dtype, device=dev)
-    rstd = torch.empty((rows,), dtype=torch.float32, device=dev)
+    """(y, h, rstd fp32 [rows]) of h = residual + dropout(x), y = RMSNorm(h); y and h of `shape`,
+    x and res its rows at strides of ldx and ldr."""
+    dev = _lib.require_gpu("dropout_add_rmsnorm", x, res, weight, state)
+    cols = weight.shape[0]
+    rows = x.numel() // cols
+    y = torch.empty(*shape, dtype=x.dtype, device=dev)
+    h = torch.empty(*shape, dtype=x.dtype, device=dev)
+    rstd = torch.empty(rows, dtype=torch.float32, device=dev)
     if rows == 0:
         return y, h, rstd
     with _lib.on_device(dev):
         check(_lib.load().ts_dropout_add_rmsnorm_fwd(
-            x2d.data_ptr(), ldx, res2d.data_ptr(), ldr, _lib.dtype_code(x2d, "dropout"),
+            x.data_ptr(), ldx, res.data_ptr(), ldr, _lib.dtype_code(x, "dropout"),
             weight.data_ptr(), _lib.dtype_code(weight, "dropout_add_rmsnorm weight"), y.data_ptr(),
             h.data_ptr(), rstd.data_ptr(), rows, cols, eps, _rng_ref(rng, state),
             _lib.stream_handle(dev)), "ts_dropout_add_rmsnorm_fwd")
@@ -831,16 +839,17 @@ def dropout_add_rmsnorm_forward(x2d: Tensor, ldx: int, res2d: Tensor, ldr: int, 
 
 
 def dropout_add_rmsnorm_backward(dy: Optional[Tensor], lddy: int, dh: Optional[Tensor], lddh: int,
-                                 h2d: Tensor, ldh: int, weight: Tensor, rstd: Tensor,
+                                 h: Tensor, ldh: int, weight: Tensor, rstd: Tensor,
                                  rng: "_lib.DropoutRng", state: Optional[Tensor], needs,
                                  shape) -> list:
     """Gradients of (x, residual, weight), None where `needs` is false, the first two of
     `shape`."""
-    dev = _lib.require_gpu("dropout_add_rmsnorm", dy, dh, h2d, weight, rstd)
-    rows, cols = h2d.shape
-    out = [torch.empty(shape, dtype=h2d.dtype, device=dev) if needs[0] else None,
-           torch.empty(shape, dtype=h2d.dtype, device=dev) if needs[1] else None,
-           torch.empty((cols,), dtype=weight.dtype, device=dev) if needs[2] else None]
+    dev = _lib.require_gpu("dropout_add_rmsnorm", dy, dh, h, weight, rstd, state)
+    rows, cols = rstd.shape[0], weight.shape[0]
+    dt = h.dtype
+    out = [torch.empty(*shape, dtype=dt, device=dev) if needs[0] else None,
+           torch.empty(*shape, dtype=dt, device=dev) if needs[1] else None,
+           torch.empty(cols, dtype=weight.dtype, device=dev) if needs[2] else None]
     lib = _lib.load()
     ws, wsb = None, 0
     if needs[2]:
@@ -849,7 +858,7 @@ def dropout_add_rmsnorm_backward(dy: Optional[Tensor], lddy: int, dh: Optional[T
     at = [0 if t is None else t.data_ptr() for t in (dy, dh, *out, ws)]
     with _lib.on_device(dev):
         check(lib.ts_dropout_add_rmsnorm_bwd(
-            at[0], lddy, at[1], lddh, h2d.data_ptr(), ldh, _lib.DTYPE_CODE[h2d.dtype],
+            at[0], lddy, at[1], lddh, h.data_ptr(), ldh, _lib.DTYPE_CODE[dt],
             weight.data_ptr(), _lib.DTYPE_CODE[weight.dtype], rstd.data_ptr(), at[2], at[3], at[4],
             rows, cols, _rng_ref(rng, state), at[5], wsb, _lib.stream_handle(dev)),
             "ts_dropout_add_rmsnorm_bwd")
