@@ -15,8 +15,10 @@
 // Every kernel gives a lane groups of 8 elements, one counter each: a group is one 16-byte access
 // (two for fp32), at any element address; a row's last, shorter group goes element by element.
 //
-// Bound by HBM; the generator's 20 products a group hide under it. Measured on MI355X: [8192, 14336]
-// bf16 80 us (5.9 TB/s); with the norm [16384, 4096] bf16 94 us forward (5.8 TB/s) and 129 + 5 us
+// Bound by HBM, with the generator's 20 products a group nearly hidden under it. Measured on MI355X,
+// [8192, 14336] bf16: 75 us (6.3 TB/s) back to back; between events 80.3, 76.5 without a mask, and
+// 83.4 with exclusive ors in pairs, each 16 bits taken apart and a division for the row. With the norm,
+// [16384, 4096] bf16 94 us forward (5.8 TB/s) and 129 + 5 us
 // backward (5.4 TB/s; much the same without the mask or dw, so what is left is memory latency), [8191,
 // 768] fp32 26 and 29 + 4 us.
 #include "common.hpp"
@@ -51,9 +53,9 @@ __device__ inline u32x4 philox(uint64_t n, Key k) {
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
     const uint64_t p0 = (uint64_t)c0 * 0xD2511F53u, p1 = (uint64_t)c2 * 0xCD9E8D57u;
-    c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k.k0;
+    c0 = __builtin_amdgcn_bitop3_b32((uint32_t)(p1 >> 32), c1, k.k0, 0x96);  // exclusive or of 3
     c1 = (uint32_t)p1;
-    c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k.k1;
+    c2 = __builtin_amdgcn_bitop3_b32((uint32_t)(p0 >> 32), c3, k.k1, 0x96);
     c3 = (uint32_t)p0;
     k.k0 += 0x9E3779B9u;
     k.k1 += 0xBB67AE85u;
@@ -61,13 +63,16 @@ __device__ inline u32x4 philox(uint64_t n, Key k) {
   return u32x4{c0, c1, c2, c3};
 }
 
-// f[i] = kept ? f[i] * scale : 0 over the 8 elements of group n.
+// f[i] = kept ? f[i] * scale : 0 over the 8 elements of group n, drop > 0. An element's 16 bits are
+// compared from the top of a word: at or above drop if the word is above 65536 drop - 1, which fits
+// 32 bits up to drop = 65536 (nothing kept).
 __device__ inline void apply_mask(float (&f)[8], uint64_t n, const Key& k, int drop, float scale) {
   const u32x4 w = philox(n, k);
+  const uint32_t limit = ((uint32_t)drop << 16) - 1u;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const int bits = i & 1 ? (int)(w[i / 2] >> 16) : (int)(w[i / 2] & 0xffffu);
-    f[i] = bits >= drop ? f[i] * scale : 0.f;
+    const uint32_t top = i & 1 ? w[i / 2] : w[i / 2] << 16;
+    f[i] = top > limit ? f[i] * scale : 0.f;
   }
 }
 
@@ -115,6 +120,7 @@ struct DropArgs {
   int64_t ldo;
   int64_t cols, groups, total;  // groups a row, groups in all
   uint64_t magic;               // ts_plan::magic64_for(groups)
+  int32_t one_row;
   Rng rng;
 };
 
@@ -122,7 +128,7 @@ template <typename T, bool kRes>
 __global__ __launch_bounds__(256) void dropout_kernel(const DropArgs a) {
   const int64_t v = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (v >= a.total) return;
-  const int64_t r = a.magic == 0 ? v : (int64_t)__umul64hi((uint64_t)v, a.magic);
+  const int64_t r = a.one_row ? 0 : a.magic == 0 ? v : (int64_t)__umul64hi((uint64_t)v, a.magic);
   const int64_t c = (v - r * a.groups) * 8;
   const int n = a.cols - c < 8 ? (int)(a.cols - c) : 8;
   float f[8], res[8];
@@ -493,8 +499,14 @@ extern "C" ts_status ts_dropout_fwd(const void* x, int64_t ldx, const void* resi
   if (rows > ((int64_t)1 << 34) / a.groups)
     return fail(TS_ERR_SHAPE, "dropout_fwd: tensor too large");
   a.total = rows * a.groups;
+  // whole groups without gaps between rows are one row of the same groups: no division
+  if (cols % 8 == 0 && ldx == cols && ldo == cols && (residual == nullptr || ldr == cols)) {
+    a.cols = rows * cols;
+    a.groups = a.total;
+  }
+  a.one_row = a.groups == a.total;
   a.magic = ts_plan::magic64_for((uint64_t)a.groups);  // total * groups < 2^64
-  if (!ts_plan::magic64_exact((uint64_t)a.total, (uint64_t)a.groups))
+  if (!a.one_row && !ts_plan::magic64_exact((uint64_t)a.total, (uint64_t)a.groups))
     return fail(TS_ERR_SHAPE, "dropout_fwd: tensor too large");
   hipStream_t st = static_cast<hipStream_t>(stream);
   switch (dtype) {
