@@ -365,3 +365,46 @@ def test_far_elements(gpu):
     bits = np.stack([v >> np.uint64(s) & np.uint64(0xFFFF) for v in words for s in (0, 16)], -1)
     keep = torch.from_numpy((bits.reshape(2, cols) >= 32768)).to(gpu)
     assert torch.equal(y[-2:] != 0, keep)
+
+
+def test_far_rows_of_the_norm(gpu):
+    """Elements past 2^32: the sum as the operator without the norm forms it (whose far mask the test
+    above holds to the generator), the last rows' norm and gradients by their formulas."""
+    rows, cols, p = (1 << 32) // 4096 + 40, 4096, 0.25
+    x = torch.full((rows, cols), 0.5, dtype=BF, device=gpu).requires_grad_()
+    res = torch.zeros(rows, cols, dtype=BF, device=gpu)
+    g = torch.Generator(device=gpu).manual_seed(3)
+    res[-32:] = torch.randn(32, cols, device=gpu, generator=g).to(BF)
+    w = torch.ones(cols, device=gpu, requires_grad=True)
+    y, h = fused_dropout_add_rms_layernorm(x, res.requires_grad_(), w, p, EPS, rng=RNG)
+    plain = fused_dropout_add(x.detach(), res.detach(), p, RNG)
+    assert torch.equal(h.detach(), plain)
+    keep = (plain - res.detach() != 0)[-32:]
+    del plain
+    dy = torch.zeros_like(y)
+    dy[-32:] = torch.randn(32, cols, device=gpu, generator=g).to(BF)
+    dx, dres, dw = torch.autograd.grad(y, (x, res, w), dy)
+    assert not dx[:-32].any() and not dres[:-32].any()
+    X, R, DY = [t[-32:].detach().double() for t in (x, res, dy)]
+    H = R + torch.where(keep, X * scale_of(p), 0.0)
+    rh = 1 / (H.square().mean(-1, keepdim=True) + EPS).sqrt()
+    k, M = (H - R).abs() + R.abs(), half(BF)
+    check(y[-32:].detach(), H * rh, 60 * U * k * rh, "y")
+    # the backward's hat comes from the rounded h: off by half a step of it
+    hat = H * rh
+    c1 = (DY * hat).mean(-1, keepdim=True)
+    t = rh * (DY - hat * c1)
+    eh = (M + 60 * U) * k * rh
+    ec = (DY.abs() * (eh + 50 * U * hat.abs())).mean(-1, keepdim=True)
+    et = rh * (eh * (c1.abs() + ec) + hat.abs() * ec) + 60 * U * rh * (DY.abs() + k * rh * c1.abs())
+    check(dres[-32:], t, et, "dres")
+    check(dx[-32:], torch.where(keep, t * scale_of(p), 0.0), et * scale_of(p) * (1 + U)
+          + 2 * U * t.abs() * scale_of(p), "dx")
+    check(dw, (DY * hat).sum(0), (DY.abs() * (eh + 220 * U * k * rh)).sum(0), "dw")
+
+
+def test_far_rows_apart(gpu):
+    """The same of rows with gaps, whose place is divided out of the group's number."""
+    x = torch.ones((1 << 32) // 4088 + 9, 4096, dtype=BF, device=gpu)[:, :4088]
+    assert x.numel() > 1 << 32
+    assert torch.equal(fused_dropout(x, 0.5, RNG), fused_dropout(x.contiguous(), 0.5, RNG))

@@ -253,3 +253,18 @@ def test_module_stream_hooks_and_graph(gpu):
         want, g = run_and_check((q.detach(), k.detach(), pos, dq, dk), m.plan)
         torch.cuda.synchronize()
         assert all(same(a, b) for a, b in zip(out, (*want, *g))), i
+
+
+def test_far_elements(gpu):
+    """Elements past 2^32: the last tokens turn as they do alone."""
+    p = RopeAxes((16, 24, 24))
+    b, s, h, d = 2, 270000, 64, 128
+    pos = torch.arange(s, device=gpu).expand(3, b, s)
+    q = torch.zeros(b, s, h, d, dtype=BF, device=gpu)
+    tail = inputs(gpu, 1, 40, h, 0, d, BF, 3, 5)[0]
+    q[1, -40:] = tail[0]
+    out = apply_rope_axes(q, None, pos, p)[0]
+    want = apply_rope_axes(tail, None, pos[:, :1, -40:], p)[0]
+    assert same(out[1, -40:], want[0]) and not out[0].any() and not out[1, :-40].any()
+    apply_rope_axes(q, None, pos, p, inplace=True)
+    assert same(q[1, -40:], want[0])
