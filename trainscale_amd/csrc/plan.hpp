@@ -404,21 +404,21 @@ struct MlpBwdPlan {
 
 // Which tiles, and how many slots K is cut into, by an estimate of the time in microseconds (the
 // host's choice follows from the shape alone, so a shape's sums keep their order). Fitted to
-// MI355X: a k-block of a 256 x 256 tile takes 1.35 us in a launch of one tile a CU and 1.65 us while
-// the whole card is at its power limit, one of a 128 x 128 tile 0.5 us on half the card's CUs, 0.75 us
-// on all of them and 1.0 us beside another on its CU; a tile's start and epilogue 4 to 5 us, 13 us
+// MI355X: a k-block of a 256 x 256 tile takes 1.25 us in a launch of one tile a CU and 1.65 us while
+// the whole card is at its power limit, one of a 128 x 128 tile 0.5 us on half the card's CUs, 0.65 us
+// on all of them and 1.0 us beside another on its CU; a tile's start and epilogue 4 to 6 us, 13 us
 // where a large tile's epilogue also moves the backward's factors and no other workgroup's products
 // run beside it; slots cost their partials' traffic and a launch. Measured against 256 x 256 tiles
 // without slots, forward and backward, N, H, F: 2045, 768, 2048 71 -> 42 and 117 -> 62 us; 256, 2048,
-// 5632 147 -> 44 and 258 -> 72; 100, 4096, 14336 402 -> 110 and 734 -> 217; of 18 shapes tried, the
-// choice was within 15% of the best of all, mostly within 5%.
+// 5632 147 -> 42 and 258 -> 72; 100, 4096, 14336 401 -> 109 and 734 -> 217; of 28 shapes tried, the
+// choice was within 10% of the best of all, mostly within 3%.
 inline int64_t mlp_kblocks(int64_t K) { return (K + kGemmBlockK - 1) / kGemmBlockK; }
 inline double mlp_time(int64_t pieces, int64_t kblocks, int waves, bool gated = false) {
   if (waves == 8)
     return (double)((pieces + 255) / 256) *
-           (kblocks * (pieces <= 256 ? 1.35 : 1.65) + (gated ? 13.0 : 5.0));
-  if (pieces <= 256) return kblocks * (pieces <= 128 ? 0.5 : 0.75) + 4.0;
-  return (double)((pieces + 511) / 512) * (kblocks * 1.0 + 5.0);
+           (kblocks * (pieces <= 256 ? 1.25 : 1.65) + (gated ? 13.0 : 6.0));
+  if (pieces <= 256) return kblocks * (pieces <= 128 ? 0.5 : 0.65) + 4.0;
+  return (double)((pieces + 511) / 512) * (kblocks * 1.0 + 6.0);
 }
 inline double mlp_slots_time(int64_t slots, int64_t M, int64_t N) {  // without the launch
   return slots > 1 ? (double)(slots * M * N) * 8.0 / 4.5e6 : 0.0;
@@ -504,9 +504,9 @@ inline MlpBwdPlan mlp_bwd_plan(const MlpShape& s) {
         const double longest = ax > aw ? ax : aw;
         // 256 x 256 tiles take a CU each, in turn; of 128 x 128 tiles two share one, the longest
         // going on alone at the end
-        double t = waves == 8 ? (tx * x + tw * w <= kCus ? 1.15 : 1.45) *
+        double t = waves == 8 ? (tx * x + tw * w <= kCus ? 1.35 : 1.45) *
                                     mlp_makespan(tx * x, ax, tw * w, aw, kCus)
-                              : (1.05 * work > 0.6 * longest ? 1.05 * work : 0.6 * longest);
+                              : (work > 0.6 * longest ? work : 0.6 * longest);
         t += mlp_slots_time(x, s.N, s.H) + 2 * mlp_slots_time(w, s.F, s.H) +
              mlp_slots_time(w, s.O, s.F);
         if (x > 1 || w > 1) t += kMlpSumLaunch;
