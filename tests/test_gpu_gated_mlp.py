@@ -171,6 +171,13 @@ def test_odd_sizes(gpu, n, h, f, o):
     run_and_check(inputs(gpu, n, h, f, 0, BF, h), "silu")
 
 
+@pytest.mark.parametrize("n", [16, 17, 31, 32, 33, 48, 49, 64])
+@pytest.mark.parametrize("h,f,o", [(72, 4104, 4120), (512, 5000, 7000), (4136, 8192, 4096),
+                                   (96, 9216, 9224)])
+def test_few_rows_of_many_features(gpu, n, h, f, o):
+    run_and_check(inputs(gpu, n, h, f, o, BF, n), "silu")
+
+
 @pytest.mark.parametrize("n,h,f", [(2048, 1024, 2816), (4100, 768, 2048), (24, 4096, 14336),
                                    (300, 4096, 14336)])
 def test_large(gpu, n, h, f):

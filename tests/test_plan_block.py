@@ -58,8 +58,18 @@ int main() {
       for (int pair = 1; pair <= 2; ++pair) {
         const int d = mlp_few_depth(tiles);
         CHECK(d >= 2 && waves * (pair + tiles) * d * 2048 <= 160 * 1024, "LDS");
+        // the waves' sums take the ring's place, and two feature tiles fit too
+        CHECK(waves * pair * tiles * 1024 <= waves * (pair + tiles) * d * 2048, "sums");
+        CHECK(waves * (2 * pair + tiles) * d * 2048 <= 160 * 1024, "LDS of two");
+        CHECK(2 * pair * tiles * 1024 <= (2 * pair + tiles) * d * 2048, "sums of two");
       }
   }
+  for (long long F = 1; F <= 40000; F += 7)
+    for (long long N : {1, 16, 17, 32, 33, 48, 49, 64})
+      for (bool pair : {false, true}) {
+        const bool two = mlp_few_two(N, F, pair);
+        CHECK(!two || (N > (pair ? 32 : 16) && F > 16 * kCus), "two tiles of %lld rows", N);
+      }
   for (long long cols = 1; cols <= kDropNormMaxCols; ++cols) {
     const long long groups = (cols + 7) / 8;
     for (int bytes : {0, 2, 4}) {  // 0: the forward

@@ -319,16 +319,17 @@ void mlp_grads(const Grads a) {
 }
 
 // ---------------------------------------------------------------------------
-// Few rows (decoding): bound by reading the weights once. A workgroup owns 16 output features and
-// every row; its waves take k-blocks of 64 in turn. Each wave streams the 128-byte runs of its 16
+// Few rows (decoding): bound by reading the weights once. A workgroup owns 16 or 32 output features
+// and every row; its waves take k-blocks of 64 in turn. Each wave streams the 128-byte runs of its 16
 // weight rows (of both projections) and of x into a ring of its own in LDS, kDepth k-blocks ahead,
 // and never waits for another wave until their sums are added in LDS, in wave order, at the end.
 // The weights are the MFMAs' first operand, so a lane ends with four features of one row.
 // The eight lanes of a load into LDS that share a row read its 128 bytes whole, where a load into
 // MFMA operands takes 16 bytes of 16 rows at a time. Measured on MI355X, 16 rows, [14336, 4096] pair
 // and [4096, 14336] (352 MB, three sets in turn): registers 85 us, LDS 72 us, the weights past the
-// caches 66 us (5.3 TB/s; one row 62 us). 64 rows: registers 157 us, LDS 107 us, products on
-// 128 x 128 tiles with K in 12 slots 103 us, but 20 against 13 us at [2048, 768].
+// caches 66 us (5.3 TB/s; one row 62 us). 64 rows: registers 157 us, LDS 107 us, with two
+// feature tiles a workgroup for the pair 96 us, products on 128 x 128 tiles with K in 12 slots 103 us (and
+// 20 against 13 us at [2048, 768]).
 // ---------------------------------------------------------------------------
 struct Few {
   const __bf16* x;
@@ -373,22 +374,23 @@ __device__ inline void few_issue(const FewTile& t, int64_t kb, bool last, uint8_
                              (int)(last ? t.tail[u] : t.off[u]), (int)(kb * 128), 0, kAux);
 }
 
-// kNT 16-row tiles of x. kStream: the weights are read past the caches.
-template <typename T, int kNT, bool kPair, bool kStream>
+// kNT 16-row tiles of x, kFT 16-feature tiles. kStream: the weights are read past the caches.
+template <typename T, int kNT, int kFT, bool kPair, bool kStream>
 __global__ __launch_bounds__(64 * ts_plan::kMlpFewWaves) void mlp_few(const Few a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  constexpr int kP = kPair ? 2 : 1;
+  constexpr int kP = (kPair ? 2 : 1) * kFT;  // weight tiles: kFT of the first product, then the other's
   constexpr int kDepth = ts_plan::mlp_few_depth(kNT);
   constexpr int kTiles = kP + kNT;
   constexpr int kStage = kTiles * 2048;
   const int lane = threadIdx.x & 63;
   const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int waves = blockDim.x >> 6;
-  const int64_t f0 = (int64_t)blockIdx.x * 16;
+  const int64_t f0 = (int64_t)blockIdx.x * (16 * kFT);
   uint8_t* ring = smem + wid * (kDepth * kStage);
   FewTile tile[kTiles];
 #pragma unroll
-  for (int p = 0; p < kP; ++p) tile[p] = few_tile(a.w[p], a.ldw[p], a.F, f0, a.K);
+  for (int p = 0; p < kP; ++p)
+    tile[p] = few_tile(a.w[p / kFT], a.ldw[p / kFT], a.F, f0 + p % kFT * 16, a.K);
 #pragma unroll
   for (int t = 0; t < kNT; ++t) tile[kP + t] = few_tile(a.x, a.ldx, a.N, t * 16, a.K);
   f32x4 acc[kP][kNT];
@@ -451,14 +453,17 @@ __global__ __launch_bounds__(64 * ts_plan::kMlpFewWaves) void mlp_few(const Few 
 #pragma unroll
     for (int t = 0; t < kNT; ++t) sums[((wid * kP + p) * kNT + t) * 64 + lane] = acc[p][t];
   __syncthreads();
-  for (int i = threadIdx.x; i < kNT * 64; i += blockDim.x) {
-    f32x4 s[kP];
+  for (int i = threadIdx.x; i < kFT * kNT * 64; i += blockDim.x) {
+    constexpr int kQ = kPair ? 2 : 1;
+    f32x4 s[kQ];
 #pragma unroll
-    for (int p = 0; p < kP; ++p) {
-      s[p] = sums[p * kNT * 64 + i];
-      for (int v = 1; v < waves; ++v) s[p] += sums[(v * kP + p) * kNT * 64 + i];
+    for (int q = 0; q < kQ; ++q) {
+      const f32x4* at = sums + q * kFT * kNT * 64 + i;
+      s[q] = at[0];
+      for (int v = 1; v < waves; ++v) s[q] += at[v * kP * kNT * 64];
     }
-    const int64_t r = (i >> 6) * 16 + (i & 15), fo = f0 + ((i & 63) >> 4) * 4;
+    const int t = i >> 6;
+    const int64_t r = t % kNT * 16 + (i & 15), fo = f0 + t / kNT * 16 + ((i & 63) >> 4) * 4;
     if (r >= a.N || fo >= a.F) continue;
     const int64_t at = r * a.F + fo;
     if constexpr (kPair) {
@@ -652,27 +657,33 @@ ts_status launch_sums(SumJobs& s, int n, hipStream_t st) {
     if (s_ != TS_OK) return s_;    \
   } while (0)
 
-template <typename T, int kNT, bool kPair>
+template <typename T, int kNT, int kFT, bool kPair>
 ts_status launch_few_rows(const Few& f, hipStream_t st) {
-  const int64_t blocks = (f.F + 15) / 16;
+  const int64_t blocks = (f.F + 16 * kFT - 1) / (16 * kFT);
   const int waves = ts_plan::mlp_few_waves(f.K);
   const size_t lds =
-      (size_t)waves * ((kPair ? 2 : 1) + kNT) * ts_plan::mlp_few_depth(kNT) * 2048;
+      (size_t)waves * ((kPair ? 2 : 1) * kFT + kNT) * ts_plan::mlp_few_depth(kNT) * 2048;
   if (ts_plan::mlp_few_stream(f.F, f.K, kPair))
-    hipLaunchKernelGGL((mlp_few<T, kNT, kPair, true>), dim3((unsigned)blocks), dim3(64 * waves),
-                       lds, st, f);
+    hipLaunchKernelGGL((mlp_few<T, kNT, kFT, kPair, true>), dim3((unsigned)blocks),
+                       dim3(64 * waves), lds, st, f);
   else
-    hipLaunchKernelGGL((mlp_few<T, kNT, kPair, false>), dim3((unsigned)blocks), dim3(64 * waves),
-                       lds, st, f);
+    hipLaunchKernelGGL((mlp_few<T, kNT, kFT, kPair, false>), dim3((unsigned)blocks),
+                       dim3(64 * waves), lds, st, f);
   return ts_host::check_launch("mlp_few");
 }
 
 template <typename T, bool kPair>
 ts_status launch_few(const Few& f, hipStream_t st) {
-  if (f.N <= 16) return launch_few_rows<T, 1, kPair>(f, st);
-  if (f.N <= 32) return launch_few_rows<T, 2, kPair>(f, st);
-  if (f.N <= 48) return launch_few_rows<T, 3, kPair>(f, st);
-  return launch_few_rows<T, 4, kPair>(f, st);
+  const bool two = ts_plan::mlp_few_two(f.N, f.F, kPair);
+  if (f.N <= 16) return launch_few_rows<T, 1, 1, kPair>(f, st);
+  if (f.N <= 32) {
+    if constexpr (!kPair)
+      if (two) return launch_few_rows<T, 2, 2, kPair>(f, st);
+    return launch_few_rows<T, 2, 1, kPair>(f, st);
+  }
+  if (f.N <= 48)
+    return two ? launch_few_rows<T, 3, 2, kPair>(f, st) : launch_few_rows<T, 3, 1, kPair>(f, st);
+  return two ? launch_few_rows<T, 4, 2, kPair>(f, st) : launch_few_rows<T, 4, 1, kPair>(f, st);
 }
 
 template <typename T>

@@ -374,10 +374,10 @@ inline int64_t mlp_tiles(int64_t M, int64_t N, int waves, bool pair) {
   const int64_t bm = 32 * waves, bn = pair ? bm / 2 : bm;
   return ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
 }
-// Few rows (mlp_few): a workgroup of up to kMlpFewWaves waves for every 16 of F features, each with
-// a ring of k-blocks in LDS, 2 KiB for the 16 rows of each operand tile. Three k-blocks deep with
+// Few rows (mlp_few): a workgroup of up to kMlpFewWaves waves for every 16 or 32 of F features, each
+// with a ring of k-blocks in LDS, 2 KiB for the 16 rows of each operand tile. Three k-blocks deep with
 // one tile of x, so that a CU holds two workgroups of a pair of projections (72 KiB); two with more
-// (up to 96 KiB). Measured on MI355X at H 4096, F 14336: 16 rows, depth 3 against 2, 72.5 and 74.4 us;
+// (up to 128 KiB). Measured on MI355X at H 4096, F 14336: 16 rows, depth 3 against 2, 72.5 and 74.4 us;
 // 32 rows 87.5 and 83.5; 4 waves against 2 and 8, 72.5, 82.4 and 76.4 us.
 constexpr int64_t kMlpFewRows = 64;
 constexpr int kMlpFewWaves = 4;
@@ -385,6 +385,19 @@ TS_HOST_DEVICE constexpr int mlp_few_depth(int row_tiles) { return row_tiles == 
 inline int mlp_few_waves(int64_t K) {
   const int64_t blocks = (K + kGemmBlockK - 1) / kGemmBlockK;
   return (int)(blocks < kMlpFewWaves ? blocks : kMlpFewWaves);
+}
+// Two 16-feature tiles a workgroup read x, which then costs the L2 more than the weights cost HBM,
+// half as often: with more than 32 rows for the pair, 16 for one product, where more workgroups than
+// CUs are there to halve and the halves' last round over the CUs is not too empty. Measured on MI355X
+// with one tile and with two: the pair at H 4096, F 14336 (448 halves), 64 rows 64 and 53 us; 48 rows 52
+// and 51; 32 rows 45 and 47; H 1536, F 8960 (280), 40 rows 14 and 18; H 6144, F 16384 (512), 82 and 74;
+// one product of 5120 features over 13824, 17 rows 39 and 32, 64 rows 72 and 50; of 9216 (288) over
+// 4096, 20 rows 20 and 25; of 4096 (128) over 14336, 64 rows 42 and 54.
+inline bool mlp_few_two(int64_t N, int64_t F, bool pair) {
+  const int64_t row_tiles = (N + 15) / 16, one = (F + 15) / 16, two = (one + 1) / 2;
+  if (row_tiles < (pair ? 3 : 2) || one <= kCus) return false;
+  const int64_t full = (two + kCus - 1) / kCus * kCus;
+  return full == kCus || full * 5 <= two * (pair && row_tiles < 4 ? 6 : 7);
 }
 // Weights of a launch above 64 MB are read past the caches: the last level's 256 MB would not keep
 // them, and their neighbours, until the next step, and not allocating there is faster (72.5 -> 66.4 us
