@@ -154,3 +154,16 @@ def test_patched_block_on_the_gpu(gpu, dtype):
         assert got.dtype == dtype
         err = (got.double() - want).norm() / want.norm()
         assert err <= 4 * torch.finfo(dtype).eps / 2, err
+
+
+@pytest.mark.parametrize("register", ["register_forward_hook", "register_forward_pre_hook",
+                                      "register_full_backward_hook",
+                                      "register_full_backward_pre_hook", "register_backward_hook"])
+def test_hooks_of_the_activation(register, monkeypatch):
+    m = LlamaMLP(act=nn.SiLU(), dtype=BF)
+    registry.auto_patch_fused_mlp(m)
+    m._trainscale_amd_forward = lambda x: x
+    hook = getattr(m.act_fn, register)(lambda *a: None)
+    assert taken(m, fake(), monkeypatch) is None
+    hook.remove()
+    assert taken(m, fake(), monkeypatch) == "silu"

@@ -117,6 +117,12 @@ _ACT_CLASSES = {"SiLUActivation": "silu", "GELUActivation": "gelu", "GELUTanh": 
                 "PytorchGELUTanh": "gelu_tanh"}
 
 
+def _watched(layer: nn.Module) -> bool:
+    """Whether calling a module does or reports more than its class's forward."""
+    return bool("forward" in vars(layer) or layer._forward_hooks or layer._forward_pre_hooks
+                or layer._backward_hooks or layer._backward_pre_hooks)
+
+
 def _activation_of(module: nn.Module):
     """The name of a gated block's activation, None where it is another's. Without an attribute it
     is SiLU, which ``auto_patch_mlp`` puts in every registered block."""
@@ -124,7 +130,7 @@ def _activation_of(module: nn.Module):
     if act is None:
         return "silu"
     if isinstance(act, nn.Module):
-        if act._forward_hooks or act._forward_pre_hooks or "forward" in vars(act):
+        if _watched(act):
             return None
         if type(act) in (nn.SiLU, nn.ReLU):
             return "silu" if type(act) is nn.SiLU else "relu"
@@ -137,17 +143,15 @@ def _activation_of(module: nn.Module):
 def _plain_linear(layer) -> bool:
     """Whether a projection is its weight's product and nothing else (no bias, adapter, hook,
     parametrization, replaced forward or distributed weight)."""
-    return (type(layer) is nn.Linear and layer.bias is None and "forward" not in vars(layer)
-            and type(layer.weight) in (nn.Parameter, torch.Tensor)
-            and not (layer._forward_hooks or layer._forward_pre_hooks or layer._backward_hooks
-                     or layer._backward_pre_hooks))
+    return (type(layer) is nn.Linear and layer.bias is None and not _watched(layer)
+            and type(layer.weight) in (nn.Parameter, torch.Tensor))
 
 
 def auto_patch_fused_mlp(module: nn.Module) -> None:
     """Routes a gate/up/down MLP through ``fused_gated_mlp``. Calls that are not the plain block in
-    bf16 or fp16 (a projection with a bias, an adapter or hooks, another activation, fp32, autocast
-    to another type, CPU tensors) keep the module's own forward; what a call is, is looked up at each
-    call, so adapters may come later."""
+    bf16 or fp16 (a projection with a bias, an adapter or hooks, another activation or one with hooks,
+    fp32, autocast to another type, CPU tensors) keep the module's own forward; what a call is, is
+    looked up at each call, so adapters may come later."""
     if not (hasattr(module, "gate_proj") and hasattr(module, "up_proj")
             and hasattr(module, "down_proj")):
         return
