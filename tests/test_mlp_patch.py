@@ -1,5 +1,6 @@
 """KernelPatcher(fuse_mlp=True): which blocks it takes, which calls keep the module's own forward."""
 import copy
+import types
 
 import pytest
 import torch
@@ -167,3 +168,52 @@ def test_hooks_of_the_activation(register, monkeypatch):
     assert taken(m, fake(), monkeypatch) is None
     hook.remove()
     assert taken(m, fake(), monkeypatch) == "silu"
+
+
+class NamedActMLP(LlamaMLP):
+    """A block of a registered shape that keeps its activation under another name."""
+
+    def __init__(self, name, act):
+        super().__init__(dtype=BF)
+        setattr(self, name, act)
+
+
+class MethodMLP(LlamaMLP):
+    def activation(self, t):
+        return F.gelu(t)
+
+
+@pytest.mark.parametrize("name,act", [
+    ("act", nn.GELU()), ("act", F.gelu), ("activation", torch.tanh), ("activation_function", F.gelu),
+    ("hidden_act", "gelu"), ("non_linearity", F.gelu), ("dropout", nn.Dropout(0.1)),
+    ("norm", nn.LayerNorm(40))])
+@pytest.mark.parametrize("act_fn", [None, nn.SiLU()])
+def test_blocks_with_more_in_them(name, act, act_fn, monkeypatch):
+    """What else a block holds may be part of its forward: the block keeps it, unless act_fn says
+    which activation it is and the rest is no layer."""
+    m = NamedActMLP(name, act)
+    if act_fn is not None:
+        m.act_fn = act_fn
+    registry.auto_patch_fused_mlp(m)
+    m._trainscale_amd_forward = lambda x: x
+    layer = isinstance(act, nn.Module)
+    assert taken(m, fake(), monkeypatch) == ("silu" if act_fn is not None and not layer else None)
+
+
+def test_activation_as_a_method(monkeypatch):
+    m = MethodMLP(dtype=BF)
+    registry.auto_patch_fused_mlp(m)
+    m._trainscale_amd_forward = lambda x: x
+    assert taken(m, fake(), monkeypatch) is None
+
+
+def test_transformers_blocks(monkeypatch):
+    """The registered blocks of the model library are still taken."""
+    pytest.importorskip("transformers")
+    from transformers.models.llama.modeling_llama import LlamaMLP as Theirs
+    for act, name in (("silu", "silu"), ("gelu_pytorch_tanh", "gelu_tanh"), ("tanh", None)):
+        m = Theirs(types.SimpleNamespace(hidden_size=24, intermediate_size=40, mlp_bias=False,
+                                         hidden_act=act)).to(BF)
+        registry.auto_patch_fused_mlp(m)
+        m._trainscale_amd_forward = lambda x: x
+        assert taken(m, fake(), monkeypatch) == name

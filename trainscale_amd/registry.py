@@ -123,12 +123,23 @@ def _watched(layer: nn.Module) -> bool:
                 or layer._backward_hooks or layer._backward_pre_hooks)
 
 
+# a gated block's own children, and other names under which blocks keep an activation
+_MLP_CHILDREN = {"gate_proj", "up_proj", "down_proj", "act_fn", "activation_fn"}
+_ACT_NAMES = ("act", "activation", "activation_function", "hidden_act", "hidden_activation")
+
+
 def _activation_of(module: nn.Module):
-    """The name of a gated block's activation, None where it is another's. Without an attribute it
-    is SiLU, which ``auto_patch_mlp`` puts in every registered block."""
+    """The name of a gated block's activation, None where it is another's or the block holds layers
+    besides its projections and activation. With nothing in it that could be an activation it is
+    SiLU, which ``auto_patch_mlp`` puts in every registered block."""
+    if any(m is not None for name, m in module._modules.items() if name not in _MLP_CHILDREN):
+        return None
     act = getattr(module, "act_fn", getattr(module, "activation_fn", None))
     if act is None:
-        return "silu"
+        other = any(hasattr(module, name) for name in _ACT_NAMES) or any(
+            callable(v) for name, v in vars(module).items()
+            if name != "forward" and not name.startswith("_"))
+        return None if other else "silu"
     if isinstance(act, nn.Module):
         if _watched(act):
             return None
@@ -150,8 +161,9 @@ def _plain_linear(layer) -> bool:
 def auto_patch_fused_mlp(module: nn.Module) -> None:
     """Routes a gate/up/down MLP through ``fused_gated_mlp``. Calls that are not the plain block in
     bf16 or fp16 (a projection with a bias, an adapter or hooks, another activation or one with hooks,
-    fp32, autocast to another type, CPU tensors) keep the module's own forward; what a call is, is
-    looked up at each call, so adapters may come later."""
+    further layers, fp32, autocast to another type, CPU tensors) keep the module's own forward; what
+    a call is, is looked up at each call, so adapters may come later. The activation is ``act_fn`` or
+    ``activation_fn``; a block without either that holds nothing like one is taken as SiLU."""
     if not (hasattr(module, "gate_proj") and hasattr(module, "up_proj")
             and hasattr(module, "down_proj")):
         return
