@@ -217,3 +217,20 @@ def test_transformers_blocks(monkeypatch):
         registry.auto_patch_fused_mlp(m)
         m._trainscale_amd_forward = lambda x: x
         assert taken(m, fake(), monkeypatch) == name
+
+
+@pytest.mark.parametrize("register", ["register_module_forward_hook",
+                                      "register_module_forward_pre_hook",
+                                      "register_module_full_backward_hook",
+                                      "register_module_full_backward_pre_hook"])
+def test_hooks_of_every_module(register, monkeypatch):
+    """Hooks for all modules (counters, profilers) fire for the projections too."""
+    m = LlamaMLP(dtype=BF)
+    registry.auto_patch_fused_mlp(m)
+    m._trainscale_amd_forward = lambda x: x
+    hook = getattr(nn.modules.module, register)(lambda *a: None)
+    try:
+        assert taken(m, fake(), monkeypatch) is None
+    finally:
+        hook.remove()
+    assert taken(m, fake(), monkeypatch) == "silu"

@@ -117,10 +117,16 @@ _ACT_CLASSES = {"SiLUActivation": "silu", "GELUActivation": "gelu", "GELUTanh": 
                 "PytorchGELUTanh": "gelu_tanh"}
 
 
+# hooks of every module, which fire for projections and activations too
+_ALL_HOOKS = [getattr(nn.modules.module, name) for name in (
+    "_global_forward_hooks", "_global_forward_pre_hooks", "_global_backward_hooks",
+    "_global_backward_pre_hooks")]
+
+
 def _watched(layer: nn.Module) -> bool:
     """Whether calling a module does or reports more than its class's forward."""
     return bool("forward" in vars(layer) or layer._forward_hooks or layer._forward_pre_hooks
-                or layer._backward_hooks or layer._backward_pre_hooks)
+                or layer._backward_hooks or layer._backward_pre_hooks or any(_ALL_HOOKS))
 
 
 # a gated block's own children, and other names under which blocks keep an activation
