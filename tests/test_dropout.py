@@ -10,6 +10,7 @@ from philox import bits16, keep_mask, philox
 from trainscale_amd import _lib
 from trainscale_amd.kernels import (FusedDropoutAddRMSNorm, fused_dropout, fused_dropout_add,
                                     fused_dropout_add_rms_layernorm)
+from trainscale_amd.kernels.dropout_kernels import _rng
 
 OK, INVALID, DTYPE, SHAPE, WORKSPACE = 0, -1, -2, -3, -4
 FAKE = 0x1000  # never dereferenced: every call below fails validation
@@ -121,3 +122,14 @@ def test_functions_refuse():
                  lambda: fused_dropout(x.requires_grad_(), 0.5)):
         with pytest.raises(RuntimeError, match="no CPU fallback"):
             call()
+
+
+@pytest.mark.parametrize("device", ["meta", "cpu"])
+def test_seed_is_drawn_on_the_cpu(device):
+    """rng=None draws from torch's CPU generator whatever the default device."""
+    torch.manual_seed(5)
+    want = [_rng("test", None, 100) for _ in range(3)]
+    torch.manual_seed(5)
+    with torch.device(device):
+        assert [_rng("test", None, 100) for _ in range(3)] == want
+    assert len(set(want)) == 3

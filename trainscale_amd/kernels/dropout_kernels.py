@@ -56,7 +56,7 @@ def _rng(what: str, rng: RngLike, drop: int):
         if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{what}: a captured graph would repeat its random numbers; pass "
                                "rng as a device tensor and change it between replays")
-        return (int(torch.empty((), dtype=torch.int64).random_()), 0)
+        return (int(torch.empty((), dtype=torch.int64, device="cpu").random_()), 0)
     if isinstance(rng, Tensor):
         if rng.dtype is not torch.int64 or rng.shape != (2,) or not rng.is_contiguous():
             raise ValueError(f"{what}: rng must be an int64 tensor [2], got {rng.dtype} "
