@@ -271,9 +271,10 @@ ts_status ts_rope_apply(const void* q_in, void* q_out,
  * be its input, and overlaps nothing else. Hq or Hk may be 0.
  * position_ids: device int64, pos[a] of token (b, s) at a * pos_sa + b * pos_sb + s * pos_ss; any
  * values.
- * turns, axis: HOST arrays of R / 2 entries, read before the call returns. turns[i] is
- * f(i) / (2 pi) modulo 1, times 2^64: with integer positions the fraction of a turn that a position
- * makes is all that matters, and its 64-bit product with a position is exact modulo a turn.
+ * turns, turns_rest, axis: HOST arrays of R / 2 entries, read before the call returns. turns[i] is
+ * f(i) / (2 pi) modulo 1, times 2^64, and turns_rest[i] what that leaves, times 2^96 (NULL: zeros):
+ * with integer positions the fraction of a turn that a position makes is all that matters, and its
+ * product with a position is exact modulo a turn. The rest matters to positions past 2^38.
  * backward 1: the transpose rotation, of gradients. R / 2 at most 256, D and heads 4096.
  */
 typedef struct ts_rope_axes_args {
@@ -289,6 +290,7 @@ typedef struct ts_rope_axes_args {
   const uint64_t* turns;
   const int32_t* axis;
   int32_t axes, dtype, interleaved, backward;
+  const int32_t* turns_rest;
 } ts_rope_axes_args;
 
 ts_status ts_rope_axes(const ts_rope_axes_args* args, ts_stream_t stream);

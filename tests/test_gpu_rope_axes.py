@@ -268,3 +268,31 @@ def test_far_elements(gpu):
     assert same(out[1, -40:], want[0]) and not out[0].any() and not out[1, :-40].any()
     apply_rope_axes(q, None, pos, p, inplace=True)
     assert same(q[1, -40:], want[0])
+
+
+def test_any_position(gpu):
+    """Positions out to both ends of int64, against angles in rational arithmetic (2 pi to 200 bits):
+    cos and sin are off by 4 u and 2 pi 2^-33."""
+    import numpy as np
+    from fractions import Fraction
+    inv = Fraction(0x28BE60DB9391054A7F09D5F47D4D377036D8A5664F10E410, 1 << 192)  # 1 / (2 pi)
+    p = RopeAxes((24, 20, 20), layout="interleaved", base=500000.0)
+    base = [1 << 20, 1 << 38, 1 << 40, 1 << 46, -(1 << 52), 1 << 57, 1 << 62, -(1 << 62),
+            (1 << 63) - 1, -(1 << 63)]
+    pos = np.array([[b // (a + 1) + (a if abs(b) < 1 << 62 else 0) for b in base] for a in range(3)],
+                   dtype=np.int64)
+    pos[:, -2:] = base[-2:]
+    turn = [[float(int(pos[a, s]) * Fraction(f) * inv % 1) for a, f in zip(p.axis, p.inv_freq.tolist())]
+            for s in range(len(base))]
+    angle = 2 * math.pi * torch.tensor(turn, dtype=torch.float64, device=gpu)[None, :, None]
+    q, _, _, dq, _ = inputs(gpu, 1, len(base), 3, 0, 128, F32, 3, 11)
+    leaf = q.requires_grad_()
+    out, _ = apply_rope_axes(leaf, None, torch.from_numpy(pos).to(gpu), p)
+    (grad,) = torch.autograd.grad(out, leaf, dq)
+    for got, x, sign in ((out.detach(), q.detach(), 1), (grad, dq, -1)):
+        lo, hi = x.double().chunk(2, -1)
+        c, s = angle.cos(), sign * angle.sin()
+        want = torch.cat((lo * c - hi * s, hi * c + lo * s), -1)
+        mag = (lo.abs() + hi.abs()).repeat(1, 1, 1, 2)
+        bad = ~((got.double() - want).abs() <= (7 * U + 2 * math.pi * 2.0 ** -33) * mag)
+        assert not bad.any(), bad.nonzero()[:3].tolist()

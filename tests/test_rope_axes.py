@@ -10,7 +10,7 @@ import torch
 
 from trainscale_amd import _lib
 from trainscale_amd.kernels import (MultiAxisRotaryEmbedding, RopeAxes, apply_rope_axes)
-from trainscale_amd.kernels.rope_kernels import _axes_positions, _turns
+from trainscale_amd.kernels.rope_kernels import _axes_positions, _turns, _turns_rest
 
 OK, INVALID, DTYPE, SHAPE = 0, -1, -2, -3
 FAKE = 0x1000
@@ -125,3 +125,24 @@ def test_functions_refuse():
         MultiAxisRotaryEmbedding((4, 4))(q, k, pos)
     assert _axes_positions(pos[:, 0], 2, 2, 3).shape == (2, 2, 3)
     assert _axes_positions(pos[:, :1].int(), 2, 2, 3).shape == (2, 2, 3)
+
+
+def test_every_position_is_exact():
+    """The fraction of a turn as the kernel forms it, 64-bit product and rest, at any int64 position:
+    off by 2^63 times half of 2^-96, and 2^-64 for the rest's own rounding."""
+    c = Fraction(inverse_two_pi(256), 1 << 256)
+    plan = RopeAxes((32, 32), base=500000.0)
+    for i, f in enumerate(plan.inv_freq.tolist()):
+        turns, rest = plan._turns_c[i], plan._rest_c[i]
+        for pos in (1, 5000, -1 << 24, (1 << 40) + 17, (1 << 46) - 3, -(1 << 52) - 1, 1 << 62,
+                    (1 << 63) - 1, -1 << 63):
+            got = (pos * turns + (pos * rest >> 32)) % (1 << 64)
+            off = (Fraction(got, 1 << 64) - pos * Fraction(f) * c) % 1
+            assert min(off, 1 - off) <= Fraction(1, 1 << 33), (f, pos)
+
+
+def test_rest_of_a_turn():
+    c = Fraction(inverse_two_pi(256), 1 << 256)
+    for f in (1.0, 0.75, 1e-8, 3.7e-5, -0.2, 12345.678, 0.0, 2.0 ** -70):
+        off = (Fraction(_turns(f), 1 << 64) + Fraction(_turns_rest(f), 1 << 96) - Fraction(f) * c) % 1
+        assert min(off, 1 - off) <= Fraction(1, 1 << 96) and abs(_turns_rest(f)) <= 1 << 31

@@ -69,7 +69,7 @@ class RopeAxesArgs(ctypes.Structure):
                 ("Hq", I64), ("Hk", I64), ("B", I64), ("S", I64), ("D", I64), ("R", I64),
                 ("position_ids", P), ("pos_sa", I64), ("pos_sb", I64), ("pos_ss", I64),
                 ("turns", P), ("axis", P), ("axes", I32), ("dtype", I32), ("interleaved", I32),
-                ("backward", I32)]
+                ("backward", I32), ("turns_rest", P)]
 
 
 class GatedMLPArgs(ctypes.Structure):

@@ -3,10 +3,11 @@
 // them stay as they are. Backward is the transpose: sin negated.
 //
 // Angles. Positions are integers, so only the fraction of a turn that a frequency makes per
-// position matters: turns[i] = f(i) / (2 pi) modulo 1 as a 64-bit fixed-point fraction, formed on
-// the host. pos * turns[i] modulo 2^64, one integer product, is then the angle's fraction of a
-// turn, exact for every 64-bit position of either sign but for the fraction's own rounding (2^-65
-// of a turn per position: 1e-12 rad at position 4 million), with no range reduction. Its nearest
+// position matters: f(i) / (2 pi) modulo 1 as a fixed-point fraction of 96 bits, turns[i] and 32
+// signed bits in rest[i], formed on the host. Its product with the position modulo a turn, to 64 bits,
+// is the angle's fraction of a turn, exact for every 64-bit position of either sign but for 2^-64 of
+// a turn and the fraction's own rounding (2^-97 of a turn per position, 4e-10 rad at 2^63; without
+// the rest 2^-65, more than fp32's rounding from 2^38 on), with no range reduction. Its nearest
 // quarter turn comes off as integers; the rest, within an eighth of a turn, is rounded to fp32
 // once, and sin and cos are Taylor polynomials there (terms past 2e-9 left out). An fp32 product of
 // position and frequency would be off by up to 2^-24 of the angle, 0.06 rad at position 1 million.
@@ -48,6 +49,7 @@ struct AxesArgs {
   int32_t Hq, Hk, half, pairs, tpb;   // pairs: rotating tasks of a head
   int32_t backward;
   uint64_t turns[kMaxHalf];
+  int32_t rest[kMaxHalf];
   uint8_t axis[kMaxHalf];
 };
 
@@ -225,8 +227,9 @@ __global__ __launch_bounds__(kMaxThreads) void rope_axes_kernel(const AxesArgs a
     const int p = idx - i * a.half;
     const int64_t t = tok0 + i, b = batch_of(t), s = t - b * a.S;
     const int64_t pos = a.pos[a.axis[p] * a.pos_sa + b * a.pos_sb + s * a.pos_ss];
+    const int64_t rest = __mul64hi(pos, (int64_t)a.rest[p] * ((int64_t)1 << 32));
     float c, w;
-    turn_cos_sin((uint64_t)pos * a.turns[p], c, w);
+    turn_cos_sin((uint64_t)pos * a.turns[p] + (uint64_t)rest, c, w);
     cs[idx] = c;
     sn[idx] = a.backward ? -w : w;
   }
@@ -336,6 +339,7 @@ extern "C" ts_status ts_rope_axes(const ts_rope_axes_args* p, ts_stream_t stream
   a.backward = p->backward;
   for (int i = 0; i < a.half; ++i) {
     a.turns[i] = p->turns[i];
+    a.rest[i] = p->turns_rest != nullptr ? p->turns_rest[i] : 0;
     a.axis[i] = (uint8_t)p->axis[i];
   }
   // in place, the elements that stay need no copy

@@ -432,6 +432,13 @@ def _turns(freq: float) -> int:
     return ((num * _INV_2PI_192 >> 127) // den + 1 >> 1) & (1 << 64) - 1
 
 
+def _turns_rest(freq: float) -> int:
+    """What _turns leaves of freq / (2 pi) modulo 1, in units of 2^-96."""
+    num, den = freq.as_integer_ratio()
+    rest = ((num * _INV_2PI_192 >> 95) // den + 1 >> 1) - (_turns(freq) << 32)
+    return min((rest + (1 << 31) & (1 << 96) - 1) - (1 << 31), (1 << 31) - 1)
+
+
 class RopeAxes:
     """How the pairs of a rotary embedding are shared out among position axes, and their
     frequencies: the plan that ``apply_rope_axes`` takes, made once.
@@ -450,7 +457,8 @@ class RopeAxes:
     elements instead of halves.
     """
 
-    __slots__ = ("sections", "layout", "interleaved", "inv_freq", "axis", "_turns_c", "_axis_c")
+    __slots__ = ("sections", "layout", "interleaved", "inv_freq", "axis", "_turns_c", "_rest_c",
+                 "_axis_c")
 
     def __init__(self, sections, layout: str = "blocks", base: float = 10000.0,
                  inv_freq: Optional[Tensor] = None, interleaved: bool = False):
@@ -479,6 +487,7 @@ class RopeAxes:
         self.interleaved = bool(interleaved)
         self.inv_freq = inv_freq
         self._turns_c = (ctypes.c_uint64 * n)(*[_turns(f) for f in inv_freq.tolist()])
+        self._rest_c = (ctypes.c_int32 * n)(*[_turns_rest(f) for f in inv_freq.tolist()])
         self._axis_c = (ctypes.c_int32 * n)(*self.axis)
 
     def __repr__(self) -> str:
@@ -521,7 +530,7 @@ def _rope_axes(plan: RopeAxes, pos: Tensor, q: Optional[Tensor], k: Optional[Ten
         outs = [t if t is None else torch.empty(*t.shape, dtype=t.dtype, device=t.device)
                 for t in (q, k)]
     if q is not None or k is not None:
-        ops.rope_axes(q, outs[0], k, outs[1], pos, plan._turns_c, plan._axis_c,
+        ops.rope_axes(q, outs[0], k, outs[1], pos, plan._turns_c, plan._rest_c, plan._axis_c,
                       len(plan.sections), 2 * len(plan.axis), plan.interleaved, backward)
     return outs[0], outs[1]
 

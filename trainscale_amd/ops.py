@@ -338,11 +338,11 @@ def rope_apply(q_in: Optional[Tensor], q_out: Optional[Tensor],
 
 
 def rope_axes(q_in: Optional[Tensor], q_out: Optional[Tensor], k_in: Optional[Tensor],
-              k_out: Optional[Tensor], position_ids: Tensor, turns, axis, axes: int, rotary: int,
-              interleaved: bool, backward: bool = False) -> None:
+              k_out: Optional[Tensor], position_ids: Tensor, turns, rest, axis, axes: int,
+              rotary: int, interleaved: bool, backward: bool = False) -> None:
     """Rotates q_in -> q_out and k_in -> k_out ([B, S, H, D], unit last stride; either pair may be
-    None; in == out is in place) at position_ids [axes, B, S] (int64, any strides). turns and axis
-    are ctypes arrays of rotary / 2 entries (ts_rope_axes)."""
+    None; in == out is in place) at position_ids [axes, B, S] (int64, any strides). turns, rest
+    and axis are ctypes arrays of rotary / 2 entries (ts_rope_axes)."""
     ref = q_in if q_in is not None else k_in
     dev = _lib.require_gpu("rope_axes", q_in, q_out, k_in, k_out, position_ids)
     B, S, _, D = ref.shape
@@ -358,7 +358,7 @@ def rope_axes(q_in: Optional[Tensor], q_out: Optional[Tensor], k_in: Optional[Te
         *side(q_in, q_out), *side(k_in, k_out), 0 if q_in is None else q_in.shape[2],
         0 if k_in is None else k_in.shape[2], B, S, D, rotary, position_ids.data_ptr(), sp[0],
         sp[1], sp[2], ctypes.addressof(turns), ctypes.addressof(axis), axes,
-        _lib.dtype_code(ref, "rope_axes"), interleaved, backward)
+        _lib.dtype_code(ref, "rope_axes"), interleaved, backward, ctypes.addressof(rest))
     with _lib.on_device(dev):
         check(_lib.load().ts_rope_axes(ctypes.byref(args), _lib.stream_handle(dev)),
               "ts_rope_axes")
