@@ -699,7 +699,8 @@ ts_status ts_gated_mlp_fwd(const ts_gated_mlp_args* args, float* keep_p, float* 
 /*
  * Gradients from dout ([N, O], or [N, F] without w_down, row stride ld_dout) and what the forward
  * kept, each contiguous in dtype and skipped where NULL: dx [N, H], dw_gate and dw_up [F, H],
- * dw_down [O, F]. The gradients of g and u are rounded to dtype between the products. N > 0.
+ * dw_down [O, F]. The gradients of g and u are rounded to dtype between the products. The first
+ * three read keep_p and keep_q, dw_down reads act; what none asked for reads may be NULL. N > 0.
  */
 ts_status ts_gated_mlp_bwd(const ts_gated_mlp_args* args, const float* keep_p,
                            const float* keep_q, const void* act, const void* dout,

@@ -132,3 +132,14 @@ def test_module():
         "gate_proj.weight": (56, 24), "up_proj.weight": (56, 24), "down_proj.weight": (24, 56)}
     with pytest.raises(ValueError, match="activation"):
         FusedGatedMLP(24, 56, "tanh")
+
+
+def test_operands_of_gradients_not_asked_for():
+    """What only skipped gradients would read may be NULL (no workspace: refused before a launch)."""
+    assert bwd(args(), act=None, dwd=None, wsb=0) == WORKSPACE
+    assert bwd(args(), gate=None, up=None, dx=None, dwg=None, dwu=None, wsb=0) == WORKSPACE
+    for k in ("dx", "dwg", "dwu"):
+        others = {n: None for n in ("dx", "dwg", "dwu", "dwd") if n != k}
+        assert bwd(args(), gate=None, **others) == INVALID
+        assert bwd(args(), up=None, **others) == INVALID
+        assert bwd(args(), act=None, wsb=0, **others) == WORKSPACE

@@ -424,3 +424,24 @@ def test_far_elements(gpu):
     assert not got["dx"][32:-32].any()
     for k in ("dwg", "dwu"):  # the other rows add exact zeros
         check(got[k], want[k], bound[k], k)
+
+
+@pytest.mark.parametrize("down", [True, False])
+def test_keeps_what_the_gradients_read(gpu, down):
+    """The fp32 factors are kept for gradients of x, gate and up, the gated product for down's."""
+    n, h, f = 200, 64, 136
+    args = inputs(gpu, n, h, f, 72 if down else 0, BF, 6)
+    ref = run(args, "silu")
+    given = {t.data_ptr() for t in args[:4] if t is not None}
+    for wanted in range(1, 16 if down else 8):
+        leaf = [t.detach().requires_grad_(bool(wanted >> i & 1)) if t is not None else None
+                for i, t in enumerate(args[:4])]
+        kept = []
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: kept.append(t) or t, lambda t: t):
+            y = (fused_gated_mlp(*leaf) if down else fused_gated_linear(*leaf[:3]))
+        new = [t for t in kept if t.data_ptr() not in given]
+        assert sum(t.numel() * t.element_size() for t in new) == \
+            (8 * n * f if wanted & 7 else 0) + (2 * n * f if wanted & 8 else 0), wanted
+        need = [i for i in range(4) if wanted >> i & 1]
+        for g, i in zip(torch.autograd.grad(y, [leaf[i] for i in need], args[4]), need):
+            assert same(g, ref[("dx", "dwg", "dwu", "dwd")[i]]), (wanted, i)

@@ -822,7 +822,9 @@ extern "C" ts_status ts_gated_mlp_bwd(const ts_gated_mlp_args* args, const float
   TS_TRY(check_args("gated_mlp_bwd", args));
   if (args->N == 0) return fail(TS_ERR_SHAPE, "gated_mlp_bwd: no rows (the gradients are zeros)");
   const bool down = args->w_down != nullptr;
-  if (keep_p == nullptr || keep_q == nullptr || dout == nullptr || (down && act == nullptr))
+  const bool inner = dx != nullptr || dw_gate != nullptr || dw_up != nullptr;
+  if ((inner && (keep_p == nullptr || keep_q == nullptr)) || dout == nullptr ||
+      (dw_down != nullptr && act == nullptr))
     return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_bwd: NULL operand");
   if (!down && dw_down != nullptr)
     return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_bwd: dw_down without w_down");

@@ -6,9 +6,10 @@ projection. Weights have ``nn.Linear``'s layout. bf16 and fp16; the sums are fp3
 between the products (the gated product forward, the gradients of both projections backward) is
 rounded to the data type once, where the unfused block rounds g, u, act(g) and the product.
 
-Where a gradient will follow, the forward keeps x, the weights, the gated product and the two
-factors of the backward in fp32 (up * act'(gate) and act(gate)): 10 N F bytes, so that no rounding
-of the projections adds to the gradients'. Otherwise only the gated product is formed.
+Where gradients of x, gate or up will follow, the forward keeps the two factors of the backward in
+fp32 (up * act'(gate) and act(gate), 8 N F bytes), so that no rounding of the projections adds to the
+gradients'; for down's it keeps the gated product (2 N F); beside them x and the weights. Otherwise
+only the gated product is formed.
 """
 from __future__ import annotations
 
@@ -72,8 +73,9 @@ class GatedMLPFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor],
                 activation: str) -> Tensor:
-        out, ctx.code, factors, act = _forward(x, gate, up, down, activation, True)
-        ctx.save_for_backward(x, gate, up, down, factors, None if down is None else act)
+        needs = ctx.needs_input_grad
+        out, ctx.code, factors, act = _forward(x, gate, up, down, activation, any(needs[:3]))
+        ctx.save_for_backward(x, gate, up, down, factors, act if needs[3] else None)
         return out
 
     @staticmethod

@@ -755,9 +755,10 @@ def gated_mlp_forward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Tens
 
 
 def gated_mlp_backward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Tensor], code: int,
-                       factors: Tensor, act: Optional[Tensor], dout: Tensor, needs) -> list:
-    """Gradients of (x2d, gate, up, down), None where `needs` is false; factors and act are the
-    forward's."""
+                       factors: Optional[Tensor], act: Optional[Tensor], dout: Tensor,
+                       needs) -> list:
+    """Gradients of (x2d, gate, up, down), None where `needs` is false; factors (for the first three)
+    and act (for down's) are the forward's."""
     dev = _lib.require_gpu("gated_mlp", x2d, gate, up, down, factors, act, dout)
     n = x2d.shape[0]
     leaves = (x2d, gate, up, down)
@@ -769,14 +770,14 @@ def gated_mlp_backward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Ten
     shapes = ((n, args.H), (args.F, args.H), (args.F, args.H), (args.O, args.F))
     out = [torch.empty(*s, dtype=x2d.dtype, device=dev) if k else None
            for s, k in zip(shapes, needs)]
-    factors = factors.contiguous()
-    act = None if act is None else act.contiguous()
-    at, step = factors.data_ptr(), 4 * n * args.F
+    factors, act = [None if t is None else t.contiguous() for t in (factors, act)]
+    p = 0 if factors is None else factors.data_ptr()
+    q = p + 4 * n * args.F if p else 0
     lib = _lib.load()
     wsb = lib.ts_gated_mlp_bwd_workspace_size(n, args.H, args.F, args.O)
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
     with _lib.on_device(dev):
-        check(lib.ts_gated_mlp_bwd(ctypes.byref(args), at, at + step,
+        check(lib.ts_gated_mlp_bwd(ctypes.byref(args), p, q,
                                    0 if act is None else act.data_ptr(), d, ldd,
                                    *[0 if t is None else t.data_ptr() for t in out],
                                    ws.data_ptr(), wsb, _lib.stream_handle(dev)),
