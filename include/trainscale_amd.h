@@ -680,9 +680,17 @@ typedef struct ts_gated_mlp_args {
   int32_t dtype;
 } ts_gated_mlp_args;
 
-/* Bytes of workspace (O = 0 without w_down); the forward's may be 0. 16-byte aligned. */
+/* Gradients that a backward is asked for. */
+enum { TS_MLP_DX = 1, TS_MLP_DW_GATE = 2, TS_MLP_DW_UP = 4, TS_MLP_DW_DOWN = 8 };
+
+/*
+ * Bytes of workspace (O = 0 without w_down), 16-byte aligned; may be 0. The backward's first is
+ * enough whichever gradients are asked for, the second for those of `grads` (TS_MLP_D*, summed).
+ */
 size_t ts_gated_mlp_fwd_workspace_size(int64_t N, int64_t H, int64_t F, int64_t O);
 size_t ts_gated_mlp_bwd_workspace_size(int64_t N, int64_t H, int64_t F, int64_t O);
+size_t ts_gated_mlp_bwd_grads_workspace_size(int64_t N, int64_t H, int64_t F, int64_t O,
+                                             int32_t grads);
 
 /*
  * g = x w_gate^T, u = x w_up^T, act = activation(g) * u, out = act w_down^T: fp32 sums, act and
@@ -700,7 +708,8 @@ ts_status ts_gated_mlp_fwd(const ts_gated_mlp_args* args, float* keep_p, float* 
  * Gradients from dout ([N, O], or [N, F] without w_down, row stride ld_dout) and what the forward
  * kept, each contiguous in dtype and skipped where NULL: dx [N, H], dw_gate and dw_up [F, H],
  * dw_down [O, F]. The gradients of g and u are rounded to dtype between the products. The first
- * three read keep_p and keep_q, dw_down reads act; what none asked for reads may be NULL. N > 0.
+ * three read keep_p and keep_q, dw_down reads act; what none asked for reads may be NULL. The order
+ * of the sums follows from the shape and from which gradients are asked for. N > 0.
  */
 ts_status ts_gated_mlp_bwd(const ts_gated_mlp_args* args, const float* keep_p,
                            const float* keep_q, const void* act, const void* dout,

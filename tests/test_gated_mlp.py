@@ -137,9 +137,28 @@ def test_module():
 def test_operands_of_gradients_not_asked_for():
     """What only skipped gradients would read may be NULL (no workspace: refused before a launch)."""
     assert bwd(args(), act=None, dwd=None, wsb=0) == WORKSPACE
-    assert bwd(args(), gate=None, up=None, dx=None, dwg=None, dwu=None, wsb=0) == WORKSPACE
+    down = dict(gate=None, up=None, dx=None, dwg=None, dwu=None)
+    assert bwd(args(N=4096), wsb=0, **down) == WORKSPACE  # sums of K slots
     for k in ("dx", "dwg", "dwu"):
         others = {n: None for n in ("dx", "dwg", "dwu", "dwd") if n != k}
         assert bwd(args(), gate=None, **others) == INVALID
         assert bwd(args(), up=None, **others) == INVALID
         assert bwd(args(), act=None, wsb=0, **others) == WORKSPACE
+
+
+def test_workspace_of_gradients_not_asked_for():
+    """Frozen weights: no room for sums of their gradients; the one size for all is enough for each."""
+    lib = _lib.load()
+    size, some = lib.ts_gated_mlp_bwd_workspace_size, lib.ts_gated_mlp_bwd_grads_workspace_size
+    for n, h, f, o in ((300, 2048, 5632, 2048), (2045, 768, 2048, 768), (2048, 4096, 14336, 4096),
+                       (64, 4096, 14336, 4096), (1000, 96, 200, 0), (8192, 4096, 14336, 4096)):
+        most = [some(n, h, f, o, g) for g in range(1, 16)]
+        assert size(n, h, f, o) == max(most) and some(n, h, f, o, 0) == 0
+        dg = 2 * ((2 * n * f + 255) // 256 * 256)
+        assert dg <= some(n, h, f, o, 1) <= dg + 16 * n * h * 4 + 1024
+        assert some(n, h, f, o, 8) <= 8 * o * f * 4 + 256  # no dg, du
+    assert some(0, 64, 64, 64, 15) == some(4, 64, 64, -1, 15) == 0
+    need = some(2045, 768, 2048, 768, 1)
+    a = args(N=2045, H=768, F=2048, O=768, ldx=768, ld_gate=768, ld_up=768, ld_down=2048)
+    others = dict(dwg=None, dwu=None, dwd=None, ldd=768)
+    assert bwd(a, wsb=need - 1, **others) == WORKSPACE

@@ -445,3 +445,19 @@ def test_keeps_what_the_gradients_read(gpu, down):
         need = [i for i in range(4) if wanted >> i & 1]
         for g, i in zip(torch.autograd.grad(y, [leaf[i] for i in need], args[4]), need):
             assert same(g, ref[("dx", "dwg", "dwu", "dwd")[i]]), (wanted, i)
+
+
+@pytest.mark.parametrize("wanted", [1, 6, 8, 9, 14])
+@pytest.mark.parametrize("n,h,f,o", [(256, 2048, 5632, 2048), (1000, 768, 2048, 264),
+                                     (2045, 768, 2048, 768), (130, 4096, 1032, 8)])
+def test_plans_of_some_gradients(gpu, n, h, f, o, wanted):
+    """Frozen operands: the others' gradients, on tiles and K slots of their own."""
+    args = inputs(gpu, n, h, f, o, BF, n)
+    want, bound = reference(*args[:4], "silu", args[4])
+    leaf = [t.detach().requires_grad_(bool(wanted >> i & 1)) for i, t in enumerate(args[:4])]
+    names = [k for i, k in enumerate(("dx", "dwg", "dwu", "dwd")) if wanted >> i & 1]
+    need = [t for t in leaf if t.requires_grad]
+    runs = [torch.autograd.grad(fused_gated_mlp(*leaf), need, args[4]) for _ in range(2)]
+    for k, g, again in zip(names, *runs):
+        check(g, want[k], bound[k], k)
+        assert same(g, again), k

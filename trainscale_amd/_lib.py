@@ -152,6 +152,7 @@ SIGNATURES = {
     "ts_rescale_inplace": ([P, I64, I32, P, P, P, P], I32),
     "ts_gated_mlp_fwd_workspace_size": ([I64, I64, I64, I64], SZ),
     "ts_gated_mlp_bwd_workspace_size": ([I64, I64, I64, I64], SZ),
+    "ts_gated_mlp_bwd_grads_workspace_size": ([I64, I64, I64, I64, I32], SZ),
     "ts_gated_mlp_fwd": ([P, P, P, P, P, P, SZ, P], I32),
     "ts_gated_mlp_bwd": ([P, P, P, P, P, I64, P, P, P, P, P, SZ, P], I32),
     "ts_pad_matrices": ([P, I32, I32, P], I32),

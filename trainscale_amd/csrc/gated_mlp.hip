@@ -557,6 +557,10 @@ ts_plan::MlpShape shape_of(const ts_gated_mlp_args& a) {
   return ts_plan::MlpShape{a.N, a.H, a.F, a.w_down != nullptr ? a.O : 0};
 }
 
+static_assert(TS_MLP_DX == ts_plan::kMlpDx && TS_MLP_DW_GATE == ts_plan::kMlpDwGate &&
+              TS_MLP_DW_UP == ts_plan::kMlpDwUp && TS_MLP_DW_DOWN == ts_plan::kMlpDwDown,
+              "the plan's gradients");
+
 constexpr int64_t kMaxDim = (int64_t)1 << 21;  // 32-bit offsets inside a tile
 
 ts_status check_args(const char* who, const ts_gated_mlp_args* a) {
@@ -782,10 +786,21 @@ extern "C" size_t ts_gated_mlp_fwd_workspace_size(int64_t N, int64_t H, int64_t 
   return (size_t)ts_plan::mlp_fwd_workspace(s, ts_plan::mlp_fwd_plan(s));
 }
 
-extern "C" size_t ts_gated_mlp_bwd_workspace_size(int64_t N, int64_t H, int64_t F, int64_t O) {
-  if (N <= 0 || H <= 0 || F <= 0 || O < 0) return 0;
+extern "C" size_t ts_gated_mlp_bwd_grads_workspace_size(int64_t N, int64_t H, int64_t F, int64_t O,
+                                                        int32_t grads) {
+  grads &= ts_plan::kMlpGrads;
+  if (N <= 0 || H <= 0 || F <= 0 || O < 0 || grads == 0) return 0;
   const ts_plan::MlpShape s{N, H, F, O};
-  return (size_t)ts_plan::mlp_bwd_workspace(s, ts_plan::mlp_bwd_plan(s)).total;
+  return (size_t)ts_plan::mlp_bwd_workspace(s, ts_plan::mlp_bwd_plan(s, grads), grads).total;
+}
+
+extern "C" size_t ts_gated_mlp_bwd_workspace_size(int64_t N, int64_t H, int64_t F, int64_t O) {
+  size_t most = 0;
+  for (int32_t grads = 1; grads <= ts_plan::kMlpGrads; ++grads) {
+    const size_t n = ts_gated_mlp_bwd_grads_workspace_size(N, H, F, O, grads);
+    if (n > most) most = n;
+  }
+  return most;
 }
 
 extern "C" ts_status ts_gated_mlp_fwd(const ts_gated_mlp_args* args, float* keep_p,
@@ -835,11 +850,15 @@ extern "C" ts_status ts_gated_mlp_bwd(const ts_gated_mlp_args* args, const float
                         (const void*)dw_up, (const void*)dw_down, (const void*)workspace})
     if (!ts_host::aligned16(p))
       return fail(TS_ERR_INVALID_ARGUMENT, "gated_mlp_bwd: buffers must be 16-byte aligned");
+  const int grads = (dx != nullptr ? TS_MLP_DX : 0) | (dw_gate != nullptr ? TS_MLP_DW_GATE : 0) |
+                    (dw_up != nullptr ? TS_MLP_DW_UP : 0) |
+                    (dw_down != nullptr ? TS_MLP_DW_DOWN : 0);
+  if (grads == 0) return TS_OK;
   const ts_plan::MlpShape s = shape_of(*args);
-  const ts_plan::MlpBwdPlan pl = ts_plan::mlp_bwd_plan(s);
-  const ts_plan::MlpBwdWorkspace w = ts_plan::mlp_bwd_workspace(s, pl);
+  const ts_plan::MlpBwdPlan pl = ts_plan::mlp_bwd_plan(s, grads);
+  const ts_plan::MlpBwdWorkspace w = ts_plan::mlp_bwd_workspace(s, pl, grads);
   const size_t need = (size_t)w.total;
-  if (workspace == nullptr || workspace_bytes < need)
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need))
     return fail(TS_ERR_WORKSPACE, "gated_mlp_bwd: workspace of %zu bytes, need %zu",
                 workspace_bytes, need);
   hipStream_t st = static_cast<hipStream_t>(stream);

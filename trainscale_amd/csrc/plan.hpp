@@ -412,8 +412,13 @@ struct MlpFwdPlan {
 };
 struct MlpBwdPlan {
   int da_waves, grad_waves;
-  KSplit dx, dw;  // dw: of all three weights
+  KSplit dx, dw;  // dw: of every weight's gradient
 };
+// Gradients asked for, as bits; dx and the weights' share a grid, so its plan depends on which. dx
+// alone, on the plan for all of them and on its own, whole backward at H 4096, F 14336: 300 rows 240
+// and 209 us, 1024 rows 443 and 351, 2048 rows 815 and 655.
+constexpr int kMlpDx = 1, kMlpDwGate = 2, kMlpDwUp = 4, kMlpDwDown = 8;
+constexpr int kMlpInner = kMlpDx | kMlpDwGate | kMlpDwUp, kMlpGrads = kMlpInner | kMlpDwDown;
 
 // Which tiles, and how many slots K is cut into, by an estimate of the time in microseconds (the
 // host's choice follows from the shape alone, so a shape's sums keep their order). Fitted to
@@ -496,32 +501,34 @@ inline MlpFwdPlan mlp_fwd_plan(const MlpShape& s) {
   }
   return p;
 }
-inline MlpBwdPlan mlp_bwd_plan(const MlpShape& s) {
+inline MlpBwdPlan mlp_bwd_plan(const MlpShape& s, int grads = kMlpGrads) {
   const KSplit one{1, 0};
   MlpBwdPlan p{s.O > 0 ? mlp_gated_waves(s.N, s.F, s.O, false) : 8, 8, one, one};
   // dx [N, H] over 2 F, then dWg and dWu [F, H] and dWd [O, F] over N, in one grid
+  const bool dx = grads & kMlpDx, down = (grads & kMlpDwDown) != 0 && s.O > 0;
+  const int inner = ((grads & kMlpDwGate) != 0) + ((grads & kMlpDwUp) != 0);
   double best = 1e30;
   const int64_t kx = mlp_kblocks(2 * s.F), kw = mlp_kblocks(s.N);
   for (int waves = 8; waves >= 4; waves -= 4) {
-    const int64_t tx = mlp_tiles(s.N, s.H, waves, false);
-    const int64_t tw = 2 * mlp_tiles(s.F, s.H, waves, false) +
-                       (s.O > 0 ? mlp_tiles(s.O, s.F, waves, false) : 0);
-    for (int64_t x = 1; x <= 16; x *= 2) {
+    const int64_t tx = dx ? mlp_tiles(s.N, s.H, waves, false) : 0;
+    const int64_t tw = inner * mlp_tiles(s.F, s.H, waves, false) +
+                       (down ? mlp_tiles(s.O, s.F, waves, false) : 0);
+    for (int64_t x = 1; x <= (dx ? 16 : 1); x *= 2) {
       if (!mlp_slots_ok(x, s.N, s.H, 2 * s.F)) break;
-      for (int64_t w = 1; w <= 8; w *= 2) {
-        if (!mlp_slots_ok(w, s.F, s.H, s.N) ||
-            (s.O > 0 && !mlp_slots_ok(w, s.O, s.F, s.N)))
+      for (int64_t w = 1; w <= (tw > 0 ? 8 : 1); w *= 2) {
+        if ((inner > 0 && !mlp_slots_ok(w, s.F, s.H, s.N)) ||
+            (down && !mlp_slots_ok(w, s.O, s.F, s.N)))
           break;
         const double ax = (double)((kx + x - 1) / x), aw = (double)((kw + w - 1) / w);
         const double work = ((double)(tx * x) * ax + (double)(tw * w) * aw) / (2.0 * kCus);
-        const double longest = ax > aw ? ax : aw;
+        const double longest = tw == 0 || (tx > 0 && ax > aw) ? ax : aw;
         // 256 x 256 tiles take a CU each, in turn; of 128 x 128 tiles two share one, the longest
         // going on alone at the end
         double t = waves == 8 ? (tx * x + tw * w <= kCus ? 1.35 : 1.45) *
                                     mlp_makespan(tx * x, ax, tw * w, aw, kCus)
                               : (work > 0.6 * longest ? work : 0.6 * longest);
-        t += mlp_slots_time(x, s.N, s.H) + 2 * mlp_slots_time(w, s.F, s.H) +
-             mlp_slots_time(w, s.O, s.F);
+        t += mlp_slots_time(x, s.N, s.H) + inner * mlp_slots_time(w, s.F, s.H) +
+             (down ? mlp_slots_time(w, s.O, s.F) : 0.0);
         if (x > 1 || w > 1) t += kMlpSumLaunch;
         if (t >= best) continue;
         best = t;
@@ -539,24 +546,25 @@ inline int64_t mlp_part_bytes(const KSplit& k, int64_t M, int64_t N) {
 inline int64_t mlp_fwd_workspace(const MlpShape& s, const MlpFwdPlan& p) {
   return s.O > 0 && s.N > kMlpFewRows ? mlp_part_bytes(p.down, s.N, s.O) : 0;
 }
-// Byte offsets in the backward's workspace: dg and du, then the partials.
+// Byte offsets in the backward's workspace: dg and du, then the partials, of what is asked for.
 struct MlpBwdWorkspace {
   int64_t dg, du, dx, dw[3], total;
 };
-inline MlpBwdWorkspace mlp_bwd_workspace(const MlpShape& s, const MlpBwdPlan& p) {
+inline MlpBwdWorkspace mlp_bwd_workspace(const MlpShape& s, const MlpBwdPlan& p,
+                                         int grads = kMlpGrads) {
   MlpBwdWorkspace w{};
   int64_t off = 0;
-  auto take = [&](int64_t bytes) {
+  auto take = [&](int for_grads, int64_t bytes) {
     const int64_t o = off;
-    off += (bytes + 255) / 256 * 256;
+    if (grads & for_grads) off += (bytes + 255) / 256 * 256;
     return o;
   };
-  w.dg = take(2 * s.N * s.F);
-  w.du = take(2 * s.N * s.F);
-  w.dx = take(mlp_part_bytes(p.dx, s.N, s.H));
-  w.dw[0] = take(mlp_part_bytes(p.dw, s.F, s.H));
-  w.dw[1] = take(mlp_part_bytes(p.dw, s.F, s.H));
-  w.dw[2] = take(s.O > 0 ? mlp_part_bytes(p.dw, s.O, s.F) : 0);
+  w.dg = take(kMlpInner, 2 * s.N * s.F);
+  w.du = take(kMlpInner, 2 * s.N * s.F);
+  w.dx = take(kMlpDx, mlp_part_bytes(p.dx, s.N, s.H));
+  w.dw[0] = take(kMlpDwGate, mlp_part_bytes(p.dw, s.F, s.H));
+  w.dw[1] = take(kMlpDwUp, mlp_part_bytes(p.dw, s.F, s.H));
+  w.dw[2] = take(kMlpDwDown, s.O > 0 ? mlp_part_bytes(p.dw, s.O, s.F) : 0);
   w.total = off;
   return w;
 }

@@ -774,7 +774,8 @@ def gated_mlp_backward(x2d: Tensor, gate: Tensor, up: Tensor, down: Optional[Ten
     p = 0 if factors is None else factors.data_ptr()
     q = p + 4 * n * args.F if p else 0
     lib = _lib.load()
-    wsb = lib.ts_gated_mlp_bwd_workspace_size(n, args.H, args.F, args.O)
+    wsb = lib.ts_gated_mlp_bwd_grads_workspace_size(n, args.H, args.F, args.O,
+                                                    sum(k << i for i, k in enumerate(needs)))
     ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
     with _lib.on_device(dev):
         check(lib.ts_gated_mlp_bwd(ctypes.byref(args), p, q,
