@@ -162,3 +162,42 @@ def test_workspace_of_gradients_not_asked_for():
     a = args(N=2045, H=768, F=2048, O=768, ldx=768, ld_gate=768, ld_up=768, ld_down=2048)
     others = dict(dwg=None, dwu=None, dwd=None, ldd=768)
     assert bwd(a, wsb=need - 1, **others) == WORKSPACE
+
+
+def test_module_refuses_projections_that_are_more_than_their_weight():
+    """The module multiplies by its projections' weights; what else a projection has come to do
+    would be lost."""
+    nn = torch.nn
+
+    class Adapter(nn.Module):  # around a linear layer, its weight in reach
+        def __init__(self, base):
+            super().__init__()
+            self.base, self.weight, self.bias = base, base.weight, None
+
+        def forward(self, t):
+            return self.base(t) + t.sum()
+
+    class Other(nn.Linear):
+        def forward(self, t):
+            return 2 * super().forward(t)
+
+    def own_forward(m):
+        m.up_proj.forward = lambda t: t
+
+    changes = [lambda m: setattr(m, "gate_proj", Adapter(m.gate_proj)), own_forward,
+               lambda m: setattr(m, "down_proj", nn.Linear(56, 24, dtype=BF)),
+               lambda m: setattr(m, "up_proj", Other(24, 56, bias=False, dtype=BF)),
+               lambda m: m.gate_proj.register_forward_hook(lambda *a: None),
+               lambda m: m.down_proj.register_forward_pre_hook(lambda *a: None),
+               lambda m: m.up_proj.register_full_backward_hook(lambda *a: None)]
+    for change in changes:
+        m = FusedGatedMLP(24, 56, dtype=BF)
+        change(m)
+        with pytest.raises(ValueError, match="FusedGatedMLP: (gate|up|down)_proj"):
+            m(torch.zeros(2, 24, dtype=BF))
+    # a weight that is computed is a weight all the same
+    m = FusedGatedMLP(24, 56, dtype=BF)
+    nn.utils.parametrizations.weight_norm(m.up_proj)
+    for plain in (m, FusedGatedMLP(24, 56, dtype=BF)):
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            plain(torch.zeros(2, 24, dtype=BF))

@@ -115,9 +115,16 @@ def fused_gated_mlp(x: Tensor, gate: Tensor, up: Tensor, down: Tensor,
     return _apply(x, gate, up, down, activation)
 
 
+def watched(layer: nn.Module) -> bool:
+    """Whether calling this module does or reports more than its class's forward."""
+    return bool("forward" in vars(layer) or layer._forward_hooks or layer._forward_pre_hooks
+                or layer._backward_hooks or layer._backward_pre_hooks)
+
+
 class FusedGatedMLP(nn.Module):
     """A gated feed-forward block on ``fused_gated_mlp`` with the weights of three bias-free
-    ``nn.Linear`` layers, under their usual names and with their initialisation."""
+    ``nn.Linear`` layers, under their usual names and with their initialisation. The layers are not
+    called: one that is more than its weight's product (an adapter, a bias, a hook) is refused."""
 
     def __init__(self, hidden_size: int, intermediate_size: int, activation: str = "silu",
                  device: Optional[torch.device] = None, dtype: Optional[torch.dtype] = None):
@@ -136,8 +143,13 @@ class FusedGatedMLP(nn.Module):
         self.down_proj = linear(intermediate_size, hidden_size)
 
     def forward(self, x: Tensor) -> Tensor:
-        return fused_gated_mlp(x, self.gate_proj.weight, self.up_proj.weight,
-                               self.down_proj.weight, self.activation)
+        layers = (self.gate_proj, self.up_proj, self.down_proj)
+        for name, layer in zip(("gate_proj", "up_proj", "down_proj"), layers):
+            if (not isinstance(layer, nn.Linear) or type(layer).forward is not nn.Linear.forward
+                    or layer.bias is not None or watched(layer)):
+                raise ValueError(f"FusedGatedMLP: {name} is more than a product with its weight "
+                                 "(an adapter, a bias or hooks), which would be lost")
+        return fused_gated_mlp(x, *[layer.weight for layer in layers], self.activation)
 
     def extra_repr(self) -> str:
         return f"{self.hidden_size}, {self.intermediate_size}, activation={self.activation!r}"

@@ -30,7 +30,7 @@ import types
 
 from .kernels.embedding_kernels import scaled_embedding
 from .kernels.fused_kernels import fast_rms_layernorm, swiglu_forward
-from .kernels.mlp_kernels import fused_gated_mlp
+from .kernels.mlp_kernels import fused_gated_mlp, watched
 from .kernels.rope_kernels import RoPEConfig, RoPEScalingType, hf_apply_rotary_pos_emb
 
 __all__ = ["LAYER_PATCHES", "NORMS_WITH_OTHER_MATH", "register_layer_patch", "auto_patch_layernorm", "auto_patch_mlp",
@@ -125,8 +125,7 @@ _ALL_HOOKS = [getattr(nn.modules.module, name) for name in (
 
 def _watched(layer: nn.Module) -> bool:
     """Whether calling a module does or reports more than its class's forward."""
-    return bool("forward" in vars(layer) or layer._forward_hooks or layer._forward_pre_hooks
-                or layer._backward_hooks or layer._backward_pre_hooks or any(_ALL_HOOKS))
+    return watched(layer) or any(_ALL_HOOKS)
 
 
 # a gated block's own children, and other names under which blocks keep an activation
