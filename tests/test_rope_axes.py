@@ -10,7 +10,7 @@ import torch
 
 from trainscale_amd import _lib
 from trainscale_amd.kernels import (MultiAxisRotaryEmbedding, RopeAxes, apply_rope_axes)
-from trainscale_amd.kernels.rope_kernels import _axes_positions, _turns, _turns_rest
+from trainscale_amd.kernels.rope_kernels import _axes_positions, _turn_parts, _turns
 
 OK, INVALID, DTYPE, SHAPE = 0, -1, -2, -3
 FAKE = 0x1000
@@ -144,5 +144,6 @@ def test_every_position_is_exact():
 def test_rest_of_a_turn():
     c = Fraction(inverse_two_pi(256), 1 << 256)
     for f in (1.0, 0.75, 1e-8, 3.7e-5, -0.2, 12345.678, 0.0, 2.0 ** -70):
-        off = (Fraction(_turns(f), 1 << 64) + Fraction(_turns_rest(f), 1 << 96) - Fraction(f) * c) % 1
-        assert min(off, 1 - off) <= Fraction(1, 1 << 96) and abs(_turns_rest(f)) <= 1 << 31
+        turns, rest = _turn_parts(f)
+        off = (Fraction(turns, 1 << 64) + Fraction(rest, 1 << 96) - Fraction(f) * c) % 1
+        assert min(off, 1 - off) <= Fraction(51, 100 << 96) and -1 << 31 <= rest < 1 << 31

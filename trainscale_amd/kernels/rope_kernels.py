@@ -426,17 +426,15 @@ def hf_apply_rotary_pos_emb(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor,
 _INV_2PI_192 = 0x28BE60DB9391054A7F09D5F47D4D377036D8A5664F10E410
 
 
+def _turn_parts(freq: float) -> Tuple[int, int]:
+    """freq / (2 pi) modulo 1: in units of 2^-64, rounded, and what that leaves in units of 2^-96."""
+    num, den = freq.as_integer_ratio()
+    whole = ((num * _INV_2PI_192 >> 95) // den + 1 >> 1) + (1 << 31)
+    return whole >> 32 & (1 << 64) - 1, (whole & (1 << 32) - 1) - (1 << 31)
+
+
 def _turns(freq: float) -> int:
-    """freq / (2 pi) modulo 1 in units of 2^-64, rounded."""
-    num, den = freq.as_integer_ratio()
-    return ((num * _INV_2PI_192 >> 127) // den + 1 >> 1) & (1 << 64) - 1
-
-
-def _turns_rest(freq: float) -> int:
-    """What _turns leaves of freq / (2 pi) modulo 1, in units of 2^-96."""
-    num, den = freq.as_integer_ratio()
-    rest = ((num * _INV_2PI_192 >> 95) // den + 1 >> 1) - (_turns(freq) << 32)
-    return min((rest + (1 << 31) & (1 << 96) - 1) - (1 << 31), (1 << 31) - 1)
+    return _turn_parts(freq)[0]
 
 
 class RopeAxes:
@@ -486,8 +484,9 @@ class RopeAxes:
         self.layout = layout
         self.interleaved = bool(interleaved)
         self.inv_freq = inv_freq
-        self._turns_c = (ctypes.c_uint64 * n)(*[_turns(f) for f in inv_freq.tolist()])
-        self._rest_c = (ctypes.c_int32 * n)(*[_turns_rest(f) for f in inv_freq.tolist()])
+        turns, rest = zip(*[_turn_parts(f) for f in inv_freq.tolist()])
+        self._turns_c = (ctypes.c_uint64 * n)(*turns)
+        self._rest_c = (ctypes.c_int32 * n)(*rest)
         self._axis_c = (ctypes.c_int32 * n)(*self.axis)
 
     def __repr__(self) -> str:
