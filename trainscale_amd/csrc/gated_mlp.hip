@@ -23,8 +23,10 @@
 // Bound by the matrix cores (at the power limit) from a few hundred rows on, by reading the weights
 // below. Measured on MI355X, N 8192, H = O = 4096, F 14336 bf16: projections 1585 us (1.21 PFLOP/s),
 // down 705 (1.37), gradients of g and u 965 (1.00: their epilogue moves 1.4 GB that no product hides;
-// starting workgroups apart changed nothing), dx and the weights' gradients 3634 (1.32); the library's
-// 8192^3 product reaches 1.38 here.
+// starting workgroups apart changed nothing), dx and the weights' gradients 3634-3707 (1.30-1.32); the
+// library's 8192^3 products reach 1.63 with k contiguous in both operands, as the first two, 1.39 in
+// one, as da and dx, and 1.21 in neither. Without w_down its place is taken by mlp_gate_bwd, 317 us
+// there (5.3 TB/s).
 #include <math.h>
 
 #include "common.hpp"

@@ -19,9 +19,9 @@
 // 16 bytes, 8 where the halves are not whole 16-byte vectors, single elements otherwise; any
 // element address will do.
 //
-// Bound by HBM. Measured on MI355X, a direction: [1, 32768, 64 + 8, 128] bf16 192 us (6.3 TB/s),
+// Bound by HBM. Measured on MI355X, a direction: [1, 32768, 64 + 8, 128] bf16 196 us (6.2 TB/s),
 // [8, 1369, 16 + 16, 80] fp16 28 us (4.4 TB/s; 2 tokens a workgroup 27, 8 of them 36), 16 tokens of 32 + 8
-// heads 4 us.
+// heads 4 us; adjacent pairs of the first 272 us (4.5 TB/s).
 #include "common.hpp"
 #include "plan.hpp"
 
